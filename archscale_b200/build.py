@@ -23,7 +23,7 @@ BUILD = os.path.join(PKG, "_build")
 OUT = os.path.join(PKG, "_C.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-PRECISE = {"gdn_pieces.cu"}     # built without --use_fast_math: expf at its documented accuracy, subnormal numbers kept
+PRECISE = {"gdn_pieces.cu", "fp8_quant.cu"}     # built without --use_fast_math: expf and divisions at their documented accuracy, subnormal numbers kept
 
 
 def _newer(src: str, dst: str, headers) -> bool:

@@ -5,6 +5,9 @@ from .attention import attention, attention_ref, pointwise_attention  # noqa: F4
 from .conv1d import causal_conv1d, causal_conv1d_ref  # noqa: F401
 from .cross_entropy import (FusedCrossEntropyLoss, FusedLinearCrossEntropyLoss, cross_entropy, cross_entropy_ref,  # noqa: F401
                             fused_linear_cross_entropy, fused_linear_cross_entropy_ref)
+from .fp8_block import (add_rms_norm_fp8, add_rms_norm_fp8_ref, add_rms_norm_linear_fp8, linear_fp8_block,  # noqa: F401
+                        linear_fp8_weight, matmul_fp8_block, matmul_fp8_block_ref, quantize_fp8_block,
+                        quantize_fp8_block_both, quantize_fp8_block_t, quantize_fp8_weight)
 from .gated_delta_rule import gated_delta_rule, gated_delta_rule_recurrent_ref  # noqa: F401
 from .gemm import linear, linear_swiglu, matmul_nn, matmul_nt, matmul_tn  # noqa: F401
 from .moe import (load_balance_loss, moe_ffn, moe_ffn_ref, router_topk_softmax, routing_metadata,  # noqa: F401

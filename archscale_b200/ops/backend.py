@@ -113,6 +113,9 @@ class NoCtx:
     def mark_non_differentiable(self, *tensors) -> None:
         pass
 
+    def set_materialize_grads(self, value: bool) -> None:
+        pass
+
 
 def apply(fn, *args):
     """``fn.apply(*args)``, or ``fn.forward`` itself where nothing can need its backward (:func:`plain_call`)."""

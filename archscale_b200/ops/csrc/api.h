@@ -281,6 +281,21 @@ int b200_gdn_state(const void* a_op, const void* c_add, const void* bm_op, const
 
 void b200_gemm_set_splitk_workspace(uint32_t* sem, int n);
 
+// e4m3 elements with one fp32 scale per block of 128 (fp8_quant.cu).  x [rows, cols] (rows ldx elements apart).  mode: 1 rows (q, s),
+// 2 columns, transposed (qt, st), 3 both, 4 tiles of 128 × 128 (q, s and, unless null, qt).  With rstd [rows] and w [cols] (mode 2) the
+// values are (x · rstd[row]) · w[col].  ldq, ldqt: bytes, multiples of 16; scales are [block][lds / ldst], of tiles [row block][column block].
+int b200_fp8_quantize(const void* x, int dtype, int64_t ldx, int rows, int cols, int mode, void* q, int64_t ldq, float* s, int64_t lds,
+                      void* qt, int64_t ldqt, float* st, int64_t ldst, const float* rstd, const void* w, int w_dtype, cudaStream_t stream);
+// x = res + h_scale · h, n = rmsnorm(x) · w quantised in blocks of 128 of a row.  res, x [rows, cols] dense (x unused without h), h bf16
+// or null, rstd [rows] or null; cols ≤ 32768.
+int b200_add_rmsnorm_fp8(const void* res, int res_dtype, const void* h, float h_scale, const void* w, int w_dtype, void* x, int x_dtype,
+                         void* q, int64_t ldq, float* s, int64_t lds, float* rstd, int rows, int cols, float eps, cudaStream_t stream);
+// out[M, N] (+)= Σ over blocks of 128 of K: sa · sb · (A block · B blockᵀ) (+ bias[N])  (gemm_fp8_block.cu).  A, B: e4m3, rows lda / ldb
+// bytes apart (multiples of 16, as the addresses); a scale belongs to one row, or (*_tile) to 128 rows, strides *_row and *_blk.
+int b200_gemm_fp8_block(const void* A, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_blk, int sa_tile, const void* B, int64_t ldb,
+                        const float* sb, int64_t sb_row, int64_t sb_blk, int sb_tile, const void* bias, int bias_dtype, void* out, int64_t ldc,
+                        int M, int N, int K, int out_f32, int accumulate, int num_sms, int* status, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

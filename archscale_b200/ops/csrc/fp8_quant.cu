@@ -1,0 +1,349 @@
+// Quantisers of the 8-bit format with one fp32 scale per block of 128 (e4m3 elements), and the residual addition + RMSNorm that
+// writes it.
+//
+// With a = max(max |x| over the block, 1e-30):  scale = a / 448,  u = 448 / a,  q = e4m3(x · u), all in fp32 with one rounding each (this
+// file is built without --use_fast_math), e4m3 rounding to nearest even.  |x · u| ≤ 448 up to one rounding, which e4m3 takes back, so nothing
+// saturates.  The floor of 1e-30 keeps u finite: an empty block gets zeros.  An infinity or NaN makes its block's scale infinite or
+// NaN and its own element NaN, so that a product shows it (magnitudes are compared as integers, where NaN is the largest).
+//
+// Scales are stored block-major, [block of 128][row] with the rows padded to a multiple of 4: the GEMM fetches one block's scales of
+// 128 neighbouring rows as 512 contiguous bytes.  Elements have rows of a multiple of 16 bytes (TMA).
+#include <cuda_fp8.h>
+
+#include "api.h"
+#include "sm100.cuh"
+
+namespace b200 {
+
+constexpr float kE4m3Max = 448.f, kBlockFloor = 1e-30f;
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ float block_amax(uint32_t bits) {                        // NaN stays NaN
+  return __uint_as_float(max(bits, __float_as_uint(kBlockFloor)));
+}
+__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
+  const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
+}
+
+// Eight neighbouring values, the first n of them inside the row (the others read as zero).  vec: whole 16-byte loads are aligned.
+__device__ __forceinline__ void load8(const float* p, int n, bool vec, float (&v)[8]) {
+  if (vec && n >= 8) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.f;
+  }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, int n, bool vec, float (&v)[8]) {
+  if (vec && n >= 8) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const float2 f = unpack_bf16x2(w[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? __bfloat162float(p[i]) : 0.f;
+  }
+}
+
+struct Fp8TileParams {
+  const void* x;
+  int64_t ldx;
+  int rows, cols, cb;           // cb: column blocks
+  int vec;
+  uint8_t* q; int64_t ldq;      // [rows][ldq]
+  float* s; int64_t lds;        // [cb][lds] per row, or [row block][cb] per tile
+  uint8_t* qt; int64_t ldqt;    // [cols][ldqt]
+  float* st; int64_t ldst;      // [row block][ldst] per column
+  const float* rstd;            // NORM: values are (x · rstd[row]) · w[col]
+  const void* w; int w_f32;
+};
+
+enum : int { FP8_ROWS = 1, FP8_COLS = 2, FP8_TILE = 4 };
+
+// One CTA per 128 × 128 tile, read once.  A thread holds 8 rows × 8 columns; magnitudes meet in shared memory, where one thread per
+// row and per column makes the two factors (and writes the scale: 512 contiguous bytes per tile).  The transposed elements turn in
+// shared memory: 16-byte pieces (rows of one column) at slot (piece ^ column / 8), two passes per access, no more conflicts.
+template <typename T, int MODE, bool NORM>
+__global__ void __launch_bounds__(256) fp8_tile_kernel(const Fp8TileParams p) {
+  __shared__ uint32_t s_row[128], s_col[8][128];
+  __shared__ __align__(16) uint8_t s_t[(MODE & FP8_COLS) || MODE == FP8_TILE ? 128 * 128 : 16];
+  const int t = threadIdx.x, warp = t >> 5, cg = t & 15, rg = t >> 4;      // column group, row group (8 each)
+  const int rb = blockIdx.x / p.cb, kb = blockIdx.x - rb * p.cb;
+  const int r0 = rb * 128 + rg * 8, c0 = kb * 128 + cg * 8;
+  const int nc = min(max(p.cols - c0, 0), 8);
+  const T* x = static_cast<const T*>(p.x) + static_cast<int64_t>(r0) * p.ldx + c0;
+  float v[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) load8(x + i * p.ldx, r0 + i < p.rows ? nc : 0, p.vec, v[i]);
+  if (NORM) {
+    float w[8];
+    if (p.w_f32) load8(static_cast<const float*>(p.w) + c0, nc, false, w);
+    else load8(static_cast<const __nv_bfloat16*>(p.w) + c0, nc, false, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float rs = r0 + i < p.rows ? p.rstd[r0 + i] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = __fmul_rn(__fmul_rn(v[i][e], rs), w[e]);
+    }
+  }
+  if (MODE == FP8_TILE) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = max(m, abs_bits(v[i][e]));
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((t & 31) == 0) s_row[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, s_row[i]);
+    const float a = block_amax(m), u = __fdiv_rn(kE4m3Max, a);
+    if (t == 0) p.s[static_cast<int64_t>(rb) * p.cb + kb] = __fdiv_rn(a, kE4m3Max);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = __fmul_rn(v[i][e], u);
+  } else {
+    if (MODE & FP8_ROWS) {
+      const uint32_t half = 0xffffu << (t & 16);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = max(m, abs_bits(v[i][e]));
+        m = __reduce_max_sync(half, m);
+        if (cg == 0) s_row[rg * 8 + i] = m;
+      }
+    }
+    if (MODE & FP8_COLS) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i][e]));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        if ((t & 16) == 0) s_col[warp][cg * 8 + e] = m;
+      }
+    }
+    __syncthreads();
+    if ((MODE & FP8_ROWS) && t < 128) {
+      const float a = block_amax(s_row[t]);
+      s_row[t] = __float_as_uint(__fdiv_rn(kE4m3Max, a));
+      if (rb * 128 + t < p.rows) p.s[kb * p.lds + rb * 128 + t] = __fdiv_rn(a, kE4m3Max);
+    }
+    if ((MODE & FP8_COLS) && t >= 128) {
+      const int c = t - 128;
+      uint32_t m = s_col[0][c];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) m = max(m, s_col[i][c]);
+      const float a = block_amax(m);
+      s_col[0][c] = __float_as_uint(__fdiv_rn(kE4m3Max, a));
+      if (kb * 128 + c < p.cols) p.st[rb * p.ldst + kb * 128 + c] = __fdiv_rn(a, kE4m3Max);
+    }
+    __syncthreads();
+  }
+  if (((MODE & FP8_ROWS) || MODE == FP8_TILE) && c0 < p.cols) {            // 8-byte pieces: rows are padded to a multiple of 16
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (r0 + i >= p.rows) break;
+      const float u = MODE == FP8_TILE ? 1.f : __uint_as_float(s_row[rg * 8 + i]);
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = MODE == FP8_TILE ? v[i][e] : __fmul_rn(v[i][e], u);
+      *reinterpret_cast<uint2*>(p.q + static_cast<int64_t>(r0 + i) * p.ldq + c0) =
+          make_uint2(pack_e4m3x4(o[0], o[1], o[2], o[3]), pack_e4m3x4(o[4], o[5], o[6], o[7]));
+    }
+  }
+  if ((MODE & FP8_COLS) || (MODE == FP8_TILE && p.qt)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = cg * 8 + e;
+      const float u = MODE == FP8_TILE ? 1.f : __uint_as_float(s_col[0][c]);
+      float o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = MODE == FP8_TILE ? v[i][e] : __fmul_rn(v[i][e], u);
+      *reinterpret_cast<uint2*>(s_t + c * 128 + (((rg >> 1) ^ (cg & 7)) << 4) + ((rg & 1) << 3)) =
+          make_uint2(pack_e4m3x4(o[0], o[1], o[2], o[3]), pack_e4m3x4(o[4], o[5], o[6], o[7]));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = i * 32 + (t >> 3), piece = t & 7;
+      const int row = rb * 128 + piece * 16;
+      if (kb * 128 + c < p.cols && row < p.rows)
+        *reinterpret_cast<uint4*>(p.qt + static_cast<int64_t>(kb * 128 + c) * p.ldqt + row) =
+            *reinterpret_cast<const uint4*>(s_t + c * 128 + ((piece ^ ((c >> 3) & 7)) << 4));
+    }
+  }
+}
+
+template <typename T, int MODE, bool NORM>
+static int launch_tile(const Fp8TileParams& p, cudaStream_t st) {
+  const int64_t tiles = static_cast<int64_t>((p.rows + 127) / 128) * p.cb;
+  if (tiles > 0x7fffffff) return -6;
+  fp8_tile_kernel<T, MODE, NORM><<<static_cast<unsigned>(tiles), 256, 0, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+// ------------------------------------------------------------------ residual addition + RMSNorm → e4m3
+//   x = res + h_scale · h (fp32, rounded to the stream's type),  n = x · rsqrt(mean x² + eps) · w (fp32),  n quantised in blocks of 128
+// n is never rounded to 16 bits: the only rounding between the stream and the tensor cores is the one to e4m3.
+struct Fp8NormParams {
+  const void* res; const __nv_bfloat16* h; const void* w;
+  float h_scale, eps;
+  int rows, cols, vec, w_vec;
+  void* x;                      // new stream (null without h)
+  uint8_t* q; int64_t ldq;
+  float* s; int64_t lds;
+  float* rstd;                  // [rows] or null
+};
+
+__device__ __forceinline__ void store8(float* p, int n, bool vec, const float (&v)[8]) {
+  if (vec && n >= 8) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) if (i < n) p[i] = v[i];
+  }
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, int n, bool vec, const float (&v)[8]) {
+  if (vec && n >= 8) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) if (i < n) p[i] = __float2bfloat16(v[i]);
+  }
+}
+__device__ __forceinline__ float round_to(float v, const float*) { return v; }
+__device__ __forceinline__ float round_to(float v, const __nv_bfloat16*) { return __bfloat162float(__float2bfloat16(v)); }
+
+// TPR threads per row, V vectors of 8 per thread: the row stays in registers.  16 neighbouring threads hold one block of 128.
+template <typename T, typename TO, int TPR, int V>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) fp8_norm_kernel(const Fp8NormParams p) {
+  constexpr int CTA = TPR < 128 ? 128 : TPR, RPC = CTA / TPR, WPR = TPR / 32;
+  __shared__ float s_sum[CTA / 32];
+  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  const int row = blockIdx.x * RPC + sub;
+  const bool live = row < p.rows;
+  const int64_t base = static_cast<int64_t>(row) * p.cols;
+  float v[V][8];
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = (t + i * TPR) * 8;
+    const int n = live ? min(max(p.cols - c, 0), 8) : 0;
+    load8(static_cast<const T*>(p.res) + base + c, n, p.vec, v[i]);
+    if (p.h) {
+      float h[8];
+      load8(p.h + base + c, n, p.vec, h);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = round_to(__fadd_rn(v[i][e], __fmul_rn(p.h_scale, h[e])), static_cast<const TO*>(nullptr));
+      if (n > 0) store8(static_cast<TO*>(p.x) + base + c, n, p.vec, v[i]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss += v[i][e] * v[i][e];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (WPR > 1) {
+    if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = ss;
+    __syncthreads();
+    ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < WPR; ++i) ss += s_sum[sub * WPR + i];
+  }
+  const float rs = rsqrtf(ss / static_cast<float>(p.cols) + p.eps);
+  if (live && t == 0 && p.rstd) p.rstd[row] = rs;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = (t + i * TPR) * 8;
+    const int n = live ? min(max(p.cols - c, 0), 8) : 0;
+    float w[8];
+    // w may be unaligned when its type differs from the stream's, so it has a rule of its own
+    if (p.w_vec & 2) load8(static_cast<const float*>(p.w) + c, n, p.w_vec & 1, w);
+    else load8(static_cast<const __nv_bfloat16*>(p.w) + c, n, p.w_vec & 1, w);
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[i][e] = __fmul_rn(__fmul_rn(v[i][e], rs), w[e]);
+      m = max(m, e < n ? abs_bits(v[i][e]) : 0u);
+    }
+    m = __reduce_max_sync(0xffffu << (threadIdx.x & 16), m);
+    if (n > 0) {
+      const float a = block_amax(m), u = __fdiv_rn(kE4m3Max, a);
+      if ((t & 15) == 0) p.s[(c >> 7) * p.lds + row] = __fdiv_rn(a, kE4m3Max);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = __fmul_rn(v[i][e], u);
+      *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) =
+          make_uint2(pack_e4m3x4(v[i][0], v[i][1], v[i][2], v[i][3]), pack_e4m3x4(v[i][4], v[i][5], v[i][6], v[i][7]));
+    }
+  }
+}
+
+template <typename T, typename TO>
+static int launch_norm(const Fp8NormParams& p, cudaStream_t st) {
+  const int vecs = (p.cols + 7) / 8;
+#define FP8_NORM(TPR, V)                                                                                     \
+  if (vecs <= TPR * V) {                                                                                     \
+    constexpr int RPC = TPR < 128 ? 128 / TPR : 1;                                                           \
+    fp8_norm_kernel<T, TO, TPR, V><<<(p.rows + RPC - 1) / RPC, TPR < 128 ? 128 : TPR, 0, st>>>(p);           \
+    return cudaGetLastError() == cudaSuccess ? 0 : -3;                                                       \
+  }
+  FP8_NORM(32, 1)
+  FP8_NORM(64, 1)
+  FP8_NORM(128, 1)
+  FP8_NORM(256, 1)
+  FP8_NORM(256, 2)
+  FP8_NORM(256, 4)
+  FP8_NORM(1024, 4)
+#undef FP8_NORM
+  return -6;
+}
+
+}  // namespace b200
+
+// x [rows, cols] (dtype 0 fp32, 1 bf16, rows ldx elements apart).  mode: 1 rows (q, s), 2 columns (qt, st), 3 both, 4 tiles of
+// 128 × 128 (q, s and, unless null, qt).  With rstd, w: the values are (x · rstd[row]) · w[col] (modes 1 to 3).  ldq, ldqt: multiples of 16.
+extern "C" int b200_fp8_quantize(const void* x, int dtype, int64_t ldx, int rows, int cols, int mode, void* q, int64_t ldq, float* s,
+                                 int64_t lds, void* qt, int64_t ldqt, float* st, int64_t ldst, const float* rstd, const void* w,
+                                 int w_dtype, cudaStream_t stream) {
+  using namespace b200;
+  if (rows < 0 || cols < 0 || (dtype != 0 && dtype != 1) || mode < 1 || mode > 4 || (rstd && mode != 2)) return -6;
+  if (rows == 0 || cols == 0) return 0;
+  const int esz = dtype == 0 ? 4 : 2;
+  Fp8TileParams p{x, ldx, rows, cols, (cols + 127) / 128,
+                  reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * esz % 16 == 0 ? 1 : 0,
+                  static_cast<uint8_t*>(q), ldq, s, lds, static_cast<uint8_t*>(qt), ldqt, st, ldst, rstd, w, w_dtype == 0 ? 1 : 0};
+  if (dtype == 0) {
+    if (rstd) return launch_tile<float, FP8_COLS, true>(p, stream);
+    if (mode == 1) return launch_tile<float, FP8_ROWS, false>(p, stream);
+    if (mode == 2) return launch_tile<float, FP8_COLS, false>(p, stream);
+    if (mode == 3) return launch_tile<float, FP8_ROWS | FP8_COLS, false>(p, stream);
+    return launch_tile<float, FP8_TILE, false>(p, stream);
+  }
+  if (rstd) return launch_tile<__nv_bfloat16, FP8_COLS, true>(p, stream);
+  if (mode == 1) return launch_tile<__nv_bfloat16, FP8_ROWS, false>(p, stream);
+  if (mode == 2) return launch_tile<__nv_bfloat16, FP8_COLS, false>(p, stream);
+  if (mode == 3) return launch_tile<__nv_bfloat16, FP8_ROWS | FP8_COLS, false>(p, stream);
+  return launch_tile<__nv_bfloat16, FP8_TILE, false>(p, stream);
+}
+
+// res, x [rows, cols] dense (dtype 0 fp32, 1 bf16; x null without h), h bf16 or null, w [cols].  cols ≤ 32768.
+extern "C" int b200_add_rmsnorm_fp8(const void* res, int res_dtype, const void* h, float h_scale, const void* w, int w_dtype, void* x,
+                                    int x_dtype, void* q, int64_t ldq, float* s, int64_t lds, float* rstd, int rows, int cols, float eps,
+                                    cudaStream_t stream) {
+  using namespace b200;
+  if (rows < 0 || cols < 1 || cols > 32768 || (x_dtype == 1 && res_dtype != 1)) return -6;
+  if (rows == 0) return 0;
+  const auto al = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; };
+  const int vec = cols % 8 == 0 && al(res) && al(h) && al(x) ? 1 : 0;
+  Fp8NormParams p{res, static_cast<const __nv_bfloat16*>(h), w, h_scale, eps, rows, cols, vec,
+                  (al(w) ? 1 : 0) | (w_dtype == 0 ? 2 : 0), x, static_cast<uint8_t*>(q), ldq, s, lds, rstd};
+  if (res_dtype == 0) return launch_norm<float, float>(p, stream);
+  return x_dtype == 0 ? launch_norm<__nv_bfloat16, float>(p, stream) : launch_norm<__nv_bfloat16, __nv_bfloat16>(p, stream);
+}

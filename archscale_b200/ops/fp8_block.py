@@ -1,0 +1,398 @@
+"""Linear layers in 8-bit floating point with one fp32 scale per block of 128 (e4m3 elements).
+
+A block is 128 neighbouring values of a row (activations, gradients) or a 128 × 128 tile (weights); the last one may be shorter.
+With ``a = max(max|block|, 1e-30)``, every operation in fp32 and rounded once,
+
+    ``scale = a / 448``,   ``q = e4m3(x · (448 / a))``,   ``x ≈ q · scale``
+
+(:func:`quantize_fp8_block`, :func:`quantize_fp8_block_both`, :func:`quantize_fp8_weight`), and the product of two such operands is
+
+    ``out[m, n] = Σ_b sa[m, b] · sb[n, b] · Σ_{k in b} a[m, k] · b[n, k]``                        (:func:`matmul_fp8_block`)
+
+with the inner sums on the tensor cores and the outer ones in fp32.  Where both scales of a block are so small that their product
+is below 2⁻¹²⁶ the block counts as zero.  Any size is taken: no dimension has to be a multiple of 128.
+
+* :func:`linear_fp8_block` trains: ``y = Q(x) Q(W)ᵀ``, ``dx = Q(dy) Q(W)``, ``dW = Qᵗ(dy)ᵀ Qᵗ(x)``, where ``Qᵗ`` takes its blocks along the
+  tokens; the rounding itself has gradient one.  Weights stay bf16 / fp32 and are quantised in every call.
+* :func:`linear_fp8_weight` serves weights that were quantised beforehand (``quantize_fp8_weight``, or a checkpoint's elements and
+  scales), from one token on.
+* :func:`add_rms_norm_fp8` is the block entry ``x = res + h_scale · h``, ``n = rmsnorm(x) · w`` with ``n`` delivered in this format (it is never
+  rounded to 16 bits); :func:`add_rms_norm_linear_fp8` trains it with the layer behind it.  Its backward makes the transposed operand of
+  the weight gradient from the residual stream, which is kept anyway, so that ``n`` itself is kept in no form.
+
+Scales are returned as ``(rows, blocks)``; in memory the rows are the fast dimension, which is what the GEMM reads.  Elements
+have rows of a multiple of 16 bytes (TMA); others are copied into such rows within the call.
+
+The functions ending in ``_ref`` are plain PyTorch restatements used as the CPU path and as test oracles.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import backend
+from .norm import fused_cols_ok
+
+BLOCK, E4M3_MAX, BLOCK_FLOOR = 128, 448.0, 1e-30
+FP8 = torch.float8_e4m3fn
+_FLOATS = (torch.bfloat16, torch.float32)
+
+
+# ------------------------------------------------------------------------------------------------ references
+def _padded(x: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    return torch.nn.functional.pad(x, (0, -x.shape[1] % cols, 0, -x.shape[0] % rows))
+
+
+def _factors(amax: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(scale, 448 / a).  Both are divisions of tensors: with a Python number torch multiplies by a rounded reciprocal."""
+    a = amax.clamp_min(BLOCK_FLOOR)
+    top = torch.full_like(a, E4M3_MAX)
+    return a / top, top / a
+
+
+def quantize_ref(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    R, C = x.shape
+    xb = _padded(x.float(), 1, BLOCK).reshape(R, -1, BLOCK)
+    scale, u = _factors(xb.abs().amax(-1))
+    return (xb * u.unsqueeze(-1)).to(FP8).reshape(R, -1)[:, :C].contiguous(), scale
+
+
+def quantize_weight_ref(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    N, K = w.shape
+    wb = _padded(w.float(), BLOCK, BLOCK)
+    nb, kb = wb.shape[0] // BLOCK, wb.shape[1] // BLOCK
+    wb = wb.view(nb, BLOCK, kb, BLOCK)
+    scale, u = _factors(wb.abs().amax((1, 3)))
+    return (wb * u.view(nb, 1, kb, 1)).to(FP8).view(nb * BLOCK, kb * BLOCK)[:N, :K].contiguous(), scale
+
+
+def dequantize_ref(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """Values of elements with one scale per row and block, or per 128 × 128 tile."""
+    R, C = q.shape
+    s = scale.to(dtype)
+    if s.shape[0] != R:
+        s = s.repeat_interleave(BLOCK, 0)[:R]
+    return q.to(dtype) * s.repeat_interleave(BLOCK, 1)[:, :C]
+
+
+def matmul_fp8_block_ref(a, a_scale, b, b_scale, bias=None, out_dtype=torch.bfloat16, acc=None):
+    y = dequantize_ref(a, a_scale) @ dequantize_ref(b, b_scale).t()
+    if bias is not None:
+        y = y + bias.float()
+    return acc.add_(y) if acc is not None else y.to(out_dtype)
+
+
+def _norm_ref(res, h, weight, eps, h_scale, stream_dtype):
+    x = res.float()
+    if h is not None:
+        x = (x + h_scale * h.float()).to(stream_dtype)
+    xf = x.float()
+    rstd = torch.rsqrt(xf.square().mean(-1, keepdim=True) + eps)
+    return (x if h is not None else res), rstd, xf * rstd * weight.float()
+
+
+def add_rms_norm_fp8_ref(res, h, weight, eps: float = 1e-5, h_scale: float = 1.0, stream_dtype: Optional[torch.dtype] = None):
+    x, _, n = _norm_ref(res, h, weight, eps, h_scale, _stream(res, stream_dtype))
+    q, scale = quantize_ref(n.reshape(-1, n.shape[-1]))
+    return x, q, scale
+
+
+# ------------------------------------------------------------------------------------------------ checks
+def _stream(res: torch.Tensor, stream_dtype: Optional[torch.dtype]) -> torch.dtype:
+    return res.dtype if stream_dtype is None else stream_dtype
+
+
+def _need_float(name: str, **tensors) -> None:
+    for what, t in tensors.items():
+        if t is not None and t.dtype not in _FLOATS:
+            raise TypeError(f"{name}: {what} must be bfloat16 or float32, got {t.dtype}")
+
+
+def _need_matrix(name: str, x: torch.Tensor) -> None:
+    if x.dim() != 2:
+        raise ValueError(f"{name}: a matrix is needed, got shape {tuple(x.shape)}")
+    _need_float(name, x=x)
+
+
+def _dense_rows(x: torch.Tensor) -> torch.Tensor:
+    return x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous()
+
+
+def _kernel(*tensors) -> bool:
+    return tensors[0].is_cuda and backend.use_cuda_kernel("fp8_block", *tensors)
+
+
+# ------------------------------------------------------------------------------------------------ quantisers
+def quantize_fp8_block(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x:(R,C) → (elements (R,C), scales (R, ⌈C/128⌉)), blocks along the rows."""
+    _need_matrix("quantize_fp8_block", x)
+    if not _kernel(x):
+        return quantize_ref(x)
+    backend.count_launch()
+    return tuple(backend.require_extension().fp8_quantize(_dense_rows(x), 1))
+
+
+def quantize_fp8_block_t(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x:(R,C) → (elements (C,R), scales (C, ⌈R/128⌉)) of the transposed matrix, blocks along the original columns."""
+    _need_matrix("quantize_fp8_block_t", x)
+    if not _kernel(x):
+        return quantize_ref(x.t())
+    backend.count_launch()
+    return tuple(backend.require_extension().fp8_quantize(_dense_rows(x), 2))
+
+
+def quantize_fp8_block_both(x: torch.Tensor):
+    """:func:`quantize_fp8_block` and :func:`quantize_fp8_block_t` from one read of x: (q, scale, q_t, scale_t)."""
+    _need_matrix("quantize_fp8_block_both", x)
+    if not _kernel(x):
+        return (*quantize_ref(x), *quantize_ref(x.t()))
+    backend.count_launch()
+    return tuple(backend.require_extension().fp8_quantize(_dense_rows(x), 3))
+
+
+def quantize_fp8_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """w:(N,K) → (elements (N,K), the same transposed (K,N), scales (⌈N/128⌉, ⌈K/128⌉) of 128 × 128 tiles)."""
+    _need_matrix("quantize_fp8_weight", w)
+    if not _kernel(w):
+        q, scale = quantize_weight_ref(w)
+        return q, q.t().contiguous(), scale
+    backend.count_launch()
+    q, scale, q_t = backend.require_extension().fp8_quantize(_dense_rows(w), 4)
+    return q, q_t, scale
+
+
+# ------------------------------------------------------------------------------------------------ product
+def _whole_rows(q: torch.Tensor) -> torch.Tensor:
+    """Elements as the GEMM reads them: dense rows that start at multiples of 16 bytes."""
+    K = q.shape[1]
+    if (q.stride(1) == 1 or K <= 1) and (q.stride(0) % 16 == 0 or q.shape[0] <= 1) and q.data_ptr() % 16 == 0:
+        return q
+    out = torch.empty(q.shape[0], (K + 15) // 16 * 16, dtype=torch.uint8, device=q.device)[:, :K]
+    out.copy_(q.view(torch.uint8) if q.stride(1) == 1 else q.contiguous().view(torch.uint8))
+    return out.view(FP8)
+
+
+def matmul_fp8_block(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                     out_dtype: torch.dtype = torch.bfloat16, acc: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``a:(M,K) · b:(N,K)ᵀ (+ bias)``, each operand with scales per row and block of 128, ``(rows, ⌈K/128⌉)``, or per 128 × 128 tile,
+    ``(⌈rows/128⌉, ⌈K/128⌉)`` → (M,N) in ``out_dtype``; with ``acc`` (fp32) the product is added to it in place."""
+    for what, t in (("a", a), ("b", b)):
+        if t.dtype != FP8 or t.dim() != 2:
+            raise TypeError(f"matmul_fp8_block: {what} must be a float8_e4m3fn matrix, got {t.dtype} {tuple(t.shape)}")
+    if a.shape[1] != b.shape[1]:
+        raise ValueError(f"matmul_fp8_block: contraction lengths differ: {a.shape[1]} and {b.shape[1]}")
+    blocks = (a.shape[1] + BLOCK - 1) // BLOCK
+    for what, q, s in (("a_scale", a, a_scale), ("b_scale", b, b_scale)):
+        if s.dtype != torch.float32 or s.dim() != 2 or s.shape[1] != blocks or s.shape[0] not in (q.shape[0], (q.shape[0] + BLOCK - 1) // BLOCK):
+            raise ValueError(f"matmul_fp8_block: {what} must be float32 ({q.shape[0]} or {(q.shape[0] + BLOCK - 1) // BLOCK}, {blocks}), "
+                             f"got {s.dtype} {tuple(s.shape)}")
+    if bias is not None and (bias.shape != (b.shape[0],) or bias.dtype not in _FLOATS):
+        raise ValueError(f"matmul_fp8_block: bias must be ({b.shape[0]},) in bfloat16 or float32, got {bias.dtype} {tuple(bias.shape)}")
+    if out_dtype not in _FLOATS:
+        raise TypeError(f"matmul_fp8_block: out_dtype must be bfloat16 or float32, got {out_dtype}")
+    if acc is not None and (acc.dtype != torch.float32 or acc.shape != (a.shape[0], b.shape[0])):
+        raise ValueError(f"matmul_fp8_block: acc must be float32 ({a.shape[0]}, {b.shape[0]}), got {acc.dtype} {tuple(acc.shape)}")
+    if not _kernel(a, a_scale, b, b_scale):
+        return matmul_fp8_block_ref(a, a_scale, b, b_scale, bias, out_dtype, acc)
+    backend.count_launch()
+    return backend.require_extension().gemm_fp8_block(_whole_rows(a), a_scale, _whole_rows(b), b_scale,
+                                                      None if bias is None else bias.contiguous(), out_dtype == torch.float32, acc)
+
+
+Quantised = Tuple[torch.Tensor, torch.Tensor]
+
+
+def linear_fp8_weight(x: Union[torch.Tensor, Quantised], weight: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                      out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``x · Wᵀ (+ bias)`` with stored elements ``weight:(N,K)`` and scales of 128 × 128 tiles.  ``x:(..., K)`` is quantised here, or is the
+    pair (elements, scales) of :func:`add_rms_norm_fp8` / :func:`quantize_fp8_block` with any leading dimensions of the elements.  No
+    gradients."""
+    if isinstance(x, torch.Tensor):
+        _need_float("linear_fp8_weight", x=x)
+        lead, out_dtype = x.shape[:-1], out_dtype or x.dtype
+        q, s = quantize_fp8_block(x.detach().reshape(-1, x.shape[-1]))
+    else:
+        q, s = x
+        lead, out_dtype = q.shape[:-1], out_dtype or torch.bfloat16
+        if q.dim() != 2:
+            q = q.reshape(-1, q.shape[-1])
+    y = matmul_fp8_block(q, s, weight, scale, bias, out_dtype)
+    return y if len(lead) == 1 else y.view(*lead, weight.shape[0])
+
+
+# ------------------------------------------------------------------------------------------------ training
+def _weight_grad(g_t, x_t, weight):
+    """dW from the operands with blocks along the tokens, into ``main_grad`` where the weight carries one."""
+    main_grad = getattr(weight, "main_grad", None)
+    if main_grad is not None:
+        matmul_fp8_block(*g_t, *x_t, acc=main_grad)
+        return None
+    return matmul_fp8_block(*g_t, *x_t, out_dtype=weight.dtype)
+
+
+def _grad_operands(gy, need_x: bool, need_w: bool):
+    if need_x and need_w:
+        q, s, q_t, s_t = quantize_fp8_block_both(gy)
+        return (q, s), (q_t, s_t)
+    return (quantize_fp8_block(gy), None) if need_x else (None, quantize_fp8_block_t(gy))
+
+
+class _LinearFP8Fn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        x2 = x.reshape(-1, x.shape[-1])
+        wq, wq_t, ws = quantize_fp8_weight(weight)
+        x_t = ()
+        if ctx.needs_input_grad and ctx.needs_input_grad[1]:
+            xq, xs, *x_t = quantize_fp8_block_both(x2)
+        else:
+            xq, xs = quantize_fp8_block(x2)
+        ctx.save_for_backward(wq_t, ws, *x_t)
+        ctx.weight, ctx.x_shape, ctx.x_dtype = weight, x.shape, x.dtype
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return matmul_fp8_block(xq, xs, wq, ws, bias, x.dtype).view(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        wq_t, ws, *x_t = ctx.saved_tensors
+        gy2 = gy.reshape(-1, gy.shape[-1])
+        need_x, need_w, need_b = ctx.needs_input_grad
+        dx = dw = None
+        if need_x or need_w:
+            g, g_t = _grad_operands(gy2, need_x, need_w)
+        if need_x:
+            dx = matmul_fp8_block(*g, wq_t, ws.t(), out_dtype=ctx.x_dtype).view(ctx.x_shape)
+        if need_w:
+            dw = _weight_grad(g_t, x_t, ctx.weight)
+        return dx, dw, (gy2.sum(0, dtype=torch.float32).to(ctx.bias_dtype) if need_b else None)
+
+
+def _check_layer(name, cols, weight, bias=None):
+    if weight.dim() != 2 or weight.shape[1] != cols:
+        raise ValueError(f"{name}: weight must be (out, {cols}), got {tuple(weight.shape)}")
+    _need_float(name, weight=weight, bias=bias)
+    if bias is not None and bias.shape != (weight.shape[0],):
+        raise ValueError(f"{name}: bias must be ({weight.shape[0]},), got {tuple(bias.shape)}")
+
+
+def linear_fp8_block(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x · weightᵀ (+ bias)`` with x:(..., K) and weight:(N, K) quantised in the call; trains (see the head of this file)."""
+    _need_float("linear_fp8_block", x=x)
+    _check_layer("linear_fp8_block", x.shape[-1], weight, bias)
+    return backend.apply(_LinearFP8Fn, x, weight, bias)
+
+
+# ------------------------------------------------------------------------------------------------ residual addition + RMSNorm
+def _check_norm(name, res, h, weight, stream_dtype):
+    _need_float(name, res=res, weight=weight)
+    if weight.shape != (res.shape[-1],):
+        raise ValueError(f"{name}: the norm's weight must be ({res.shape[-1]},), got {tuple(weight.shape)}")
+    if h is not None and (h.shape != res.shape or h.dtype != torch.bfloat16):
+        raise ValueError(f"{name}: the branch must be bfloat16 {tuple(res.shape)}, got {h.dtype} {tuple(h.shape)}")
+    if stream_dtype not in _FLOATS or (stream_dtype == torch.bfloat16 and res.dtype != torch.bfloat16):
+        raise TypeError(f"{name}: a {res.dtype} residual stream cannot be kept in {stream_dtype}")
+
+
+def _norm_kernel(res, h, weight, eps, h_scale, stream_dtype, want_rstd):
+    """(x, q, scale, rstd) on two-dimensional operands."""
+    if not _kernel(res, h, weight) or not 1 <= res.shape[1] <= 32768:
+        x, rstd, n = _norm_ref(res, h, weight, eps, h_scale, stream_dtype)
+        return (x, *quantize_ref(n), rstd.reshape(-1))
+    backend.count_launch()
+    return backend.require_extension().add_rmsnorm_fp8(res.contiguous(), None if h is None else h.contiguous(), h_scale, weight.contiguous(), eps,
+                                                       stream_dtype == torch.bfloat16, want_rstd)
+
+
+def add_rms_norm_fp8(res: torch.Tensor, h: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-5, h_scale: float = 1.0,
+                     stream_dtype: Optional[torch.dtype] = None):
+    """``x = res + h_scale · h`` (fp32, kept in ``stream_dtype``, by default the type of ``res``; without ``h`` x is ``res``) and ``rmsnorm(x) · weight`` as
+    elements and scales: (x of the shape of res, elements (rows, C), scales (rows, ⌈C/128⌉)).  No gradients: training goes through
+    :func:`add_rms_norm_linear_fp8`."""
+    stream_dtype = _stream(res, stream_dtype)
+    _check_norm("add_rms_norm_fp8", res, h, weight, stream_dtype)
+    C = res.shape[-1]
+    with torch.no_grad():
+        x, q, scale, _ = _norm_kernel(res.reshape(-1, C), None if h is None else h.reshape(-1, C), weight, eps, h_scale, stream_dtype, False)
+    return (res if h is None else x.view(res.shape)), q, scale
+
+
+def _norm_backward_ref(gx, dn, x, weight, rstd, h_scale, want_h):
+    """Formula of the norm's gradients in fp32: (d_res fp32, d_h | None, d_weight fp32)."""
+    xhat = x.float() * rstd.view(-1, 1)
+    t = dn.float() * weight.float()
+    d = rstd.view(-1, 1) * (t - xhat * (t * xhat).mean(-1, keepdim=True))
+    if gx is not None:
+        d = d + gx.float()
+    return d, ((h_scale * d).to(torch.bfloat16) if want_h else None), (dn.float() * xhat).sum(0)
+
+
+class _AddNormLinearFP8Fn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, res, h, norm_weight, weight, bias, eps, h_scale, stream_dtype):
+        C = res.shape[-1]
+        res2, h2 = res.reshape(-1, C), None if h is None else h.reshape(-1, C)
+        x, q, s, rstd = _norm_kernel(res2, h2, norm_weight, eps, h_scale, stream_dtype, True)
+        wq, wq_t, ws = quantize_fp8_weight(weight)
+        ctx.save_for_backward(x, rstd, norm_weight, wq_t, ws)
+        ctx.weight, ctx.shape, ctx.res_dtype, ctx.h_scale, ctx.has_h = weight, res.shape, res.dtype, h_scale, h is not None
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.set_materialize_grads(False)
+        y = matmul_fp8_block(q, s, wq, ws, bias, torch.bfloat16).view(*res.shape[:-1], weight.shape[0])
+        return (x.view(res.shape) if h is not None else res.view_as(res)), y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gx, gy):
+        x, rstd, norm_weight, wq_t, ws = ctx.saved_tensors
+        C = ctx.shape[-1]
+        need_res, need_h, need_nw, need_w, need_b = ctx.needs_input_grad[:5]
+        need_n = need_res or need_h or need_nw
+        gx2 = None if gx is None else gx.reshape(-1, C)
+        dw = db = dres = dh = dnw = None
+        if gy is None:
+            dn = None
+        else:
+            gy2 = gy.reshape(-1, gy.shape[-1])
+            g, g_t = _grad_operands(gy2, need_n, need_w) if need_n or need_w else (None, None)
+            if need_w:
+                dw = _weight_grad(g_t, _normed_t(x, rstd, norm_weight), ctx.weight)
+            if need_b:
+                db = gy2.sum(0, dtype=torch.float32).to(ctx.bias_dtype)
+            # the norm's backward kernel reads bf16: one rounding of dn, as in the bf16 layers
+            fused = _kernel(x, norm_weight) and fused_cols_ok(C)
+            dn = matmul_fp8_block(*g, wq_t, ws.t(), out_dtype=torch.bfloat16 if fused else torch.float32) if need_n else None
+        if need_n:
+            if dn is None:
+                dres = gx2
+                dh = None if gx2 is None or not need_h else (ctx.h_scale * gx2.float()).to(torch.bfloat16)
+            elif fused:
+                bf16_stream = x.dtype == torch.bfloat16
+                gx3 = None if gx2 is None else gx2.to(x.dtype).contiguous()
+                dres, dh, dnw = backend.require_extension().add_rmsnorm_bwd(gx3, dn, x, norm_weight, rstd, ctx.has_h and need_h, ctx.h_scale,
+                                                                           bf16_stream)
+                backend.count_launch(2)
+            else:
+                dres, dh, dnw = _norm_backward_ref(gx2, dn, x, norm_weight, rstd, ctx.h_scale, ctx.has_h and need_h)
+        return (dres.to(ctx.res_dtype).view(ctx.shape) if need_res and dres is not None else None,
+                dh.view(ctx.shape) if need_h and dh is not None else None,
+                dnw.to(norm_weight.dtype) if need_nw and dnw is not None else None, dw, db, None, None, None)
+
+
+def _normed_t(x, rstd, weight):
+    """The normalised values again, quantised with blocks along the tokens: (elements (C, rows), scales)."""
+    if not _kernel(x, rstd, weight):
+        return quantize_ref((x.float() * rstd.view(-1, 1) * weight.float()).t())
+    backend.count_launch()
+    return tuple(backend.require_extension().fp8_quantize(x, 2, rstd, weight.contiguous()))
+
+
+def add_rms_norm_linear_fp8(res: torch.Tensor, h: Optional[torch.Tensor], norm_weight: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5,
+                            h_scale: float = 1.0, stream_dtype: Optional[torch.dtype] = None, bias: Optional[torch.Tensor] = None):
+    """``x = res + h_scale · h``, ``y = Q(rmsnorm(x) · norm_weight) · Q(weight)ᵀ (+ bias)`` → (x, y in bf16), with gradients of all inputs."""
+    stream_dtype = _stream(res, stream_dtype)
+    _check_norm("add_rms_norm_linear_fp8", res, h, norm_weight, stream_dtype)
+    _check_layer("add_rms_norm_linear_fp8", res.shape[-1], weight, bias)
+    return backend.apply(_AddNormLinearFP8Fn, res, h, norm_weight, weight, bias, eps, h_scale, stream_dtype)
