@@ -173,11 +173,20 @@ int make_tmap_2d_u8(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t 
 // (or groups of 128 rows: *_tile) and between blocks of 128 along K.  out [M, N] fp32 (accumulate: added to) or bf16; bias [N] or null.
 extern "C" int b200_gemm_fp8_block(const void* A, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_blk, int sa_tile, const void* B,
                                    int64_t ldb, const float* sb, int64_t sb_row, int64_t sb_blk, int sb_tile, const void* bias, int bias_dtype,
-                                   void* out, int64_t ldc, int M, int N, int K, int out_f32, int accumulate, int num_sms, int* status,
+                                   void* out, int64_t ldc, int M, int N, int K, int out_f32, int accumulate, int pair, int num_sms, int* status,
                                    cudaStream_t stream) {
   using namespace b200;
   if (M < 0 || N < 0 || K < 1 || lda % 16 || ldb % 16 || (accumulate && !out_f32)) return -6;
   if (M == 0 || N == 0) return 0;
+  if (pair) {
+    const auto rows = [](const float* s, int64_t row, int64_t blk) { return row == 1 && blk % 4 == 0 && reinterpret_cast<uintptr_t>(s) % 16 == 0; };
+    if (sa_tile || !rows(sa, sa_row, sa_blk) || (!sb_tile && !rows(sb, sb_row, sb_blk))) return -6;
+    const int64_t m = (M + 255) / 256, pairs = num_sms / 2;
+    // tiles of half the width take 0.55 of the time (a little more than half): narrower where that saves enough of the last wave
+    const int64_t wide = (m * ((N + 255) / 256) + pairs - 1) / pairs * 100, narrow = (m * ((N + 127) / 128) + pairs - 1) / pairs * 55;
+    return b200_gemm2_fp8_block(A, lda, sa, sa_blk, B, ldb, sb, sb_row, sb_blk, sb_tile, bias, bias_dtype == 0 ? 1 : 0, out, ldc, M, N, K, out_f32,
+                                accumulate, narrow < wide ? 128 : 256, num_sms, status, stream);
+  }
   CUtensorMap ta, tb;
   int rc = make_tmap_2d_u8(&ta, A, K, M, lda, FB_BK, FB_BM);
   if (rc) return rc;
