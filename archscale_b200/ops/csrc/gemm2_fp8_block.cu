@@ -3,61 +3,105 @@
 //
 // Two CTAs share a 256 × NT tile; each stages its 128 rows of A and half of the rows of B.  A block of 128 along K is one accumulation
 // of four MMAs into one of two accumulators in tensor memory (2 × NT columns), while eight warps read the other one and add it, scaled, to
-// fp32 sums in registers: thread = row, NT / 2 columns.  Scales travel in a ring of their own, deeper than that of the operands, since
-// they are needed up to two blocks after the operands' stage is free.
+// fp32 sums in registers: thread = row, NT / 2 columns.
 //
-// 320 threads: warp 0 TMA, warp 1 MMA (leader CTA), warps 2..9 sums (two warps per lane quarter, one per half of the columns).
+// What bounds it is that read-out: per block a warp has to see the products done, bring 128 columns to registers and spend 128
+// multiply-adds on them (two warps share a scheduler: 256 cycles of the 512 that the products take), and everything that stands beside these
+// in its one chain of instructions adds to the block's time.  Hence: the row's scales of eight blocks are loaded together (the wait for them is
+// paid once in eight; fetched block by block through a TMA ring, as the operands are, they cost 150 cycles a block), scales of 128 rows of B
+// are folded into them there, and only scales per row of B go through shared memory (copied asynchronously, each warp its own columns).
+// Loads, products and their commits are issued by one elected lane of a converged warp: four loads a block from a branch of one lane
+// took longer than the block's products.  Two half-width streams with an MMA warp each read operands twice and were slower.
+//
+// 384 threads: warp 0 TMA, warp 1 MMA (leader CTA), warps 4..11 sums (two warps per lane quarter, one per half of the columns).  A sums
+// thread holds 128 sums and 64 values on their way from tensor memory: the first warpgroup gives it registers (56 + 224 + 224 = 3 · 168).
+// Tiles leave by TMA from shared memory, a piece of 32 rows × 128 bytes per warp at a time, under the next tile's first blocks; an output
+// that TMA cannot write (rows not a multiple of 16 bytes) is stored from the same pieces, a row at a time.
 #include "api.h"
 #include "sm100.cuh"
 
 namespace b200 {
 
-constexpr int F2_BK = 128, F2_THREADS = 320, F2_GROUP_M = 8, F2_SLOTS = 8;
+constexpr int F2_BK = 128, F2_THREADS = 384, F2_GROUP_M = 8;
+constexpr int F2_PIECE = 32 * 128, F2_RING = 4;        // bytes of a piece of the tile; blocks of B's scales on their way
 
 template <int NT, bool BTILE>
 struct F2 {
   static constexpr int A_BYTES = 128 * F2_BK, B_BYTES = NT / 2 * F2_BK, STAGE = A_BYTES + B_BYTES;
-  static constexpr int SLOT = 512 + (BTILE ? 0 : NT * 4);                       // scales of A, then of B
-  static constexpr int STAGES = NT == 256 ? 6 : 8;
-  static constexpr int SMEM = STAGES * STAGE + F2_SLOTS * SLOT + 1024 + 512;
+  static constexpr int STAGES = NT == 256 ? 5 : 7;
+  static constexpr int SV = BTILE ? 0 : F2_RING * NT / 2 * 4;      // bytes of B's scales per warp
+  static constexpr int SMEM = STAGES * STAGE + 8 * (F2_PIECE + SV) + 1024 + 256;
 };
 
 struct F2Params {
   void* out;
   const void* bias;
-  const float* sb;                 // BTILE: scales of 128 rows of B
-  int64_t sb_row, sb_blk, ldc;
+  const float *sa, *sb;
+  int64_t ldc, sa_blk, sb_row, sb_blk;
   int M, N, K;
-  int out_f32, accumulate, bias_f32;
+  int out_f32, accumulate, bias_f32, tma_out;
   int* status;
 };
 
 __device__ __forceinline__ void f2_mma(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-  if (elect_one_sync())
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
-        "}\n" ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
-        : "memory");
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// tcgen05.wait::ld that the registers of the load pass through, so that nothing which uses them can be placed before it.
+__device__ __forceinline__ void f2_ld_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                 "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                 "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ void f2_cp_async16(uint32_t dst, const float* src, int bytes) {      // what is past `bytes` is zero
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void f2_tma_add_2d(const CUtensorMap* map, const void* smem_src, int x, int y) {
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(smem_src)), "r"(x), "r"(y) : "memory");
+}
+// A piece of 32 × 32 fp32 values to an output that TMA cannot write: lane = column, one row after the other.
+__device__ __forceinline__ void f2_store_piece(const uint8_t* piece, const F2Params& p, int row0, int col0, int lane) {
+  const int rows = min(p.M - row0, 32), col = col0 + lane;
+  if (col >= p.N) return;
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r) {
+    const float v = *reinterpret_cast<const float*>(piece + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + ((lane & 3) << 2));
+    const int64_t at = static_cast<int64_t>(row0 + r) * p.ldc + col;
+    if (p.out_f32) {
+      float* o = static_cast<float*>(p.out) + at;
+      *o = p.accumulate ? *o + v : v;
+    } else {
+      static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16(v);
+    }
+  }
 }
 
 template <int NT, bool BTILE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F2_THREADS, 1)
 gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                       const __grid_constant__ CUtensorMap tmap_sa, const __grid_constant__ CUtensorMap tmap_sb, const F2Params p) {
+                       const __grid_constant__ CUtensorMap tmap_out, const F2Params p) {
   using T = F2<NT, BTILE>;
   constexpr int W = NT / 2;                            // columns per thread
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* slots = smem + T::STAGES * T::STAGE;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(slots + F2_SLOTS * T::SLOT);
+  uint8_t* pieces = smem + T::STAGES * T::STAGE;
+  uint8_t* svs = pieces + 8 * F2_PIECE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(svs + 8 * T::SV);
   uint64_t* full_bar = bars;                           // [STAGES] used in the leader CTA
   uint64_t* empty_bar = full_bar + T::STAGES;          // [STAGES] each CTA's producer waits on its own
-  uint64_t* sfull_bar = empty_bar + T::STAGES;         // [SLOTS]  scales, per CTA
-  uint64_t* sempty_bar = sfull_bar + F2_SLOTS;         // [SLOTS]  eight warps
-  uint64_t* tmem_full = sempty_bar + F2_SLOTS;         // [2]      each CTA's sums wait on their own
+  uint64_t* tmem_full = empty_bar + T::STAGES;         // [2]      each CTA's sums wait on their own
   uint64_t* tmem_empty = tmem_full + 2;                // [2]      used in the leader CTA, 16 warps
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(tmem_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
@@ -71,12 +115,11 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < T::STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-    for (int s = 0; s < F2_SLOTS; ++s) { mbar_init(&sfull_bar[s], 1); mbar_init(&sempty_bar[s], 8); }
     for (int a = 0; a < 2; ++a) { mbar_init(&tmem_full[a], 1); mbar_init(&tmem_empty[a], 16); }
     *abort_flag = 0;
     mbar_fence_init();
-    tma_prefetch_desc(&tmap_a); tma_prefetch_desc(&tmap_b); tma_prefetch_desc(&tmap_sa);
-    if (!BTILE) tma_prefetch_desc(&tmap_sb);
+    tma_prefetch_desc(&tmap_a); tma_prefetch_desc(&tmap_b);
+    if (p.tma_out) tma_prefetch_desc(&tmap_out);
   }
   if (warp == 1) { tmem_alloc_2sm(tmem_ptr, 2 * NT); tmem_relinquish_2sm(); }
   tc_fence_before();
@@ -94,29 +137,26 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     n0 = (r / gsz) * NT;
   };
 
-  if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0, slot = 0; uint32_t phase = 0, sphase = 0;
-      for (int t = pair; t < num_tiles; t += n_pair) {
-        int m0, n0; tile_coords(t, m0, n0);
-        const int ma = m0 + rank * 128, nb = n0 + rank * (NT / 2);
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, STATUS_TIMEOUT_EMPTY)) goto done;
-          uint8_t* sa = smem + stage * T::STAGE;
+  if (warp == 0) {                                     // converged: a load from inside a branch of one lane takes longer to issue
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    int stage = 0; uint32_t phase = 0;
+    for (int t = pair; t < num_tiles; t += n_pair) {
+      int m0, n0; tile_coords(t, m0, n0);
+      const int ma = m0 + rank * 128, nb = n0 + rank * (NT / 2);
+      for (int kb = 0; kb < num_kb; ++kb) {
+        if (!mbar_wait_warp(&empty_bar[stage], phase ^ 1, abort_flag, p.status, STATUS_TIMEOUT_EMPTY)) goto done;
+        uint8_t* sa = smem + stage * T::STAGE;
+        if (elect_one_sync()) {
           if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * T::STAGE);       // both CTAs' loads
           tma_load_2d_2sm(sa, &tmap_a, &full_bar[stage], kb * F2_BK, ma);
           tma_load_2d_2sm(sa + T::A_BYTES, &tmap_b, &full_bar[stage], kb * F2_BK, nb);
-          if (!mbar_wait(&sempty_bar[slot], sphase ^ 1, abort_flag, p.status, STATUS_TIMEOUT_EMPTY)) goto done;
-          mbar_arrive_expect_tx(&sfull_bar[slot], T::SLOT);
-          tma_load_2d(slots + slot * T::SLOT, &tmap_sa, &sfull_bar[slot], ma, kb);
-          if (!BTILE) tma_load_2d(slots + slot * T::SLOT + 512, &tmap_sb, &sfull_bar[slot], n0, kb);
-          if (++stage == T::STAGES) { stage = 0; phase ^= 1; }
-          if (++slot == F2_SLOTS) { slot = 0; sphase ^= 1; }
         }
+        if (++stage == T::STAGES) { stage = 0; phase ^= 1; }
       }
     }
   } else if (warp == 1) {
-    if (rank == 0) {                                   // the whole warp, converged: one lane is elected per instruction
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (rank == 0) {                                   // the whole warp, converged; one lane is elected per block
       // e4m3 × e4m3, fp32 accumulate, both operands K-major
       constexpr uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(NT >> 3) << 17) | (static_cast<uint32_t>(256 >> 4) << 24);
       int stage = 0; uint32_t phase = 0, it = 0;
@@ -128,106 +168,147 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + stage * T::STAGE);
           const uint64_t da = make_smem_desc(sa, 16, 1024), db = make_smem_desc(sa + T::A_BYTES, 16, 1024);
+          if (elect_one_sync()) {
 #pragma unroll
-          for (uint32_t k = 0; k < F2_BK / 32; ++k)
-            f2_mma(tmem_base + acc * NT, da + static_cast<uint64_t>(k * 2), db + static_cast<uint64_t>(k * 2), idesc, k != 0 ? 1u : 0u);
-          if (elect_one_sync()) { umma_commit_2sm(&empty_bar[stage], 3); umma_commit_2sm(&tmem_full[acc], 3); }
+            for (uint32_t k = 0; k < F2_BK / 32; ++k)
+              f2_mma(tmem_base + acc * NT, da + static_cast<uint64_t>(k * 2), db + static_cast<uint64_t>(k * 2), idesc, k != 0 ? 1u : 0u);
+            umma_commit_2sm(&tmem_full[acc], 3);
+            umma_commit_2sm(&empty_bar[stage], 3);
+          }
           if (++stage == T::STAGES) { stage = 0; phase ^= 1; }
         }
       }
     }
+  } else if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");      // every warp of the group has to give its registers back
   } else {
-    const int q = warp & 3, half = (warp - 2) >> 2;    // lane quarter, half of the columns
-    const int esz = p.out_f32 ? 4 : 2;
-    const bool wide = p.ldc * esz % 32 == 0 && reinterpret_cast<uintptr_t>(p.out) % 32 == 0;      // whole sectors per lane
-    int slot = 0; uint32_t sphase = 0, it = 0;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const int q = warp & 3, half = (warp - 4) >> 2;    // lane quarter, half of the columns
+    uint8_t* piece = pieces + (warp - 4) * F2_PIECE;
+    uint8_t* sv = svs + (warp - 4) * T::SV;
+    uint32_t it = 0;
     for (int t = pair; t < num_tiles; t += n_pair) {
       int m0, n0; tile_coords(t, m0, n0);
-      const int row = m0 + rank * 128 + q * 32 + lane, c0 = n0 + half * W;
-      const float* sb = BTILE ? p.sb + static_cast<int64_t>(min(c0, p.N - 1) >> 7) * p.sb_row : nullptr;
-      float fb = BTILE ? sb[0] : 0.f;
-      float2 sum[W / 2];
+      const int row0 = m0 + rank * 128 + q * 32, c0 = n0 + half * W;
+      const float* sa = p.sa + min(row0 + lane, p.M - 1);
+      const float* sb = BTILE ? p.sb + static_cast<int64_t>(min(c0, p.N - 1) >> 7) * p.sb_row : p.sb + min(c0 + 4 * lane, (p.N - 1) & ~3);
+      // scales of B's rows: each lane copies four columns of a block
+      const int sv_bytes = BTILE || lane >= W / 4 ? 0 : max(min(p.N - c0 - 4 * lane, 4), 0) * 4;
+      auto copy_sv = [&](int kb) {
+        if (!BTILE) {
+          if (lane < W / 4)
+            f2_cp_async16(smem_u32(sv + (kb % F2_RING) * (W * 4) + lane * 16), sb + min(kb, num_kb - 1) * p.sb_blk, kb < num_kb ? sv_bytes : 0);
+          asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+      };
+      float sum[W], scale[8];
 #pragma unroll
-      for (int i = 0; i < W / 2; ++i) sum[i] = make_float2(0.f, 0.f);
+      for (int i = 0; i < W; ++i) sum[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < F2_RING - 1; ++j) copy_sv(j);
       for (int kb = 0; kb < num_kb; ++kb, ++it) {
         const int acc = it & 1; const uint32_t acc_phase = (it >> 1) & 1;
         const uint32_t taddr = tmem_base + acc * NT + half * W + (static_cast<uint32_t>(q * 32) << 16);
-        if (!mbar_wait_warp(&sfull_bar[slot], sphase, abort_flag, p.status, STATUS_TIMEOUT_FULL)) goto done;
-        const float* ss = reinterpret_cast<const float*>(slots + slot * T::SLOT);
-        float fa = ss[q * 32 + lane];
-        const float2* sv = reinterpret_cast<const float2*>(ss + 128 + half * W);
-        if (BTILE) {
-          fa *= fb;
-          if (kb + 1 < num_kb) fb = sb[(kb + 1) * p.sb_blk];
+        if ((kb & 7) == 0) {                           // the row's scales of eight blocks
+#pragma unroll
+          for (int j = 0; j < 8; ++j) scale[j] = sa[min(kb + j, num_kb - 1) * p.sa_blk];
+          if (BTILE) {
+            const float b = sb[min(kb + (lane & 7), num_kb - 1) * p.sb_blk];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) scale[j] *= __shfl_sync(0xffffffffu, b, j);
+          }
         }
-        const float2 fa2 = make_float2(fa, fa);
+        const float s01 = (kb & 1) ? scale[1] : scale[0], s23 = (kb & 1) ? scale[3] : scale[2];
+        const float s45 = (kb & 1) ? scale[5] : scale[4], s67 = (kb & 1) ? scale[7] : scale[6];
+        const float f = (kb & 4) ? ((kb & 2) ? s67 : s45) : ((kb & 2) ? s23 : s01);
         if (!mbar_wait_warp(&tmem_full[acc], acc_phase, abort_flag, p.status, STATUS_TIMEOUT_TMEM_FULL)) goto done;
         tc_fence_after();
-        uint32_t r[2][16];
-        tmem_ld_32x16(taddr, r[0]);
-        tmem_ld_wait();
+        uint32_t r[2][32];
+        tmem_ld_32x32(taddr, r[0]);
+        if (!BTILE) {                                  // block kb has arrived; its slot's predecessor was read by every lane
+          copy_sv(kb + F2_RING - 1);
+          asm volatile("cp.async.wait_group %0;" ::"n"(F2_RING - 1) : "memory");
+          __syncwarp();
+        }
+        const float4* bv = reinterpret_cast<const float4*>(sv + (kb % F2_RING) * (W * 4));
 #pragma unroll
-        for (int c = 0; c < W / 16; ++c) {
-          if (c + 1 < W / 16) tmem_ld_32x16(taddr + (c + 1) * 16, r[(c + 1) & 1]);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float2 v = make_float2(__uint_as_float(r[c & 1][2 * i]), __uint_as_float(r[c & 1][2 * i + 1]));
-            if (!BTILE) v = mul_f32x2(v, sv[c * 8 + i]);
-            sum[c * 8 + i] = fma_f32x2(v, fa2, sum[c * 8 + i]);
-          }
-          if (c + 1 < W / 16) tmem_ld_wait();
-          if (c + 2 == W / 16) {                       // the last columns are in registers: the accumulator is free
+        for (int c = 0; c < W / 32; ++c) {
+          f2_ld_wait(r[c & 1]);
+          if (c + 1 < W / 32) {
+            tmem_ld_32x32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
+          } else {                                     // the last columns are in registers: the accumulator is free
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_leader(&tmem_empty[acc]);
           }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sempty_bar[slot]);
-        if (++slot == F2_SLOTS) { slot = 0; sphase ^= 1; }
-      }
-      if (row < p.M) {
+          const uint32_t (&w)[32] = r[c & 1];
+          float* o = sum + c * 32;
+          if (BTILE) {
 #pragma unroll
-        for (int c = 0; c < W / 16; ++c) {
-          const int col = c0 + c * 16;
-          float v[16];
+            for (int i = 0; i < 32; ++i) o[i] = fmaf(__uint_as_float(w[i]), f, o[i]);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) { v[2 * i] = sum[c * 8 + i].x; v[2 * i + 1] = sum[c * 8 + i].y; }
-          if (p.bias) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (col + i < p.N)
-                v[i] += p.bias_f32 ? static_cast<const float*>(p.bias)[col + i] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col + i]);
+            for (int i = 0; i < 32; i += 4) {
+              const float4 b = bv[c * 8 + i / 4];
+              const float2 f2 = make_float2(f, f);
+              const float2 x = fma_f32x2(mul_f32x2(make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1])), make_float2(b.x, b.y)), f2,
+                                         make_float2(o[i], o[i + 1]));
+              const float2 y = fma_f32x2(mul_f32x2(make_float2(__uint_as_float(w[i + 2]), __uint_as_float(w[i + 3])), make_float2(b.z, b.w)), f2,
+                                         make_float2(o[i + 2], o[i + 3]));
+              o[i] = x.x; o[i + 1] = x.y; o[i + 2] = y.x; o[i + 3] = y.y;
+            }
           }
-          const int64_t at = static_cast<int64_t>(row) * p.ldc + col;
-          if (p.out_f32) {
-            float* o = static_cast<float*>(p.out) + at;
-            if (wide && col + 16 <= p.N) {
+        }
+        if (!BTILE) __syncwarp();                      // every lane has read its slot
+      }
+      if (!BTILE) asm volatile("cp.async.wait_group 0;" ::: "memory");      // copies past the last block (of zeros)
+      if (p.bias) {
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                uint32_t w[8];
-                if (p.accumulate) load_32b(o + 8 * j, w);
+        for (int c = 0; c < W / 32; ++c) {
+          const int col = min(c0 + c * 32 + lane, p.N - 1);
+          const float b = p.bias_f32 ? static_cast<const float*>(p.bias)[col] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(p.accumulate ? __uint_as_float(w[e]) + v[8 * j + e] : v[8 * j + e]);
-                store_32b(o + 8 * j, w);
-              }
-            } else {
+          for (int i = 0; i < 32; ++i) sum[c * 32 + i] += __shfl_sync(0xffffffffu, b, i);
+        }
+      }
+      // pieces of 32 rows × 128 bytes: 16-byte parts at part ^ (row % 8), the order of the output's tensor map
+      auto part = [&](int j) { return reinterpret_cast<uint4*>(piece + lane * 128 + ((j ^ (lane & 7)) << 4)); };
+      if (p.tma_out && !p.out_f32) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (col + i < p.N) o[i] = p.accumulate ? o[i] + v[i] : v[i];
+        for (int c = 0; c < W / 64; ++c) {
+          if (lane == 0) tma_store_wait_read<0>();
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float* v = sum + c * 64 + j * 8;
+            *part(j) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && row0 < p.M && c0 + c * 64 < p.N) { tma_store_2d(&tmap_out, piece, c0 + c * 64, row0); tma_store_commit(); }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < W / 32; ++c) {
+          if (lane == 0) tma_store_wait_read<0>();
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float* v = sum + c * 32 + j * 4;
+            *part(j) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+          }
+          if (p.tma_out) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && row0 < p.M && c0 + c * 32 < p.N) {
+              if (p.accumulate) f2_tma_add_2d(&tmap_out, piece, c0 + c * 32, row0);
+              else tma_store_2d(&tmap_out, piece, c0 + c * 32, row0);
+              tma_store_commit();
             }
           } else {
-            __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + at;
-            if (wide && col + 16 <= p.N) {
-              uint32_t w[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
-              store_32b(o, w);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (col + i < p.N) o[i] = __float2bfloat16(v[i]);
-            }
+            __syncwarp();
+            f2_store_piece(piece, p, row0, c0 + c * 32, lane);
+            __syncwarp();
           }
         }
       }
@@ -235,6 +316,10 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
   }
 
 done:
+  if (warp >= 4) {
+    tmem_ld_wait();                    // a wait that gave up can leave a load on its way
+    tma_store_wait<0>();
+  }
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();
@@ -248,8 +333,8 @@ done:
 int make_tmap_2d_u8(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
                     uint32_t box_inner, uint32_t box_outer);
 
-// Scales [blocks][ld] of `rows` rows, boxes of `box` rows of one block (rows past the end read as zeros).
-static int make_tmap_scales(CUtensorMap* map, const float* ptr, uint64_t rows, uint64_t blocks, uint64_t ld, uint32_t box) {
+// The output in boxes of 32 rows × 128 bytes, 16-byte parts swizzled by the row.
+static int make_tmap_out(CUtensorMap* map, void* ptr, int f32, uint64_t cols, uint64_t rows, uint64_t ld) {
   typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
   static Encode fn = nullptr;
@@ -259,46 +344,41 @@ static int make_tmap_scales(CUtensorMap* map, const float* ptr, uint64_t rows, u
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &res) != cudaSuccess || res != cudaDriverEntryPointSuccess) return -1;
     fn = reinterpret_cast<Encode>(f);
   }
-  const cuuint64_t dim[2] = {rows, blocks}, stride[1] = {ld * 4};
-  const cuuint32_t boxes[2] = {box, 1}, step[2] = {1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<float*>(ptr), dim, stride, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint64_t dim[2] = {cols, rows}, stride[1] = {ld * (f32 ? 4 : 2)};
+  const cuuint32_t box[2] = {f32 ? 32u : 64u, 32}, step[2] = {1, 1};
+  const CUresult r = fn(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, dim, stride, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : static_cast<int>(r);
 }
 
 template <int NT, bool BTILE>
-static int launch_f2(const void* A, int64_t lda, const float* sa, int64_t sa_blk, const void* B, int64_t ldb, const float* sb, const F2Params& p,
-                     int num_sms, cudaStream_t st) {
+static int launch_f2(const void* A, int64_t lda, const void* B, int64_t ldb, const F2Params& p, int num_sms, cudaStream_t st) {
   using T = F2<NT, BTILE>;
-  CUtensorMap ta, tb, tsa, tsb;
-  const uint64_t blocks = (p.K + F2_BK - 1) / F2_BK;
+  CUtensorMap ta, tb, to;
   int rc = make_tmap_2d_u8(&ta, A, p.K, p.M, lda, F2_BK, 128);
   if (!rc) rc = make_tmap_2d_u8(&tb, B, p.K, p.N, ldb, F2_BK, NT / 2);
-  if (!rc) rc = make_tmap_scales(&tsa, sa, p.M, blocks, sa_blk, 128);
-  tsb = tsa;
-  if (!rc && !BTILE) rc = make_tmap_scales(&tsb, sb, p.N, blocks, p.sb_blk, NT);
+  to = tb;
+  if (!rc && p.tma_out) rc = make_tmap_out(&to, p.out, p.out_f32, p.N, p.M, p.ldc);
   if (rc) return rc;
   auto kern = gemm2_fp8_block_kernel<NT, BTILE>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM) != cudaSuccess) return -2;
   const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + NT - 1) / NT);
   if (tiles > 0x3fffffff) return -6;
   const int pairs = num_sms / 2;
-  kern<<<2 * (tiles < pairs ? static_cast<int>(tiles) : pairs), F2_THREADS, T::SMEM, st>>>(ta, tb, tsa, tsb, p);
+  kern<<<2 * (tiles < pairs ? static_cast<int>(tiles) : pairs), F2_THREADS, T::SMEM, st>>>(ta, tb, to, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
 }  // namespace b200
 
-// Contract of b200_gemm_fp8_block, which checks the arguments and calls this: scales of A are per row, stored [block][sa_blk], those
-// of B too unless sb_tile; addresses of such scales and their strides are multiples of 16 bytes.
+// Contract of b200_gemm_fp8_block, which checks the arguments and calls this: scales of A are per row, those of B per row or (sb_tile) per 128
+// rows; scales per row are stored [block][*_blk], those of B 16-byte aligned.
 extern "C" int b200_gemm2_fp8_block(const void* A, int64_t lda, const float* sa, int64_t sa_blk, const void* B, int64_t ldb, const float* sb,
                                     int64_t sb_row, int64_t sb_blk, int sb_tile, const void* bias, int bias_f32, void* out, int64_t ldc, int M,
                                     int N, int K, int out_f32, int accumulate, int nt, int num_sms, int* status, cudaStream_t stream) {
   using namespace b200;
-  const F2Params p{out, bias, sb, sb_row, sb_blk, ldc, M, N, K, out_f32, accumulate, bias_f32, status};
-  if (nt == 256)
-    return sb_tile ? launch_f2<256, true>(A, lda, sa, sa_blk, B, ldb, sb, p, num_sms, stream)
-                   : launch_f2<256, false>(A, lda, sa, sa_blk, B, ldb, sb, p, num_sms, stream);
-  return sb_tile ? launch_f2<128, true>(A, lda, sa, sa_blk, B, ldb, sb, p, num_sms, stream)
-                 : launch_f2<128, false>(A, lda, sa, sa_blk, B, ldb, sb, p, num_sms, stream);
+  const int tma_out = ldc * (out_f32 ? 4 : 2) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 ? 1 : 0;
+  const F2Params p{out, bias, sa, sb, ldc, sa_blk, sb_row, sb_blk, M, N, K, out_f32, accumulate, bias_f32, tma_out, status};
+  if (nt == 256) return sb_tile ? launch_f2<256, true>(A, lda, B, ldb, p, num_sms, stream) : launch_f2<256, false>(A, lda, B, ldb, p, num_sms, stream);
+  return sb_tile ? launch_f2<128, true>(A, lda, B, ldb, p, num_sms, stream) : launch_f2<128, false>(A, lda, B, ldb, p, num_sms, stream);
 }
