@@ -27,26 +27,50 @@ __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float
   return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
 }
 
-// Eight neighbouring values, the first n of them inside the row (the others read as zero).  vec: whole 16-byte loads are aligned.
-__device__ __forceinline__ void load8(const float* p, int n, bool vec, float (&v)[8]) {
-  if (vec && n >= 8) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+// Eight neighbouring values of a row, the first n of them inside it (the others are zero).
+template <typename T> struct Raw8;
+template <> struct Raw8<float> { float4 a, b; };
+template <> struct Raw8<__nv_bfloat16> { uint4 a; };
+// VEC: rows are whole 16-byte pieces, so that n is 8 or not positive: one or two predicated loads, which the compiler issues together
+// (with a branch per vector for the general case in between, a tile of bf16 took 3.5 times as long).
+template <bool VEC>
+__device__ __forceinline__ void load_raw(const float* p, int n, Raw8<float>& r) {
+  if (VEC) {
+    r.a = r.b = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (n > 0) { r.a = *reinterpret_cast<const float4*>(p); r.b = *reinterpret_cast<const float4*>(p + 4); }
   } else {
+    float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.f;
+    r.a = make_float4(v[0], v[1], v[2], v[3]);
+    r.b = make_float4(v[4], v[5], v[6], v[7]);
   }
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, int n, bool vec, float (&v)[8]) {
-  if (vec && n >= 8) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { const float2 f = unpack_bf16x2(w[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
+template <bool VEC>
+__device__ __forceinline__ void load_raw(const __nv_bfloat16* p, int n, Raw8<__nv_bfloat16>& r) {
+  if (VEC) {
+    r.a = make_uint4(0u, 0u, 0u, 0u);
+    if (n > 0) r.a = *reinterpret_cast<const uint4*>(p);
   } else {
+    uint32_t v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? __bfloat162float(p[i]) : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[i]) : 0u;
+    r.a = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
   }
+}
+__device__ __forceinline__ void unpack8(const Raw8<float>& r, float (&v)[8]) {
+  v[0] = r.a.x; v[1] = r.a.y; v[2] = r.a.z; v[3] = r.a.w; v[4] = r.b.x; v[5] = r.b.y; v[6] = r.b.z; v[7] = r.b.w;
+}
+__device__ __forceinline__ void unpack8(const Raw8<__nv_bfloat16>& r, float (&v)[8]) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+template <bool VEC, typename T>
+__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
+  Raw8<T> r;
+  load_raw<VEC>(p, n, r);
+  unpack8(r, v);
 }
 
 struct Fp8TileParams {
@@ -67,9 +91,10 @@ enum : int { FP8_ROWS = 1, FP8_COLS = 2, FP8_TILE = 4 };
 // One CTA per 128 × 128 tile, read once.  A thread holds 8 rows × 8 columns; magnitudes meet in shared memory, where one thread per
 // row and per column makes the two factors (and writes the scale: 512 contiguous bytes per tile).  The transposed elements turn in
 // shared memory: 16-byte pieces (rows of one column) at slot (piece ^ column / 8), two passes per access, no more conflicts.
-template <typename T, int MODE, bool NORM>
+template <typename T, int MODE, bool NORM, bool VEC>
 __global__ void __launch_bounds__(256) fp8_tile_kernel(const Fp8TileParams p) {
-  __shared__ uint32_t s_row[128], s_col[8][128];
+  __shared__ uint32_t s_row[128];
+  __shared__ __align__(16) uint32_t s_col[8][128];
   __shared__ __align__(16) uint8_t s_t[(MODE & FP8_COLS) || MODE == FP8_TILE ? 128 * 128 : 16];
   const int t = threadIdx.x, warp = t >> 5, cg = t & 15, rg = t >> 4;      // column group, row group (8 each)
   const int rb = blockIdx.x / p.cb, kb = blockIdx.x - rb * p.cb;
@@ -77,12 +102,17 @@ __global__ void __launch_bounds__(256) fp8_tile_kernel(const Fp8TileParams p) {
   const int nc = min(max(p.cols - c0, 0), 8);
   const T* x = static_cast<const T*>(p.x) + static_cast<int64_t>(r0) * p.ldx + c0;
   float v[8][8];
+  {
+    Raw8<T> raw[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) load8(x + i * p.ldx, r0 + i < p.rows ? nc : 0, p.vec, v[i]);
+    for (int i = 0; i < 8; ++i) load_raw<VEC>(x + i * p.ldx, r0 + i < p.rows ? nc : 0, raw[i]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) unpack8(raw[i], v[i]);
+  }
   if (NORM) {
     float w[8];
-    if (p.w_f32) load8(static_cast<const float*>(p.w) + c0, nc, false, w);
-    else load8(static_cast<const __nv_bfloat16*>(p.w) + c0, nc, false, w);
+    if (p.w_f32) load8<false>(static_cast<const float*>(p.w) + c0, nc, w);
+    else load8<false>(static_cast<const __nv_bfloat16*>(p.w) + c0, nc, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float rs = r0 + i < p.rows ? p.rstd[r0 + i] : 0.f;
@@ -109,25 +139,41 @@ __global__ void __launch_bounds__(256) fp8_tile_kernel(const Fp8TileParams p) {
       for (int e = 0; e < 8; ++e) v[i][e] = __fmul_rn(v[i][e], u);
   } else {
     if (MODE & FP8_ROWS) {
-      const uint32_t half = 0xffffu << (t & 16);
+      // eight rows over 16 lanes: at every step a lane hands half of its rows to a neighbour and keeps the other half
+      uint32_t m[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        uint32_t m = 0;
+        m[i] = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m = max(m, abs_bits(v[i][e]));
-        m = __reduce_max_sync(half, m);
-        if (cg == 0) s_row[rg * 8 + i] = m;
+        for (int e = 0; e < 8; ++e) m[i] = max(m[i], abs_bits(v[i][e]));
       }
+#pragma unroll
+      for (int h = 4; h > 0; h >>= 1) {
+        const bool up = (t & (2 * h)) != 0;
+#pragma unroll
+        for (int i = 0; i < h; ++i) {
+          const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? m[i] : m[i + h], 2 * h);
+          m[i] = max(up ? m[i + h] : m[i], got);
+        }
+      }
+      m[0] = max(m[0], __shfl_xor_sync(0xffffffffu, m[0], 1));
+      if ((t & 1) == 0) s_row[rg * 8 + (cg >> 1)] = m[0];
     }
-    if (MODE & FP8_COLS) {
+    if (MODE & FP8_COLS) {                               // two row groups of a warp meet: a lane keeps four of its columns
+      uint32_t m[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        uint32_t m = 0;
+        m[e] = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i][e]));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        if ((t & 16) == 0) s_col[warp][cg * 8 + e] = m;
+        for (int i = 0; i < 8; ++i) m[e] = max(m[e], abs_bits(v[i][e]));
       }
+      const bool up = (t & 16) != 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? m[e] : m[e + 4], 16);
+        m[e] = max(up ? m[e + 4] : m[e], got);
+      }
+      *reinterpret_cast<uint4*>(&s_col[warp][cg * 8 + (up ? 4 : 0)]) = make_uint4(m[0], m[1], m[2], m[3]);
     }
     __syncthreads();
     if ((MODE & FP8_ROWS) && t < 128) {
@@ -185,7 +231,8 @@ template <typename T, int MODE, bool NORM>
 static int launch_tile(const Fp8TileParams& p, cudaStream_t st) {
   const int64_t tiles = static_cast<int64_t>((p.rows + 127) / 128) * p.cb;
   if (tiles > 0x7fffffff) return -6;
-  fp8_tile_kernel<T, MODE, NORM><<<static_cast<unsigned>(tiles), 256, 0, st>>>(p);
+  if (p.vec) fp8_tile_kernel<T, MODE, NORM, true><<<static_cast<unsigned>(tiles), 256, 0, st>>>(p);
+  else fp8_tile_kernel<T, MODE, NORM, false><<<static_cast<unsigned>(tiles), 256, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
@@ -195,7 +242,7 @@ static int launch_tile(const Fp8TileParams& p, cudaStream_t st) {
 struct Fp8NormParams {
   const void* res; const __nv_bfloat16* h; const void* w;
   float h_scale, eps;
-  int rows, cols, vec, w_vec;
+  int rows, cols, vec, w_f32;
   void* x;                      // new stream (null without h)
   uint8_t* q; int64_t ldq;
   float* s; int64_t lds;
@@ -223,7 +270,7 @@ __device__ __forceinline__ float round_to(float v, const float*) { return v; }
 __device__ __forceinline__ float round_to(float v, const __nv_bfloat16*) { return __bfloat162float(__float2bfloat16(v)); }
 
 // TPR threads per row, V vectors of 8 per thread: the row stays in registers.  16 neighbouring threads hold one block of 128.
-template <typename T, typename TO, int TPR, int V>
+template <typename T, typename TO, int TPR, int V, bool VEC>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) fp8_norm_kernel(const Fp8NormParams p) {
   constexpr int CTA = TPR < 128 ? 128 : TPR, RPC = CTA / TPR, WPR = TPR / 32;
   __shared__ float s_sum[CTA / 32];
@@ -237,13 +284,13 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) fp8_norm_kernel(const F
   for (int i = 0; i < V; ++i) {
     const int c = (t + i * TPR) * 8;
     const int n = live ? min(max(p.cols - c, 0), 8) : 0;
-    load8(static_cast<const T*>(p.res) + base + c, n, p.vec, v[i]);
+    load8<VEC>(static_cast<const T*>(p.res) + base + c, n, v[i]);
     if (p.h) {
       float h[8];
-      load8(p.h + base + c, n, p.vec, h);
+      load8<VEC>(p.h + base + c, n, h);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] = round_to(__fadd_rn(v[i][e], __fmul_rn(p.h_scale, h[e])), static_cast<const TO*>(nullptr));
-      if (n > 0) store8(static_cast<TO*>(p.x) + base + c, n, p.vec, v[i]);
+      if (n > 0) store8(static_cast<TO*>(p.x) + base + c, n, VEC, v[i]);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss += v[i][e] * v[i][e];
@@ -264,16 +311,16 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) fp8_norm_kernel(const F
     const int c = (t + i * TPR) * 8;
     const int n = live ? min(max(p.cols - c, 0), 8) : 0;
     float w[8];
-    // w may be unaligned when its type differs from the stream's, so it has a rule of its own
-    if (p.w_vec & 2) load8(static_cast<const float*>(p.w) + c, n, p.w_vec & 1, w);
-    else load8(static_cast<const __nv_bfloat16*>(p.w) + c, n, p.w_vec & 1, w);
+    if (p.w_f32) load8<VEC>(static_cast<const float*>(p.w) + c, n, w);
+    else load8<VEC>(static_cast<const __nv_bfloat16*>(p.w) + c, n, w);
     uint32_t m = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       v[i][e] = __fmul_rn(__fmul_rn(v[i][e], rs), w[e]);
       m = max(m, e < n ? abs_bits(v[i][e]) : 0u);
     }
-    m = __reduce_max_sync(0xffffu << (threadIdx.x & 16), m);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (n > 0) {
       const float a = block_amax(m), u = __fdiv_rn(kE4m3Max, a);
       if ((t & 15) == 0) p.s[(c >> 7) * p.lds + row] = __fdiv_rn(a, kE4m3Max);
@@ -291,7 +338,9 @@ static int launch_norm(const Fp8NormParams& p, cudaStream_t st) {
 #define FP8_NORM(TPR, V)                                                                                     \
   if (vecs <= TPR * V) {                                                                                     \
     constexpr int RPC = TPR < 128 ? 128 / TPR : 1;                                                           \
-    fp8_norm_kernel<T, TO, TPR, V><<<(p.rows + RPC - 1) / RPC, TPR < 128 ? 128 : TPR, 0, st>>>(p);           \
+    const int grid = (p.rows + RPC - 1) / RPC, block = TPR < 128 ? 128 : TPR;                                \
+    if (p.vec) fp8_norm_kernel<T, TO, TPR, V, true><<<grid, block, 0, st>>>(p);                              \
+    else fp8_norm_kernel<T, TO, TPR, V, false><<<grid, block, 0, st>>>(p);                                   \
     return cudaGetLastError() == cudaSuccess ? 0 : -3;                                                       \
   }
   FP8_NORM(32, 1)
@@ -317,7 +366,7 @@ extern "C" int b200_fp8_quantize(const void* x, int dtype, int64_t ldx, int rows
   if (rows == 0 || cols == 0) return 0;
   const int esz = dtype == 0 ? 4 : 2;
   Fp8TileParams p{x, ldx, rows, cols, (cols + 127) / 128,
-                  reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * esz % 16 == 0 ? 1 : 0,
+                  cols % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * esz % 16 == 0 ? 1 : 0,
                   static_cast<uint8_t*>(q), ldq, s, lds, static_cast<uint8_t*>(qt), ldqt, st, ldst, rstd, w, w_dtype == 0 ? 1 : 0};
   if (dtype == 0) {
     if (rstd) return launch_tile<float, FP8_COLS, true>(p, stream);
@@ -341,9 +390,9 @@ extern "C" int b200_add_rmsnorm_fp8(const void* res, int res_dtype, const void* 
   if (rows < 0 || cols < 1 || cols > 32768 || (x_dtype == 1 && res_dtype != 1)) return -6;
   if (rows == 0) return 0;
   const auto al = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; };
-  const int vec = cols % 8 == 0 && al(res) && al(h) && al(x) ? 1 : 0;
+  const int vec = cols % 8 == 0 && al(res) && al(h) && al(x) && al(w) ? 1 : 0;
   Fp8NormParams p{res, static_cast<const __nv_bfloat16*>(h), w, h_scale, eps, rows, cols, vec,
-                  (al(w) ? 1 : 0) | (w_dtype == 0 ? 2 : 0), x, static_cast<uint8_t*>(q), ldq, s, lds, rstd};
+                  w_dtype == 0 ? 1 : 0, x, static_cast<uint8_t*>(q), ldq, s, lds, rstd};
   if (res_dtype == 0) return launch_norm<float, float>(p, stream);
   return x_dtype == 0 ? launch_norm<__nv_bfloat16, float>(p, stream) : launch_norm<__nv_bfloat16, __nv_bfloat16>(p, stream);
 }
