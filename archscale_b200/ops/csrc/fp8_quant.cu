@@ -88,65 +88,75 @@ struct Fp8TileParams {
 
 enum : int { FP8_ROWS = 1, FP8_COLS = 2, FP8_TILE = 4 };
 
-// One CTA per 128 × 128 tile, read once.  A thread holds 8 rows × 8 columns; magnitudes meet in shared memory, where one thread per
-// row and per column makes the two factors (and writes the scale: 512 contiguous bytes per tile).  The transposed elements turn in
-// shared memory: 16-byte pieces (rows of one column) at slot (piece ^ column / 8), two passes per access, no more conflicts.
-template <typename T, int MODE, bool NORM, bool VEC>
-__global__ void __launch_bounds__(256) fp8_tile_kernel(const Fp8TileParams p) {
-  __shared__ uint32_t s_row[128];
-  __shared__ __align__(16) uint32_t s_col[8][128];
-  __shared__ __align__(16) uint8_t s_t[(MODE & FP8_COLS) || MODE == FP8_TILE ? 128 * 128 : 16];
+// Largest magnitudes of a thread's 8 × 8 values, as the bits of fp32 numbers: per row, per column, over all.  bf16 is compared two at a
+// time as 16-bit integers (NaN is the largest there too).
+__device__ __forceinline__ void row_max(const Raw8<float> (&r)[8], uint32_t (&m)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float v[8] = {r[i].a.x, r[i].a.y, r[i].a.z, r[i].a.w, r[i].b.x, r[i].b.y, r[i].b.z, r[i].b.w};
+    m[i] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m[i] = max(m[i], abs_bits(v[e]));
+  }
+}
+__device__ __forceinline__ void row_max(const Raw8<__nv_bfloat16> (&r)[8], uint32_t (&m)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t k = 0x7fff7fffu;
+    const uint32_t t = __vmaxu2(__vmaxu2(r[i].a.x & k, r[i].a.y & k), __vmaxu2(r[i].a.z & k, r[i].a.w & k));
+    m[i] = max(t & 0xffff0000u, t << 16);
+  }
+}
+__device__ __forceinline__ void col_max(const Raw8<float> (&r)[8], uint32_t (&m)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m[e] = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float v[8] = {r[i].a.x, r[i].a.y, r[i].a.z, r[i].a.w, r[i].b.x, r[i].b.y, r[i].b.z, r[i].b.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m[e] = max(m[e], abs_bits(v[e]));
+  }
+}
+__device__ __forceinline__ void col_max(const Raw8<__nv_bfloat16> (&r)[8], uint32_t (&m)[8]) {
+  uint32_t t[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t w[4] = {r[i].a.x, r[i].a.y, r[i].a.z, r[i].a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = __vmaxu2(t[j], w[j] & 0x7fff7fffu);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) { m[2 * j] = t[j] << 16; m[2 * j + 1] = t[j] & 0xffff0000u; }
+}
+
+// A 128 × 128 tile of which a thread holds 8 rows × 8 columns.  Magnitudes meet in shared memory, where one thread per row and per column
+// makes the two factors (and writes the scale: 512 contiguous bytes per tile).  The transposed elements turn in shared memory: 16-byte
+// pieces (rows of one column) at slot (piece ^ column / 8), two passes per access, no more conflicts.
+template <typename T, int MODE>
+__device__ __forceinline__ void fp8_tile(const Fp8TileParams& p, const Raw8<T> (&raw)[8], uint32_t* s_row, uint32_t (*s_col)[128], uint8_t* s_t,
+                                         int rb, int kb) {
   const int t = threadIdx.x, warp = t >> 5, cg = t & 15, rg = t >> 4;      // column group, row group (8 each)
-  const int rb = blockIdx.x / p.cb, kb = blockIdx.x - rb * p.cb;
   const int r0 = rb * 128 + rg * 8, c0 = kb * 128 + cg * 8;
-  const int nc = min(max(p.cols - c0, 0), 8);
-  const T* x = static_cast<const T*>(p.x) + static_cast<int64_t>(r0) * p.ldx + c0;
-  float v[8][8];
-  {
-    Raw8<T> raw[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) load_raw<VEC>(x + i * p.ldx, r0 + i < p.rows ? nc : 0, raw[i]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) unpack8(raw[i], v[i]);
-  }
-  if (NORM) {
-    float w[8];
-    if (p.w_f32) load8<false>(static_cast<const float*>(p.w) + c0, nc, w);
-    else load8<false>(static_cast<const __nv_bfloat16*>(p.w) + c0, nc, w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float rs = r0 + i < p.rows ? p.rstd[r0 + i] : 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = __fmul_rn(__fmul_rn(v[i][e], rs), w[e]);
-    }
-  }
+  float u_tile = 1.f;
   if (MODE == FP8_TILE) {
-    uint32_t m = 0;
+    uint32_t m[8];
+    col_max(raw, m);
+    uint32_t a = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = max(m, abs_bits(v[i][e]));
-    m = __reduce_max_sync(0xffffffffu, m);
-    if ((t & 31) == 0) s_row[warp] = m;
+    for (int i = 0; i < 8; ++i) a = max(a, m[i]);
+    a = __reduce_max_sync(0xffffffffu, a);
+    if ((t & 31) == 0) s_row[warp] = a;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, s_row[i]);
-    const float a = block_amax(m), u = __fdiv_rn(kE4m3Max, a);
-    if (t == 0) p.s[static_cast<int64_t>(rb) * p.cb + kb] = __fdiv_rn(a, kE4m3Max);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = __fmul_rn(v[i][e], u);
+    for (int i = 0; i < 8; ++i) a = max(a, s_row[i]);
+    const float top = block_amax(a);
+    u_tile = __fdiv_rn(kE4m3Max, top);
+    if (t == 0) p.s[static_cast<int64_t>(rb) * p.cb + kb] = __fdiv_rn(top, kE4m3Max);
   } else {
     if (MODE & FP8_ROWS) {
       // eight rows over 16 lanes: at every step a lane hands half of its rows to a neighbour and keeps the other half
       uint32_t m[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        m[i] = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m[i] = max(m[i], abs_bits(v[i][e]));
-      }
+      row_max(raw, m);
 #pragma unroll
       for (int h = 4; h > 0; h >>= 1) {
         const bool up = (t & (2 * h)) != 0;
@@ -161,12 +171,7 @@ __global__ void __launch_bounds__(256) fp8_tile_kernel(const Fp8TileParams p) {
     }
     if (MODE & FP8_COLS) {                               // two row groups of a warp meet: a lane keeps four of its columns
       uint32_t m[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        m[e] = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m[e] = max(m[e], abs_bits(v[i][e]));
-      }
+      col_max(raw, m);
       const bool up = (t & 16) != 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -193,26 +198,34 @@ __global__ void __launch_bounds__(256) fp8_tile_kernel(const Fp8TileParams p) {
     __syncthreads();
   }
   if (((MODE & FP8_ROWS) || MODE == FP8_TILE) && c0 < p.cols) {            // 8-byte pieces: rows are padded to a multiple of 16
+    uint8_t* q = p.q + static_cast<int64_t>(r0) * p.ldq + c0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (r0 + i >= p.rows) break;
-      const float u = MODE == FP8_TILE ? 1.f : __uint_as_float(s_row[rg * 8 + i]);
+      const float u = MODE == FP8_TILE ? u_tile : __uint_as_float(s_row[rg * 8 + i]);
       float o[8];
+      unpack8(raw[i], o);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = MODE == FP8_TILE ? v[i][e] : __fmul_rn(v[i][e], u);
-      *reinterpret_cast<uint2*>(p.q + static_cast<int64_t>(r0 + i) * p.ldq + c0) =
-          make_uint2(pack_e4m3x4(o[0], o[1], o[2], o[3]), pack_e4m3x4(o[4], o[5], o[6], o[7]));
+      for (int e = 0; e < 8; ++e) o[e] = __fmul_rn(o[e], u);
+      if (r0 + i < p.rows)
+        *reinterpret_cast<uint2*>(q + i * p.ldq) = make_uint2(pack_e4m3x4(o[0], o[1], o[2], o[3]), pack_e4m3x4(o[4], o[5], o[6], o[7]));
     }
   }
   if ((MODE & FP8_COLS) || (MODE == FP8_TILE && p.qt)) {
+    float v[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) unpack8(raw[i], v[i]);
+    float uc[8];
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const float4 f = MODE == FP8_TILE ? make_float4(u_tile, u_tile, u_tile, u_tile) : *reinterpret_cast<const float4*>(&s_col[0][cg * 8 + e]);
+      uc[e] = f.x; uc[e + 1] = f.y; uc[e + 2] = f.z; uc[e + 3] = f.w;
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int c = cg * 8 + e;
-      const float u = MODE == FP8_TILE ? 1.f : __uint_as_float(s_col[0][c]);
       float o[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = MODE == FP8_TILE ? v[i][e] : __fmul_rn(v[i][e], u);
-      *reinterpret_cast<uint2*>(s_t + c * 128 + (((rg >> 1) ^ (cg & 7)) << 4) + ((rg & 1) << 3)) =
+      for (int i = 0; i < 8; ++i) o[i] = __fmul_rn(v[i][e], uc[e]);
+      *reinterpret_cast<uint2*>(s_t + (cg * 8 + e) * 128 + (((rg >> 1) ^ (cg & 7)) << 4) + ((rg & 1) << 3)) =
           make_uint2(pack_e4m3x4(o[0], o[1], o[2], o[3]), pack_e4m3x4(o[4], o[5], o[6], o[7]));
     }
     __syncthreads();
@@ -224,6 +237,41 @@ __global__ void __launch_bounds__(256) fp8_tile_kernel(const Fp8TileParams p) {
         *reinterpret_cast<uint4*>(p.qt + static_cast<int64_t>(kb * 128 + c) * p.ldqt + row) =
             *reinterpret_cast<const uint4*>(s_t + c * 128 + ((piece ^ ((c >> 3) & 7)) << 4));
     }
+  }
+}
+
+// One CTA per tile, read once.
+template <typename T, int MODE, bool NORM, bool VEC>
+__global__ void __launch_bounds__(256) fp8_tile_kernel(const Fp8TileParams p) {
+  __shared__ uint32_t s_row[128];
+  __shared__ __align__(16) uint32_t s_col[8][128];
+  __shared__ __align__(16) uint8_t s_t[(MODE & FP8_COLS) || MODE == FP8_TILE ? 128 * 128 : 16];
+  const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4;      // column group, row group (8 each)
+  const int rb = blockIdx.x / p.cb, kb = blockIdx.x - rb * p.cb;
+  const int r0 = rb * 128 + rg * 8, c0 = kb * 128 + cg * 8;
+  const int nc = min(max(p.cols - c0, 0), 8);
+  const T* x = static_cast<const T*>(p.x) + static_cast<int64_t>(r0) * p.ldx + c0;
+  Raw8<T> raw[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) load_raw<VEC>(x + i * p.ldx, r0 + i < p.rows ? nc : 0, raw[i]);
+  if (NORM) {                                            // (x · rstd[row]) · w[col] in fp32, kept in registers
+    float w[8];
+    if (p.w_f32) load8<false>(static_cast<const float*>(p.w) + c0, nc, w);
+    else load8<false>(static_cast<const __nv_bfloat16*>(p.w) + c0, nc, w);
+    Raw8<float> v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float rs = r0 + i < p.rows ? p.rstd[r0 + i] : 0.f;
+      float t[8];
+      unpack8(raw[i], t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t[e] = __fmul_rn(__fmul_rn(t[e], rs), w[e]);
+      v[i].a = make_float4(t[0], t[1], t[2], t[3]);
+      v[i].b = make_float4(t[4], t[5], t[6], t[7]);
+    }
+    fp8_tile<float, MODE>(p, v, s_row, s_col, s_t, rb, kb);
+  } else {
+    fp8_tile<T, MODE>(p, raw, s_row, s_col, s_t, rb, kb);
   }
 }
 
@@ -269,25 +317,35 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, int n, bool vec, const 
 __device__ __forceinline__ float round_to(float v, const float*) { return v; }
 __device__ __forceinline__ float round_to(float v, const __nv_bfloat16*) { return __bfloat162float(__float2bfloat16(v)); }
 
-// TPR threads per row, V vectors of 8 per thread: the row stays in registers.  16 neighbouring threads hold one block of 128.
-template <typename T, typename TO, int TPR, int V, bool VEC>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) fp8_norm_kernel(const Fp8NormParams p) {
-  constexpr int CTA = TPR < 128 ? 128 : TPR, RPC = CTA / TPR, WPR = TPR / 32;
-  __shared__ float s_sum[CTA / 32];
-  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+// PACK threads per row (0: the whole block, one row), V vectors of 8 per thread: the row stays in registers.  16 neighbouring threads
+// hold one block of 128.
+template <typename T, typename TO, int PACK, int V, bool VEC, bool H>
+__global__ void __launch_bounds__(PACK ? 128 : V > 2 ? 1024 : 512) fp8_norm_kernel(const Fp8NormParams p) {
+  __shared__ float s_sum[32];
+  const int TPR = PACK ? PACK : blockDim.x, RPC = PACK ? 128 / PACK : 1, WPR = TPR / 32;
+  const int t = PACK ? threadIdx.x % PACK : threadIdx.x, sub = PACK ? threadIdx.x / PACK : 0;
   const int row = blockIdx.x * RPC + sub;
   const bool live = row < p.rows;
   const int64_t base = static_cast<int64_t>(row) * p.cols;
+  Raw8<T> xr[V];
+  Raw8<__nv_bfloat16> hr[H ? V : 1];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {                          // all of the row's loads first
+    const int c = (t + i * TPR) * 8;
+    const int n = live ? min(max(p.cols - c, 0), 8) : 0;
+    load_raw<VEC>(static_cast<const T*>(p.res) + base + c, n, xr[i]);
+    if (H) load_raw<VEC>(p.h + base + c, n, hr[i]);
+  }
   float v[V][8];
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = (t + i * TPR) * 8;
     const int n = live ? min(max(p.cols - c, 0), 8) : 0;
-    load8<VEC>(static_cast<const T*>(p.res) + base + c, n, v[i]);
-    if (p.h) {
+    unpack8(xr[i], v[i]);
+    if (H) {
       float h[8];
-      load8<VEC>(p.h + base + c, n, h);
+      unpack8(hr[i], h);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] = round_to(__fadd_rn(v[i][e], __fmul_rn(p.h_scale, h[e])), static_cast<const TO*>(nullptr));
       if (n > 0) store8(static_cast<TO*>(p.x) + base + c, n, VEC, v[i]);
@@ -301,7 +359,6 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) fp8_norm_kernel(const F
     if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = ss;
     __syncthreads();
     ss = 0.f;
-#pragma unroll
     for (int i = 0; i < WPR; ++i) ss += s_sum[sub * WPR + i];
   }
   const float rs = rsqrtf(ss / static_cast<float>(p.cols) + p.eps);
@@ -335,21 +392,21 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) fp8_norm_kernel(const F
 template <typename T, typename TO>
 static int launch_norm(const Fp8NormParams& p, cudaStream_t st) {
   const int vecs = (p.cols + 7) / 8;
-#define FP8_NORM(TPR, V)                                                                                     \
-  if (vecs <= TPR * V) {                                                                                     \
-    constexpr int RPC = TPR < 128 ? 128 / TPR : 1;                                                           \
-    const int grid = (p.rows + RPC - 1) / RPC, block = TPR < 128 ? 128 : TPR;                                \
-    if (p.vec) fp8_norm_kernel<T, TO, TPR, V, true><<<grid, block, 0, st>>>(p);                              \
-    else fp8_norm_kernel<T, TO, TPR, V, false><<<grid, block, 0, st>>>(p);                                   \
+#define FP8_NORM(PACK, V, BLOCK)                                                                             \
+  {                                                                                                          \
+    constexpr int RPC = PACK ? 128 / (PACK ? PACK : 1) : 1;                                                  \
+    const int grid = (p.rows + RPC - 1) / RPC, block = BLOCK;                                                \
+    if (p.vec && p.h) fp8_norm_kernel<T, TO, PACK, V, true, true><<<grid, block, 0, st>>>(p);                \
+    else if (p.vec) fp8_norm_kernel<T, TO, PACK, V, true, false><<<grid, block, 0, st>>>(p);                 \
+    else if (p.h) fp8_norm_kernel<T, TO, PACK, V, false, true><<<grid, block, 0, st>>>(p);                   \
+    else fp8_norm_kernel<T, TO, PACK, V, false, false><<<grid, block, 0, st>>>(p);                           \
     return cudaGetLastError() == cudaSuccess ? 0 : -3;                                                       \
   }
-  FP8_NORM(32, 1)
-  FP8_NORM(64, 1)
-  FP8_NORM(128, 1)
-  FP8_NORM(256, 1)
-  FP8_NORM(256, 2)
-  FP8_NORM(256, 4)
-  FP8_NORM(1024, 4)
+  // narrow rows share a block; wider ones have as many threads as leave none idle (2560 columns: 160), two vectors each
+  if (vecs <= 64) FP8_NORM(32, 2, 128)
+  if (vecs <= 128) FP8_NORM(64, 2, 128)
+  if (vecs <= 1024) FP8_NORM(0, 2, (vecs + 63) / 64 * 32)
+  if (vecs <= 4096) FP8_NORM(0, 4, 1024)
 #undef FP8_NORM
   return -6;
 }

@@ -6,16 +6,28 @@
 // fp32 scales, so the products of one block of K are accumulated in tensor memory (exact to fp32 rounding over 128 terms), read
 // back, scaled and added to fp32 sums in registers.
 //
-// 128 × 128 tile per CTA, six stages of 32 KB; two accumulators in tensor memory, so that the products of a block run while the
-// one before is read.  192 threads: warp 0 TMA, warp 1 MMA, warps 2..5 sums (thread = row of the tile, 128 sums each).
+// This file: the form for few rows of A (single tokens to a few hundred) and for outputs too small to fill the machine with the 256-row
+// tiles of gemm2_fp8_block.cu.  It is bound by reading B once (one token: 11264 × 2048 weights, 23 MB, 3.5 µs at the copy rate) and, at
+// this size, by the latency of one CTA's chain.  So 128 rows of B are the M side of the MMA and BT rows of A (16 to 128) its N side, which
+// makes neighbouring lanes neighbouring columns of the output, and the blocks of K are split over a cluster of up to eight CTAs.  The
+// first loads are issued before tensor memory is allocated.  The CTAs' sums meet in shared memory, in the place of the stages; every CTA
+// adds its share of the rows over the ranks in rank order (distributed shared memory), so a result does not depend on scheduling.
+//
+// 192 threads: warp 0 TMA, warp 1 MMA, warps 2..5 sums (thread = row of B, BT sums); all of them add.
 #include "api.h"
 #include "sm100.cuh"
 
 namespace b200 {
 
-constexpr int FB_BM = 128, FB_BN = 128, FB_BK = 128, FB_STAGES = 6, FB_THREADS = 192;
-constexpr int FB_A = FB_BM * FB_BK, FB_B = FB_BN * FB_BK, FB_STAGE = FB_A + FB_B;
-constexpr int FB_SMEM = FB_STAGES * FB_STAGE + 1024 + 256;
+constexpr int FS_BN = 128, FS_BK = 128, FS_STAGES = 4, FS_THREADS = 192, FS_CHUNK = 32;
+
+template <int BT>
+struct FS {
+  static constexpr int B_BYTES = FS_BN * FS_BK, A_BYTES = BT * FS_BK, STAGE = B_BYTES + A_BYTES;
+  static constexpr int TMEM = 2 * BT < 32 ? 32 : 2 * BT;
+  static constexpr int SMEM = FS_STAGES * STAGE + FS_CHUNK * BT * 4 + 1024 + 256;
+  static_assert(BT * FS_BN * 4 <= FS_STAGES * STAGE, "the sums take the place of the stages");
+};
 
 struct Fp8Scale {
   const float* p;
@@ -23,149 +35,242 @@ struct Fp8Scale {
   int shift;              // 0: one scale per row, 7: per 128 rows
 };
 
-struct Fp8GemmParams {
+struct FsParams {
   void* out;
   const void* bias;
   Fp8Scale sa, sb;
   int M, N, K;
   int64_t ldc;
-  int out_f32, accumulate, bias_f32;
+  int out_f32, accumulate, bias_f32, vec;
   int* status;
 };
 
-__device__ __forceinline__ void umma_fp8_warp(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-  if (elect_one_sync())
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
-        "}\n" ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
-        : "memory");
+__device__ __forceinline__ void fs_mma(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
-// e4m3 × e4m3 (format code 0 in both operand fields), fp32 accumulate, both operands K-major
-__host__ __device__ constexpr uint32_t make_idesc_e4m3(int M, int N) {
-  return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+__device__ __forceinline__ float4 fs_ld_cluster(uint32_t smem_addr, int rank) {
+  uint32_t a;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
 }
 
-__global__ void __launch_bounds__(FB_THREADS, 1)
-gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const Fp8GemmParams p) {
+template <int BT, int S>
+__global__ void __launch_bounds__(FS_THREADS, BT <= 64 ? 2 : 1)
+gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const FsParams p) {
+  using T = FS<BT>;
+  constexpr int PC = BT < 32 ? BT : 32;                // columns that a load from tensor memory brings
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + FB_STAGES * FB_STAGE);
+  float* part = reinterpret_cast<float*>(smem);        // [BT][128] sums of this CTA, once the stages are read
+  float* table = reinterpret_cast<float*>(smem + FS_STAGES * T::STAGE);      // [FS_CHUNK][BT] scales of A
+  uint64_t* bars = reinterpret_cast<uint64_t*>(table + FS_CHUNK * BT);
   uint64_t* full_bar = bars;
-  uint64_t* empty_bar = bars + FB_STAGES;
-  uint64_t* tmem_full = bars + 2 * FB_STAGES;          // [2]
-  uint64_t* tmem_empty = bars + 2 * FB_STAGES + 2;     // [2], four warps
-  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(bars + 2 * FB_STAGES + 4);
+  uint64_t* empty_bar = bars + FS_STAGES;
+  uint64_t* tmem_full = bars + 2 * FS_STAGES;          // [2]
+  uint64_t* tmem_empty = bars + 2 * FS_STAGES + 2;     // [2], four warps
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(bars + 2 * FS_STAGES + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int num_m = (p.M + FB_BM - 1) / FB_BM;
-  const int m0 = static_cast<int>(blockIdx.x) % num_m * FB_BM, n0 = static_cast<int>(blockIdx.x) / num_m * FB_BN;
-  const int num_kb = (p.K + FB_BK - 1) / FB_BK;
+  const int rank = S > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int num_n = (p.N + FS_BN - 1) / FS_BN;
+  const int tile = static_cast<int>(blockIdx.x) / S, n0 = tile % num_n * FS_BN, m0 = tile / num_n * BT;
+  const int num_kb = (p.K + FS_BK - 1) / FS_BK, per = (num_kb + S - 1) / S;
+  const int kb0 = min(rank * per, num_kb), nkb = min(kb0 + per, num_kb) - kb0;      // the last ranks may have no share
 
+  auto load = [&](int i, int st) {
+    uint8_t* sb = smem + st * T::STAGE;
+    mbar_arrive_expect_tx(&full_bar[st], T::STAGE);
+    tma_load_2d(sb, &tmap_b, &full_bar[st], (kb0 + i) * FS_BK, n0);
+    tma_load_2d(sb + T::B_BYTES, &tmap_a, &full_bar[st], (kb0 + i) * FS_BK, m0);
+  };
   if (threadIdx.x == 0) {
-    for (int s = 0; s < FB_STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    for (int s = 0; s < FS_STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
     for (int a = 0; a < 2; ++a) { mbar_init(&tmem_full[a], 1); mbar_init(&tmem_empty[a], 4); }
     *abort_flag = 0;
     mbar_fence_init();
-    tma_prefetch_desc(&tmap_a);
-    tma_prefetch_desc(&tmap_b);
+    fence_proxy_async_smem();
+    for (int i = 0; i < FS_STAGES && i < nkb; ++i) load(i, i);      // the ring is empty: no wait, and under the set-up
   }
-  if (warp == 1) { tmem_alloc(tmem_ptr, 256); tmem_relinquish(); }
+  if (warp == 1) { tmem_alloc(tmem_ptr, T::TMEM); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
 
   if (warp == 0) {
-    if (lane == 0) {
-      for (int kb = 0; kb < num_kb; ++kb) {
-        const int st = kb % FB_STAGES; const uint32_t ph = (kb / FB_STAGES) & 1;
-        if (!mbar_wait(&empty_bar[st], ph ^ 1, abort_flag, p.status, STATUS_TIMEOUT_EMPTY)) break;
-        uint8_t* sa = smem + st * FB_STAGE;
-        mbar_arrive_expect_tx(&full_bar[st], FB_STAGE);
-        tma_load_2d(sa, &tmap_a, &full_bar[st], kb * FB_BK, m0);
-        tma_load_2d(sa + FB_A, &tmap_b, &full_bar[st], kb * FB_BK, n0);
-      }
+    for (int i = FS_STAGES; i < nkb; ++i) {
+      const int st = i % FS_STAGES; const uint32_t ph = (i / FS_STAGES) & 1;
+      if (!mbar_wait_warp(&empty_bar[st], ph ^ 1, abort_flag, p.status, STATUS_TIMEOUT_EMPTY)) break;
+      if (elect_one_sync()) load(i, st);
     }
   } else if (warp == 1) {
-    constexpr uint32_t idesc = make_idesc_e4m3(FB_BM, FB_BN);
-    for (int kb = 0; kb < num_kb; ++kb) {
-      const int st = kb % FB_STAGES; const uint32_t ph = (kb / FB_STAGES) & 1;
-      const int acc = kb & 1; const uint32_t aph = (kb >> 1) & 1;
-      if (!mbar_wait_warp(&tmem_empty[acc], aph ^ 1, abort_flag, p.status, STATUS_TIMEOUT_TMEM_EMPTY)) break;
+    // e4m3 × e4m3, fp32 accumulate, both operands K-major
+    constexpr uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(BT >> 3) << 17) | (static_cast<uint32_t>(FS_BN >> 4) << 24);
+    for (int i = 0; i < nkb; ++i) {
+      const int st = i % FS_STAGES; const uint32_t ph = (i / FS_STAGES) & 1;
+      const int acc = i & 1; const uint32_t aph = (i >> 1) & 1;
       if (!mbar_wait_warp(&full_bar[st], ph, abort_flag, p.status, STATUS_TIMEOUT_FULL)) break;
+      if (!mbar_wait_warp(&tmem_empty[acc], aph ^ 1, abort_flag, p.status, STATUS_TIMEOUT_TMEM_EMPTY)) break;
       tc_fence_after();
-      const uint32_t sa = smem_u32(smem + st * FB_STAGE);
-      const uint64_t da = make_smem_desc(sa, 16, 1024), db = make_smem_desc(sa + FB_A, 16, 1024);
+      const uint32_t sb = smem_u32(smem + st * T::STAGE);
+      const uint64_t db = make_smem_desc(sb, 16, 1024), da = make_smem_desc(sb + T::B_BYTES, 16, 1024);
+      if (elect_one_sync()) {
 #pragma unroll
-      for (uint32_t k = 0; k < FB_BK / 32; ++k)
-        umma_fp8_warp(tmem_base + acc * FB_BN, da + static_cast<uint64_t>(2 * k), db + static_cast<uint64_t>(2 * k), idesc, k != 0 ? 1u : 0u);
-      umma_commit_warp(&empty_bar[st]);
-      umma_commit_warp(&tmem_full[acc]);
+        for (uint32_t k = 0; k < FS_BK / 32; ++k)
+          fs_mma(tmem_base + acc * BT, db + static_cast<uint64_t>(2 * k), da + static_cast<uint64_t>(2 * k), idesc, k != 0 ? 1u : 0u);
+        umma_commit(&tmem_full[acc]);
+        umma_commit(&empty_bar[st]);
+      }
     }
   } else {
-    const int q = warp & 3;
-    const int row = m0 + q * 32 + lane;
-    const bool live = row < p.M;
-    const float* sa = p.sa.p + static_cast<int64_t>(live ? row >> p.sa.shift : 0) * p.sa.row;
-    float sum[FB_BN];
+    const int q = warp & 3, t = threadIdx.x - 64;
+    const int n = n0 + q * 32 + lane;
+    const float* sb = p.sb.p + static_cast<int64_t>(min(n, p.N - 1) >> p.sb.shift) * p.sb.row + kb0 * p.sb.blk;
+    float sum[BT], scale[8];
 #pragma unroll
-    for (int i = 0; i < FB_BN; ++i) sum[i] = 0.f;
+    for (int i = 0; i < BT; ++i) sum[i] = 0.f;
     bool ok = true;
-    for (int kb = 0; kb < num_kb; ++kb) {
-      const int acc = kb & 1; const uint32_t aph = (kb >> 1) & 1;
-      const float fa = live ? sa[kb * p.sa.blk] : 0.f;
-      const float* sb = p.sb.p + kb * p.sb.blk;
-      ok = mbar_wait(&tmem_full[acc], aph, abort_flag, p.status, STATUS_TIMEOUT_TMEM_FULL);
-      ok = __all_sync(0xffffffffu, ok);
+    for (int i = 0; i < nkb; ++i) {
+      const int acc = i & 1; const uint32_t aph = (i >> 1) & 1;
+      if (i % FS_CHUNK == 0) {                         // scales of A of the next blocks: the same for all rows of B
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const int blocks = min(FS_CHUNK, nkb - i);
+        for (int j = t; j < blocks * BT; j += 128) {
+          const int m = m0 + j % BT;
+          table[j] = m < p.M ? p.sa.p[static_cast<int64_t>(m >> p.sa.shift) * p.sa.row + (kb0 + i + j / BT) * p.sa.blk] : 0.f;
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      }
+      if ((i & 7) == 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) scale[j] = sb[min(i + j, nkb - 1) * p.sb.blk];
+      }
+      const float s01 = (i & 1) ? scale[1] : scale[0], s23 = (i & 1) ? scale[3] : scale[2];
+      const float s45 = (i & 1) ? scale[5] : scale[4], s67 = (i & 1) ? scale[7] : scale[6];
+      const float f = (i & 4) ? ((i & 2) ? s67 : s45) : ((i & 2) ? s23 : s01);
+      const float4* sa = reinterpret_cast<const float4*>(table + i % FS_CHUNK * BT);
+      ok = mbar_wait_warp(&tmem_full[acc], aph, abort_flag, p.status, STATUS_TIMEOUT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after();
+      const uint32_t taddr = tmem_base + acc * BT + (static_cast<uint32_t>(q * 32) << 16);
 #pragma unroll
-      for (int c = 0; c < FB_BN / 32; ++c) {
-        uint32_t r[32];
-        tmem_ld_32x32(tmem_base + acc * FB_BN + c * 32 + (static_cast<uint32_t>(q * 32) << 16), r);
+      for (int c = 0; c < BT / PC; ++c) {
+        uint32_t r[PC];
+        if constexpr (PC == 32) tmem_ld_32x32(taddr + c * PC, r);
+        else tmem_ld_32x16(taddr + c * PC, r);
         tmem_ld_wait();
+        if (c + 1 == BT / PC) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tmem_empty[acc]);
+        }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int col = n0 + c * 32 + i;
-          const float fb = col < p.N ? sb[static_cast<int64_t>(col >> p.sb.shift) * p.sb.row] : 0.f;
-          sum[c * 32 + i] += __uint_as_float(r[i]) * (fa * fb);
+        for (int j = 0; j < PC; j += 4) {
+          const float4 a = sa[(c * PC + j) / 4];
+          float* o = sum + c * PC + j;
+          o[0] = fmaf(__uint_as_float(r[j]) * a.x, f, o[0]);
+          o[1] = fmaf(__uint_as_float(r[j + 1]) * a.y, f, o[1]);
+          o[2] = fmaf(__uint_as_float(r[j + 2]) * a.z, f, o[2]);
+          o[3] = fmaf(__uint_as_float(r[j + 3]) * a.w, f, o[3]);
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&tmem_empty[acc]);
     }
-    if (ok && live) {
+    // the last products were waited for, so the loads before them have landed and the stages may be written
+    if (ok) {
 #pragma unroll
-      for (int i = 0; i < FB_BN; ++i) {
-        const int col = n0 + i;
-        if (col < p.N) {
-          float v = sum[i];
-          if (p.bias) v += p.bias_f32 ? static_cast<const float*>(p.bias)[col] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col]);
-          const int64_t at = static_cast<int64_t>(row) * p.ldc + col;
-          if (p.out_f32) {
-            float* o = static_cast<float*>(p.out) + at;
-            *o = p.accumulate ? *o + v : v;
-          } else {
-            static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16(v);
-          }
-        }
-      }
+      for (int i = 0; i < BT; ++i) part[i * FS_BN + q * 32 + lane] = sum[i];
     }
   }
   tc_fence_before();
   __syncthreads();
+  if (S > 1) cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, 256);
+    tmem_dealloc(tmem_base, T::TMEM);
   }
+  // rows of the output: every CTA of the cluster adds its share over the ranks
+  const int rows = min(p.M - m0, BT), first = rank * BT / S, last = min((rank + 1) * BT / S, rows);
+  const int col = n0 + lane * 4;
+  const uint32_t part_addr = smem_u32(part);
+  for (int m = first + warp; m < last; m += FS_THREADS / 32) {
+    float4 v[S];
+#pragma unroll
+    for (int r = 0; r < S; ++r) {
+      if (S > 1) v[r] = fs_ld_cluster(part_addr + (m * FS_BN + lane * 4) * 4, r);
+      else v[r] = *reinterpret_cast<const float4*>(part + m * FS_BN + lane * 4);
+    }
+#pragma unroll
+    for (int r = 1; r < S; ++r) { v[0].x += v[r].x; v[0].y += v[r].y; v[0].z += v[r].z; v[0].w += v[r].w; }
+    float o[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+    if (p.bias) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (col + e < p.N) o[e] += p.bias_f32 ? static_cast<const float*>(p.bias)[col + e] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col + e]);
+    }
+    const int64_t at = static_cast<int64_t>(m0 + m) * p.ldc + col;
+    if (p.out_f32) {
+      float* d = static_cast<float*>(p.out) + at;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (col + e < p.N) d[e] = p.accumulate ? d[e] + o[e] : o[e];
+    } else {
+      __nv_bfloat16* d = static_cast<__nv_bfloat16*>(p.out) + at;
+      if (p.vec && col + 4 <= p.N) {
+        *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < p.N) d[e] = __float2bfloat16(o[e]);
+      }
+    }
+  }
+  if (S > 1) cluster_sync_all();                       // nobody leaves while its sums are read
 }
 
 int make_tmap_2d_u8(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
                     uint32_t box_inner, uint32_t box_outer);
+
+template <int BT, int S>
+static int launch_fs(const CUtensorMap& ta, const CUtensorMap& tb, const FsParams& p, unsigned tiles, cudaStream_t st) {
+  auto kern = gemm_fp8_block_kernel<BT, S>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FS<BT>::SMEM) != cudaSuccess) return -2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(tiles * S);
+  cfg.blockDim = dim3(FS_THREADS);
+  cfg.dynamicSmemBytes = FS<BT>::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = S; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = S > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, ta, tb, p) == cudaSuccess ? 0 : -3;
+}
+template <int BT>
+static int launch_fs(const void* A, int64_t lda, const void* B, int64_t ldb, const FsParams& p, int num_sms, cudaStream_t st) {
+  CUtensorMap ta, tb;
+  int rc = make_tmap_2d_u8(&ta, A, p.K, p.M, lda, FS_BK, BT);
+  if (!rc) rc = make_tmap_2d_u8(&tb, B, p.K, p.N, ldb, FS_BK, FS_BN);
+  if (rc) return rc;
+  const int64_t tiles = static_cast<int64_t>((p.M + BT - 1) / BT) * ((p.N + FS_BN - 1) / FS_BN);
+  if (tiles > 0xfffffff) return -6;
+  // K is split as far as the CTAs fit the machine at once and have a block each
+  const int64_t room = static_cast<int64_t>(num_sms) * (BT <= 64 ? 2 : 1);
+  const int num_kb = (p.K + FS_BK - 1) / FS_BK;
+  int s = 1;
+  while (s < 8 && tiles * 2 * s <= room && 2 * s <= num_kb) s *= 2;
+  const unsigned t = static_cast<unsigned>(tiles);
+  return s == 8 ? launch_fs<BT, 8>(ta, tb, p, t, st) : s == 4 ? launch_fs<BT, 4>(ta, tb, p, t, st)
+       : s == 2 ? launch_fs<BT, 2>(ta, tb, p, t, st) : launch_fs<BT, 1>(ta, tb, p, t, st);
+}
 
 }  // namespace b200
 
@@ -178,25 +283,25 @@ extern "C" int b200_gemm_fp8_block(const void* A, int64_t lda, const float* sa, 
   using namespace b200;
   if (M < 0 || N < 0 || K < 1 || lda % 16 || ldb % 16 || (accumulate && !out_f32)) return -6;
   if (M == 0 || N == 0) return 0;
+  static thread_local bool ctx_bound = false;          // tensor maps are encoded by the driver, which wants a context on this thread
+  if (!ctx_bound) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return -5;
+    ctx_bound = true;
+  }
   if (pair) {
     const auto rows = [](const float* s, int64_t row, int64_t blk) { return row == 1 && blk % 4 == 0 && reinterpret_cast<uintptr_t>(s) % 16 == 0; };
-    if (sa_tile || !rows(sa, sa_row, sa_blk) || (!sb_tile && !rows(sb, sb_row, sb_blk))) return -6;
+    if (sa_tile || sa_row != 1 || (!sb_tile && !rows(sb, sb_row, sb_blk))) return -6;
     const int64_t m = (M + 255) / 256, pairs = num_sms / 2;
-    // tiles of half the width take 0.55 of the time (a little more than half): narrower where that saves enough of the last wave
-    const int64_t wide = (m * ((N + 255) / 256) + pairs - 1) / pairs * 100, narrow = (m * ((N + 127) / 128) + pairs - 1) / pairs * 55;
+    // tiles of half the width take 0.62 of the time: narrower where that saves enough of the last wave
+    const int64_t wide = (m * ((N + 255) / 256) + pairs - 1) / pairs * 100, narrow = (m * ((N + 127) / 128) + pairs - 1) / pairs * 62;
     return b200_gemm2_fp8_block(A, lda, sa, sa_blk, B, ldb, sb, sb_row, sb_blk, sb_tile, bias, bias_dtype == 0 ? 1 : 0, out, ldc, M, N, K, out_f32,
                                 accumulate, narrow < wide ? 128 : 256, num_sms, status, stream);
   }
-  CUtensorMap ta, tb;
-  int rc = make_tmap_2d_u8(&ta, A, K, M, lda, FB_BK, FB_BM);
-  if (rc) return rc;
-  rc = make_tmap_2d_u8(&tb, B, K, N, ldb, FB_BK, FB_BN);
-  if (rc) return rc;
-  const Fp8GemmParams p{out, bias, {sa, sa_row, sa_blk, sa_tile ? 7 : 0}, {sb, sb_row, sb_blk, sb_tile ? 7 : 0}, M, N, K, ldc,
-                        out_f32, accumulate, bias_dtype == 0 ? 1 : 0, status};
-  if (cudaFuncSetAttribute(gemm_fp8_block_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FB_SMEM) != cudaSuccess) return -2;
-  const int64_t tiles = static_cast<int64_t>((M + FB_BM - 1) / FB_BM) * ((N + FB_BN - 1) / FB_BN);
-  if (tiles > 0x7fffffff) return -6;
-  gemm_fp8_block_kernel<<<static_cast<unsigned>(tiles), FB_THREADS, FB_SMEM, stream>>>(ta, tb, p);
-  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+  const FsParams p{out, bias, {sa, sa_row, sa_blk, sa_tile ? 7 : 0}, {sb, sb_row, sb_blk, sb_tile ? 7 : 0}, M, N, K, ldc, out_f32, accumulate,
+                   bias_dtype == 0 ? 1 : 0, ldc % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0 ? 1 : 0, status};
+  if (M <= 16) return launch_fs<16>(A, lda, B, ldb, p, num_sms, stream);
+  if (M <= 32) return launch_fs<32>(A, lda, B, ldb, p, num_sms, stream);
+  if (M <= 64) return launch_fs<64>(A, lda, B, ldb, p, num_sms, stream);
+  return launch_fs<128>(A, lda, B, ldb, p, num_sms, stream);
 }
