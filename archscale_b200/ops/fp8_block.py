@@ -100,6 +100,7 @@ def add_rms_norm_fp8_ref(res, h, weight, eps: float = 1e-5, h_scale: float = 1.0
 
 
 # ------------------------------------------------------------------------------------------------ checks
+# The bindings check the operands of the kernels (and raise the same exceptions); these are for the restatements.
 def _stream(res: torch.Tensor, stream_dtype: Optional[torch.dtype]) -> torch.dtype:
     return res.dtype if stream_dtype is None else stream_dtype
 
@@ -116,73 +117,64 @@ def _need_matrix(name: str, x: torch.Tensor) -> None:
     _need_float(name, x=x)
 
 
-def _dense_rows(x: torch.Tensor) -> torch.Tensor:
-    return x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous()
+def _kernel(x: torch.Tensor) -> bool:
+    return x.is_cuda and backend.use_cuda_kernel("fp8_block", x)
 
 
-def _kernel(*tensors) -> bool:
-    return tensors[0].is_cuda and backend.use_cuda_kernel("fp8_block", *tensors)
+def _ext():
+    backend.count_launch()
+    return backend.require_extension()
 
 
 # ------------------------------------------------------------------------------------------------ quantisers
 def quantize_fp8_block(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x:(R,C) → (elements (R,C), scales (R, ⌈C/128⌉)), blocks along the rows."""
+    if _kernel(x):
+        return tuple(_ext().fp8_quantize(x, 1))
     _need_matrix("quantize_fp8_block", x)
-    if not _kernel(x):
-        return quantize_ref(x)
-    backend.count_launch()
-    return tuple(backend.require_extension().fp8_quantize(_dense_rows(x), 1))
+    return quantize_ref(x)
 
 
 def quantize_fp8_block_t(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x:(R,C) → (elements (C,R), scales (C, ⌈R/128⌉)) of the transposed matrix, blocks along the original columns."""
+    if _kernel(x):
+        return tuple(_ext().fp8_quantize(x, 2))
     _need_matrix("quantize_fp8_block_t", x)
-    if not _kernel(x):
-        return quantize_ref(x.t())
-    backend.count_launch()
-    return tuple(backend.require_extension().fp8_quantize(_dense_rows(x), 2))
+    return quantize_ref(x.t())
 
 
 def quantize_fp8_block_both(x: torch.Tensor):
     """:func:`quantize_fp8_block` and :func:`quantize_fp8_block_t` from one read of x: (q, scale, q_t, scale_t)."""
+    if _kernel(x):
+        return tuple(_ext().fp8_quantize(x, 3))
     _need_matrix("quantize_fp8_block_both", x)
-    if not _kernel(x):
-        return (*quantize_ref(x), *quantize_ref(x.t()))
-    backend.count_launch()
-    return tuple(backend.require_extension().fp8_quantize(_dense_rows(x), 3))
+    return (*quantize_ref(x), *quantize_ref(x.t()))
 
 
 def quantize_fp8_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """w:(N,K) → (elements (N,K), the same transposed (K,N), scales (⌈N/128⌉, ⌈K/128⌉) of 128 × 128 tiles)."""
+    if _kernel(w):
+        return tuple(_ext().fp8_quantize(w, 4))
     _need_matrix("quantize_fp8_weight", w)
-    if not _kernel(w):
-        q, scale = quantize_weight_ref(w)
-        return q, q.t().contiguous(), scale
-    backend.count_launch()
-    q, scale, q_t = backend.require_extension().fp8_quantize(_dense_rows(w), 4)
-    return q, q_t, scale
+    q, scale = quantize_weight_ref(w)
+    return q, q.t().contiguous(), scale
 
 
 # ------------------------------------------------------------------------------------------------ product
-def _whole_rows(q: torch.Tensor) -> torch.Tensor:
-    """Elements as the GEMM reads them: dense rows that start at multiples of 16 bytes."""
-    K = q.shape[1]
-    if (q.stride(1) == 1 or K <= 1) and (q.stride(0) % 16 == 0 or q.shape[0] <= 1) and q.data_ptr() % 16 == 0:
-        return q
-    out = torch.empty(q.shape[0], (K + 15) // 16 * 16, dtype=torch.uint8, device=q.device)[:, :K]
-    out.copy_(q.view(torch.uint8) if q.stride(1) == 1 else q.contiguous().view(torch.uint8))
-    return out.view(FP8)
-
-
 def matmul_fp8_block(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
                      out_dtype: torch.dtype = torch.bfloat16, acc: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``a:(M,K) · b:(N,K)ᵀ (+ bias)``, each operand with scales per row and block of 128, ``(rows, ⌈K/128⌉)``, or per 128 × 128 tile,
-    ``(⌈rows/128⌉, ⌈K/128⌉)`` → (M,N) in ``out_dtype``; with ``acc`` (fp32) the product is added to it in place."""
-    for what, t in (("a", a), ("b", b)):
-        if t.dtype != FP8 or t.dim() != 2:
-            raise TypeError(f"matmul_fp8_block: {what} must be a float8_e4m3fn matrix, got {t.dtype} {tuple(t.shape)}")
-    if a.shape[1] != b.shape[1]:
-        raise ValueError(f"matmul_fp8_block: contraction lengths differ: {a.shape[1]} and {b.shape[1]}")
+    ``(⌈rows/128⌉, ⌈K/128⌉)`` → (M,N) in ``out_dtype``; with ``acc`` (fp32) the product is added to it in place.  ``a`` may have more leading
+    dimensions than one (M: their product), which the result then has too."""
+    if out_dtype not in _FLOATS:
+        raise TypeError(f"matmul_fp8_block: out_dtype must be bfloat16 or float32, got {out_dtype}")
+    if _kernel(a):
+        return _ext().gemm_fp8_block(a, a_scale, b, b_scale, bias, out_dtype is torch.float32, acc)
+    if a.dtype != FP8 or b.dtype != FP8:
+        raise TypeError(f"matmul_fp8_block: operands must be float8_e4m3fn, got {a.dtype} and {b.dtype}")
+    if a.dim() < 2 or b.dim() != 2 or a.shape[-1] != b.shape[1]:
+        raise ValueError(f"matmul_fp8_block: contraction lengths differ: {tuple(a.shape)} and {tuple(b.shape)}")
+    lead, a = a.shape[:-1], a.reshape(-1, a.shape[-1])
     blocks = (a.shape[1] + BLOCK - 1) // BLOCK
     for what, q, s in (("a_scale", a, a_scale), ("b_scale", b, b_scale)):
         if s.dtype != torch.float32 or s.dim() != 2 or s.shape[1] != blocks or s.shape[0] not in (q.shape[0], (q.shape[0] + BLOCK - 1) // BLOCK):
@@ -190,15 +182,10 @@ def matmul_fp8_block(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_
                              f"got {s.dtype} {tuple(s.shape)}")
     if bias is not None and (bias.shape != (b.shape[0],) or bias.dtype not in _FLOATS):
         raise ValueError(f"matmul_fp8_block: bias must be ({b.shape[0]},) in bfloat16 or float32, got {bias.dtype} {tuple(bias.shape)}")
-    if out_dtype not in _FLOATS:
-        raise TypeError(f"matmul_fp8_block: out_dtype must be bfloat16 or float32, got {out_dtype}")
     if acc is not None and (acc.dtype != torch.float32 or acc.shape != (a.shape[0], b.shape[0])):
         raise ValueError(f"matmul_fp8_block: acc must be float32 ({a.shape[0]}, {b.shape[0]}), got {acc.dtype} {tuple(acc.shape)}")
-    if not _kernel(a, a_scale, b, b_scale):
-        return matmul_fp8_block_ref(a, a_scale, b, b_scale, bias, out_dtype, acc)
-    backend.count_launch()
-    return backend.require_extension().gemm_fp8_block(_whole_rows(a), a_scale, _whole_rows(b), b_scale,
-                                                      None if bias is None else bias.contiguous(), out_dtype == torch.float32, acc)
+    y = matmul_fp8_block_ref(a, a_scale, b, b_scale, bias, out_dtype, acc)
+    return y if len(lead) == 1 or acc is not None else y.view(*lead, b.shape[0])
 
 
 Quantised = Tuple[torch.Tensor, torch.Tensor]
@@ -209,17 +196,12 @@ def linear_fp8_weight(x: Union[torch.Tensor, Quantised], weight: torch.Tensor, s
     """``x · Wᵀ (+ bias)`` with stored elements ``weight:(N,K)`` and scales of 128 × 128 tiles.  ``x:(..., K)`` is quantised here, or is the
     pair (elements, scales) of :func:`add_rms_norm_fp8` / :func:`quantize_fp8_block` with any leading dimensions of the elements.  No
     gradients."""
-    if isinstance(x, torch.Tensor):
-        _need_float("linear_fp8_weight", x=x)
-        lead, out_dtype = x.shape[:-1], out_dtype or x.dtype
-        q, s = quantize_fp8_block(x.detach().reshape(-1, x.shape[-1]))
-    else:
-        q, s = x
-        lead, out_dtype = q.shape[:-1], out_dtype or torch.bfloat16
-        if q.dim() != 2:
-            q = q.reshape(-1, q.shape[-1])
-    y = matmul_fp8_block(q, s, weight, scale, bias, out_dtype)
-    return y if len(lead) == 1 else y.view(*lead, weight.shape[0])
+    if not isinstance(x, torch.Tensor):
+        return matmul_fp8_block(x[0], x[1], weight, scale, bias, out_dtype or torch.bfloat16)
+    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    q, s = quantize_fp8_block(flat)
+    y = matmul_fp8_block(q, s, weight, scale, bias, out_dtype or x.dtype)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
 
 
 # ------------------------------------------------------------------------------------------------ training
@@ -297,13 +279,13 @@ def _check_norm(name, res, h, weight, stream_dtype):
 
 
 def _norm_kernel(res, h, weight, eps, h_scale, stream_dtype, want_rstd):
-    """(x, q, scale, rstd) on two-dimensional operands."""
-    if not _kernel(res, h, weight) or not 1 <= res.shape[1] <= 32768:
-        x, rstd, n = _norm_ref(res, h, weight, eps, h_scale, stream_dtype)
-        return (x, *quantize_ref(n), rstd.reshape(-1))
-    backend.count_launch()
-    return backend.require_extension().add_rmsnorm_fp8(res.contiguous(), None if h is None else h.contiguous(), h_scale, weight.contiguous(), eps,
-                                                       stream_dtype == torch.bfloat16, want_rstd)
+    """(x of the shape of res, elements (rows, C), scales, 1 / rms (rows,))."""
+    C = res.shape[-1]
+    if not _kernel(res) or not 1 <= C <= 32768:
+        _check_norm("add_rms_norm_fp8", res, h, weight, _stream(res, stream_dtype))
+        x, rstd, n = _norm_ref(res, h, weight, eps, h_scale, _stream(res, stream_dtype))
+        return (x, *quantize_ref(n.reshape(-1, C)), rstd.reshape(-1))
+    return _ext().add_rmsnorm_fp8(res, h, weight, eps, h_scale, -1 if stream_dtype is None else int(stream_dtype is torch.bfloat16), want_rstd)
 
 
 def add_rms_norm_fp8(res: torch.Tensor, h: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-5, h_scale: float = 1.0,
@@ -311,12 +293,8 @@ def add_rms_norm_fp8(res: torch.Tensor, h: Optional[torch.Tensor], weight: torch
     """``x = res + h_scale · h`` (fp32, kept in ``stream_dtype``, by default the type of ``res``; without ``h`` x is ``res``) and ``rmsnorm(x) · weight`` as
     elements and scales: (x of the shape of res, elements (rows, C), scales (rows, ⌈C/128⌉)).  No gradients: training goes through
     :func:`add_rms_norm_linear_fp8`."""
-    stream_dtype = _stream(res, stream_dtype)
-    _check_norm("add_rms_norm_fp8", res, h, weight, stream_dtype)
-    C = res.shape[-1]
-    with torch.no_grad():
-        x, q, scale, _ = _norm_kernel(res.reshape(-1, C), None if h is None else h.reshape(-1, C), weight, eps, h_scale, stream_dtype, False)
-    return (res if h is None else x.view(res.shape)), q, scale
+    x, q, scale, _ = _norm_kernel(res, h, weight, eps, h_scale, stream_dtype, False)
+    return x, q, scale
 
 
 def _norm_backward_ref(gx, dn, x, weight, rstd, h_scale, want_h):
@@ -332,22 +310,21 @@ def _norm_backward_ref(gx, dn, x, weight, rstd, h_scale, want_h):
 class _AddNormLinearFP8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, res, h, norm_weight, weight, bias, eps, h_scale, stream_dtype):
-        C = res.shape[-1]
-        res2, h2 = res.reshape(-1, C), None if h is None else h.reshape(-1, C)
-        x, q, s, rstd = _norm_kernel(res2, h2, norm_weight, eps, h_scale, stream_dtype, True)
+        x, q, s, rstd = _norm_kernel(res, h, norm_weight, eps, h_scale, stream_dtype, True)
         wq, wq_t, ws = quantize_fp8_weight(weight)
         ctx.save_for_backward(x, rstd, norm_weight, wq_t, ws)
         ctx.weight, ctx.shape, ctx.res_dtype, ctx.h_scale, ctx.has_h = weight, res.shape, res.dtype, h_scale, h is not None
         ctx.bias_dtype = None if bias is None else bias.dtype
         ctx.set_materialize_grads(False)
         y = matmul_fp8_block(q, s, wq, ws, bias, torch.bfloat16).view(*res.shape[:-1], weight.shape[0])
-        return (x.view(res.shape) if h is not None else res.view_as(res)), y
+        return (x if h is not None else res.view_as(res)), y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gx, gy):
         x, rstd, norm_weight, wq_t, ws = ctx.saved_tensors
         C = ctx.shape[-1]
+        x = x.reshape(-1, C)
         need_res, need_h, need_nw, need_w, need_b = ctx.needs_input_grad[:5]
         need_n = need_res or need_h or need_nw
         gx2 = None if gx is None else gx.reshape(-1, C)
@@ -362,7 +339,7 @@ class _AddNormLinearFP8Fn(torch.autograd.Function):
             if need_b:
                 db = gy2.sum(0, dtype=torch.float32).to(ctx.bias_dtype)
             # the norm's backward kernel reads bf16: one rounding of dn, as in the bf16 layers
-            fused = _kernel(x, norm_weight) and fused_cols_ok(C)
+            fused = _kernel(x) and fused_cols_ok(C)
             dn = matmul_fp8_block(*g, wq_t, ws.t(), out_dtype=torch.bfloat16 if fused else torch.float32) if need_n else None
         if need_n:
             if dn is None:
@@ -383,10 +360,9 @@ class _AddNormLinearFP8Fn(torch.autograd.Function):
 
 def _normed_t(x, rstd, weight):
     """The normalised values again, quantised with blocks along the tokens: (elements (C, rows), scales)."""
-    if not _kernel(x, rstd, weight):
+    if not _kernel(x):
         return quantize_ref((x.float() * rstd.view(-1, 1) * weight.float()).t())
-    backend.count_launch()
-    return tuple(backend.require_extension().fp8_quantize(x, 2, rstd, weight.contiguous()))
+    return tuple(_ext().fp8_quantize(x, 2, rstd, weight.contiguous()))
 
 
 def add_rms_norm_linear_fp8(res: torch.Tensor, h: Optional[torch.Tensor], norm_weight: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5,
