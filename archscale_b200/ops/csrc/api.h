@@ -295,12 +295,14 @@ int b200_add_rmsnorm_fp8(const void* res, int res_dtype, const void* h, float h_
 // pair: on SM pairs; scales of A then belong to rows, and scales of rows are stored [block][*_blk], at multiples of 16 bytes.
 int b200_gemm_fp8_block(const void* A, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_blk, int sa_tile, const void* B, int64_t ldb,
                         const float* sb, int64_t sb_row, int64_t sb_blk, int sb_tile, const void* bias, int bias_dtype, void* out, int64_t ldc,
-                        int M, int N, int K, int out_f32, int accumulate, int pair, int num_sms, int* status, cudaStream_t stream);
+                        int M, int N, int K, int out_f32, int accumulate, int pair, void* ws, int num_sms, int* status,
+                        cudaStream_t stream);
 // The same on SM pairs (gemm2_fp8_block.cu), called by the one above with `pair`: scales per row are stored [block][blk],
 // those of B 16-byte aligned.
 int b200_gemm2_fp8_block(const void* A, int64_t lda, const float* sa, int64_t sa_blk, const void* B, int64_t ldb, const float* sb, int64_t sb_row,
                          int64_t sb_blk, int sb_tile, const void* bias, int bias_f32, void* out, int64_t ldc, int M, int N, int K, int out_f32,
-                         int accumulate, int nt, int num_sms, int* status, cudaStream_t stream);
+                         int accumulate, void* ws, int num_sms, int* status, cudaStream_t stream);
+int64_t b200_gemm2_fp8_block_workspace(int M, int N, int K, int num_sms);      // bytes
 
 #ifdef __cplusplus
 }

@@ -9,9 +9,16 @@
 // multiply-adds on them (two warps share a scheduler: 256 cycles of the 512 that the products take), and everything that stands beside these
 // in its one chain of instructions adds to the block's time.  Hence: the row's scales of eight blocks are loaded together (the wait for them is
 // paid once in eight; fetched block by block through a TMA ring, as the operands are, they cost 150 cycles a block), scales of 128 rows of B
-// are folded into them there, and only scales per row of B go through shared memory (copied asynchronously, each warp its own columns).
+// are folded into them there.  Scales per row of B make two operations of every multiply-add and go through shared memory (copied
+// asynchronously, each warp its own rows and columns); there a warp reads its accumulator in the shape that gives a thread 4 rows × 32 columns
+// instead of one row × 128: with a row per thread, 32 broadcast reads of 16 bytes per block and warp kept the shared memory's port busy for
+// twice the time of the products.
 // Loads, products and their commits are issued by one elected lane of a converged warp: four loads a block from a branch of one lane
 // took longer than the block's products.  Two half-width streams with an MMA warp each read operands twice and were slower.
+//
+// Tiles that do not fill a last wave of pairs are split along K over the pairs that would be idle.  Each part's sums go to a workspace, and the
+// warp that finds itself the last of a region's parts (a counter per region) adds all of them, in the order of K, and stores: nobody waits, and
+// the result does not depend on who came last.
 //
 // 384 threads: warp 0 TMA, warp 1 MMA (leader CTA), warps 4..11 sums (two warps per lane quarter, one per half of the columns).  A sums
 // thread holds 128 sums and 64 values on their way from tensor memory: the first warpgroup gives it registers (56 + 224 + 224 = 3 · 168).
@@ -29,7 +36,8 @@ template <int NT, bool BTILE>
 struct F2 {
   static constexpr int A_BYTES = 128 * F2_BK, B_BYTES = NT / 2 * F2_BK, STAGE = A_BYTES + B_BYTES;
   static constexpr int STAGES = NT == 256 ? 5 : 7;
-  static constexpr int SV = BTILE ? 0 : F2_RING * NT / 2 * 4;      // bytes of B's scales per warp
+  static constexpr int SLOT = NT / 2 * 4 + 128;                    // scales of a block: a warp's columns, then its rows
+  static constexpr int SV = BTILE ? 0 : F2_RING * SLOT;
   static constexpr int SMEM = STAGES * STAGE + 8 * (F2_PIECE + SV) + 1024 + 256;
 };
 
@@ -40,6 +48,9 @@ struct F2Params {
   int64_t ldc, sa_blk, sb_row, sb_blk;
   int M, N, K;
   int out_f32, accumulate, bias_f32, tma_out;
+  int whole, splits, per;          // tiles computed whole; parts of each of the others and their blocks of K
+  float* ws;                       // [part][CTA of the pair][warp][column][32 rows] sums of the parts
+  int* arrived;                    // [split tile][CTA][warp] parts that have arrived
   int* status;
 };
 
@@ -66,6 +77,23 @@ __device__ __forceinline__ void f2_ld_wait(uint32_t (&r)[32]) {
 
 __device__ __forceinline__ void f2_cp_async16(uint32_t dst, const float* src, int bytes) {      // what is past `bytes` is zero
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void f2_cp_async4(uint32_t dst, const float* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// 16 lanes × 64 fp32 columns → 32 registers: thread t has columns 8 i + 2 (t % 4) + {0, 1} of rows t / 4 (registers 4 i, 4 i + 1) and
+// t / 4 + 8 (4 i + 2, 4 i + 3).
+__device__ __forceinline__ void f2_ld_16x64(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
 }
 __device__ __forceinline__ void f2_tma_add_2d(const CUtensorMap* map, const void* smem_src, int x, int y) {
   asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
@@ -110,8 +138,8 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
   const int rank = static_cast<int>(cluster_ctarank());
   const int pair = static_cast<int>(blockIdx.x) >> 1, n_pair = static_cast<int>(gridDim.x) >> 1;
   const int num_m = (p.M + 255) / 256, num_n = (p.N + NT - 1) / NT;
-  const int num_tiles = num_m * num_n;
-  const int num_kb = (p.K + F2_BK - 1) / F2_BK;
+  const int all_kb = (p.K + F2_BK - 1) / F2_BK;
+  const int num_units = p.whole + (num_m * num_n - p.whole) * p.splits;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < T::STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
@@ -128,7 +156,15 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
 
-  auto tile_coords = [&](int t, int& m0, int& n0) {
+  // work of a pair: a tile, or (past the whole ones) one of the parts of a tile along K
+  auto unit = [&](int u, int& m0, int& n0, int& kb0, int& kb1) {
+    int t = u;
+    kb0 = 0; kb1 = all_kb;
+    if (u >= p.whole) {
+      const int v = u - p.whole, part = v % p.splits;
+      t = p.whole + v / p.splits;
+      kb0 = part * p.per; kb1 = min(kb0 + p.per, all_kb);
+    }
     const int per_group = F2_GROUP_M * num_n;
     const int g = t / per_group, first_m = g * F2_GROUP_M;
     const int gsz = min(num_m - first_m, F2_GROUP_M);
@@ -140,10 +176,10 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
   if (warp == 0) {                                     // converged: a load from inside a branch of one lane takes longer to issue
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     int stage = 0; uint32_t phase = 0;
-    for (int t = pair; t < num_tiles; t += n_pair) {
-      int m0, n0; tile_coords(t, m0, n0);
+    for (int u = pair; u < num_units; u += n_pair) {
+      int m0, n0, kb0, kb1; unit(u, m0, n0, kb0, kb1);
       const int ma = m0 + rank * 128, nb = n0 + rank * (NT / 2);
-      for (int kb = 0; kb < num_kb; ++kb) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         if (!mbar_wait_warp(&empty_bar[stage], phase ^ 1, abort_flag, p.status, STATUS_TIMEOUT_EMPTY)) goto done;
         uint8_t* sa = smem + stage * T::STAGE;
         if (elect_one_sync()) {
@@ -160,8 +196,9 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
       // e4m3 × e4m3, fp32 accumulate, both operands K-major
       constexpr uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(NT >> 3) << 17) | (static_cast<uint32_t>(256 >> 4) << 24);
       int stage = 0; uint32_t phase = 0, it = 0;
-      for (int t = pair; t < num_tiles; t += n_pair) {
-        for (int kb = 0; kb < num_kb; ++kb, ++it) {
+      for (int u = pair; u < num_units; u += n_pair) {
+        int m0, n0, kb0, kb1; unit(u, m0, n0, kb0, kb1);
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int acc = it & 1; const uint32_t acc_phase = (it >> 1) & 1;
           if (!mbar_wait_warp(&full_bar[stage], phase, abort_flag, p.status, STATUS_TIMEOUT_FULL)) goto done;
           if (!mbar_wait_warp(&tmem_empty[acc], acc_phase ^ 1, abort_flag, p.status, STATUS_TIMEOUT_TMEM_EMPTY)) goto done;
@@ -187,17 +224,19 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     uint8_t* piece = pieces + (warp - 4) * F2_PIECE;
     uint8_t* sv = svs + (warp - 4) * T::SV;
     uint32_t it = 0;
-    for (int t = pair; t < num_tiles; t += n_pair) {
-      int m0, n0; tile_coords(t, m0, n0);
+    for (int u = pair; u < num_units; u += n_pair) {
+      int m0, n0, kb0, kb1; unit(u, m0, n0, kb0, kb1);
       const int row0 = m0 + rank * 128 + q * 32, c0 = n0 + half * W;
       const float* sa = p.sa + min(row0 + lane, p.M - 1);
       const float* sb = BTILE ? p.sb + static_cast<int64_t>(min(c0, p.N - 1) >> 7) * p.sb_row : p.sb + min(c0 + 4 * lane, (p.N - 1) & ~3);
-      // scales of B's rows: each lane copies four columns of a block
+      // scales per row of both: each lane copies four columns and one row of a block
       const int sv_bytes = BTILE || lane >= W / 4 ? 0 : max(min(p.N - c0 - 4 * lane, 4), 0) * 4;
       auto copy_sv = [&](int kb) {
         if (!BTILE) {
-          if (lane < W / 4)
-            f2_cp_async16(smem_u32(sv + (kb % F2_RING) * (W * 4) + lane * 16), sb + min(kb, num_kb - 1) * p.sb_blk, kb < num_kb ? sv_bytes : 0);
+          const uint32_t slot = smem_u32(sv + (kb % F2_RING) * T::SLOT);
+          const int k = min(kb, kb1 - 1);
+          if (lane < W / 4) f2_cp_async16(slot + lane * 16, sb + k * p.sb_blk, kb < kb1 ? sv_bytes : 0);
+          f2_cp_async4(slot + W * 4 + lane * 4, sa + k * p.sa_blk, kb < kb1 ? 4 : 0);
           asm volatile("cp.async.commit_group;" ::: "memory");
         }
       };
@@ -205,74 +244,127 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
 #pragma unroll
       for (int i = 0; i < W; ++i) sum[i] = 0.f;
 #pragma unroll
-      for (int j = 0; j < F2_RING - 1; ++j) copy_sv(j);
-      for (int kb = 0; kb < num_kb; ++kb, ++it) {
+      for (int j = 0; j < F2_RING - 1; ++j) copy_sv(kb0 + j);
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int acc = it & 1; const uint32_t acc_phase = (it >> 1) & 1;
         const uint32_t taddr = tmem_base + acc * NT + half * W + (static_cast<uint32_t>(q * 32) << 16);
-        if ((kb & 7) == 0) {                           // the row's scales of eight blocks
+        if constexpr (BTILE) {
+          const int g = (kb - kb0) & 7;
+          if (g == 0) {                                // the row's scales of eight blocks
 #pragma unroll
-          for (int j = 0; j < 8; ++j) scale[j] = sa[min(kb + j, num_kb - 1) * p.sa_blk];
-          if (BTILE) {
-            const float b = sb[min(kb + (lane & 7), num_kb - 1) * p.sb_blk];
+            for (int j = 0; j < 8; ++j) scale[j] = sa[min(kb + j, kb1 - 1) * p.sa_blk];
+            const float b = sb[min(kb + (lane & 7), kb1 - 1) * p.sb_blk];
 #pragma unroll
             for (int j = 0; j < 8; ++j) scale[j] *= __shfl_sync(0xffffffffu, b, j);
           }
-        }
-        const float s01 = (kb & 1) ? scale[1] : scale[0], s23 = (kb & 1) ? scale[3] : scale[2];
-        const float s45 = (kb & 1) ? scale[5] : scale[4], s67 = (kb & 1) ? scale[7] : scale[6];
-        const float f = (kb & 4) ? ((kb & 2) ? s67 : s45) : ((kb & 2) ? s23 : s01);
-        if (!mbar_wait_warp(&tmem_full[acc], acc_phase, abort_flag, p.status, STATUS_TIMEOUT_TMEM_FULL)) goto done;
-        tc_fence_after();
-        uint32_t r[2][32];
-        tmem_ld_32x32(taddr, r[0]);
-        if (!BTILE) {                                  // block kb has arrived; its slot's predecessor was read by every lane
-          copy_sv(kb + F2_RING - 1);
-          asm volatile("cp.async.wait_group %0;" ::"n"(F2_RING - 1) : "memory");
-          __syncwarp();
-        }
-        const float4* bv = reinterpret_cast<const float4*>(sv + (kb % F2_RING) * (W * 4));
+          const float s01 = (g & 1) ? scale[1] : scale[0], s23 = (g & 1) ? scale[3] : scale[2];
+          const float s45 = (g & 1) ? scale[5] : scale[4], s67 = (g & 1) ? scale[7] : scale[6];
+          const float f = (g & 4) ? ((g & 2) ? s67 : s45) : ((g & 2) ? s23 : s01);
+          if (!mbar_wait_warp(&tmem_full[acc], acc_phase, abort_flag, p.status, STATUS_TIMEOUT_TMEM_FULL)) goto done;
+          tc_fence_after();
+          uint32_t r[2][32];
+          tmem_ld_32x32(taddr, r[0]);
 #pragma unroll
-        for (int c = 0; c < W / 32; ++c) {
-          f2_ld_wait(r[c & 1]);
-          if (c + 1 < W / 32) {
-            tmem_ld_32x32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
-          } else {                                     // the last columns are in registers: the accumulator is free
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_leader(&tmem_empty[acc]);
-          }
-          const uint32_t (&w)[32] = r[c & 1];
-          float* o = sum + c * 32;
-          if (BTILE) {
+          for (int c = 0; c < W / 32; ++c) {
+            f2_ld_wait(r[c & 1]);
+            if (c + 1 < W / 32) {
+              tmem_ld_32x32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
+            } else {                                   // the last columns are in registers: the accumulator is free
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_leader(&tmem_empty[acc]);
+            }
+            const uint32_t (&w)[32] = r[c & 1];
+            float* o = sum + c * 32;
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = fmaf(__uint_as_float(w[i]), f, o[i]);
-          } else {
+          }
+        } else {                                       // piece c: columns 64 (c / 2) .., rows 16 (c % 2) ..
+          if (!mbar_wait_warp(&tmem_full[acc], acc_phase, abort_flag, p.status, STATUS_TIMEOUT_TMEM_FULL)) goto done;
+          tc_fence_after();
+          uint32_t r[2][32];
+          f2_ld_16x64(taddr, r[0]);
+          copy_sv(kb + F2_RING - 1);                   // into the slot of block kb - 1, which every lane has read
+          asm volatile("cp.async.wait_group %0;" ::"n"(F2_RING - 1) : "memory");
+          __syncwarp();                                // block kb has arrived
+          const float* slot = reinterpret_cast<const float*>(sv + (kb % F2_RING) * T::SLOT);
+          float fa[4];
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 b = bv[c * 8 + i / 4];
-              const float2 f2 = make_float2(f, f);
-              const float2 x = fma_f32x2(mul_f32x2(make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1])), make_float2(b.x, b.y)), f2,
-                                         make_float2(o[i], o[i + 1]));
-              const float2 y = fma_f32x2(mul_f32x2(make_float2(__uint_as_float(w[i + 2]), __uint_as_float(w[i + 3])), make_float2(b.z, b.w)), f2,
-                                         make_float2(o[i + 2], o[i + 3]));
-              o[i] = x.x; o[i + 1] = x.y; o[i + 2] = y.x; o[i + 3] = y.y;
+          for (int j = 0; j < 4; ++j) fa[j] = slot[W + j * 8 + (lane >> 2)];
+          float2 fb[8];
+#pragma unroll
+          for (int c = 0; c < W / 32; ++c) {
+            if ((c & 1) == 0) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) fb[i] = *reinterpret_cast<const float2*>(slot + (c >> 1) * 64 + i * 8 + (lane & 3) * 2);
+            }
+            f2_ld_wait(r[c & 1]);
+            if (c + 1 < W / 32) {
+              f2_ld_16x64(taddr + ((c + 1) >> 1) * 64 + (static_cast<uint32_t>(((c + 1) & 1) * 16) << 16), r[(c + 1) & 1]);
+            } else {
+              tc_fence_before();
+              __syncwarp();                            // (every lane has read its scales, too)
+              if (lane == 0) mbar_arrive_leader(&tmem_empty[acc]);
+            }
+            const uint32_t (&w)[32] = r[c & 1];
+            float* o = sum + c * 32;
+            const float2 f0 = make_float2(fa[(c & 1) * 2], fa[(c & 1) * 2]), f1 = make_float2(fa[(c & 1) * 2 + 1], fa[(c & 1) * 2 + 1]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float2 x = fma_f32x2(mul_f32x2(make_float2(__uint_as_float(w[4 * i]), __uint_as_float(w[4 * i + 1])), fb[i]), f0,
+                                         make_float2(o[4 * i], o[4 * i + 1]));
+              const float2 y = fma_f32x2(mul_f32x2(make_float2(__uint_as_float(w[4 * i + 2]), __uint_as_float(w[4 * i + 3])), fb[i]), f1,
+                                         make_float2(o[4 * i + 2], o[4 * i + 3]));
+              o[4 * i] = x.x; o[4 * i + 1] = x.y; o[4 * i + 2] = y.x; o[4 * i + 3] = y.y;
             }
           }
         }
-        if (!BTILE) __syncwarp();                      // every lane has read its slot
       }
       if (!BTILE) asm volatile("cp.async.wait_group 0;" ::: "memory");      // copies past the last block (of zeros)
+      if (u >= p.whole) {                              // one of the parts of a tile
+        const int v = u - p.whole, w = rank * 8 + warp - 4;
+        float* mine = p.ws + (static_cast<int64_t>(v) * 16 + w) * (W * 32) + lane;
+#pragma unroll
+        for (int i = 0; i < W; ++i) __stcg(mine + i * 32, sum[i]);
+        __threadfence();
+        __syncwarp();
+        int before = 0;
+        if (lane == 0) before = atomicAdd(p.arrived + v / p.splits * 16 + w, 1);
+        if (__shfl_sync(0xffffffffu, before, 0) != p.splits - 1) continue;
+        __threadfence();
+        const float* part = p.ws + (static_cast<int64_t>(v / p.splits * p.splits) * 16 + w) * (W * 32) + lane;
+#pragma unroll
+        for (int i = 0; i < W; ++i) sum[i] = __ldcg(part + i * 32);
+        for (int s = 1; s < p.splits; ++s) {
+          part += 16 * W * 32;
+#pragma unroll
+          for (int i = 0; i < W; ++i) sum[i] += __ldcg(part + i * 32);
+        }
+      }
       if (p.bias) {
 #pragma unroll
         for (int c = 0; c < W / 32; ++c) {
           const int col = min(c0 + c * 32 + lane, p.N - 1);
           const float b = p.bias_f32 ? static_cast<const float*>(p.bias)[col] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col]);
+          if (BTILE) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) sum[c * 32 + i] += __shfl_sync(0xffffffffu, b, i);
+            for (int i = 0; i < 32; ++i) sum[c * 32 + i] += __shfl_sync(0xffffffffu, b, i);
+          } else {                                     // columns 32 (c % 2) .. of pieces c / 2 · 2 and the one after
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float v = __shfl_sync(0xffffffffu, b, i * 8 + (lane & 3) * 2 + e);
+                float* o = sum + (c >> 1) * 64 + (c & 1) * 16 + i * 4 + e;
+                o[0] += v; o[2] += v; o[32] += v; o[34] += v;
+              }
+            }
+          }
         }
       }
       // pieces of 32 rows × 128 bytes: 16-byte parts at part ^ (row % 8), the order of the output's tensor map
       auto part = [&](int j) { return reinterpret_cast<uint4*>(piece + lane * 128 + ((j ^ (lane & 7)) << 4)); };
+      auto frag = [&](int g, int j) { return piece + (g * 8 + (lane >> 2)) * 128 + ((j ^ (lane >> 2)) << 4); };      // part j of row 8 g + lane / 4
       if (p.tma_out && !p.out_f32) {
 #pragma unroll
         for (int c = 0; c < W / 64; ++c) {
@@ -280,8 +372,16 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float* v = sum + c * 64 + j * 8;
-            *part(j) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+            if (BTILE) {
+              const float* v = sum + c * 64 + j * 8;
+              *part(j) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+            } else {
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {            // rows 8 g + lane / 4
+                const float* v = sum + c * 64 + (g >> 1) * 32 + j * 4 + (g & 1) * 2;
+                *reinterpret_cast<uint32_t*>(frag(g, j) + (lane & 3) * 4) = pack_bf16x2(v[0], v[1]);
+              }
+            }
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -294,8 +394,16 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float* v = sum + c * 32 + j * 4;
-            *part(j) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+            if (BTILE) {
+              const float* v = sum + c * 32 + j * 4;
+              *part(j) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+            } else if (j < 4) {
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const float* v = sum + (c >> 1) * 64 + (g >> 1) * 32 + (c & 1) * 16 + j * 4 + (g & 1) * 2;
+                *reinterpret_cast<float2*>(frag(g, 2 * j + ((lane & 3) >> 1)) + (lane & 1) * 8) = make_float2(v[0], v[1]);
+              }
+            }
           }
           if (p.tma_out) {
             fence_proxy_async_smem();
@@ -363,22 +471,73 @@ static int launch_f2(const void* A, int64_t lda, const void* B, int64_t ldb, con
   auto kern = gemm2_fp8_block_kernel<NT, BTILE>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM) != cudaSuccess) return -2;
   const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + NT - 1) / NT);
-  if (tiles > 0x3fffffff) return -6;
+  const int64_t units = p.whole + (tiles - p.whole) * p.splits;
+  if (units > 0x3fffffff) return -6;
+  if (p.splits > 1 && cudaMemsetAsync(p.arrived, 0, (tiles - p.whole) * 16 * sizeof(int), st) != cudaSuccess) return -4;
   const int pairs = num_sms / 2;
-  kern<<<2 * (tiles < pairs ? static_cast<int>(tiles) : pairs), F2_THREADS, T::SMEM, st>>>(ta, tb, to, p);
+  kern<<<2 * (units < pairs ? static_cast<int>(units) : pairs), F2_THREADS, T::SMEM, st>>>(ta, tb, to, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
 }  // namespace b200
 
+// How a product is laid over the pairs of SMs: the width of its tiles, and the split of those that do not fill a last wave.
+namespace b200 {
+struct F2Plan { int nt, whole, splits, per; int64_t ws_floats; int counters; };
+static F2Plan f2_plan(int M, int N, int K, int num_sms) {
+  const int pairs = num_sms / 2, num_kb = (K + F2_BK - 1) / F2_BK;
+  F2Plan best{};
+  double best_cost = 0;
+  for (int nt = 256; nt >= 128; nt /= 2) {
+    const int64_t tiles = static_cast<int64_t>((M + 255) / 256) * ((N + nt - 1) / nt);
+    const int rest = static_cast<int>(tiles % pairs);
+    // in blocks of 256 columns: a block of 128 columns takes 0.62 of the time; a tile's set-up and end take 4 blocks, the sums of a split tile
+    // (written, counted and read again) 10 and 3 per part: 2048 × 5632 × 16384 294 µs whole, 257 with its last tiles split, 1024 × 1024 × 16384 81 and 53, but
+    // 700 × 7680 × 2560 33 and 35, 16384 × 5632 × 2048 190 and 199, 128 × 2048 × 5632 25 and 29
+    const double blk = nt == 256 ? 1.0 : 0.62, tile = num_kb * blk + 4;
+    int splits = 1, per = num_kb;
+    double last = rest ? tile : 0;
+    if (rest) {
+      int s = pairs / rest;
+      s = s < 8 ? s : 8;
+      s = s < num_kb / 2 ? s : num_kb / 2;
+      if (s > 1) {
+        const int pk = (num_kb + s - 1) / s;
+        s = (num_kb + pk - 1) / pk;
+        const double split = pk * blk + 4 + 10 + 3 * s;
+        if (split < last) { last = split; splits = s; per = pk; }
+      }
+    }
+    const double cost = static_cast<double>(tiles / pairs) * tile + last;
+    if (nt == 256 || cost < best_cost) {
+      const int64_t parts = splits > 1 ? static_cast<int64_t>(rest) * splits : 0;
+      best = F2Plan{nt, static_cast<int>(splits > 1 ? tiles - rest : tiles), splits, per, parts * 256 * nt, splits > 1 ? rest * 16 : 0};
+      best_cost = cost;
+    }
+  }
+  return best;
+}
+}  // namespace b200
+
+// Bytes of workspace that b200_gemm2_fp8_block needs for these sizes (0: none).
+extern "C" int64_t b200_gemm2_fp8_block_workspace(int M, int N, int K, int num_sms) {
+  const b200::F2Plan plan = b200::f2_plan(M, N, K, num_sms);
+  return plan.ws_floats * 4 + plan.counters * 4;
+}
+
 // Contract of b200_gemm_fp8_block, which checks the arguments and calls this: scales of A are per row, those of B per row or (sb_tile) per 128
-// rows; scales per row are stored [block][*_blk], those of B 16-byte aligned.
+// rows; scales per row are stored [block][*_blk], those of B 16-byte aligned.  ws: the bytes that b200_gemm2_fp8_block_workspace names.
 extern "C" int b200_gemm2_fp8_block(const void* A, int64_t lda, const float* sa, int64_t sa_blk, const void* B, int64_t ldb, const float* sb,
                                     int64_t sb_row, int64_t sb_blk, int sb_tile, const void* bias, int bias_f32, void* out, int64_t ldc, int M,
-                                    int N, int K, int out_f32, int accumulate, int nt, int num_sms, int* status, cudaStream_t stream) {
+                                    int N, int K, int out_f32, int accumulate, void* ws, int num_sms, int* status, cudaStream_t stream) {
   using namespace b200;
   const int tma_out = ldc * (out_f32 ? 4 : 2) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 ? 1 : 0;
-  const F2Params p{out, bias, sa, sb, ldc, sa_blk, sb_row, sb_blk, M, N, K, out_f32, accumulate, bias_f32, tma_out, status};
-  if (nt == 256) return sb_tile ? launch_f2<256, true>(A, lda, B, ldb, p, num_sms, stream) : launch_f2<256, false>(A, lda, B, ldb, p, num_sms, stream);
+  const F2Plan plan = f2_plan(M, N, K, num_sms);
+  if (plan.splits > 1 && !ws) return -6;
+  float* sums = static_cast<float*>(ws);
+  const F2Params p{out, bias, sa, sb, ldc, sa_blk, sb_row, sb_blk, M, N, K, out_f32, accumulate, bias_f32, tma_out, plan.whole, plan.splits,
+                   plan.per, sums, reinterpret_cast<int*>(sums + plan.ws_floats), status};
+  if (plan.nt == 256)
+    return sb_tile ? launch_f2<256, true>(A, lda, B, ldb, p, num_sms, stream) : launch_f2<256, false>(A, lda, B, ldb, p, num_sms, stream);
   return sb_tile ? launch_f2<128, true>(A, lda, B, ldb, p, num_sms, stream) : launch_f2<128, false>(A, lda, B, ldb, p, num_sms, stream);
 }

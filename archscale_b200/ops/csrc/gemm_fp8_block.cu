@@ -24,7 +24,8 @@ constexpr int FS_BN = 128, FS_BK = 128, FS_STAGES = 4, FS_THREADS = 192, FS_CHUN
 template <int BT>
 struct FS {
   static constexpr int B_BYTES = FS_BN * FS_BK, A_BYTES = BT * FS_BK, STAGE = B_BYTES + A_BYTES;
-  static constexpr int TMEM = 2 * BT < 32 ? 32 : 2 * BT;
+  static constexpr int ACC = BT <= 32 ? 8 : BT == 64 ? 4 : 2;      // accumulators: products run ahead of the sums
+  static constexpr int TMEM = ACC * BT;
   static constexpr int SMEM = FS_STAGES * STAGE + FS_CHUNK * BT * 4 + 1024 + 256;
   static_assert(BT * FS_BN * 4 <= FS_STAGES * STAGE, "the sums take the place of the stages");
 };
@@ -74,9 +75,9 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   uint64_t* bars = reinterpret_cast<uint64_t*>(table + FS_CHUNK * BT);
   uint64_t* full_bar = bars;
   uint64_t* empty_bar = bars + FS_STAGES;
-  uint64_t* tmem_full = bars + 2 * FS_STAGES;          // [2]
-  uint64_t* tmem_empty = bars + 2 * FS_STAGES + 2;     // [2], four warps
-  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(bars + 2 * FS_STAGES + 4);
+  uint64_t* tmem_full = bars + 2 * FS_STAGES;          // [ACC]
+  uint64_t* tmem_empty = tmem_full + T::ACC;           // [ACC], four warps
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(tmem_empty + T::ACC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = S > 1 ? static_cast<int>(cluster_ctarank()) : 0;
@@ -93,7 +94,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   };
   if (threadIdx.x == 0) {
     for (int s = 0; s < FS_STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(&tmem_full[a], 1); mbar_init(&tmem_empty[a], 4); }
+    for (int a = 0; a < T::ACC; ++a) { mbar_init(&tmem_full[a], 1); mbar_init(&tmem_empty[a], 4); }
     *abort_flag = 0;
     mbar_fence_init();
     fence_proxy_async_smem();
@@ -116,7 +117,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     constexpr uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(BT >> 3) << 17) | (static_cast<uint32_t>(FS_BN >> 4) << 24);
     for (int i = 0; i < nkb; ++i) {
       const int st = i % FS_STAGES; const uint32_t ph = (i / FS_STAGES) & 1;
-      const int acc = i & 1; const uint32_t aph = (i >> 1) & 1;
+      const int acc = i % T::ACC; const uint32_t aph = (i / T::ACC) & 1;
       if (!mbar_wait_warp(&full_bar[st], ph, abort_flag, p.status, STATUS_TIMEOUT_FULL)) break;
       if (!mbar_wait_warp(&tmem_empty[acc], aph ^ 1, abort_flag, p.status, STATUS_TIMEOUT_TMEM_EMPTY)) break;
       tc_fence_after();
@@ -139,7 +140,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     for (int i = 0; i < BT; ++i) sum[i] = 0.f;
     bool ok = true;
     for (int i = 0; i < nkb; ++i) {
-      const int acc = i & 1; const uint32_t aph = (i >> 1) & 1;
+      const int acc = i % T::ACC; const uint32_t aph = (i / T::ACC) & 1;
       if (i % FS_CHUNK == 0) {                         // scales of A of the next blocks: the same for all rows of B
         asm volatile("bar.sync 1, 128;" ::: "memory");
         const int blocks = min(FS_CHUNK, nkb - i);
@@ -276,10 +277,11 @@ static int launch_fs(const void* A, int64_t lda, const void* B, int64_t ldb, con
 
 // A [M, K], B [N, K]: e4m3, rows lda / ldb bytes apart (multiples of 16, as the addresses).  sa, sb: scales with strides between rows
 // (or groups of 128 rows: *_tile) and between blocks of 128 along K.  out [M, N] fp32 (accumulate: added to) or bf16; bias [N] or null.
+// pair: on SM pairs, with the workspace that b200_gemm2_fp8_block_workspace names.
 extern "C" int b200_gemm_fp8_block(const void* A, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_blk, int sa_tile, const void* B,
                                    int64_t ldb, const float* sb, int64_t sb_row, int64_t sb_blk, int sb_tile, const void* bias, int bias_dtype,
-                                   void* out, int64_t ldc, int M, int N, int K, int out_f32, int accumulate, int pair, int num_sms, int* status,
-                                   cudaStream_t stream) {
+                                   void* out, int64_t ldc, int M, int N, int K, int out_f32, int accumulate, int pair, void* ws, int num_sms,
+                                   int* status, cudaStream_t stream) {
   using namespace b200;
   if (M < 0 || N < 0 || K < 1 || lda % 16 || ldb % 16 || (accumulate && !out_f32)) return -6;
   if (M == 0 || N == 0) return 0;
@@ -292,11 +294,8 @@ extern "C" int b200_gemm_fp8_block(const void* A, int64_t lda, const float* sa, 
   if (pair) {
     const auto rows = [](const float* s, int64_t row, int64_t blk) { return row == 1 && blk % 4 == 0 && reinterpret_cast<uintptr_t>(s) % 16 == 0; };
     if (sa_tile || sa_row != 1 || (!sb_tile && !rows(sb, sb_row, sb_blk))) return -6;
-    const int64_t m = (M + 255) / 256, pairs = num_sms / 2;
-    // tiles of half the width take 0.62 of the time: narrower where that saves enough of the last wave
-    const int64_t wide = (m * ((N + 255) / 256) + pairs - 1) / pairs * 100, narrow = (m * ((N + 127) / 128) + pairs - 1) / pairs * 62;
     return b200_gemm2_fp8_block(A, lda, sa, sa_blk, B, ldb, sb, sb_row, sb_blk, sb_tile, bias, bias_dtype == 0 ? 1 : 0, out, ldc, M, N, K, out_f32,
-                                accumulate, narrow < wide ? 128 : 256, num_sms, status, stream);
+                                accumulate, ws, num_sms, status, stream);
   }
   const FsParams p{out, bias, {sa, sa_row, sa_blk, sa_tile ? 7 : 0}, {sb, sb_row, sb_blk, sb_tile ? 7 : 0}, M, N, K, ldc, out_f32, accumulate,
                    bias_dtype == 0 ? 1 : 0, ldc % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0 ? 1 : 0, status};
