@@ -13,21 +13,24 @@
 // first loads are issued before tensor memory is allocated.  The CTAs' sums meet in shared memory, in the place of the stages; every CTA
 // adds its share of the rows over the ranks in rank order (distributed shared memory), so a result does not depend on scheduling.
 //
-// 192 threads: warp 0 TMA, warp 1 MMA, warps 2..5 sums (thread = row of B, BT sums); all of them add.
+// Warp 0 TMA, warp 1 MMA, then four warps of sums for every 32 rows of A (thread = row of B, up to 32 sums); all of them add.
 #include "api.h"
 #include "sm100.cuh"
 
 namespace b200 {
 
-constexpr int FS_BN = 128, FS_BK = 128, FS_STAGES = 4, FS_THREADS = 192, FS_CHUNK = 32;
+constexpr int FS_BN = 128, FS_BK = 128, FS_CHUNK = 32;
 
 template <int BT>
 struct FS {
   static constexpr int B_BYTES = FS_BN * FS_BK, A_BYTES = BT * FS_BK, STAGE = B_BYTES + A_BYTES;
+  static constexpr int STAGES = BT == 16 ? 6 : BT == 32 ? 5 : 4;        // two CTAs fit an SM (BT 128: one)
   static constexpr int ACC = BT <= 32 ? 8 : BT == 64 ? 4 : 2;      // accumulators: products run ahead of the sums
   static constexpr int TMEM = ACC * BT;
-  static constexpr int SMEM = FS_STAGES * STAGE + FS_CHUNK * BT * 4 + 1024 + 256;
-  static_assert(BT * FS_BN * 4 <= FS_STAGES * STAGE, "the sums take the place of the stages");
+  static constexpr int W = BT < 32 ? BT : 32, GROUPS = BT / W;     // sums of a thread; teams of four warps
+  static constexpr int SUMMERS = 128 * GROUPS, THREADS = 64 + SUMMERS;
+  static constexpr int SMEM = STAGES * STAGE + FS_CHUNK * BT * 4 + 1024 + 256;
+  static_assert(BT * FS_BN * 4 <= STAGES * STAGE, "the sums take the place of the stages");
 };
 
 struct Fp8Scale {
@@ -64,19 +67,19 @@ __device__ __forceinline__ float4 fs_ld_cluster(uint32_t smem_addr, int rank) {
 }
 
 template <int BT, int S>
-__global__ void __launch_bounds__(FS_THREADS, BT <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(FS<BT>::THREADS, BT <= 64 ? 2 : 1)
 gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const FsParams p) {
   using T = FS<BT>;
-  constexpr int PC = BT < 32 ? BT : 32;                // columns that a load from tensor memory brings
+  constexpr int W = T::W;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* part = reinterpret_cast<float*>(smem);        // [BT][128] sums of this CTA, once the stages are read
-  float* table = reinterpret_cast<float*>(smem + FS_STAGES * T::STAGE);      // [FS_CHUNK][BT] scales of A
+  float* table = reinterpret_cast<float*>(smem + T::STAGES * T::STAGE);      // [FS_CHUNK][BT] scales of A
   uint64_t* bars = reinterpret_cast<uint64_t*>(table + FS_CHUNK * BT);
   uint64_t* full_bar = bars;
-  uint64_t* empty_bar = bars + FS_STAGES;
-  uint64_t* tmem_full = bars + 2 * FS_STAGES;          // [ACC]
-  uint64_t* tmem_empty = tmem_full + T::ACC;           // [ACC], four warps
+  uint64_t* empty_bar = bars + T::STAGES;
+  uint64_t* tmem_full = bars + 2 * T::STAGES;          // [ACC]
+  uint64_t* tmem_empty = tmem_full + T::ACC;           // [ACC], the warps of sums
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(tmem_empty + T::ACC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -93,12 +96,12 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     tma_load_2d(sb + T::B_BYTES, &tmap_a, &full_bar[st], (kb0 + i) * FS_BK, m0);
   };
   if (threadIdx.x == 0) {
-    for (int s = 0; s < FS_STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-    for (int a = 0; a < T::ACC; ++a) { mbar_init(&tmem_full[a], 1); mbar_init(&tmem_empty[a], 4); }
+    for (int s = 0; s < T::STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    for (int a = 0; a < T::ACC; ++a) { mbar_init(&tmem_full[a], 1); mbar_init(&tmem_empty[a], 4 * T::GROUPS); }
     *abort_flag = 0;
     mbar_fence_init();
     fence_proxy_async_smem();
-    for (int i = 0; i < FS_STAGES && i < nkb; ++i) load(i, i);      // the ring is empty: no wait, and under the set-up
+    for (int i = 0; i < T::STAGES && i < nkb; ++i) load(i, i);      // the ring is empty: no wait, and under the set-up
   }
   if (warp == 1) { tmem_alloc(tmem_ptr, T::TMEM); tmem_relinquish(); }
   tc_fence_before();
@@ -107,8 +110,8 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
 
   if (warp == 0) {
-    for (int i = FS_STAGES; i < nkb; ++i) {
-      const int st = i % FS_STAGES; const uint32_t ph = (i / FS_STAGES) & 1;
+    for (int i = T::STAGES; i < nkb; ++i) {
+      const int st = i % T::STAGES; const uint32_t ph = (i / T::STAGES) & 1;
       if (!mbar_wait_warp(&empty_bar[st], ph ^ 1, abort_flag, p.status, STATUS_TIMEOUT_EMPTY)) break;
       if (elect_one_sync()) load(i, st);
     }
@@ -116,7 +119,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     // e4m3 × e4m3, fp32 accumulate, both operands K-major
     constexpr uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(BT >> 3) << 17) | (static_cast<uint32_t>(FS_BN >> 4) << 24);
     for (int i = 0; i < nkb; ++i) {
-      const int st = i % FS_STAGES; const uint32_t ph = (i / FS_STAGES) & 1;
+      const int st = i % T::STAGES; const uint32_t ph = (i / T::STAGES) & 1;
       const int acc = i % T::ACC; const uint32_t aph = (i / T::ACC) & 1;
       if (!mbar_wait_warp(&full_bar[st], ph, abort_flag, p.status, STATUS_TIMEOUT_FULL)) break;
       if (!mbar_wait_warp(&tmem_empty[acc], aph ^ 1, abort_flag, p.status, STATUS_TIMEOUT_TMEM_EMPTY)) break;
@@ -132,62 +135,56 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
       }
     }
   } else {
-    const int q = warp & 3, t = threadIdx.x - 64;
+    const int q = warp & 3, t = threadIdx.x - 64, c0 = (warp - 2) / 4 * W;      // lane quarter, first row of A
     const int n = n0 + q * 32 + lane;
     const float* sb = p.sb.p + static_cast<int64_t>(min(n, p.N - 1) >> p.sb.shift) * p.sb.row + kb0 * p.sb.blk;
-    float sum[BT], scale[8];
+    float sum[W], scale[8];
 #pragma unroll
-    for (int i = 0; i < BT; ++i) sum[i] = 0.f;
+    for (int i = 0; i < W; ++i) sum[i] = 0.f;
     bool ok = true;
     for (int i = 0; i < nkb; ++i) {
       const int acc = i % T::ACC; const uint32_t aph = (i / T::ACC) & 1;
-      if (i % FS_CHUNK == 0) {                         // scales of A of the next blocks: the same for all rows of B
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        const int blocks = min(FS_CHUNK, nkb - i);
-        for (int j = t; j < blocks * BT; j += 128) {
-          const int m = m0 + j % BT;
-          table[j] = m < p.M ? p.sa.p[static_cast<int64_t>(m >> p.sa.shift) * p.sa.row + (kb0 + i + j / BT) * p.sa.blk] : 0.f;
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-      }
       if ((i & 7) == 0) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) scale[j] = sb[min(i + j, nkb - 1) * p.sb.blk];
       }
+      if (i % FS_CHUNK == 0) {                         // scales of A of the next blocks: the same for all rows of B
+        if (i) asm volatile("bar.sync 1, %0;" ::"n"(T::SUMMERS) : "memory");
+        const int blocks = min(FS_CHUNK, nkb - i);
+        for (int j = t; j < blocks * BT; j += T::SUMMERS) {
+          const int m = m0 + j % BT;
+          table[j] = m < p.M ? p.sa.p[static_cast<int64_t>(m >> p.sa.shift) * p.sa.row + (kb0 + i + j / BT) * p.sa.blk] : 0.f;
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(T::SUMMERS) : "memory");
+      }
       const float s01 = (i & 1) ? scale[1] : scale[0], s23 = (i & 1) ? scale[3] : scale[2];
       const float s45 = (i & 1) ? scale[5] : scale[4], s67 = (i & 1) ? scale[7] : scale[6];
       const float f = (i & 4) ? ((i & 2) ? s67 : s45) : ((i & 2) ? s23 : s01);
-      const float4* sa = reinterpret_cast<const float4*>(table + i % FS_CHUNK * BT);
+      const float4* sa = reinterpret_cast<const float4*>(table + i % FS_CHUNK * BT + c0);
       ok = mbar_wait_warp(&tmem_full[acc], aph, abort_flag, p.status, STATUS_TIMEOUT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + acc * BT + (static_cast<uint32_t>(q * 32) << 16);
+      uint32_t r[W];
+      const uint32_t taddr = tmem_base + acc * BT + c0 + (static_cast<uint32_t>(q * 32) << 16);
+      if constexpr (W == 32) tmem_ld_32x32(taddr, r);
+      else tmem_ld_32x16(taddr, r);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tmem_empty[acc]);
 #pragma unroll
-      for (int c = 0; c < BT / PC; ++c) {
-        uint32_t r[PC];
-        if constexpr (PC == 32) tmem_ld_32x32(taddr + c * PC, r);
-        else tmem_ld_32x16(taddr + c * PC, r);
-        tmem_ld_wait();
-        if (c + 1 == BT / PC) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&tmem_empty[acc]);
-        }
-#pragma unroll
-        for (int j = 0; j < PC; j += 4) {
-          const float4 a = sa[(c * PC + j) / 4];
-          float* o = sum + c * PC + j;
-          o[0] = fmaf(__uint_as_float(r[j]) * a.x, f, o[0]);
-          o[1] = fmaf(__uint_as_float(r[j + 1]) * a.y, f, o[1]);
-          o[2] = fmaf(__uint_as_float(r[j + 2]) * a.z, f, o[2]);
-          o[3] = fmaf(__uint_as_float(r[j + 3]) * a.w, f, o[3]);
-        }
+      for (int j = 0; j < W; j += 4) {
+        const float4 a = sa[j / 4];
+        sum[j] = fmaf(__uint_as_float(r[j]) * a.x, f, sum[j]);
+        sum[j + 1] = fmaf(__uint_as_float(r[j + 1]) * a.y, f, sum[j + 1]);
+        sum[j + 2] = fmaf(__uint_as_float(r[j + 2]) * a.z, f, sum[j + 2]);
+        sum[j + 3] = fmaf(__uint_as_float(r[j + 3]) * a.w, f, sum[j + 3]);
       }
     }
     // the last products were waited for, so the loads before them have landed and the stages may be written
     if (ok) {
 #pragma unroll
-      for (int i = 0; i < BT; ++i) part[i * FS_BN + q * 32 + lane] = sum[i];
+      for (int i = 0; i < W; ++i) part[(c0 + i) * FS_BN + q * 32 + lane] = sum[i];
     }
   }
   tc_fence_before();
@@ -201,7 +198,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   const int rows = min(p.M - m0, BT), first = rank * BT / S, last = min((rank + 1) * BT / S, rows);
   const int col = n0 + lane * 4;
   const uint32_t part_addr = smem_u32(part);
-  for (int m = first + warp; m < last; m += FS_THREADS / 32) {
+  for (int m = first + warp; m < last; m += T::THREADS / 32) {
     float4 v[S];
 #pragma unroll
     for (int r = 0; r < S; ++r) {
@@ -245,7 +242,7 @@ static int launch_fs(const CUtensorMap& ta, const CUtensorMap& tb, const FsParam
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FS<BT>::SMEM) != cudaSuccess) return -2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tiles * S);
-  cfg.blockDim = dim3(FS_THREADS);
+  cfg.blockDim = dim3(FS<BT>::THREADS);
   cfg.dynamicSmemBytes = FS<BT>::SMEM;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
