@@ -411,6 +411,146 @@ static int launch_norm(const Fp8NormParams& p, cudaStream_t st) {
   return -6;
 }
 
+// ------------------------------------------------------------------ gradients of the norm and the addition
+// With x̂ = x · rstd, t = dn · w:   d_res = g_x + rstd · (t − x̂ · mean(t · x̂)),   d_h = h_scale · d_res,   d_w = Σ_rows dn · x̂.
+// dn is the fp32 output of the product behind the norm: rounded to bf16 it made the sums over rows 1.5 times as far off.
+// Threads hold the columns that they hold in the forward kernel, so that d_w is summed in registers over a block's rows; the blocks' sums meet in
+// a second kernel, in a fixed order.  Bound by memory: 12 bytes per element with a bf16 stream.
+struct Fp8NormBwdParams {
+  const float* dn; const void *x, *gx, *w;
+  const float* rstd;
+  void* dres; __nv_bfloat16* dh;
+  float* dw_part;               // [grid][cols] or null
+  float h_scale;
+  int rows, cols, vec, w_f32;
+};
+
+template <typename T, int PACK, int V, bool VEC>
+__global__ void __launch_bounds__(PACK ? 128 : V > 2 ? 1024 : 512) fp8_norm_bwd_kernel(const Fp8NormBwdParams p) {
+  constexpr int RPC = PACK ? 128 / (PACK ? PACK : 1) : 1;
+  __shared__ float s_sum[2][32];
+  __shared__ float s_dw[PACK ? 128 * V * 8 : 1];
+  const int TPR = PACK ? PACK : blockDim.x, WPR = TPR / 32;
+  const int t = PACK ? threadIdx.x % PACK : threadIdx.x, sub = PACK ? threadIdx.x / PACK : 0;
+  float w[V][8], dw[V][8];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = (t + i * TPR) * 8, n = min(max(p.cols - c, 0), 8);
+    if (p.w_f32) load8<VEC>(static_cast<const float*>(p.w) + c, n, w[i]);
+    else load8<VEC>(static_cast<const __nv_bfloat16*>(p.w) + c, n, w[i]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[i][e] = 0.f;
+  }
+  int it = 0;
+  for (int r0 = blockIdx.x * RPC; r0 < p.rows; r0 += gridDim.x * RPC, ++it) {      // the same number of turns for all threads of a block
+    const int row = r0 + sub;
+    const bool live = row < p.rows;
+    const int64_t base = static_cast<int64_t>(row) * p.cols;
+    Raw8<float> dr[V];
+    Raw8<T> xr[V], gr[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (t + i * TPR) * 8;
+      const int n = live ? min(max(p.cols - c, 0), 8) : 0;
+      load_raw<VEC>(p.dn + base + c, n, dr[i]);
+      load_raw<VEC>(static_cast<const T*>(p.x) + base + c, n, xr[i]);
+      load_raw<VEC>(static_cast<const T*>(p.gx) + base + c, p.gx ? n : 0, gr[i]);
+    }
+    const float rs = live ? p.rstd[row] : 0.f;
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float d[8], x[8];
+      unpack8(dr[i], d); unpack8(xr[i], x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float xhat = x[e] * rs;
+        dot += d[e] * w[i][e] * xhat;
+        dw[i][e] += d[e] * xhat;
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if (WPR > 1) {                                       // two buffers: one barrier per row
+      if ((threadIdx.x & 31) == 0) s_sum[it & 1][threadIdx.x >> 5] = dot;
+      __syncthreads();
+      dot = 0.f;
+      for (int i = 0; i < WPR; ++i) dot += s_sum[it & 1][sub * WPR + i];
+    }
+    const float mean = dot / static_cast<float>(p.cols);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (t + i * TPR) * 8;
+      const int n = live ? min(max(p.cols - c, 0), 8) : 0;
+      float d[8], x[8], g[8];
+      unpack8(dr[i], d); unpack8(xr[i], x); unpack8(gr[i], g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[e] += rs * (d[e] * w[i][e] - x[e] * rs * mean);
+      if (n > 0) {
+        if (p.dres) store8(static_cast<T*>(p.dres) + base + c, n, VEC, g);
+        if (p.dh) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[e] *= p.h_scale;
+          store8(p.dh + base + c, n, VEC, g);
+        }
+      }
+    }
+  }
+  if (!p.dw_part) return;
+  float* out = p.dw_part + static_cast<int64_t>(blockIdx.x) * p.cols;
+  if (PACK) {                                            // the block's rows in order
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s_dw[(i * 8 + e) * 128 + threadIdx.x] = dw[i][e];
+    __syncthreads();
+    if (sub == 0) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          for (int j = 1; j < RPC; ++j) dw[i][e] += s_dw[(i * 8 + e) * 128 + t + j * PACK];
+    }
+  }
+  if (sub == 0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (t + i * TPR) * 8;
+      store8(out + c, min(max(p.cols - c, 0), 8), false, dw[i]);
+    }
+  }
+}
+__global__ void __launch_bounds__(1024) fp8_norm_dw_kernel(const float* __restrict__ part, float* __restrict__ out, int n, int cols) {
+  const float t = column_sum_block(part, n, cols);
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  if (threadIdx.x < 32 && c < cols) out[c] = t;
+}
+
+// Blocks of the backward kernel (and rows of its partial sums): as many as fit the machine at once.
+static int norm_bwd_grid(int rows, int cols, int num_sms) {
+  const int vecs = (cols + 7) / 8, rpc = vecs <= 64 ? 4 : vecs <= 128 ? 2 : 1;
+  const int threads = vecs <= 128 ? 128 : vecs <= 1024 ? (vecs + 63) / 64 * 32 : 1024;
+  const int64_t need = (static_cast<int64_t>(rows) + rpc - 1) / rpc, room = static_cast<int64_t>(num_sms) * max(1, 768 / threads);
+  return static_cast<int>(need < room ? need : room);
+}
+
+template <typename T>
+static int launch_norm_bwd(const Fp8NormBwdParams& p, int grid, cudaStream_t st) {
+  const int vecs = (p.cols + 7) / 8;
+#define FP8_NORM_BWD(PACK, V, BLOCK)                                                                         \
+  {                                                                                                          \
+    if (p.vec) fp8_norm_bwd_kernel<T, PACK, V, true><<<grid, BLOCK, 0, st>>>(p);                             \
+    else fp8_norm_bwd_kernel<T, PACK, V, false><<<grid, BLOCK, 0, st>>>(p);                                  \
+    return cudaGetLastError() == cudaSuccess ? 0 : -3;                                                       \
+  }
+  if (vecs <= 64) FP8_NORM_BWD(32, 2, 128)
+  if (vecs <= 128) FP8_NORM_BWD(64, 2, 128)
+  if (vecs <= 1024) FP8_NORM_BWD(0, 2, (vecs + 63) / 64 * 32)
+  if (vecs <= 4096) FP8_NORM_BWD(0, 4, 1024)
+#undef FP8_NORM_BWD
+  return -6;
+}
+
 }  // namespace b200
 
 // x [rows, cols] (dtype 0 fp32, 1 bf16, rows ldx elements apart).  mode: 1 rows (q, s), 2 columns (qt, st), 3 both, 4 tiles of
@@ -452,4 +592,23 @@ extern "C" int b200_add_rmsnorm_fp8(const void* res, int res_dtype, const void* 
                   w_dtype == 0 ? 1 : 0, x, static_cast<uint8_t*>(q), ldq, s, lds, rstd};
   if (res_dtype == 0) return launch_norm<float, float>(p, stream);
   return x_dtype == 0 ? launch_norm<__nv_bfloat16, float>(p, stream) : launch_norm<__nv_bfloat16, __nv_bfloat16>(p, stream);
+}
+
+// dn fp32, x, gx (or null) of x_dtype, all [rows, cols] dense; dres (x_dtype), dh (bf16), dw (fp32 [cols], with dw_part [grid][cols]): null if not
+// wanted.  grid: b200_add_rmsnorm_fp8_bwd_grid.
+extern "C" int b200_add_rmsnorm_fp8_bwd_grid(int rows, int cols, int num_sms) { return b200::norm_bwd_grid(rows, cols, num_sms); }
+extern "C" int b200_add_rmsnorm_fp8_bwd(const float* dn, const void* x, int x_dtype, const void* gx, const void* w, int w_dtype, const float* rstd,
+                                        void* dres, void* dh, float h_scale, float* dw_part, float* dw, int rows, int cols, int grid,
+                                        cudaStream_t stream) {
+  using namespace b200;
+  if (rows < 0 || cols < 1 || cols > 32768) return -6;
+  if (rows == 0) return dw && cudaMemsetAsync(dw, 0, cols * sizeof(float), stream) != cudaSuccess ? -4 : 0;
+  const auto al = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; };
+  const int vec = cols % 8 == 0 && al(dn) && al(x) && al(gx) && al(w) && al(dres) && al(dh) ? 1 : 0;
+  const Fp8NormBwdParams p{dn, x, gx, w, rstd, dres, static_cast<__nv_bfloat16*>(dh), dw ? dw_part : nullptr, h_scale, rows, cols, vec,
+                           w_dtype == 0 ? 1 : 0};
+  const int rc = x_dtype == 0 ? launch_norm_bwd<float>(p, grid, stream) : launch_norm_bwd<__nv_bfloat16>(p, grid, stream);
+  if (rc || !dw) return rc;
+  fp8_norm_dw_kernel<<<(cols + 31) / 32, 1024, 0, stream>>>(dw_part, dw, grid, cols);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }

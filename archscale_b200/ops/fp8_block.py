@@ -33,7 +33,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import backend
-from .norm import fused_cols_ok
 
 BLOCK, E4M3_MAX, BLOCK_FLOOR = 128, 448.0, 1e-30
 FP8 = torch.float8_e4m3fn
@@ -205,50 +204,49 @@ def linear_fp8_weight(x: Union[torch.Tensor, Quantised], weight: torch.Tensor, s
 
 
 # ------------------------------------------------------------------------------------------------ training
-def _weight_grad(g_t, x_t, weight):
-    """dW from the operands with blocks along the tokens, into ``main_grad`` where the weight carries one."""
+def _layer_forward(x2, weight, bias, out_dtype, want_t):
+    """(y, Wᵀ elements, scales of W, *(xᵀ elements, scales) with ``want_t``)."""
+    if _kernel(x2):
+        backend.count_launch(3)
+        return backend.require_extension().linear_fp8_fwd(x2, weight, bias, out_dtype is torch.float32, want_t)
+    wq, w_t, w_scale = quantize_fp8_weight(weight)
+    q, scale, *x_t = quantize_fp8_block_both(x2) if want_t else quantize_fp8_block(x2)
+    return (matmul_fp8_block(q, scale, wq, w_scale, bias, out_dtype), w_t, w_scale, *x_t)
+
+
+def _layer_backward(gy2, w_t, w_scale, x_t, weight, want_x, x_dtype, want_w):
+    """(dx | None, dW | None); dW goes into ``main_grad`` where the weight carries one.  ``x_t``: (elements, scales) of xᵀ."""
     main_grad = getattr(weight, "main_grad", None)
-    if main_grad is not None:
-        matmul_fp8_block(*g_t, *x_t, acc=main_grad)
-        return None
-    return matmul_fp8_block(*g_t, *x_t, out_dtype=weight.dtype)
-
-
-def _grad_operands(gy, need_x: bool, need_w: bool):
-    if need_x and need_w:
-        q, s, q_t, s_t = quantize_fp8_block_both(gy)
-        return (q, s), (q_t, s_t)
-    return (quantize_fp8_block(gy), None) if need_x else (None, quantize_fp8_block_t(gy))
+    if _kernel(gy2):
+        backend.count_launch(1 + want_x + want_w)
+        return backend.require_extension().linear_fp8_bwd(gy2, w_t, w_scale, *(x_t or (None, None)), want_x, x_dtype is torch.float32, want_w,
+                                                          weight.dtype is torch.float32, main_grad)
+    dx = matmul_fp8_block(*quantize_fp8_block(gy2), w_t, w_scale.t(), out_dtype=x_dtype) if want_x else None
+    dw = matmul_fp8_block(*quantize_fp8_block_t(gy2), *x_t, out_dtype=weight.dtype, acc=main_grad) if want_w else None
+    return dx, (None if main_grad is not None else dw)
 
 
 class _LinearFP8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        x2 = x.reshape(-1, x.shape[-1])
-        wq, wq_t, ws = quantize_fp8_weight(weight)
-        x_t = ()
-        if ctx.needs_input_grad and ctx.needs_input_grad[1]:
-            xq, xs, *x_t = quantize_fp8_block_both(x2)
-        else:
-            xq, xs = quantize_fp8_block(x2)
-        ctx.save_for_backward(wq_t, ws, *x_t)
+        need = ctx.needs_input_grad
+        y, *saved = _layer_forward(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), weight, bias, x.dtype, bool(need) and need[1])
+        ctx.save_for_backward(*saved)
         ctx.weight, ctx.x_shape, ctx.x_dtype = weight, x.shape, x.dtype
         ctx.bias_dtype = None if bias is None else bias.dtype
-        return matmul_fp8_block(xq, xs, wq, ws, bias, x.dtype).view(*x.shape[:-1], weight.shape[0])
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        wq_t, ws, *x_t = ctx.saved_tensors
-        gy2 = gy.reshape(-1, gy.shape[-1])
+        w_t, w_scale, *x_t = ctx.saved_tensors
+        gy2 = gy if gy.dim() == 2 else gy.reshape(-1, gy.shape[-1])
         need_x, need_w, need_b = ctx.needs_input_grad
         dx = dw = None
         if need_x or need_w:
-            g, g_t = _grad_operands(gy2, need_x, need_w)
-        if need_x:
-            dx = matmul_fp8_block(*g, wq_t, ws.t(), out_dtype=ctx.x_dtype).view(ctx.x_shape)
-        if need_w:
-            dw = _weight_grad(g_t, x_t, ctx.weight)
+            dx, dw = _layer_backward(gy2, w_t, w_scale, x_t, ctx.weight, need_x, ctx.x_dtype, need_w)
+        if dx is not None and len(ctx.x_shape) != 2:
+            dx = dx.view(ctx.x_shape)
         return dx, dw, (gy2.sum(0, dtype=torch.float32).to(ctx.bias_dtype) if need_b else None)
 
 
@@ -311,48 +309,41 @@ class _AddNormLinearFP8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, res, h, norm_weight, weight, bias, eps, h_scale, stream_dtype):
         x, q, s, rstd = _norm_kernel(res, h, norm_weight, eps, h_scale, stream_dtype, True)
-        wq, wq_t, ws = quantize_fp8_weight(weight)
-        ctx.save_for_backward(x, rstd, norm_weight, wq_t, ws)
+        wq, w_t, w_scale = quantize_fp8_weight(weight)
+        ctx.save_for_backward(x, rstd, norm_weight, w_t, w_scale)
         ctx.weight, ctx.shape, ctx.res_dtype, ctx.h_scale, ctx.has_h = weight, res.shape, res.dtype, h_scale, h is not None
         ctx.bias_dtype = None if bias is None else bias.dtype
         ctx.set_materialize_grads(False)
-        y = matmul_fp8_block(q, s, wq, ws, bias, torch.bfloat16).view(*res.shape[:-1], weight.shape[0])
-        return (x if h is not None else res.view_as(res)), y
+        y = matmul_fp8_block(q, s, wq, w_scale, bias, torch.bfloat16)
+        return (x if h is not None else res.view_as(res)), (y if res.dim() == 2 else y.view(*res.shape[:-1], weight.shape[0]))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gx, gy):
-        x, rstd, norm_weight, wq_t, ws = ctx.saved_tensors
+        x, rstd, norm_weight, w_t, w_scale = ctx.saved_tensors
         C = ctx.shape[-1]
         x = x.reshape(-1, C)
         need_res, need_h, need_nw, need_w, need_b = ctx.needs_input_grad[:5]
         need_n = need_res or need_h or need_nw
         gx2 = None if gx is None else gx.reshape(-1, C)
-        dw = db = dres = dh = dnw = None
-        if gy is None:
-            dn = None
-        else:
+        dn = dw = db = dres = dh = dnw = None
+        if gy is not None:
             gy2 = gy.reshape(-1, gy.shape[-1])
-            g, g_t = _grad_operands(gy2, need_n, need_w) if need_n or need_w else (None, None)
-            if need_w:
-                dw = _weight_grad(g_t, _normed_t(x, rstd, norm_weight), ctx.weight)
+            if need_n or need_w:
+                x_t = _normed_t(x, rstd, norm_weight) if need_w else None
+                dn, dw = _layer_backward(gy2, w_t, w_scale, x_t, ctx.weight, need_n, torch.float32, need_w)
             if need_b:
                 db = gy2.sum(0, dtype=torch.float32).to(ctx.bias_dtype)
-            # the norm's backward kernel reads bf16: one rounding of dn, as in the bf16 layers
-            fused = _kernel(x) and fused_cols_ok(C)
-            dn = matmul_fp8_block(*g, wq_t, ws.t(), out_dtype=torch.bfloat16 if fused else torch.float32) if need_n else None
-        if need_n:
-            if dn is None:
-                dres = gx2
-                dh = None if gx2 is None or not need_h else (ctx.h_scale * gx2.float()).to(torch.bfloat16)
-            elif fused:
-                bf16_stream = x.dtype == torch.bfloat16
-                gx3 = None if gx2 is None else gx2.to(x.dtype).contiguous()
-                dres, dh, dnw = backend.require_extension().add_rmsnorm_bwd(gx3, dn, x, norm_weight, rstd, ctx.has_h and need_h, ctx.h_scale,
-                                                                           bf16_stream)
-                backend.count_launch(2)
-            else:
-                dres, dh, dnw = _norm_backward_ref(gx2, dn, x, norm_weight, rstd, ctx.h_scale, ctx.has_h and need_h)
+        if dn is None:                                           # the layer behind the norm was not used
+            dres = gx2
+            dh = (ctx.h_scale * gx2.float()).to(torch.bfloat16) if need_h and gx2 is not None else None
+        elif _kernel(x) and C <= 32768:
+            gx3 = None if gx2 is None else gx2.to(x.dtype).contiguous()
+            dres, dh, dnw = backend.require_extension().add_rmsnorm_fp8_bwd(gx3, dn, x.contiguous(), norm_weight.contiguous(), rstd, ctx.h_scale,
+                                                                           need_res, need_h, need_nw)
+            backend.count_launch(1 + need_nw)
+        else:
+            dres, dh, dnw = _norm_backward_ref(gx2, dn, x, norm_weight, rstd, ctx.h_scale, need_h)
         return (dres.to(ctx.res_dtype).view(ctx.shape) if need_res and dres is not None else None,
                 dh.view(ctx.shape) if need_h and dh is not None else None,
                 dnw.to(norm_weight.dtype) if need_nw and dnw is not None else None, dw, db, None, None, None)
