@@ -108,7 +108,10 @@ class LLaMAMLP(nn.Module):
                 if self.config.ffn_norm:
                     h = self.norm(h)
                 return self.w3(h), gmu_mems
-        h = self.w1(x)
+        return self.after_w1(self.w1(x), layer_idx, gmu_mems)
+
+    def after_w1(self, h: torch.Tensor, layer_idx: int, gmu_mems=None):
+        """The rest of the layer, from the output of the gate and up projections."""
         if self.relu2:
             h = F.relu(h).square()
         else:
@@ -256,6 +259,25 @@ class Block(nn.Module):
                 and not hasattr(self, "layer_configurator") and type(self.norm_1) in (FusedRMSNorm,)
                 and type(self.norm_2) in (FusedRMSNorm,) and not (self.training and residual_dropout > 0))
 
+    def _fp8_mlp(self, x, compute_dtype) -> bool:
+        """Whether the second norm may deliver 8-bit operands to the MLP: nothing but its first layer reads the normalised values."""
+        mlp = self.mlp
+        return (type(mlp) is LLaMAMLP and mlp.w1.fp8_block and not (mlp.w1.mxfp8 or mlp.w1.nvfp4) and ops.gemm.bare_linear(mlp.w1)
+                and "forward" not in mlp.__dict__ and not (mlp._forward_hooks or mlp._forward_pre_hooks or mlp._backward_hooks
+                                                           or mlp._backward_pre_hooks or self.norm_2._forward_hooks or self.norm_2._forward_pre_hooks)
+                and compute_dtype == torch.bfloat16 and x.dtype in (torch.bfloat16, torch.float32))
+
+    def _norm_w1_fp8(self, x, h, scale, stream):
+        w1, norm = self.mlp.w1, self.norm_2
+        g = getattr(w1.weight, "_fsdp_group", None)
+        if g is not None and getattr(g, "ag_pending", False):
+            w1.weight._fsdp_engine.finish_pending_gather(g)
+        stored = w1.stored_fp8()
+        if stored is None:
+            return ops.add_rms_norm_linear_fp8(x, h, norm.weight, w1.weight, norm.eps, scale, stream)
+        x, q, s = ops.add_rms_norm_fp8(x, h, norm.weight, norm.eps, scale, stream)
+        return x, ops.linear_fp8_weight((q.view(x.shape), s), *stored)
+
     def forward_deferred(self, x, h_pending, input_embed, rope, max_seq_length, seq_meta, kv_cache, gmu_mems,
                          compute_dtype):
         """Same math as :meth:`forward`; takes the residual stream ``x`` plus the not-yet-added branch
@@ -284,11 +306,15 @@ class Block(nn.Module):
                 self.attn_output_rmsnorm = compute_rmsnorm(h) * scale
                 self.attn_outlier_pct = compute_outlier_percentage(h)
                 self.attn_z_mean = getattr(self.attn, "z_mean", None)
-        x, n_2 = ops.add_rms_norm(x, h.to(compute_dtype), self.norm_2.weight, self.norm_2.eps, scale, compute_dtype, stream)
-        if cfg.moe:
-            h = self.mlp(n_2)
+        if self._fp8_mlp(x, compute_dtype):             # the norm writes the 8-bit operand of the gate and up projections itself
+            x, h = self._norm_w1_fp8(x, h.to(compute_dtype), scale, stream)
+            h, gmu_mems = self.mlp.after_w1(h, self.layer_idx, gmu_mems)
         else:
-            h, gmu_mems = self.mlp(n_2, self.layer_idx, gmu_mems)
+            x, n_2 = ops.add_rms_norm(x, h.to(compute_dtype), self.norm_2.weight, self.norm_2.eps, scale, compute_dtype, stream)
+            if cfg.moe:
+                h = self.mlp(n_2)
+            else:
+                h, gmu_mems = self.mlp(n_2, self.layer_idx, gmu_mems)
         if self.collect_stats:
             with torch.no_grad():
                 self.mlp_output_rmsnorm = compute_rmsnorm(h) * scale

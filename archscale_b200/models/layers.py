@@ -16,20 +16,27 @@ class Linear(nn.Linear):
       (replaces the ``te.Linear`` swap of the reference, `precision.py:192-251`);
     * ``nvfp4=True`` → NVFP4 GEMM (e2m1 elements, E4M3 block scales; the ``--fp4`` recipe, `precision.py:92-96`),
       emulated in PyTorch off the GPU;
+    * ``fp8_block=True`` → E4M3 GEMM with one fp32 scale per 128 elements (``ops.linear_fp8_block``), for weights of any size; after
+      :func:`freeze_fp8_block` calls without gradients read the stored 8-bit weight (``ops.linear_fp8_weight``);
     * anything else (CPU, fp32) → ``F.linear``.
     The weight is cast to the activation dtype when they differ (fp32 masters, bf16 compute).
     """
 
     mxfp8: bool = False
     nvfp4: bool = False
+    fp8_block: bool = False
+    fp8_stored = None           # (elements, scales, version of the weight) of a frozen layer
     widen: bool = False         # odd feature counts on operands widened to a multiple of 8 (``ops.gemm.linear_widened``)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         w, b = self.weight, self.bias
         g = getattr(w, "_fsdp_group", None)
-        if g is not None and getattr(g, "ag_pending", False) and (self.mxfp8 or self.nvfp4 or not (
+        if g is not None and getattr(g, "ag_pending", False) and (self.mxfp8 or self.nvfp4 or self.fp8_block or not (
                 w._fsdp_first and x.is_cuda and x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16)):
             w._fsdp_engine.finish_pending_gather(g)
+        if self.fp8_block:
+            stored = self.stored_fp8()
+            return ops.linear_fp8_block(x, w, b) if stored is None else ops.linear_fp8_weight(x, *stored, b)
         if w.dtype != x.dtype:
             w = w.to(x.dtype)
             b = b.to(x.dtype) if b is not None else None
@@ -42,6 +49,15 @@ class Linear(nn.Linear):
         if self.widen and b is None and gemm.widened_ok(x, w):
             return gemm.linear_widened(x, w)
         return ops.linear(x, w, b)
+
+    def stored_fp8(self):
+        """(elements, scales) of a frozen layer in a call without gradients, else None.  Raises when the weight was written since."""
+        if self.fp8_stored is None or torch.is_grad_enabled():
+            return None
+        q, scale, version = self.fp8_stored
+        if version != self.weight._version or q.device != self.weight.device:
+            raise RuntimeError("the weight of a frozen 8-bit layer has changed: call freeze_fp8_block(model) again")
+        return q, scale
 
     plain_forward = forward     # what ``ops.gemm.plain_linear`` compares with: a replaced ``forward`` is never passed by
 
@@ -67,5 +83,32 @@ def apply_nvfp4(model: nn.Module, skip=("lm_head", "lc_proj")) -> int:
         if isinstance(mod, Linear) and not any(s in name for s in skip) \
                 and mod.in_features % 256 == 0 and mod.out_features % 256 == 0:
             mod.nvfp4 = True
+            n += 1
+    return n
+
+
+def apply_fp8_block(model: nn.Module, skip=("lm_head", "lc_proj")) -> int:
+    """Switch every :class:`Linear` of ``model`` to 8-bit operands with an fp32 scale per 128 elements, except modules whose name
+    contains one of ``skip``.  Returns the number of layers switched."""
+    n = 0
+    for name, mod in model.named_modules():
+        if isinstance(mod, Linear) and not any(s in name for s in skip):
+            mod.fp8_block = True
+            n += 1
+    return n
+
+
+@torch.no_grad()
+def freeze_fp8_block(model: nn.Module, frozen: bool = True) -> int:
+    """Store the 8-bit form of the weights of all ``fp8_block`` layers for calls without gradients (evaluation, generation), which otherwise
+    quantise them every time; ``frozen=False`` drops it.  Weights that change afterwards make such a call raise.  Returns the number of
+    layers."""
+    n = 0
+    for mod in model.modules():
+        if isinstance(mod, Linear) and mod.fp8_block:
+            mod.fp8_stored = None
+            if frozen:
+                q, _, scale = ops.quantize_fp8_weight(mod.weight)
+                mod.fp8_stored = (q, scale, mod.weight._version)
             n += 1
     return n

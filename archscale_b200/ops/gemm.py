@@ -367,14 +367,19 @@ class _MultiLinearFn(torch.autograd.Function):
         return (dx,) + tuple(outs)
 
 
-def plain_linear(l) -> bool:
-    """True when a call of the layer ``l`` is the product with its weight and nothing else, so that a fused route may pass the
-    module by: a ``Linear`` without bias or low-precision operands, hooks, or another ``forward`` than its own."""
+def bare_linear(l) -> bool:
+    """True when calling the layer ``l`` runs its own ``forward`` and nothing else, so that a fused route may pass the module by: a
+    ``Linear`` without bias, hooks, or another ``forward`` than its own."""
     cls, d = type(l), l.__dict__
     return (cls.__name__ == "Linear" and cls.forward is getattr(cls, "plain_forward", None) and "forward" not in d
-            and d["_parameters"].get("bias") is None and not l.mxfp8 and not l.nvfp4
+            and d["_parameters"].get("bias") is None
             and not (d["_forward_hooks"] or d["_forward_pre_hooks"] or d["_backward_hooks"] or d["_backward_pre_hooks"])
             and l._compiled_call_impl is None and not _has_any_global_hook())
+
+
+def plain_linear(l) -> bool:
+    """A :func:`bare_linear` without low-precision operands: its call is the product with its weight."""
+    return bare_linear(l) and not l.mxfp8 and not l.nvfp4 and not l.fp8_block
 
 
 def linear_multi(x: torch.Tensor, layers, keep_fused: bool = False):

@@ -368,6 +368,11 @@ class Trainer:
             from archscale_b200.models.layers import apply_nvfp4
             n_fp4 = apply_nvfp4(self.model)
             self.print(f"NVFP4: {n_fp4} linear layers run the block-scaled e2m1 GEMM")
+        if self.config.fp8_block:
+            if self.config.mxfp8 or self.config.nvfp4 or self.config.tp_size > 1:
+                raise ValueError("fp8_block goes with neither --fp8, --fp4 nor tensor parallelism")
+            from archscale_b200.models.layers import apply_fp8_block
+            self.print(f"FP8: {apply_fp8_block(self.model)} linear layers run the e4m3 GEMM with fp32 scales per 128 elements")
         if self.config.tp_size > 1:
             from archscale_b200.parallel import tp as tp_mod
             tp_mod.apply_tensor_parallel(self.model, mesh)
