@@ -442,10 +442,9 @@ __global__ void __launch_bounds__(PACK ? 128 : V > 2 ? 1024 : 512) fp8_norm_bwd_
     for (int e = 0; e < 8; ++e) dw[i][e] = 0.f;
   }
   int it = 0;
-  for (int r0 = blockIdx.x * RPC; r0 < p.rows; r0 += gridDim.x * RPC, ++it) {      // the same number of turns for all threads of a block
-    const int row = r0 + sub;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * RPC; r0 < p.rows; r0 += gridDim.x * RPC, ++it) {      // as many turns for all threads of a block
+    const int64_t row = r0 + sub, base = row * p.cols;
     const bool live = row < p.rows;
-    const int64_t base = static_cast<int64_t>(row) * p.cols;
     Raw8<float> dr[V];
     Raw8<T> xr[V], gr[V];
 #pragma unroll

@@ -6,9 +6,8 @@
 // fp32 scales, so the products of one block of K are accumulated in tensor memory (exact to fp32 rounding over 128 terms), read
 // back, scaled and added to fp32 sums in registers.
 //
-// This file: the form for few rows of A (single tokens to a few hundred) and for outputs too small to fill the machine with the 256-row
-// tiles of gemm2_fp8_block.cu.  It is bound by reading B once (one token: 11264 × 2048 weights, 23 MB, 3.5 µs at the copy rate) and, at
-// this size, by the latency of one CTA's chain.  So 128 rows of B are the M side of the MMA and BT rows of A (16 to 128) its N side, which
+// This file: the form for up to 64 rows of A (single tokens, a batch in decoding).  It is bound by reading B once (one token: 11264 × 2048 weights, 23 MB, 3.5 µs at the copy rate) and, at
+// this size, by the latency of one CTA's chain.  So 128 rows of B are the M side of the MMA and BT rows of A (16, 32 or 64) its N side, which
 // makes neighbouring lanes neighbouring columns of the output, and the blocks of K are split over a cluster of up to eight CTAs.  The
 // first loads are issued before tensor memory is allocated.  The CTAs' sums meet in shared memory, in the place of the stages; every CTA
 // adds its share of the rows over the ranks in rank order (distributed shared memory), so a result does not depend on scheduling.
@@ -24,8 +23,8 @@ constexpr int FS_BN = 128, FS_BK = 128, FS_CHUNK = 32;
 template <int BT>
 struct FS {
   static constexpr int B_BYTES = FS_BN * FS_BK, A_BYTES = BT * FS_BK, STAGE = B_BYTES + A_BYTES;
-  static constexpr int STAGES = BT == 16 ? 6 : BT == 32 ? 5 : 4;        // two CTAs fit an SM (BT 128: one)
-  static constexpr int ACC = BT <= 32 ? 8 : BT == 64 ? 4 : 2;      // accumulators: products run ahead of the sums
+  static constexpr int STAGES = BT == 16 ? 6 : BT == 32 ? 5 : 4;        // two CTAs fit an SM
+  static constexpr int ACC = BT <= 32 ? 8 : 4;                     // accumulators: products run ahead of the sums
   static constexpr int TMEM = ACC * BT;
   static constexpr int W = BT < 32 ? BT : 32, GROUPS = BT / W;     // sums of a thread; teams of four warps
   static constexpr int SUMMERS = 128 * GROUPS, THREADS = 64 + SUMMERS;
@@ -67,7 +66,7 @@ __device__ __forceinline__ float4 fs_ld_cluster(uint32_t smem_addr, int rank) {
 }
 
 template <int BT, int S>
-__global__ void __launch_bounds__(FS<BT>::THREADS, BT <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(FS<BT>::THREADS, 2)
 gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const FsParams p) {
   using T = FS<BT>;
   constexpr int W = T::W;
@@ -261,7 +260,7 @@ static int launch_fs(const void* A, int64_t lda, const void* B, int64_t ldb, con
   const int64_t tiles = static_cast<int64_t>((p.M + BT - 1) / BT) * ((p.N + FS_BN - 1) / FS_BN);
   if (tiles > 0xfffffff) return -6;
   // K is split as far as the CTAs fit the machine at once and have a block each
-  const int64_t room = static_cast<int64_t>(num_sms) * (BT <= 64 ? 2 : 1);
+  const int64_t room = 2 * static_cast<int64_t>(num_sms);
   const int num_kb = (p.K + FS_BK - 1) / FS_BK;
   int s = 1;
   while (s < 8 && tiles * 2 * s <= room && 2 * s <= num_kb) s *= 2;
@@ -298,6 +297,5 @@ extern "C" int b200_gemm_fp8_block(const void* A, int64_t lda, const float* sa, 
                    bias_dtype == 0 ? 1 : 0, ldc % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0 ? 1 : 0, status};
   if (M <= 16) return launch_fs<16>(A, lda, B, ldb, p, num_sms, stream);
   if (M <= 32) return launch_fs<32>(A, lda, B, ldb, p, num_sms, stream);
-  if (M <= 64) return launch_fs<64>(A, lda, B, ldb, p, num_sms, stream);
-  return launch_fs<128>(A, lda, B, ldb, p, num_sms, stream);
+  return launch_fs<64>(A, lda, B, ldb, p, num_sms, stream);
 }

@@ -120,6 +120,12 @@ def _kernel(x: torch.Tensor) -> bool:
     return x.is_cuda and backend.use_cuda_kernel("fp8_block", x)
 
 
+def _no_grad(name: str, *tensors) -> None:
+    """A call that has no gradients must not cut a graph silently."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no gradients: call it under torch.no_grad(), or use the training form")
+
+
 def _ext():
     backend.count_launch()
     return backend.require_extension()
@@ -193,10 +199,11 @@ Quantised = Tuple[torch.Tensor, torch.Tensor]
 def linear_fp8_weight(x: Union[torch.Tensor, Quantised], weight: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
                       out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``x · Wᵀ (+ bias)`` with stored elements ``weight:(N,K)`` and scales of 128 × 128 tiles.  ``x:(..., K)`` is quantised here, or is the
-    pair (elements, scales) of :func:`add_rms_norm_fp8` / :func:`quantize_fp8_block` with any leading dimensions of the elements.  No
-    gradients."""
+    pair (elements, scales) of :func:`add_rms_norm_fp8` / :func:`quantize_fp8_block` with any leading dimensions of the elements.  It has
+    no gradients and refuses operands that ask for one."""
     if not isinstance(x, torch.Tensor):
         return matmul_fp8_block(x[0], x[1], weight, scale, bias, out_dtype or torch.bfloat16)
+    _no_grad("linear_fp8_weight", x, bias)
     flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     q, s = quantize_fp8_block(flat)
     y = matmul_fp8_block(q, s, weight, scale, bias, out_dtype or x.dtype)
@@ -289,8 +296,9 @@ def _norm_kernel(res, h, weight, eps, h_scale, stream_dtype, want_rstd):
 def add_rms_norm_fp8(res: torch.Tensor, h: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-5, h_scale: float = 1.0,
                      stream_dtype: Optional[torch.dtype] = None):
     """``x = res + h_scale · h`` (fp32, kept in ``stream_dtype``, by default the type of ``res``; without ``h`` x is ``res``) and ``rmsnorm(x) · weight`` as
-    elements and scales: (x of the shape of res, elements (rows, C), scales (rows, ⌈C/128⌉)).  No gradients: training goes through
-    :func:`add_rms_norm_linear_fp8`."""
+    elements and scales: (x of the shape of res, elements (rows, C), scales (rows, ⌈C/128⌉)).  It has no gradients and refuses operands that
+    ask for one: training goes through :func:`add_rms_norm_linear_fp8`."""
+    _no_grad("add_rms_norm_fp8", res, h, weight)
     x, q, scale, _ = _norm_kernel(res, h, weight, eps, h_scale, stream_dtype, False)
     return x, q, scale
 

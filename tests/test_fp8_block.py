@@ -9,6 +9,7 @@ import torch
 
 from archscale_b200 import ops
 from archscale_b200.ops import backend, fp8_block as fb
+from archscale_b200.utils import canary
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 
@@ -131,6 +132,44 @@ def test_product(M, N, K, kinds):
     _close_product(acc, a, sa, b, sb, base=0.5)
     assert torch.equal(out, ops.matmul_fp8_block(a, sa, b, sb, out_dtype=torch.float32))      # the same from call to call
     assert backend.require_extension().device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(256, 256, 16384), (257, 300, 9000), (100, 1001, 12800), (512, 640, 20000)])
+@pytest.mark.parametrize("kinds", ["row,tile", "row,row"])
+def test_long_contractions_are_split(M, N, K, kinds):
+    """Few tiles and many blocks: every tile is the sum of parts, added in the order of K by whichever comes last."""
+    a, sa = ops.quantize_fp8_block(_rand((M, K), torch.bfloat16, "cuda", 1))
+    w = _rand((N, K), torch.bfloat16, "cuda", 2)
+    b, sb = ops.quantize_fp8_weight(w)[::2] if kinds == "row,tile" else ops.quantize_fp8_block(w)
+    out = ops.matmul_fp8_block(a, sa, b, sb, out_dtype=torch.float32)
+    _close_product(out, a, sa, b, sb)
+    for _ in range(5):
+        assert torch.equal(out, ops.matmul_fp8_block(a, sa, b, sb, out_dtype=torch.float32))
+    bias = _rand((N,), torch.float32, "cuda", 3)
+    _close_product(ops.matmul_fp8_block(a, sa, b, sb, bias=bias), a, sa, b, sb, base=bias.double())
+    acc = torch.full((M, N), -2.0, device="cuda")
+    _close_product(ops.matmul_fp8_block(a, sa, b, sb, acc=acc), a, sa, b, sb, base=-2.0)
+    # two streams at once: each call has its own workspace
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for st in streams:
+        with torch.cuda.stream(st):
+            outs.append(ops.matmul_fp8_block(a, sa, b, sb, out_dtype=torch.float32))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, out) for o in outs) and backend.require_extension().device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N", [(7, 131), (64, 300), (300, 520), (301, 523)])
+def test_outputs_stay_inside(M, N):
+    acc, raw = canary.guarded((M, N), torch.float32, "cuda")
+    a, b = (ops.quantize_fp8_block(_rand((r, 512), torch.bfloat16, "cuda", r)) for r in (M, N))
+    want = acc.clone()
+    ops.matmul_fp8_block(*a, *b, acc=acc)
+    torch.cuda.synchronize()
+    assert canary.guards_intact(acc, raw)
+    _close_product(acc, *a, *b, base=want.double())
 
 
 @pytest.mark.gpu
@@ -410,7 +449,14 @@ def test_refusals(device):
         ops.add_rms_norm_fp8(x, None, torch.ones(256, device=device), stream_dtype=torch.bfloat16)
     with pytest.raises(ValueError):
         ops.add_rms_norm_linear_fp8(x, None, torch.ones(256, device=device), w[:, :128])
-    y = ops.linear_fp8_block(x.requires_grad_(), w.requires_grad_())
+    with pytest.raises(ValueError):
+        ops.matmul_fp8_block(q, s, wq, ws, acc=torch.zeros(1, 6, device=device).expand(4, 6)[:, :5])
+    x.requires_grad_()
+    with pytest.raises(RuntimeError):
+        ops.linear_fp8_weight(x, wq, ws)                                              # these two have no gradients
+    with pytest.raises(RuntimeError):
+        ops.add_rms_norm_fp8(x, None, torch.ones(256, device=device))
+    y = ops.linear_fp8_block(x, w.requires_grad_())
     g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()                                                            # no gradient of the gradient
