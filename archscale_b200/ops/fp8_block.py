@@ -104,6 +104,12 @@ def _stream(res: torch.Tensor, stream_dtype: Optional[torch.dtype]) -> torch.dty
     return res.dtype if stream_dtype is None else stream_dtype
 
 
+def _stream_code(stream_dtype: Optional[torch.dtype]) -> int:
+    if stream_dtype is not None and stream_dtype not in _FLOATS:
+        raise TypeError(f"a residual stream is kept in bfloat16 or float32, not in {stream_dtype}")
+    return -1 if stream_dtype is None else int(stream_dtype is torch.bfloat16)
+
+
 def _need_float(name: str, **tensors) -> None:
     for what, t in tensors.items():
         if t is not None and t.dtype not in _FLOATS:
@@ -211,23 +217,10 @@ def linear_fp8_weight(x: Union[torch.Tensor, Quantised], weight: torch.Tensor, s
 
 
 # ------------------------------------------------------------------------------------------------ training
-def _layer_forward(x2, weight, bias, out_dtype, want_t):
-    """(y, Wᵀ elements, scales of W, *(xᵀ elements, scales) with ``want_t``)."""
-    if _kernel(x2):
-        backend.count_launch(3)
-        return backend.require_extension().linear_fp8_fwd(x2, weight, bias, out_dtype is torch.float32, want_t)
-    wq, w_t, w_scale = quantize_fp8_weight(weight)
-    q, scale, *x_t = quantize_fp8_block_both(x2) if want_t else quantize_fp8_block(x2)
-    return (matmul_fp8_block(q, scale, wq, w_scale, bias, out_dtype), w_t, w_scale, *x_t)
-
-
+# CUDA operands go through the autograd nodes of the bindings (``csrc/bindings_fp8.inc``); these are the same on the restatements.
 def _layer_backward(gy2, w_t, w_scale, x_t, weight, want_x, x_dtype, want_w):
     """(dx | None, dW | None); dW goes into ``main_grad`` where the weight carries one.  ``x_t``: (elements, scales) of xᵀ."""
     main_grad = getattr(weight, "main_grad", None)
-    if _kernel(gy2):
-        backend.count_launch(1 + want_x + want_w)
-        return backend.require_extension().linear_fp8_bwd(gy2, w_t, w_scale, *(x_t or (None, None)), want_x, x_dtype is torch.float32, want_w,
-                                                          weight.dtype is torch.float32, main_grad)
     dx = matmul_fp8_block(*quantize_fp8_block(gy2), w_t, w_scale.t(), out_dtype=x_dtype) if want_x else None
     dw = matmul_fp8_block(*quantize_fp8_block_t(gy2), *x_t, out_dtype=weight.dtype, acc=main_grad) if want_w else None
     return dx, (None if main_grad is not None else dw)
@@ -236,25 +229,23 @@ def _layer_backward(gy2, w_t, w_scale, x_t, weight, want_x, x_dtype, want_w):
 class _LinearFP8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        need = ctx.needs_input_grad
-        y, *saved = _layer_forward(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), weight, bias, x.dtype, bool(need) and need[1])
-        ctx.save_for_backward(*saved)
+        x2 = x.reshape(-1, x.shape[-1])
+        wq, w_t, w_scale = quantize_fp8_weight(weight)
+        q, scale = quantize_fp8_block(x2)
+        need_w = bool(ctx.needs_input_grad) and ctx.needs_input_grad[1]
+        ctx.save_for_backward(w_t, w_scale, *(quantize_fp8_block_t(x2) if need_w else ()))
         ctx.weight, ctx.x_shape, ctx.x_dtype = weight, x.shape, x.dtype
         ctx.bias_dtype = None if bias is None else bias.dtype
-        return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
+        return matmul_fp8_block(q, scale, wq, w_scale, bias, x.dtype).view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
         w_t, w_scale, *x_t = ctx.saved_tensors
-        gy2 = gy if gy.dim() == 2 else gy.reshape(-1, gy.shape[-1])
+        gy2 = gy.reshape(-1, gy.shape[-1])
         need_x, need_w, need_b = ctx.needs_input_grad
-        dx = dw = None
-        if need_x or need_w:
-            dx, dw = _layer_backward(gy2, w_t, w_scale, x_t, ctx.weight, need_x, ctx.x_dtype, need_w)
-        if dx is not None and len(ctx.x_shape) != 2:
-            dx = dx.view(ctx.x_shape)
-        return dx, dw, (gy2.sum(0, dtype=torch.float32).to(ctx.bias_dtype) if need_b else None)
+        dx, dw = _layer_backward(gy2, w_t, w_scale, x_t, ctx.weight, need_x, ctx.x_dtype, need_w)
+        return (None if dx is None else dx.view(ctx.x_shape)), dw, (gy2.sum(0, dtype=torch.float32).to(ctx.bias_dtype) if need_b else None)
 
 
 def _check_layer(name, cols, weight, bias=None):
@@ -267,6 +258,9 @@ def _check_layer(name, cols, weight, bias=None):
 
 def linear_fp8_block(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x · weightᵀ (+ bias)`` with x:(..., K) and weight:(N, K) quantised in the call; trains (see the head of this file)."""
+    if _kernel(x):
+        backend.count_launch(3)
+        return backend.require_extension().linear_fp8(x, weight, bias)
     _need_float("linear_fp8_block", x=x)
     _check_layer("linear_fp8_block", x.shape[-1], weight, bias)
     return backend.apply(_LinearFP8Fn, x, weight, bias)
@@ -290,7 +284,7 @@ def _norm_kernel(res, h, weight, eps, h_scale, stream_dtype, want_rstd):
         _check_norm("add_rms_norm_fp8", res, h, weight, _stream(res, stream_dtype))
         x, rstd, n = _norm_ref(res, h, weight, eps, h_scale, _stream(res, stream_dtype))
         return (x, *quantize_ref(n.reshape(-1, C)), rstd.reshape(-1))
-    return _ext().add_rmsnorm_fp8(res, h, weight, eps, h_scale, -1 if stream_dtype is None else int(stream_dtype is torch.bfloat16), want_rstd)
+    return _ext().add_rmsnorm_fp8(res, h, weight, eps, h_scale, _stream_code(stream_dtype), want_rstd)
 
 
 def add_rms_norm_fp8(res: torch.Tensor, h: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-5, h_scale: float = 1.0,
@@ -338,18 +332,13 @@ class _AddNormLinearFP8Fn(torch.autograd.Function):
         if gy is not None:
             gy2 = gy.reshape(-1, gy.shape[-1])
             if need_n or need_w:
-                x_t = _normed_t(x, rstd, norm_weight) if need_w else None
+                x_t = quantize_ref((x.float() * rstd.view(-1, 1) * norm_weight.float()).t()) if need_w else None
                 dn, dw = _layer_backward(gy2, w_t, w_scale, x_t, ctx.weight, need_n, torch.float32, need_w)
             if need_b:
                 db = gy2.sum(0, dtype=torch.float32).to(ctx.bias_dtype)
         if dn is None:                                           # the layer behind the norm was not used
             dres = gx2
             dh = (ctx.h_scale * gx2.float()).to(torch.bfloat16) if need_h and gx2 is not None else None
-        elif _kernel(x) and C <= 32768:
-            gx3 = None if gx2 is None else gx2.to(x.dtype).contiguous()
-            dres, dh, dnw = backend.require_extension().add_rmsnorm_fp8_bwd(gx3, dn, x.contiguous(), norm_weight.contiguous(), rstd, ctx.h_scale,
-                                                                           need_res, need_h, need_nw)
-            backend.count_launch(1 + need_nw)
         else:
             dres, dh, dnw = _norm_backward_ref(gx2, dn, x, norm_weight, rstd, ctx.h_scale, need_h)
         return (dres.to(ctx.res_dtype).view(ctx.shape) if need_res and dres is not None else None,
@@ -357,16 +346,12 @@ class _AddNormLinearFP8Fn(torch.autograd.Function):
                 dnw.to(norm_weight.dtype) if need_nw and dnw is not None else None, dw, db, None, None, None)
 
 
-def _normed_t(x, rstd, weight):
-    """The normalised values again, quantised with blocks along the tokens: (elements (C, rows), scales)."""
-    if not _kernel(x):
-        return quantize_ref((x.float() * rstd.view(-1, 1) * weight.float()).t())
-    return tuple(_ext().fp8_quantize(x, 2, rstd, weight.contiguous()))
-
-
 def add_rms_norm_linear_fp8(res: torch.Tensor, h: Optional[torch.Tensor], norm_weight: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5,
                             h_scale: float = 1.0, stream_dtype: Optional[torch.dtype] = None, bias: Optional[torch.Tensor] = None):
     """``x = res + h_scale · h``, ``y = Q(rmsnorm(x) · norm_weight) · Q(weight)ᵀ (+ bias)`` → (x, y in bf16), with gradients of all inputs."""
+    if _kernel(res) and 1 <= res.shape[-1] <= 32768:
+        backend.count_launch(3)
+        return tuple(backend.require_extension().add_norm_linear_fp8(res, h, norm_weight, weight, eps, h_scale, _stream_code(stream_dtype), bias))
     stream_dtype = _stream(res, stream_dtype)
     _check_norm("add_rms_norm_linear_fp8", res, h, norm_weight, stream_dtype)
     _check_layer("add_rms_norm_linear_fp8", res.shape[-1], weight, bias)
