@@ -290,9 +290,10 @@ int b200_fp8_quantize(const void* x, int dtype, int64_t ldx, int rows, int cols,
 // or null, rstd [rows] or null; cols ≤ 32768.
 int b200_add_rmsnorm_fp8(const void* res, int res_dtype, const void* h, float h_scale, const void* w, int w_dtype, void* x, int x_dtype,
                          void* q, int64_t ldq, float* s, int64_t lds, float* rstd, int rows, int cols, float eps, cudaStream_t stream);
-// Its gradients: dn fp32, x and gx (or null) of x_dtype; dres (x_dtype), dh (bf16), dw (fp32, with dw_part [grid][cols]) null if not wanted.
+// Its gradients: dn fp32 (rows ld_dn apart, a multiple of 8, 16-byte aligned), x and gx (or null) of x_dtype; dres (x_dtype), dh (bf16), dw (fp32,
+// with dw_part [grid][cols]) null if not wanted.
 int b200_add_rmsnorm_fp8_bwd_grid(int rows, int cols, int num_sms);
-int b200_add_rmsnorm_fp8_bwd(const float* dn, const void* x, int x_dtype, const void* gx, const void* w, int w_dtype, const float* rstd, void* dres,
+int b200_add_rmsnorm_fp8_bwd(const float* dn, int64_t ld_dn, const void* x, int x_dtype, const void* gx, const void* w, int w_dtype, const float* rstd, void* dres,
                              void* dh, float h_scale, float* dw_part, float* dw, int rows, int cols, int grid, cudaStream_t stream);
 // out[M, N] (+)= Σ over blocks of 128 of K: sa · sb · (A block · B blockᵀ) (+ bias[N])  (gemm_fp8_block.cu).  A, B: e4m3, rows lda / ldb
 // bytes apart (multiples of 16, as the addresses); a scale belongs to one row, or (*_tile) to 128 rows, strides *_row and *_blk.

@@ -31,8 +31,12 @@ __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float
 template <typename T> struct Raw8;
 template <> struct Raw8<float> { float4 a, b; };
 template <> struct Raw8<__nv_bfloat16> { uint4 a; };
+
 // VEC: rows are whole 16-byte pieces, so that n is 8 or not positive: one or two predicated loads, which the compiler issues together
-// (with a branch per vector for the general case in between, a tile of bf16 took 3.5 times as long).
+// (with a branch per vector for the general case in between, a tile of bf16 took 3.5 times as long).  Otherwise the row starts anywhere, and
+// fp32 is loaded one value at a time; of bf16 the aligned 16-byte pieces that hold at least one of the values are loaded and shifted
+// (30568 x 7981 in both orientations 266 µs instead of 317; fp32 that way 457 instead of 336).  Such a piece never leaves the 16-byte granule of
+// memory that the value lies in.
 template <bool VEC>
 __device__ __forceinline__ void load_raw(const float* p, int n, Raw8<float>& r) {
   if (VEC) {
@@ -48,14 +52,24 @@ __device__ __forceinline__ void load_raw(const float* p, int n, Raw8<float>& r) 
 }
 template <bool VEC>
 __device__ __forceinline__ void load_raw(const __nv_bfloat16* p, int n, Raw8<__nv_bfloat16>& r) {
+  r.a = make_uint4(0u, 0u, 0u, 0u);
   if (VEC) {
-    r.a = make_uint4(0u, 0u, 0u, 0u);
     if (n > 0) r.a = *reinterpret_cast<const uint4*>(p);
-  } else {
-    uint32_t v[8];
+  } else if (n > 0) {
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
+    const uint4* base = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) - off);
+    const uint4 c0 = base[0], c1 = static_cast<int>(off) + n * 2 > 16 ? base[1] : make_uint4(0u, 0u, 0u, 0u);
+    const uint32_t w[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+    uint32_t t[6], u[5], o[4];                          // by two words, by one, by half of one
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[i]) : 0u;
-    r.a = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+    for (int i = 0; i < 6; ++i) t[i] = (off & 8) ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) u[i] = (off & 4) ? t[i + 1] : t[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __funnelshift_r(u[i], u[i + 1], (off & 2) * 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = 2 * i + 1 < n ? o[i] : 2 * i < n ? o[i] & 0xffffu : 0u;
+    r.a = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 __device__ __forceinline__ void unpack8(const Raw8<float>& r, float (&v)[8]) {
@@ -309,6 +323,14 @@ __device__ __forceinline__ void store8(float* p, int n, bool vec, const float (&
 __device__ __forceinline__ void store8(__nv_bfloat16* p, int n, bool vec, const float (&v)[8]) {
   if (vec && n >= 8) {
     *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  } else if (n >= 8 && (reinterpret_cast<uintptr_t>(p) & 2)) {       // pairs that lie on 4 bytes
+    p[0] = __float2bfloat16(v[0]);
+#pragma unroll
+    for (int i = 1; i < 7; i += 2) *reinterpret_cast<uint32_t*>(p + i) = pack_bf16x2(v[i], v[i + 1]);
+    p[7] = __float2bfloat16(v[7]);
+  } else if (n >= 8) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) *reinterpret_cast<uint32_t*>(p + i) = pack_bf16x2(v[i], v[i + 1]);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) if (i < n) p[i] = __float2bfloat16(v[i]);
@@ -417,7 +439,8 @@ static int launch_norm(const Fp8NormParams& p, cudaStream_t st) {
 // Threads hold the columns that they hold in the forward kernel, so that d_w is summed in registers over a block's rows; the blocks' sums meet in
 // a second kernel, in a fixed order.  Bound by memory: 12 bytes per element with a bf16 stream.
 struct Fp8NormBwdParams {
-  const float* dn; const void *x, *gx, *w;
+  const float* dn; int64_t ld_dn;       // rows of whole 32-byte pieces, whatever cols is
+  const void *x, *gx, *w;
   const float* rstd;
   void* dres; __nv_bfloat16* dh;
   float* dw_part;               // [grid][cols] or null
@@ -451,7 +474,7 @@ __global__ void __launch_bounds__(PACK ? 128 : V > 2 ? 1024 : 512) fp8_norm_bwd_
     for (int i = 0; i < V; ++i) {
       const int c = (t + i * TPR) * 8;
       const int n = live ? min(max(p.cols - c, 0), 8) : 0;
-      load_raw<VEC>(p.dn + base + c, n, dr[i]);
+      load_raw<true>(p.dn + row * p.ld_dn + c, n, dr[i]);
       load_raw<VEC>(static_cast<const T*>(p.x) + base + c, n, xr[i]);
       load_raw<VEC>(static_cast<const T*>(p.gx) + base + c, p.gx ? n : 0, gr[i]);
     }
@@ -459,8 +482,13 @@ __global__ void __launch_bounds__(PACK ? 128 : V > 2 ? 1024 : 512) fp8_norm_bwd_
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
+      const int c = (t + i * TPR) * 8;
       float d[8], x[8];
       unpack8(dr[i], d); unpack8(xr[i], x);
+      if (!VEC && c + 8 > p.cols) {                      // what lies past the row is anything
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] = c + e < p.cols ? d[e] : 0.f;
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float xhat = x[e] * rs;
@@ -594,18 +622,18 @@ extern "C" int b200_add_rmsnorm_fp8(const void* res, int res_dtype, const void* 
   return x_dtype == 0 ? launch_norm<__nv_bfloat16, float>(p, stream) : launch_norm<__nv_bfloat16, __nv_bfloat16>(p, stream);
 }
 
-// dn fp32, x, gx (or null) of x_dtype, all [rows, cols] dense; dres (x_dtype), dh (bf16), dw (fp32 [cols], with dw_part [grid][cols]): null if not
-// wanted.  grid: b200_add_rmsnorm_fp8_bwd_grid.
+// x, gx (or null) of x_dtype [rows, cols] dense; dn fp32, 16-byte aligned, its rows ld_dn apart, a multiple of 8 (the last row's padding is
+// read too); dres (x_dtype), dh (bf16), dw (fp32 [cols], with dw_part [grid][cols]): null if not wanted.  grid: b200_add_rmsnorm_fp8_bwd_grid.
 extern "C" int b200_add_rmsnorm_fp8_bwd_grid(int rows, int cols, int num_sms) { return b200::norm_bwd_grid(rows, cols, num_sms); }
-extern "C" int b200_add_rmsnorm_fp8_bwd(const float* dn, const void* x, int x_dtype, const void* gx, const void* w, int w_dtype, const float* rstd,
+extern "C" int b200_add_rmsnorm_fp8_bwd(const float* dn, int64_t ld_dn, const void* x, int x_dtype, const void* gx, const void* w, int w_dtype, const float* rstd,
                                         void* dres, void* dh, float h_scale, float* dw_part, float* dw, int rows, int cols, int grid,
                                         cudaStream_t stream) {
   using namespace b200;
-  if (rows < 0 || cols < 1 || cols > 32768) return -6;
+  if (rows < 0 || cols < 1 || cols > 32768 || ld_dn % 8 || ld_dn < cols || reinterpret_cast<uintptr_t>(dn) % 16) return -6;
   if (rows == 0) return dw && cudaMemsetAsync(dw, 0, cols * sizeof(float), stream) != cudaSuccess ? -4 : 0;
   const auto al = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; };
-  const int vec = cols % 8 == 0 && al(dn) && al(x) && al(gx) && al(w) && al(dres) && al(dh) ? 1 : 0;
-  const Fp8NormBwdParams p{dn, x, gx, w, rstd, dres, static_cast<__nv_bfloat16*>(dh), dw ? dw_part : nullptr, h_scale, rows, cols, vec,
+  const int vec = cols % 8 == 0 && al(x) && al(gx) && al(w) && al(dres) && al(dh) ? 1 : 0;
+  const Fp8NormBwdParams p{dn, ld_dn, x, gx, w, rstd, dres, static_cast<__nv_bfloat16*>(dh), dw ? dw_part : nullptr, h_scale, rows, cols, vec,
                            w_dtype == 0 ? 1 : 0};
   const int rc = x_dtype == 0 ? launch_norm_bwd<float>(p, grid, stream) : launch_norm_bwd<__nv_bfloat16>(p, grid, stream);
   if (rc || !dw) return rc;
