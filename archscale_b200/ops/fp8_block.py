@@ -210,9 +210,15 @@ def linear_fp8_weight(x: Union[torch.Tensor, Quantised], weight: torch.Tensor, s
     if not isinstance(x, torch.Tensor):
         return matmul_fp8_block(x[0], x[1], weight, scale, bias, out_dtype or torch.bfloat16)
     _no_grad("linear_fp8_weight", x, bias)
+    dtype = out_dtype or x.dtype
+    if dtype not in _FLOATS:
+        raise TypeError(f"linear_fp8_weight: results are bfloat16 or float32, not {dtype}")
+    if _kernel(x):
+        backend.count_launch(2)
+        return backend.require_extension().linear_fp8_stored(x, weight, scale, bias, dtype is torch.float32)
     flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     q, s = quantize_fp8_block(flat)
-    y = matmul_fp8_block(q, s, weight, scale, bias, out_dtype or x.dtype)
+    y = matmul_fp8_block(q, s, weight, scale, bias, dtype)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
 
 
