@@ -304,8 +304,44 @@ def bench_nvfp4(res: list) -> None:
         print(res[-1], flush=True)
 
 
+def bench_fp8_block(res: list) -> None:
+    """e4m3 GEMM with fp32 scales per block of 128 (weights in 128 × 128 tiles, and both operands per row), its quantisers and the norm that writes
+    the format, against the bf16 and MXFP8 kernels on the same shapes."""
+    from archscale_b200.ops import mxfp8
+    ext = backend.require_extension()
+    pk = peaks()
+    for (M, N, K, what) in [(1, 11264, 2048, "one token w1 d16"), (48, 2048, 5632, "48 tokens w3 d16"), (1000, 11264, 2048, "1000 tokens w1 d16"),
+                            (32768, 11264, 2048, "fwd w1 d16"), (32768, 2048, 5632, "fwd w3 d16"), (8192, 8192, 8192, "square 8192")]:
+        a, b = torch.randn(M, K, device="cuda").bfloat16(), torch.randn(N, K, device="cuda").bfloat16()
+        aq, asc = ops.quantize_fp8_block(a)
+        wq, _, wsc = ops.quantize_fp8_weight(b)
+        bq, bsc = ops.quantize_fp8_block(b)
+        t_w = time_ms(lambda: ops.matmul_fp8_block(aq, asc, wq, wsc))
+        t_r = time_ms(lambda: ops.matmul_fp8_block(aq, asc, bq, bsc))
+        t_b = time_ms(lambda: ext.gemm_bf16(a, b, 0, torch.bfloat16, None))
+        r = {"kernel": "gemm_fp8_block", "case": what, "M": M, "N": N, "K": K, "tile_scales_ms": t_w, "row_scales_ms": t_r,
+             "tile_scales_tflops": 2.0 * M * N * K / t_w / 1e9, "row_scales_tflops": 2.0 * M * N * K / t_r / 1e9, "bf16_kernel_ms": t_b}
+        if M >= 128 and M % 128 == 0:
+            (ma, msa), (mb, msb) = mxfp8.quantize(a), mxfp8.quantize(b)
+            r["mxfp8_kernel_ms"] = time_ms(lambda: mxfp8.gemm(ma, msa, mb, msb))
+        res.append(r)
+        print(r, flush=True)
+    for (R, C) in [(1, 2048), (1001, 1501), (32768, 2048), (32768, 11264)]:
+        x, h, w = (torch.randn(R, C, device="cuda").bfloat16() for _ in range(3))
+        g = w[0].contiguous()
+        dn, rstd = torch.randn(R, (C + 7) // 8 * 8, device="cuda")[:, :C], torch.rand(R, device="cuda")
+        r = {"kernel": "fp8_block quantisers and norm", "rows": R, "cols": C}
+        for name, nbytes, fn in (("quantize", 3, lambda: ops.quantize_fp8_block(x)), ("quantize_both", 4, lambda: ops.quantize_fp8_block_both(x)),
+                                 ("quantize_weight", 4, lambda: ops.quantize_fp8_weight(x)), ("add_rms_norm", 7, lambda: ops.add_rms_norm_fp8(x, h, g)),
+                                 ("add_rms_norm_bwd", 12, lambda: ext.add_rmsnorm_fp8_bwd(h, dn, x, g, rstd, 0.5, True, True, True))):
+            t = time_ms(fn)
+            r[name + "_ms"], r[name + "_frac_of_" + pk["kind"] + "_hbm"] = t, nbytes * R * C / t / 1e6 / pk["hbm_gbs"]
+        res.append(r)
+        print(r, flush=True)
+
+
 ALL = {"gemm": bench_gemm, "rmsnorm": bench_rmsnorm, "swiglu": bench_swiglu, "ce": bench_ce, "rope": bench_rope,
-       "attn": bench_attn, "mamba": bench_mamba, "mxfp8": bench_mxfp8, "nvfp4": bench_nvfp4, "gdn": bench_gdn}
+       "attn": bench_attn, "mamba": bench_mamba, "mxfp8": bench_mxfp8, "nvfp4": bench_nvfp4, "fp8_block": bench_fp8_block, "gdn": bench_gdn}
 
 
 def main() -> None:

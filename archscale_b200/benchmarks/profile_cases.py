@@ -51,6 +51,22 @@ def case_nvfp4():
     _run(lambda: nvfp4.gemm(qa, qb))
 
 
+def case_fp8_block():
+    """Both products (scales of weight tiles, scales per row), quantiser of both orientations and norm."""
+    a, b = torch.randn(8192, 4096, device="cuda").bfloat16(), torch.randn(8192, 4096, device="cuda").bfloat16()
+    aq, asc, _, _ = ops.quantize_fp8_block_both(a)
+    wq, _, wsc = ops.quantize_fp8_weight(b)
+    bq, bsc = ops.quantize_fp8_block(b)
+    w = torch.randn(4096, device="cuda").bfloat16()
+
+    def once():
+        ops.matmul_fp8_block(aq, asc, wq, wsc)
+        ops.matmul_fp8_block(aq, asc, bq, bsc)
+        ops.add_rms_norm_fp8(a, b, w)
+        ops.matmul_fp8_block(aq[:48], asc[:48], wq, wsc)
+    _run(once)
+
+
 def _qkv(B=4, T=4096, H=16, G=4, D=128):
     mk = lambda h: torch.randn(B, T, h, D, device="cuda").bfloat16().requires_grad_()
     return mk(H), mk(G), mk(G)

@@ -339,14 +339,37 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, int n, bool vec, const 
 __device__ __forceinline__ float round_to(float v, const float*) { return v; }
 __device__ __forceinline__ float round_to(float v, const __nv_bfloat16*) { return __bfloat162float(__float2bfloat16(v)); }
 
-// PACK threads per row (0: the whole block, one row), V vectors of 8 per thread: the row stays in registers.  16 neighbouring threads
-// hold one block of 128.
-template <typename T, typename TO, int PACK, int V, bool VEC, bool H>
-__global__ void __launch_bounds__(PACK ? 128 : V > 2 ? 1024 : 512) fp8_norm_kernel(const Fp8NormParams p) {
-  __shared__ float s_sum[32];
+// The sum of `v` over the CTAs of a cluster, which each have the threads' sums of one part of a row: every CTA writes its own to all of them
+// (part: a buffer that nobody reads any more) and adds them in the order of the ranks.
+template <int CL>
+__device__ __forceinline__ float cluster_row_sum(float v, float* warps, float* part, int n_warps) {
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x < CL) {
+    v = 0.f;
+    for (int i = 0; i < n_warps; ++i) v += warps[i];
+    uint32_t to;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(part + cluster_ctarank())), "r"(threadIdx.x));
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
+  }
+  __syncwarp();
+  cluster_sync_all();
+  v = 0.f;
+#pragma unroll
+  for (int r = 0; r < CL; ++r) v += part[r];
+  return v;
+}
+
+constexpr int NORM_V = 2;       // vectors of 8 values per thread
+// PACK threads per row, or (0) a whole block, or a cluster of CL blocks: the row stays in registers.  16 neighbouring threads hold one block
+// of 128.
+template <typename T, typename TO, int PACK, int CL, bool VEC, bool H>
+__global__ void __launch_bounds__(PACK ? 128 : 512) fp8_norm_kernel(const Fp8NormParams p) {
+  constexpr int V = NORM_V;
+  __shared__ float s_sum[32], s_part[CL];
   const int TPR = PACK ? PACK : blockDim.x, RPC = PACK ? 128 / PACK : 1, WPR = TPR / 32;
-  const int t = PACK ? threadIdx.x % PACK : threadIdx.x, sub = PACK ? threadIdx.x / PACK : 0;
-  const int row = blockIdx.x * RPC + sub;
+  const int t = (PACK ? threadIdx.x % PACK : threadIdx.x) + (CL > 1 ? static_cast<int>(cluster_ctarank()) * TPR * V : 0);
+  const int sub = PACK ? threadIdx.x / PACK : 0, row = static_cast<int>(blockIdx.x) / CL * RPC + sub;
   const bool live = row < p.rows;
   const int64_t base = static_cast<int64_t>(row) * p.cols;
   Raw8<T> xr[V];
@@ -358,6 +381,7 @@ __global__ void __launch_bounds__(PACK ? 128 : V > 2 ? 1024 : 512) fp8_norm_kern
     load_raw<VEC>(static_cast<const T*>(p.res) + base + c, n, xr[i]);
     if (H) load_raw<VEC>(p.h + base + c, n, hr[i]);
   }
+  if (CL > 1) cluster_sync_all();                        // every block of the cluster has started
   float v[V][8];
   float ss = 0.f;
 #pragma unroll
@@ -377,7 +401,9 @@ __global__ void __launch_bounds__(PACK ? 128 : V > 2 ? 1024 : 512) fp8_norm_kern
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (WPR > 1) {
+  if (CL > 1) {
+    ss = cluster_row_sum<CL>(ss, s_sum, s_part, WPR);
+  } else if (WPR > 1) {
     if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = ss;
     __syncthreads();
     ss = 0.f;
@@ -411,24 +437,43 @@ __global__ void __launch_bounds__(PACK ? 128 : V > 2 ? 1024 : 512) fp8_norm_kern
   }
 }
 
+// Rows share a block up to 1024 columns; wider ones have as many threads as leave none idle (2560 columns: 160), and past 8192 columns a
+// cluster of blocks.  (One block of 1024 threads with four vectors each leaves 64 registers a thread: 32768 rows of 11264 bf16 took 1075 µs
+// instead of 590 and their gradients 6775 instead of 1091; 8192 rows of 32768 2144 instead of 820, but the norm itself 383 instead of 473.)
+struct NormShape { int pack, cl, threads; };
+static NormShape norm_shape(int cols) {
+  const int vecs = (cols + 7) / 8;
+  if (vecs <= 64) return {32, 1, 128};
+  if (vecs <= 128) return {64, 1, 128};
+  const int cl = vecs <= 1024 ? 1 : vecs <= 2048 ? 2 : 4;
+  return {0, cl, ((vecs + cl - 1) / cl + 32 * NORM_V - 1) / (32 * NORM_V) * 32};
+}
+template <typename P>
+static int launch_rows(void (*kern)(P), const P& p, int blocks, const NormShape& shape, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks * shape.cl);
+  cfg.blockDim = dim3(shape.threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = shape.cl; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = shape.cl > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? 0 : -3;
+}
+
 template <typename T, typename TO>
 static int launch_norm(const Fp8NormParams& p, cudaStream_t st) {
-  const int vecs = (p.cols + 7) / 8;
-#define FP8_NORM(PACK, V, BLOCK)                                                                             \
-  {                                                                                                          \
-    constexpr int RPC = PACK ? 128 / (PACK ? PACK : 1) : 1;                                                  \
-    const int grid = (p.rows + RPC - 1) / RPC, block = BLOCK;                                                \
-    if (p.vec && p.h) fp8_norm_kernel<T, TO, PACK, V, true, true><<<grid, block, 0, st>>>(p);                \
-    else if (p.vec) fp8_norm_kernel<T, TO, PACK, V, true, false><<<grid, block, 0, st>>>(p);                 \
-    else if (p.h) fp8_norm_kernel<T, TO, PACK, V, false, true><<<grid, block, 0, st>>>(p);                   \
-    else fp8_norm_kernel<T, TO, PACK, V, false, false><<<grid, block, 0, st>>>(p);                           \
-    return cudaGetLastError() == cudaSuccess ? 0 : -3;                                                       \
-  }
-  // narrow rows share a block; wider ones have as many threads as leave none idle (2560 columns: 160), two vectors each
-  if (vecs <= 64) FP8_NORM(32, 2, 128)
-  if (vecs <= 128) FP8_NORM(64, 2, 128)
-  if (vecs <= 1024) FP8_NORM(0, 2, (vecs + 63) / 64 * 32)
-  if (vecs <= 4096) FP8_NORM(0, 4, 1024)
+  const NormShape shape = norm_shape(p.cols);
+  const int rpc = shape.pack ? 128 / shape.pack : 1;
+  const int64_t blocks = (static_cast<int64_t>(p.rows) + rpc - 1) / rpc;
+  if (blocks * shape.cl > 0x7fffffff) return -6;
+#define FP8_NORM(PACK, CL)                                                                                                       \
+  if (shape.pack == PACK && shape.cl == CL)                                                                                      \
+    return launch_rows(p.vec ? (p.h ? fp8_norm_kernel<T, TO, PACK, CL, true, true> : fp8_norm_kernel<T, TO, PACK, CL, true, false>) \
+                             : (p.h ? fp8_norm_kernel<T, TO, PACK, CL, false, true> : fp8_norm_kernel<T, TO, PACK, CL, false, false>), \
+                       p, static_cast<int>(blocks), shape, st);
+  FP8_NORM(32, 1) FP8_NORM(64, 1) FP8_NORM(0, 1) FP8_NORM(0, 2) FP8_NORM(0, 4)
 #undef FP8_NORM
   return -6;
 }
@@ -448,13 +493,14 @@ struct Fp8NormBwdParams {
   int rows, cols, vec, w_f32;
 };
 
-template <typename T, int PACK, int V, bool VEC>
-__global__ void __launch_bounds__(PACK ? 128 : V > 2 ? 1024 : 512) fp8_norm_bwd_kernel(const Fp8NormBwdParams p) {
-  constexpr int RPC = PACK ? 128 / (PACK ? PACK : 1) : 1;
-  __shared__ float s_sum[2][32];
+template <typename T, int PACK, int CL, bool VEC>
+__global__ void __launch_bounds__(PACK ? 128 : 512) fp8_norm_bwd_kernel(const Fp8NormBwdParams p) {
+  constexpr int RPC = PACK ? 128 / (PACK ? PACK : 1) : 1, V = NORM_V;
+  __shared__ float s_sum[2][32], s_part[2][CL];
   __shared__ float s_dw[PACK ? 128 * V * 8 : 1];
   const int TPR = PACK ? PACK : blockDim.x, WPR = TPR / 32;
-  const int t = PACK ? threadIdx.x % PACK : threadIdx.x, sub = PACK ? threadIdx.x / PACK : 0;
+  const int t = (PACK ? threadIdx.x % PACK : threadIdx.x) + (CL > 1 ? static_cast<int>(cluster_ctarank()) * TPR * V : 0);
+  const int sub = PACK ? threadIdx.x / PACK : 0, blk = static_cast<int>(blockIdx.x) / CL, blks = static_cast<int>(gridDim.x) / CL;
   float w[V][8], dw[V][8];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -464,8 +510,9 @@ __global__ void __launch_bounds__(PACK ? 128 : V > 2 ? 1024 : 512) fp8_norm_bwd_
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[i][e] = 0.f;
   }
+  if (CL > 1) cluster_sync_all();                        // every block of the cluster has started
   int it = 0;
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * RPC; r0 < p.rows; r0 += gridDim.x * RPC, ++it) {      // as many turns for all threads of a block
+  for (int64_t r0 = static_cast<int64_t>(blk) * RPC; r0 < p.rows; r0 += blks * RPC, ++it) {      // as many turns for all threads of a block or cluster
     const int64_t row = r0 + sub, base = row * p.cols;
     const bool live = row < p.rows;
     Raw8<float> dr[V];
@@ -498,7 +545,9 @@ __global__ void __launch_bounds__(PACK ? 128 : V > 2 ? 1024 : 512) fp8_norm_bwd_
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if (WPR > 1) {                                       // two buffers: one barrier per row
+    if (CL > 1) {                                        // two buffers: one barrier per row
+      dot = cluster_row_sum<CL>(dot, s_sum[it & 1], s_part[it & 1], WPR);
+    } else if (WPR > 1) {
       if ((threadIdx.x & 31) == 0) s_sum[it & 1][threadIdx.x >> 5] = dot;
       __syncthreads();
       dot = 0.f;
@@ -524,7 +573,7 @@ __global__ void __launch_bounds__(PACK ? 128 : V > 2 ? 1024 : 512) fp8_norm_bwd_
     }
   }
   if (!p.dw_part) return;
-  float* out = p.dw_part + static_cast<int64_t>(blockIdx.x) * p.cols;
+  float* out = p.dw_part + static_cast<int64_t>(blk) * p.cols;
   if (PACK) {                                            // the block's rows in order
 #pragma unroll
     for (int i = 0; i < V; ++i)
@@ -553,28 +602,24 @@ __global__ void __launch_bounds__(1024) fp8_norm_dw_kernel(const float* __restri
   if (threadIdx.x < 32 && c < cols) out[c] = t;
 }
 
-// Blocks of the backward kernel (and rows of its partial sums): as many as fit the machine at once (≈ 100 registers a thread; one more block
-// per SM than fit, and a second wave of a few took 194 µs instead of 161 at 32768 × 2048).
+// Blocks (or clusters) of the backward kernel, and rows of its partial sums: as many blocks as fit the machine at once (≈ 100 registers a thread;
+// one more block per SM than fit, and a second wave of a few took 194 µs instead of 161 at 32768 × 2048).  How many clusters fit depends on the
+// machine's groups of SMs, so there are several times as many, which even out.
 static int norm_bwd_grid(int rows, int cols, int num_sms) {
-  const int vecs = (cols + 7) / 8, rpc = vecs <= 64 ? 4 : vecs <= 128 ? 2 : 1;
-  const int threads = vecs <= 128 ? 128 : vecs <= 1024 ? (vecs + 63) / 64 * 32 : 1024;
-  const int64_t need = (static_cast<int64_t>(rows) + rpc - 1) / rpc, room = static_cast<int64_t>(num_sms) * max(1, 640 / threads);
+  const NormShape shape = norm_shape(cols);
+  const int rpc = shape.pack ? 128 / shape.pack : 1;
+  const int64_t need = (static_cast<int64_t>(rows) + rpc - 1) / rpc;
+  const int64_t room = shape.cl > 1 ? num_sms : static_cast<int64_t>(num_sms) * max(1, 640 / shape.threads);
   return static_cast<int>(need < room ? need : room);
 }
 
 template <typename T>
 static int launch_norm_bwd(const Fp8NormBwdParams& p, int grid, cudaStream_t st) {
-  const int vecs = (p.cols + 7) / 8;
-#define FP8_NORM_BWD(PACK, V, BLOCK)                                                                         \
-  {                                                                                                          \
-    if (p.vec) fp8_norm_bwd_kernel<T, PACK, V, true><<<grid, BLOCK, 0, st>>>(p);                             \
-    else fp8_norm_bwd_kernel<T, PACK, V, false><<<grid, BLOCK, 0, st>>>(p);                                  \
-    return cudaGetLastError() == cudaSuccess ? 0 : -3;                                                       \
-  }
-  if (vecs <= 64) FP8_NORM_BWD(32, 2, 128)
-  if (vecs <= 128) FP8_NORM_BWD(64, 2, 128)
-  if (vecs <= 1024) FP8_NORM_BWD(0, 2, (vecs + 63) / 64 * 32)
-  if (vecs <= 4096) FP8_NORM_BWD(0, 4, 1024)
+  const NormShape shape = norm_shape(p.cols);
+#define FP8_NORM_BWD(PACK, CL)                                                                                                       \
+  if (shape.pack == PACK && shape.cl == CL)                                                                                          \
+    return launch_rows(p.vec ? fp8_norm_bwd_kernel<T, PACK, CL, true> : fp8_norm_bwd_kernel<T, PACK, CL, false>, p, grid, shape, st);
+  FP8_NORM_BWD(32, 1) FP8_NORM_BWD(64, 1) FP8_NORM_BWD(0, 1) FP8_NORM_BWD(0, 2) FP8_NORM_BWD(0, 4)
 #undef FP8_NORM_BWD
   return -6;
 }

@@ -460,3 +460,30 @@ def test_refusals(device):
     g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()                                                            # no gradient of the gradient
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [7, 200, 1001, 2048, 8192, 8200, 12001, 16384, 16392, 20000, 32767])
+@pytest.mark.parametrize("stream", [torch.bfloat16, torch.float32])
+def test_norm_backward_kernel(cols, stream):
+    """The norm's gradients of given fp32 dn, with more rows than blocks or clusters of blocks at every width, against 64 bits: a sum of `cols`
+    terms and a handful of roundings, then one to the output's type (2⁻⁸ for bf16)."""
+    from archscale_b200.ops import backend
+    rows, hs = (300 if cols > 2048 else 4000), 0.7
+    x = _rand((rows, cols), stream, "cuda", 1)
+    gx = _rand((rows, cols), stream, "cuda", 2)
+    dn = torch.full((rows, (cols + 7) // 8 * 8), float("nan"), device="cuda")[:, :cols]             # what lies past a row is not used
+    dn.copy_(_rand((rows, cols), torch.float32, "cuda", 3))
+    w = (1 + 0.1 * torch.randn(cols, device="cuda")).to(torch.bfloat16 if cols % 2 else torch.float32)
+    rstd = torch.rsqrt(x.float().square().mean(1) + 1e-5)
+    dres, dh, dw = backend.require_extension().add_rmsnorm_fp8_bwd(gx, dn, x, w, rstd, hs, True, True, True)
+    xhat, t = x.double() * rstd.double()[:, None], dn.double() * w.double()
+    r = rstd.double()[:, None]
+    want = gx.double() + r * (t - xhat * (t * xhat).mean(1, keepdim=True))
+    mag = gx.double().abs() + r * (t.abs() + xhat.abs() * (t * xhat).abs().mean(1, keepdim=True))
+    slack, out = (cols + 16) * 2.0 ** -24, 2.0 ** -8 if stream == torch.bfloat16 else 2.0 ** -24
+    assert ((dres.double() - want).abs() <= slack * mag + out * want.abs() * (1 + slack)).all()
+    assert ((dh.double() - hs * want).abs() <= slack * hs * mag + 2.0 ** -8 * (hs * want).abs() * (1 + slack)).all()
+    assert ((dw.double() - (dn.double() * xhat).sum(0)).abs() <= (rows + 8) * 2.0 ** -24 * (dn.double() * xhat).abs().sum(0)).all()
+    again = backend.require_extension().add_rmsnorm_fp8_bwd(gx, dn, x, w, rstd, hs, True, True, True)
+    assert all(torch.equal(a, b) for a, b in zip(again, (dres, dh, dw)))
