@@ -17,14 +17,37 @@ namespace b200 {
 
 constexpr float kE4m3Max = 448.f, kBlockFloor = 1e-30f;
 
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ float block_amax(uint32_t bits) {                        // NaN stays NaN
   return __uint_as_float(max(bits, __float_as_uint(kBlockFloor)));
+}
+__device__ __forceinline__ float max_abs(float a, float b, float c) {               // NaN if one of them is
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
   const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
   const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
   return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
+}
+
+// Two values at a time, each rounded as by itself.
+__device__ __forceinline__ void scale8(float (&v)[8], float u) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2 t = mul_f32x2(make_float2(v[e], v[e + 1]), make_float2(u, u));
+    v[e] = t.x; v[e + 1] = t.y;
+  }
+}
+__device__ __forceinline__ void mul8(float (&v)[8], const float (&w)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2 t = mul_f32x2(make_float2(v[e], v[e + 1]), make_float2(w[e], w[e + 1]));
+    v[e] = t.x; v[e + 1] = t.y;
+  }
+}
+__device__ __forceinline__ uint2 pack_e4m3x8(const float (&v)[8]) {
+  return make_uint2(pack_e4m3x4(v[0], v[1], v[2], v[3]), pack_e4m3x4(v[4], v[5], v[6], v[7]));
 }
 
 // Eight neighbouring values of a row, the first n of them inside it (the others are zero).
@@ -107,10 +130,8 @@ enum : int { FP8_ROWS = 1, FP8_COLS = 2, FP8_TILE = 4 };
 __device__ __forceinline__ void row_max(const Raw8<float> (&r)[8], uint32_t (&m)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float v[8] = {r[i].a.x, r[i].a.y, r[i].a.z, r[i].a.w, r[i].b.x, r[i].b.y, r[i].b.z, r[i].b.w};
-    m[i] = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m[i] = max(m[i], abs_bits(v[e]));
+    const float4 a = r[i].a, b = r[i].b;
+    m[i] = __float_as_uint(max_abs(max_abs(max_abs(a.x, a.y, a.z), a.w, b.x), b.y, max_abs(b.z, b.w, 0.f)));
   }
 }
 __device__ __forceinline__ void row_max(const Raw8<__nv_bfloat16> (&r)[8], uint32_t (&m)[8]) {
@@ -122,14 +143,17 @@ __device__ __forceinline__ void row_max(const Raw8<__nv_bfloat16> (&r)[8], uint3
   }
 }
 __device__ __forceinline__ void col_max(const Raw8<float> (&r)[8], uint32_t (&m)[8]) {
+  float t[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) m[e] = 0;
+  for (int e = 0; e < 8; ++e) t[e] = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float v[8] = {r[i].a.x, r[i].a.y, r[i].a.z, r[i].a.w, r[i].b.x, r[i].b.y, r[i].b.z, r[i].b.w};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m[e] = max(m[e], abs_bits(v[e]));
+  for (int i = 0; i < 8; i += 2) {
+    const float4 a = r[i].a, b = r[i].b, c = r[i + 1].a, d = r[i + 1].b;
+    t[0] = max_abs(t[0], a.x, c.x); t[1] = max_abs(t[1], a.y, c.y); t[2] = max_abs(t[2], a.z, c.z); t[3] = max_abs(t[3], a.w, c.w);
+    t[4] = max_abs(t[4], b.x, d.x); t[5] = max_abs(t[5], b.y, d.y); t[6] = max_abs(t[6], b.z, d.z); t[7] = max_abs(t[7], b.w, d.w);
   }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m[e] = __float_as_uint(t[e]);
 }
 __device__ __forceinline__ void col_max(const Raw8<__nv_bfloat16> (&r)[8], uint32_t (&m)[8]) {
   uint32_t t[4] = {0u, 0u, 0u, 0u};
@@ -218,10 +242,8 @@ __device__ __forceinline__ void fp8_tile(const Fp8TileParams& p, const Raw8<T> (
       const float u = MODE == FP8_TILE ? u_tile : __uint_as_float(s_row[rg * 8 + i]);
       float o[8];
       unpack8(raw[i], o);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = __fmul_rn(o[e], u);
-      if (r0 + i < p.rows)
-        *reinterpret_cast<uint2*>(q + i * p.ldq) = make_uint2(pack_e4m3x4(o[0], o[1], o[2], o[3]), pack_e4m3x4(o[4], o[5], o[6], o[7]));
+      scale8(o, u);
+      if (r0 + i < p.rows) *reinterpret_cast<uint2*>(q + i * p.ldq) = pack_e4m3x8(o);
     }
   }
   if ((MODE & FP8_COLS) || (MODE == FP8_TILE && p.qt)) {
@@ -238,9 +260,9 @@ __device__ __forceinline__ void fp8_tile(const Fp8TileParams& p, const Raw8<T> (
     for (int e = 0; e < 8; ++e) {
       float o[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = __fmul_rn(v[i][e], uc[e]);
-      *reinterpret_cast<uint2*>(s_t + (cg * 8 + e) * 128 + (((rg >> 1) ^ (cg & 7)) << 4) + ((rg & 1) << 3)) =
-          make_uint2(pack_e4m3x4(o[0], o[1], o[2], o[3]), pack_e4m3x4(o[4], o[5], o[6], o[7]));
+      for (int i = 0; i < 8; ++i) o[i] = v[i][e];
+      scale8(o, uc[e]);
+      *reinterpret_cast<uint2*>(s_t + (cg * 8 + e) * 128 + (((rg >> 1) ^ (cg & 7)) << 4) + ((rg & 1) << 3)) = pack_e4m3x8(o);
     }
     __syncthreads();
 #pragma unroll
@@ -254,9 +276,10 @@ __device__ __forceinline__ void fp8_tile(const Fp8TileParams& p, const Raw8<T> (
   }
 }
 
-// One CTA per tile, read once.
+// One CTA per tile, read once.  Four fit an SM with bf16 (the form for any alignment has to be told: with 70 registers 317 µs instead of 270 at
+// 30568 × 7981); fp32 takes the registers that it needs.
 template <typename T, int MODE, bool NORM, bool VEC>
-__global__ void __launch_bounds__(256) fp8_tile_kernel(const Fp8TileParams p) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && !NORM && !VEC ? 4 : 0) fp8_tile_kernel(const Fp8TileParams p) {
   __shared__ uint32_t s_row[128];
   __shared__ __align__(16) uint32_t s_col[8][128];
   __shared__ __align__(16) uint8_t s_t[(MODE & FP8_COLS) || MODE == FP8_TILE ? 128 * 128 : 16];
@@ -278,8 +301,8 @@ __global__ void __launch_bounds__(256) fp8_tile_kernel(const Fp8TileParams p) {
       const float rs = r0 + i < p.rows ? p.rstd[r0 + i] : 0.f;
       float t[8];
       unpack8(raw[i], t);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) t[e] = __fmul_rn(__fmul_rn(t[e], rs), w[e]);
+      scale8(t, rs);
+      mul8(t, w);
       v[i].a = make_float4(t[0], t[1], t[2], t[3]);
       v[i].b = make_float4(t[4], t[5], t[6], t[7]);
     }
@@ -362,9 +385,11 @@ __device__ __forceinline__ float cluster_row_sum(float v, float* warps, float* p
 
 constexpr int NORM_V = 2;       // vectors of 8 values per thread
 // PACK threads per row, or (0) a whole block, or a cluster of CL blocks: the row stays in registers.  16 neighbouring threads hold one block
-// of 128.
+// of 128.  Instructions cost nearly as much as bytes do (81 % of the issue slots were taken), hence values in pairs, maxima of three, and a
+// half warp's four divisions at once: 16384 × 8192 bf16 149 µs (6.3 TB/s) instead of 189, 32768 × 2048 76 (6.2 TB/s) instead of 85.  40 registers
+// (1536 threads per SM) are worth the few that are spilled: fp32 at 30568 × 7981 874 µs, 1002 with 44 to 51.
 template <typename T, typename TO, int PACK, int CL, bool VEC, bool H>
-__global__ void __launch_bounds__(PACK ? 128 : 512) fp8_norm_kernel(const Fp8NormParams p) {
+__global__ void __launch_bounds__(PACK ? 128 : 512, PACK ? 12 : 3) fp8_norm_kernel(const Fp8NormParams p) {
   constexpr int V = NORM_V;
   __shared__ float s_sum[32], s_part[CL];
   const int TPR = PACK ? PACK : blockDim.x, RPC = PACK ? 128 / PACK : 1, WPR = TPR / 32;
@@ -392,8 +417,9 @@ __global__ void __launch_bounds__(PACK ? 128 : 512) fp8_norm_kernel(const Fp8Nor
     if (H) {
       float h[8];
       unpack8(hr[i], h);
+      scale8(h, p.h_scale);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = round_to(__fadd_rn(v[i][e], __fmul_rn(p.h_scale, h[e])), static_cast<const TO*>(nullptr));
+      for (int e = 0; e < 8; ++e) v[i][e] = round_to(__fadd_rn(v[i][e], h[e]), static_cast<const TO*>(nullptr));
       if (n > 0) store8(static_cast<TO*>(p.x) + base + c, n, VEC, v[i]);
     }
 #pragma unroll
@@ -411,6 +437,7 @@ __global__ void __launch_bounds__(PACK ? 128 : 512) fp8_norm_kernel(const Fp8Nor
   }
   const float rs = rsqrtf(ss / static_cast<float>(p.cols) + p.eps);
   if (live && t == 0 && p.rstd) p.rstd[row] = rs;
+  float m[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = (t + i * TPR) * 8;
@@ -418,21 +445,24 @@ __global__ void __launch_bounds__(PACK ? 128 : 512) fp8_norm_kernel(const Fp8Nor
     float w[8];
     if (p.w_f32) load8<VEC>(static_cast<const float*>(p.w) + c, n, w);
     else load8<VEC>(static_cast<const __nv_bfloat16*>(p.w) + c, n, w);
-    uint32_t m = 0;
+    scale8(v[i], rs);                                    // (zeros past the row stay zeros, or rs is no number and neither is any value of the row)
+    mul8(v[i], w);
+    m[i] = max_abs(max_abs(max_abs(v[i][0], v[i][1], v[i][2]), v[i][3], v[i][4]), v[i][5], max_abs(v[i][6], v[i][7], 0.f));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[i][e] = __fmul_rn(__fmul_rn(v[i][e], rs), w[e]);
-      m = max(m, e < n ? abs_bits(v[i][e]) : 0u);
-    }
+    for (int o = 8; o > 0; o >>= 1) m[i] = max_abs(m[i], __shfl_xor_sync(0xffffffffu, m[i], o), kBlockFloor);
+  }
+  // the four divisions of two blocks on four lanes of each half warp: scales on the even ones
+  static_assert(V == 2);
+  const float a = (t & 2) ? m[1] : m[0];
+  const float f = __fdiv_rn((t & 1) ? kE4m3Max : a, (t & 1) ? a : kE4m3Max);
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (n > 0) {
-      const float a = block_amax(m), u = __fdiv_rn(kE4m3Max, a);
-      if ((t & 15) == 0) p.s[(c >> 7) * p.lds + row] = __fdiv_rn(a, kE4m3Max);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = __fmul_rn(v[i][e], u);
-      *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) =
-          make_uint2(pack_e4m3x4(v[i][0], v[i][1], v[i][2], v[i][3]), pack_e4m3x4(v[i][4], v[i][5], v[i][6], v[i][7]));
+  for (int i = 0; i < V; ++i) {
+    const int c = (t + i * TPR) * 8;
+    const float u = __shfl_sync(0xffffffffu, f, 2 * i + 1, 16);
+    if (live && (t & 15) == 2 * i && c - 16 * i < p.cols) p.s[(c >> 7) * p.lds + row] = f;
+    if (live && c < p.cols) {
+      scale8(v[i], u);
+      *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) = pack_e4m3x8(v[i]);
     }
   }
 }
