@@ -512,7 +512,7 @@ static int launch_norm(const Fp8NormParams& p, cudaStream_t st) {
 // With x̂ = x · rstd, t = dn · w:   d_res = g_x + rstd · (t − x̂ · mean(t · x̂)),   d_h = h_scale · d_res,   d_w = Σ_rows dn · x̂.
 // dn is the fp32 output of the product behind the norm: rounded to bf16 it made the sums over rows 1.5 times as far off.
 // Threads hold the columns that they hold in the forward kernel, so that d_w is summed in registers over a block's rows; the blocks' sums meet in
-// a second kernel, in a fixed order.  Bound by memory: 12 bytes per element with a bf16 stream.
+// a second kernel, in a fixed order.  Bound by memory: 12 bytes per element with a bf16 stream (32768 × 2048 142 µs, 5.7 TB/s).
 struct Fp8NormBwdParams {
   const float* dn; int64_t ld_dn;       // rows of whole 32-byte pieces, whatever cols is
   const void *x, *gx, *w;
@@ -524,7 +524,7 @@ struct Fp8NormBwdParams {
 };
 
 template <typename T, int PACK, int CL, bool VEC>
-__global__ void __launch_bounds__(PACK ? 128 : 512) fp8_norm_bwd_kernel(const Fp8NormBwdParams p) {
+__global__ void __maxnreg__(CL > 1 ? 128 : 96) fp8_norm_bwd_kernel(const Fp8NormBwdParams p) {
   constexpr int RPC = PACK ? 128 / (PACK ? PACK : 1) : 1, V = NORM_V;
   __shared__ float s_sum[2][32], s_part[2][CL];
   __shared__ float s_dw[PACK ? 128 * V * 8 : 1];
@@ -632,9 +632,9 @@ __global__ void __launch_bounds__(1024) fp8_norm_dw_kernel(const float* __restri
   if (threadIdx.x < 32 && c < cols) out[c] = t;
 }
 
-// Blocks (or clusters) of the backward kernel, and rows of its partial sums: as many blocks as fit the machine at once (≈ 100 registers a thread;
-// one more block per SM than fit, and a second wave of a few took 194 µs instead of 161 at 32768 × 2048).  How many clusters fit depends on the
-// machine's groups of SMs, so there are several times as many, which even out.
+// Blocks (or clusters) of the backward kernel, and rows of its partial sums: as many blocks as fit the machine at once (96 registers a thread; with
+// up to 128, as the compiler chose, only four of the five blocks per SM fit and 32768 × 2048 took 177 µs instead of 142).  How many clusters fit
+// depends on the machine's groups of SMs, so there are several times as many, which even out.
 static int norm_bwd_grid(int rows, int cols, int num_sms) {
   const NormShape shape = norm_shape(cols);
   const int rpc = shape.pack ? 128 / shape.pack : 1;
