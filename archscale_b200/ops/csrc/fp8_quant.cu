@@ -323,7 +323,10 @@ static int launch_tile(const Fp8TileParams& p, cudaStream_t st) {
 
 // ------------------------------------------------------------------ residual addition + RMSNorm → e4m3
 //   x = res + h_scale · h (fp32, rounded to the stream's type),  n = x · rsqrt(mean x² + eps) · w (fp32),  n quantised in blocks of 128
-// n is never rounded to 16 bits: the only rounding between the stream and the tensor cores is the one to e4m3.
+// n is never rounded to 16 bits: the only rounding between the stream and the tensor cores is the one to e4m3.  1 / rms is common to a block, so
+// with y = x · w (exact for bf16) and m = max |y| of the block, a = m / rms and n · 448 / a is y · (448 / m), where 448 / m is held with its rest
+// in two numbers: what is rounded to e4m3 is off by half a unit of fp32, and values half way between two of e4m3, which factors of 8 bits
+// make one in ten thousand, are found to be so.  Blocks at the floor of a, or with m below it, take (y / rms) · (448 / a).
 struct Fp8NormParams {
   const void* res; const __nv_bfloat16* h; const void* w;
   float h_scale, eps;
@@ -445,23 +448,33 @@ __global__ void __launch_bounds__(PACK ? 128 : 512, PACK ? 12 : 3) fp8_norm_kern
     float w[8];
     if (p.w_f32) load8<VEC>(static_cast<const float*>(p.w) + c, n, w);
     else load8<VEC>(static_cast<const __nv_bfloat16*>(p.w) + c, n, w);
-    scale8(v[i], rs);                                    // (zeros past the row stay zeros, or rs is no number and neither is any value of the row)
     mul8(v[i], w);
     m[i] = max_abs(max_abs(max_abs(v[i][0], v[i][1], v[i][2]), v[i][3], v[i][4]), v[i][5], max_abs(v[i][6], v[i][7], 0.f));
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m[i] = max_abs(m[i], __shfl_xor_sync(0xffffffffu, m[i], o), kBlockFloor);
+    for (int o = 8; o > 0; o >>= 1) m[i] = max_abs(m[i], __shfl_xor_sync(0xffffffffu, m[i], o), 0.f);
   }
-  // the four divisions of two blocks on four lanes of each half warp: scales on the even ones
+  // the four divisions of two blocks on four lanes of each half warp: scales on the even ones, on the odd ones u = 448 / m and its rest, or,
+  // marked by a rest that is no number, 448 / a
   static_assert(V == 2);
-  const float a = (t & 2) ? m[1] : m[0];
-  const float f = __fdiv_rn((t & 1) ? kE4m3Max : a, (t & 1) ? a : kE4m3Max);
+  const bool odd = (t & 1) != 0;
+  const float top = (t & 2) ? m[1] : m[0], a = max_abs(__fmul_rn(top, rs), kBlockFloor, 0.f);
+  const bool large = a > kBlockFloor && top > kBlockFloor;
+  const float f = __fdiv_rn(odd ? kE4m3Max : a, !odd ? kE4m3Max : large ? top : a);
+  const float rest = large ? fmaf(-f, top, kE4m3Max) * f * (1.f / kE4m3Max) : __int_as_float(0x7fffffff);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = (t + i * TPR) * 8;
     const float u = __shfl_sync(0xffffffffu, f, 2 * i + 1, 16);
+    float u2 = __shfl_sync(0xffffffffu, rest, 2 * i + 1, 16);
     if (live && (t & 15) == 2 * i && c - 16 * i < p.cols) p.s[(c >> 7) * p.lds + row] = f;
     if (live && c < p.cols) {
-      scale8(v[i], u);
+      if (u2 != u2) { scale8(v[i], rs); u2 = 0.f; }
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float2 y = make_float2(v[i][e], v[i][e + 1]);
+        const float2 z = fma_f32x2(y, make_float2(u, u), mul_f32x2(y, make_float2(u2, u2)));
+        v[i][e] = z.x; v[i][e + 1] = z.y;
+      }
       *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) = pack_e4m3x8(v[i]);
     }
   }

@@ -487,3 +487,25 @@ def test_norm_backward_kernel(cols, stream):
     assert ((dw.double() - (dn.double() * xhat).sum(0)).abs() <= (rows + 8) * 2.0 ** -24 * (dn.double() * xhat).abs().sum(0)).all()
     again = backend.require_extension().add_rmsnorm_fp8_bwd(gx, dn, x, w, rstd, hs, True, True, True)
     assert all(torch.equal(a, b) for a, b in zip(again, (dres, dh, dw)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [128, 1001, 2048, 8320])
+def test_norm_elements_of_16_bit_factors_are_those_of_the_reals(cols):
+    """With bf16 stream and weight, n · 448 / a = 448 · y / max|y| with y = x · w of 16 bits: its distance from a value half way between two of e4m3
+    is nothing or more than 2⁻²² of it, so that half a unit of fp32 cannot change an element.  Rows at the floor of a only get a bound."""
+    size = torch.tensor([0.0, 1e-33, 1e-31, 1e-20, 1e-3, 1.0, 30.0, 1e15], device="cuda").repeat_interleave(40)[:, None]
+    x = (_rand((size.shape[0], cols), torch.float32, "cuda", 1) * size).to(torch.bfloat16)
+    w = (1 + 0.1 * torch.randn(cols, generator=_gen(2, "cuda"), device="cuda")).to(torch.bfloat16)
+    _, q, s = ops.add_rms_norm_fp8(x, None, w)
+    y = torch.nn.functional.pad(x.double() * w.double(), (0, -cols % 128)).view(len(x), -1, 128)
+    r = 1 / (x.double().square().mean(1) + 1e-5).sqrt()
+    a = (y.abs().amax(-1) * r[:, None]).clamp_min(1e-30)
+    v = y * r[:, None, None] * 448 / a[..., None]
+    exact = torch.where(a[..., None] > 1e-30, y * 448 / y.abs().amax(-1, keepdim=True), v)               # one rounding, so that halves stay halves
+    want = exact.float().to(torch.float8_e4m3fn).float().view(len(x), -1)[:, :cols]
+    large = (y.abs().amax(-1) > 1e-30).repeat_interleave(128, 1)[:, :cols]
+    got, v = q.float(), v.view(len(x), -1)[:, :cols]
+    assert large.any() and (~large).any() and (got[large] == want[large]).all()
+    assert ((got.double() - v).abs() <= v.abs() * 2.0 ** -4 * (1 + 1e-5) + 2.0 ** -10 * (1 + 1e-5)).all()
+    assert ((s.double() - a / 448).abs() <= (cols + 16) * 2.0 ** -24 * a / 448 + 1e-45).all()
