@@ -337,26 +337,76 @@ struct Fp8NormParams {
   float* rstd;                  // [rows] or null
 };
 
-__device__ __forceinline__ void store8(float* p, int n, bool vec, const float (&v)[8]) {
-  if (vec && n >= 8) {
+// Eight values of a row per lane, neighbouring lanes' next to each other, by all lanes of a warp (n ≤ 0: none of this lane's).  Rows that start
+// anywhere leave in aligned 16-byte pieces all the same: a lane gives its first values to the lane before it and takes the next one's; what no
+// whole piece covers goes value by value.
+template <bool VEC>
+__device__ __forceinline__ void store_row(float* p, int n, const float (&v)[8]) {
+  if (VEC) {
+    if (n <= 0) return;
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
     *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) if (i < n) p[i] = v[i];
+    return;
   }
+  const int lane = threadIdx.x & 31, s = (-static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 2)) & 3;       // values up to a boundary
+  float w[11], t[9];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = v[i];
+#pragma unroll
+  for (int i = 0; i < 3; ++i) w[8 + i] = __shfl_down_sync(0xffffffffu, v[i], 1);
+  const int behind = __shfl_down_sync(0xffffffffu, n, 1);
+  const bool one = n >= s + 4, two = n >= 8 && (s == 0 || (lane < 31 && behind >= s));
+  const bool before = __shfl_up_sync(0xffffffffu, two ? 1 : 0, 1) && lane > 0;
+#pragma unroll
+  for (int i = 0; i < 9; ++i) t[i] = (s & 2) ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = (s & 1) ? t[i + 1] : t[i];
+  if (one) *reinterpret_cast<float4*>(p + s) = make_float4(w[0], w[1], w[2], w[3]);
+  if (two) *reinterpret_cast<float4*>(p + s + 4) = make_float4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) if (e < n && !(e < s ? before : e < s + 4 ? one : two)) p[e] = v[e];
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, int n, bool vec, const float (&v)[8]) {
-  if (vec && n >= 8) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-  } else if (n >= 8 && (reinterpret_cast<uintptr_t>(p) & 2)) {       // pairs that lie on 4 bytes
-    p[0] = __float2bfloat16(v[0]);
+template <bool VEC>
+__device__ __forceinline__ void store_row(__nv_bfloat16* p, int n, const float (&v)[8]) {
+  uint32_t w[8];
 #pragma unroll
-    for (int i = 1; i < 7; i += 2) *reinterpret_cast<uint32_t*>(p + i) = pack_bf16x2(v[i], v[i + 1]);
-    p[7] = __float2bfloat16(v[7]);
-  } else if (n >= 8) {
+  for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+  if (VEC) {
+    if (n > 0) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    return;
+  }
+  const int lane = threadIdx.x & 31, s = (-static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1)) & 7;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) *reinterpret_cast<uint32_t*>(p + i) = pack_bf16x2(v[i], v[i + 1]);
+  for (int i = 0; i < 4; ++i) w[4 + i] = __shfl_down_sync(0xffffffffu, w[i], 1);
+  const int behind = __shfl_down_sync(0xffffffffu, n, 1);
+  const bool full = n >= 8 && (s == 0 || (lane < 31 && behind >= s));
+  const bool before = __shfl_up_sync(0xffffffffu, full ? 1 : 0, 1) && lane > 0;
+  uint32_t t[6], u[5], o[4];
+#pragma unroll
+  for (int i = 0; i < 6; ++i) t[i] = (s & 4) ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) u[i] = (s & 2) ? t[i + 1] : t[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = __funnelshift_r(u[i], u[i + 1], (s & 1) * 16);
+  if (full) *reinterpret_cast<uint4*>(p + s) = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < n && !(e < s ? before : full)) p[e] = __ushort_as_bfloat16(static_cast<unsigned short>(w[e >> 1] >> ((e & 1) * 16)));
+}
+// bf16 in pairs that lie on 4 bytes: fewer instructions, which the norm itself is bound by (30568 × 7981: 515 µs this way, 584 in whole pieces,
+// while its gradients take 1392 and 1183; fp32 880 and 642, 1834 and 1148).
+__device__ __forceinline__ void store_pairs(__nv_bfloat16* p, int n, const float (&v)[8]) {
+  if (n >= 8) {
+    const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 1;
+    if (odd) {
+      p[0] = __float2bfloat16(v[0]);
+#pragma unroll
+      for (int i = 1; i < 7; i += 2) *reinterpret_cast<uint32_t*>(p + i) = pack_bf16x2(v[i], v[i + 1]);
+      p[7] = __float2bfloat16(v[7]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) *reinterpret_cast<uint32_t*>(p + i) = pack_bf16x2(v[i], v[i + 1]);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) if (i < n) p[i] = __float2bfloat16(v[i]);
@@ -423,7 +473,8 @@ __global__ void __launch_bounds__(PACK ? 128 : 512, PACK ? 12 : 3) fp8_norm_kern
       scale8(h, p.h_scale);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] = round_to(__fadd_rn(v[i][e], h[e]), static_cast<const TO*>(nullptr));
-      if (n > 0) store8(static_cast<TO*>(p.x) + base + c, n, VEC, v[i]);
+      if constexpr (!VEC && sizeof(TO) == 2) store_pairs(static_cast<TO*>(p.x) + base + c, n, v[i]);
+      else store_row<VEC>(static_cast<TO*>(p.x) + base + c, n, v[i]);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss += v[i][e] * v[i][e];
@@ -525,7 +576,7 @@ static int launch_norm(const Fp8NormParams& p, cudaStream_t st) {
 // With x̂ = x · rstd, t = dn · w:   d_res = g_x + rstd · (t − x̂ · mean(t · x̂)),   d_h = h_scale · d_res,   d_w = Σ_rows dn · x̂.
 // dn is the fp32 output of the product behind the norm: rounded to bf16 it made the sums over rows 1.5 times as far off.
 // Threads hold the columns that they hold in the forward kernel, so that d_w is summed in registers over a block's rows; the blocks' sums meet in
-// a second kernel, in a fixed order.  Bound by memory: 12 bytes per element with a bf16 stream (32768 × 2048 142 µs, 5.7 TB/s).
+// a second kernel, in a fixed order.  Bound by memory: 12 bytes per element with a bf16 stream (32768 × 2048 136 µs, 5.9 TB/s).
 struct Fp8NormBwdParams {
   const float* dn; int64_t ld_dn;       // rows of whole 32-byte pieces, whatever cols is
   const void *x, *gx, *w;
@@ -605,13 +656,10 @@ __global__ void __maxnreg__(CL > 1 ? 128 : 96) fp8_norm_bwd_kernel(const Fp8Norm
       unpack8(dr[i], d); unpack8(xr[i], x); unpack8(gr[i], g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) g[e] += rs * (d[e] * w[i][e] - x[e] * rs * mean);
-      if (n > 0) {
-        if (p.dres) store8(static_cast<T*>(p.dres) + base + c, n, VEC, g);
-        if (p.dh) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) g[e] *= p.h_scale;
-          store8(p.dh + base + c, n, VEC, g);
-        }
+      if (p.dres) store_row<VEC>(static_cast<T*>(p.dres) + base + c, n, g);
+      if (p.dh) {
+        scale8(g, p.h_scale);
+        store_row<VEC>(p.dh + base + c, n, g);
       }
     }
   }
@@ -635,7 +683,7 @@ __global__ void __maxnreg__(CL > 1 ? 128 : 96) fp8_norm_bwd_kernel(const Fp8Norm
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int c = (t + i * TPR) * 8;
-      store8(out + c, min(max(p.cols - c, 0), 8), false, dw[i]);
+      store_row<VEC>(out + c, min(max(p.cols - c, 0), 8), dw[i]);
     }
   }
 }
