@@ -99,20 +99,64 @@ __device__ __forceinline__ void f2_tma_add_2d(const CUtensorMap* map, const void
   asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
                ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(smem_src)), "r"(x), "r"(y) : "memory");
 }
-// A piece of 32 × 32 fp32 values to an output that TMA cannot write: lane = column, one row after the other.
-__device__ __forceinline__ void f2_store_piece(const uint8_t* piece, const F2Params& p, int row0, int col0, int lane) {
-  const int rows = min(p.M - row0, 32), col = col0 + lane;
-  if (col >= p.N) return;
-#pragma unroll 4
-  for (int r = 0; r < rows; ++r) {
-    const float v = *reinterpret_cast<const float*>(piece + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + ((lane & 3) << 2));
-    const int64_t at = static_cast<int64_t>(row0 + r) * p.ldc + col;
-    if (p.out_f32) {
-      float* o = static_cast<float*>(p.out) + at;
-      *o = p.accumulate ? *o + v : v;
-    } else {
-      static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16(v);
+// Pieces to an output that TMA cannot write.  Two warps per scheduler have nothing to hide instructions behind, so these are few per row: eight
+// rows on their way at a time, pointers that advance, all that depends on the alignment outside the loop (a plain loop over rows took 25 instructions
+// for 32 columns, and 2048 × 11263 × 256 49 µs instead of 33; 11264 columns, by TMA, 21).
+// 32 × 32 fp32 values, lane = column.
+__device__ __forceinline__ void f2_store_piece32(const uint8_t* piece, const F2Params& p, int row0, int col0, int lane) {
+  const int rows = col0 + lane < p.N ? p.M - row0 : 0;
+  float* o = static_cast<float*>(p.out) + static_cast<int64_t>(row0) * p.ldc + col0 + lane;
+#pragma unroll 1
+  for (int r0 = 0; r0 < 32; r0 += 8) {
+    float v[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v[r] = *reinterpret_cast<const float*>(piece + (r0 + r) * 128 + (((lane >> 2) ^ r) << 4) + ((lane & 3) << 2));
+    if (p.accumulate) {
+      float old[8];
+      const float* in = o;
+#pragma unroll
+      for (int r = 0; r < 8; ++r, in += p.ldc) old[r] = r0 + r < rows ? *in : 0.f;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v[r] += old[r];
     }
+#pragma unroll
+    for (int r = 0; r < 8; ++r, o += p.ldc) if (r0 + r < rows) *o = v[r];
+  }
+}
+// 32 × 64 bf16 values, two per lane: the rows K, K + STEP, ..  They start on 4 bytes, or (ODD) 2 bytes after such an address, and then get their pairs
+// one column later, and the first value and the last by themselves.
+template <int STEP, int K, bool ODD>
+__device__ __forceinline__ void f2_store_rows(const uint8_t* piece, __nv_bfloat16* o, int64_t ldc, int rows, int cols, int lane) {
+  const int c = 2 * lane + (ODD ? 1 : 0);
+  const int pair = c + 1 < cols ? rows : 0, last = c < cols && !pair ? rows : 0, first = ODD && lane == 0 && cols > 0 ? rows : 0;
+  o += K * ldc;
+#pragma unroll 1
+  for (int r0 = K; r0 < 32; r0 += 8 * STEP) {
+    uint32_t v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = *reinterpret_cast<const uint32_t*>(piece + (r0 + i * STEP) * 128 + (((lane >> 2) ^ ((K + i * STEP) & 7)) << 4) + ((lane & 3) << 2));
+#pragma unroll
+    for (int i = 0; i < 8; ++i, o += STEP * ldc) {
+      const int r = r0 + i * STEP;
+      const uint32_t w = ODD ? __funnelshift_r(v[i], __shfl_down_sync(0xffffffffu, v[i], 1), 16) : v[i];
+      if (r < pair) *reinterpret_cast<uint32_t*>(o + c) = w;
+      if (r < last) o[c] = __ushort_as_bfloat16(static_cast<unsigned short>(w));
+      if (r < first) o[0] = __ushort_as_bfloat16(static_cast<unsigned short>(v[i]));
+    }
+  }
+}
+__device__ __forceinline__ void f2_store_piece16(const uint8_t* piece, const F2Params& p, int row0, int col0, int lane) {
+  const int rows = p.M - row0, cols = p.N - col0 < 64 ? p.N - col0 : 64;
+  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(row0) * p.ldc + col0;
+  const bool odd = (reinterpret_cast<uintptr_t>(o) & 2) != 0;
+  if (p.ldc & 1) {
+    if (odd) { f2_store_rows<2, 0, true>(piece, o, p.ldc, rows, cols, lane); f2_store_rows<2, 1, false>(piece, o, p.ldc, rows, cols, lane); }
+    else { f2_store_rows<2, 0, false>(piece, o, p.ldc, rows, cols, lane); f2_store_rows<2, 1, true>(piece, o, p.ldc, rows, cols, lane); }
+  } else if (odd) {
+    f2_store_rows<1, 0, true>(piece, o, p.ldc, rows, cols, lane);
+  } else {
+    f2_store_rows<1, 0, false>(piece, o, p.ldc, rows, cols, lane);
   }
 }
 
@@ -365,7 +409,7 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
       // pieces of 32 rows × 128 bytes: 16-byte parts at part ^ (row % 8), the order of the output's tensor map
       auto part = [&](int j) { return reinterpret_cast<uint4*>(piece + lane * 128 + ((j ^ (lane & 7)) << 4)); };
       auto frag = [&](int g, int j) { return piece + (g * 8 + (lane >> 2)) * 128 + ((j ^ (lane >> 2)) << 4); };      // part j of row 8 g + lane / 4
-      if (p.tma_out && !p.out_f32) {
+      if (!p.out_f32) {
 #pragma unroll
         for (int c = 0; c < W / 64; ++c) {
           if (lane == 0) tma_store_wait_read<0>();
@@ -383,9 +427,15 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
               }
             }
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0 && row0 < p.M && c0 + c * 64 < p.N) { tma_store_2d(&tmap_out, piece, c0 + c * 64, row0); tma_store_commit(); }
+          if (p.tma_out) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && row0 < p.M && c0 + c * 64 < p.N) { tma_store_2d(&tmap_out, piece, c0 + c * 64, row0); tma_store_commit(); }
+          } else {
+            __syncwarp();
+            f2_store_piece16(piece, p, row0, c0 + c * 64, lane);
+            __syncwarp();
+          }
         }
       } else {
 #pragma unroll
@@ -415,7 +465,7 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             }
           } else {
             __syncwarp();
-            f2_store_piece(piece, p, row0, c0 + c * 32, lane);
+            f2_store_piece32(piece, p, row0, c0 + c * 32, lane);
             __syncwarp();
           }
         }
