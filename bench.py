@@ -271,7 +271,7 @@ def run_ours(args) -> None:
             "metric": "train tokens/sec (whole job; per GPU = value / n_gpus), device-timed, max over ranks",
             "value": value, "unit": "tokens/s", "n_gpus": world, "steps": args.steps, "warmup": args.warmup,
             "ms_per_step": ms_per_step, "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
-            "dtype": "nvfp4 linears (bf16 elsewhere)" if args.fp4 else "mxfp8 linears (bf16 elsewhere)" if args.fp8 else "bf16", "data": "synthetic uniform-random token ids (seed 0), random-init weights",
+            "dtype": "nvfp4 linears (bf16 elsewhere)" if args.fp4 else "mxfp8 linears (bf16 elsewhere)" if args.fp8 else "e4m3 linears with fp32 block scales (bf16 elsewhere)" if cfg.fp8_block else "bf16", "data": "synthetic uniform-random token ids (seed 0), random-init weights",
             "tokens_per_sec_per_gpu": value / world,
             "mfu": flops_step / max(args.tp, 1) / (ms_per_step / 1e3) / 2.25e15,   # per GPU: tp peers share a micro-batch
             "mfu_with_lm_head": flops_step_head / max(args.tp, 1) / (ms_per_step / 1e3) / 2.25e15,
