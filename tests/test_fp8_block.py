@@ -509,3 +509,33 @@ def test_norm_elements_of_16_bit_factors_are_those_of_the_reals(cols):
     assert large.any() and (~large).any() and (got[large] == want[large]).all()
     assert ((got.double() - v).abs() <= v.abs() * 2.0 ** -4 * (1 + 1e-5) + 2.0 ** -10 * (1 + 1e-5)).all()
     assert ((s.double() - a / 448).abs() <= (cols + 16) * 2.0 ** -24 * a / 448 + 1e-45).all()
+
+
+@pytest.mark.gpu
+def test_offsets_past_31_bits():
+    """Matrices of more than 2³¹ elements: their last rows are what those rows give by themselves."""
+    from archscale_b200.ops import backend
+    R, C, last = 264192, 8200, 128
+    x = torch.empty(R, C, device="cuda", dtype=torch.bfloat16)
+    for i in range(0, R, 33024):
+        x[i:i + 33024] = _rand((min(33024, R - i), C), torch.bfloat16, "cuda", i)
+    w = (1 + 0.1 * torch.randn(C, device="cuda")).to(torch.bfloat16)
+    q, s, qt, st = ops.quantize_fp8_block_both(x)
+    want = ops.quantize_fp8_block_both(x[-last:])
+    assert torch.equal(q[-last:].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(s[-last:], want[1])
+    assert torch.equal(qt[:, -last:].contiguous().view(torch.uint8), want[2].contiguous().view(torch.uint8)) and torch.equal(st[:, -1:], want[3])
+    del qt, st
+    wq, _, ws = ops.quantize_fp8_weight(_rand((8200, 200), torch.bfloat16, "cuda", 5))
+    a, sa = ops.quantize_fp8_block(x[:, :200])
+    y = ops.matmul_fp8_block(a, sa, wq, ws)                            # more than 2³¹ values of the result
+    assert torch.equal(y[-last:], ops.matmul_fp8_block(a[-last:], sa[-last:], wq, ws))
+    del y, q, s
+    z, n, ns = ops.add_rms_norm_fp8(x, x, w)
+    zw, nw, nsw = ops.add_rms_norm_fp8(x[-last:], x[-last:], w)
+    assert torch.equal(z[-last:], zw) and torch.equal(n[-last:].view(torch.uint8), nw.view(torch.uint8)) and torch.equal(ns[-last:], nsw)
+    del z, n, ns
+    rstd, dn = torch.rand(R, device="cuda"), torch.randn(R, C, device="cuda")
+    ext = backend.require_extension()
+    dres, dh, _ = ext.add_rmsnorm_fp8_bwd(x, dn, x, w, rstd, 0.5, True, True, False)
+    dw, hw, _ = ext.add_rmsnorm_fp8_bwd(x[-last:], dn[-last:], x[-last:], w, rstd[-last:], 0.5, True, True, False)
+    assert torch.equal(dres[-last:], dw) and torch.equal(dh[-last:], hw)
