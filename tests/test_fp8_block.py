@@ -539,3 +539,31 @@ def test_offsets_past_31_bits():
     dres, dh, _ = ext.add_rmsnorm_fp8_bwd(x, dn, x, w, rstd, 0.5, True, True, False)
     dw, hw, _ = ext.add_rmsnorm_fp8_bwd(x[-last:], dn[-last:], x[-last:], w, rstd[-last:], 0.5, True, True, False)
     assert torch.equal(dres[-last:], dw) and torch.equal(dh[-last:], hw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 48, 300])
+def test_graph_capture(T):
+    """A decoding step's calls in a CUDA graph, replayed on other inputs: what the calls give by themselves."""
+    C, N = 1024, 2500
+    wn = torch.ones(C, device="cuda", dtype=torch.bfloat16)
+    wq, _, ws = ops.quantize_fp8_weight(_rand((N, C), torch.bfloat16, "cuda", 1))
+    w2, _, s2 = ops.quantize_fp8_weight(_rand((C, N), torch.bfloat16, "cuda", 2))
+    res, h = _rand((T, C), torch.bfloat16, "cuda", 3), _rand((T, C), torch.bfloat16, "cuda", 4)
+
+    def step():
+        x, n, s = ops.add_rms_norm_fp8(res, h, wn)
+        return x, ops.linear_fp8_weight(ops.linear_fp8_weight((n, s), wq, ws), w2, s2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (5, 6):
+        res.copy_(_rand((T, C), torch.bfloat16, "cuda", seed))
+        graph.replay()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
