@@ -302,6 +302,8 @@ int b200_gemm_fp8_block(const void* A, int64_t lda, const float* sa, int64_t sa_
                         const float* sb, int64_t sb_row, int64_t sb_blk, int sb_tile, const void* bias, int bias_dtype, void* out, int64_t ldc,
                         int M, int N, int K, int out_f32, int accumulate, int pair, void* ws, int num_sms, int* status,
                         cudaStream_t stream);
+// Whether a product is faster on SM pairs, where scales of A are per row.
+int b200_gemm_fp8_block_pairs(int M, int N, int K, int sb_tile, int num_sms);
 // The same on SM pairs (gemm2_fp8_block.cu), called by the one above with `pair`: scales per row are stored [block][blk],
 // those of B 16-byte aligned.
 int b200_gemm2_fp8_block(const void* A, int64_t lda, const float* sa, int64_t sa_blk, const void* B, int64_t ldb, const float* sb, int64_t sb_row,

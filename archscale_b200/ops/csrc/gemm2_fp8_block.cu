@@ -533,11 +533,10 @@ static int launch_f2(const void* A, int64_t lda, const void* B, int64_t ldb, con
 
 // How a product is laid over the pairs of SMs: the width of its tiles, and the split of those that do not fill a last wave.
 namespace b200 {
-struct F2Plan { int nt, whole, splits, per; int64_t ws_floats; int counters; };
+struct F2Plan { int nt, whole, splits, per; int64_t ws_floats; int counters; double cost; };
 static F2Plan f2_plan(int M, int N, int K, int num_sms) {
   const int pairs = num_sms / 2, num_kb = (K + F2_BK - 1) / F2_BK;
   F2Plan best{};
-  double best_cost = 0;
   for (int nt = 256; nt >= 128; nt /= 2) {
     const int64_t tiles = static_cast<int64_t>((M + 255) / 256) * ((N + nt - 1) / nt);
     const int rest = static_cast<int>(tiles % pairs);
@@ -559,13 +558,18 @@ static F2Plan f2_plan(int M, int N, int K, int num_sms) {
       }
     }
     const double cost = static_cast<double>(tiles / pairs) * tile + last;
-    if (nt == 256 || cost < best_cost) {
+    if (nt == 256 || cost < best.cost) {
       const int64_t parts = splits > 1 ? static_cast<int64_t>(rest) * splits : 0;
-      best = F2Plan{nt, static_cast<int>(splits > 1 ? tiles - rest : tiles), splits, per, parts * 256 * nt, splits > 1 ? rest * 16 : 0};
-      best_cost = cost;
+      best = F2Plan{nt, static_cast<int>(splits > 1 ? tiles - rest : tiles), splits, per, parts * 256 * nt, splits > 1 ? rest * 16 : 0, cost};
     }
   }
   return best;
+}
+// About how many µs the product takes, to choose between this kernel and the one for few rows (a line through 64 to 512 rows by 256 to 11264
+// columns, K 256 to 8192).
+double f2_microseconds(int M, int N, int K, int sb_tile, int num_sms) {
+  const double cost = f2_plan(M, N, K, num_sms).cost;
+  return sb_tile ? 2.6 + 0.52 * cost : 3.0 + 0.8 * cost;
 }
 }  // namespace b200
 

@@ -6,8 +6,8 @@
 // fp32 scales, so the products of one block of K are accumulated in tensor memory (exact to fp32 rounding over 128 terms), read
 // back, scaled and added to fp32 sums in registers.
 //
-// This file: the form for up to 64 rows of A (single tokens, a batch in decoding).  It is bound by reading B once (one token: 11264 × 2048 weights, 23 MB, 3.5 µs at the copy rate) and, at
-// this size, by the latency of one CTA's chain.  So 128 rows of B are the M side of the MMA and BT rows of A (16, 32 or 64) its N side, which
+// This file: the form for few rows of A (single tokens, a batch in decoding, small results of a long K).  It is bound by reading B once (one token:
+// 11264 × 2048 weights, 23 MB, 3.5 µs at the copy rate) and, at this size, by the latency of one CTA's chain (7.2 µs).  So 128 rows of B are the M side of the MMA and BT rows of A (16, 32 or 64) its N side, which
 // makes neighbouring lanes neighbouring columns of the output, and the blocks of K are split over a cluster of up to eight CTAs.  The
 // first loads are issued before tensor memory is allocated.  The CTAs' sums meet in shared memory, in the place of the stages; every CTA
 // adds its share of the rows over the ranks in rank order (distributed shared memory), so a result does not depend on scheduling.
@@ -235,6 +235,15 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
 int make_tmap_2d_u8(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
                     uint32_t box_inner, uint32_t box_outer);
 
+// K is split as far as the CTAs fit the machine at once and have a block each.
+static int fs_split(int64_t tiles, int K, int num_sms) {
+  const int num_kb = (K + FS_BK - 1) / FS_BK;
+  int s = 1;
+  while (s < 8 && tiles * 2 * s <= 2 * static_cast<int64_t>(num_sms) && 2 * s <= num_kb) s *= 2;
+  return s;
+}
+double f2_microseconds(int M, int N, int K, int sb_tile, int num_sms);
+
 template <int BT, int S>
 static int launch_fs(const CUtensorMap& ta, const CUtensorMap& tb, const FsParams& p, unsigned tiles, cudaStream_t st) {
   auto kern = gemm_fp8_block_kernel<BT, S>;
@@ -259,17 +268,26 @@ static int launch_fs(const void* A, int64_t lda, const void* B, int64_t ldb, con
   if (rc) return rc;
   const int64_t tiles = static_cast<int64_t>((p.M + BT - 1) / BT) * ((p.N + FS_BN - 1) / FS_BN);
   if (tiles > 0xfffffff) return -6;
-  // K is split as far as the CTAs fit the machine at once and have a block each
-  const int64_t room = 2 * static_cast<int64_t>(num_sms);
-  const int num_kb = (p.K + FS_BK - 1) / FS_BK;
-  int s = 1;
-  while (s < 8 && tiles * 2 * s <= room && 2 * s <= num_kb) s *= 2;
+  const int s = fs_split(tiles, p.K, num_sms);
   const unsigned t = static_cast<unsigned>(tiles);
   return s == 8 ? launch_fs<BT, 8>(ta, tb, p, t, st) : s == 4 ? launch_fs<BT, 4>(ta, tb, p, t, st)
        : s == 2 ? launch_fs<BT, 2>(ta, tb, p, t, st) : launch_fs<BT, 1>(ta, tb, p, t, st);
 }
 
 }  // namespace b200
+
+// Whether a product with one scale per row of A runs on SM pairs.  Up to 64 rows never do.  From there this file's kernel has a fixed time (one more
+// microsecond where two CTAs share an SM) and reads 24 KB per tile of 64 x 128 and block of K at 8 TB/s; it wins while its tiles are few: µs of
+// it and of the pairs, weight tiles / scales per row, 2048 x 5632 weights 128 rows 11.8 and 18.2 / 11.8 and 28.2, 256 14.3 and 18.7 / 14.4 and 27.3,
+// 384 21.5 and 19.1 / 21.6 and 28.3; 11264 x 2048 128 rows 15.9 and 13.2 / 15.9 and 16.5, 512 38 and 22 / 39 and 29.  Over 90 random sizes (65 to 2500 rows)
+// what it picks takes 1.010 of the better one's time, the pairs alone 1.25.
+extern "C" int b200_gemm_fp8_block_pairs(int M, int N, int K, int sb_tile, int num_sms) {
+  using namespace b200;
+  if (M <= 64) return 0;
+  const int64_t tiles = static_cast<int64_t>((M + 63) / 64) * ((N + FS_BN - 1) / FS_BN);
+  const double few = 6.0 + (tiles * fs_split(tiles, K, num_sms) > num_sms ? 1.0 : 0.0) + 0.0031 * static_cast<double>(tiles) * ((K + FS_BK - 1) / FS_BK);
+  return few < f2_microseconds(M, N, K, sb_tile, num_sms) ? 0 : 1;
+}
 
 // A [M, K], B [N, K]: e4m3, rows lda / ldb bytes apart (multiples of 16, as the addresses).  sa, sb: scales with strides between rows
 // (or groups of 128 rows: *_tile) and between blocks of 128 along K.  out [M, N] fp32 (accumulate: added to) or bf16; bias [N] or null.
