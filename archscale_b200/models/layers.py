@@ -25,7 +25,7 @@ class Linear(nn.Linear):
     mxfp8: bool = False
     nvfp4: bool = False
     fp8_block: bool = False
-    fp8_stored = None           # (elements, scales, version of the weight) of a frozen layer
+    fp8_stored = None           # StoredFP8 of a frozen layer
     widen: bool = False         # odd feature counts on operands widened to a multiple of 8 (``ops.gemm.linear_widened``)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
@@ -52,12 +52,16 @@ class Linear(nn.Linear):
 
     def stored_fp8(self):
         """(elements, scales) of a frozen layer in a call without gradients, else None.  Raises when the weight was written since."""
-        if self.fp8_stored is None or torch.is_grad_enabled():
+        s = self.fp8_stored
+        if s is None:
             return None
-        q, scale, version = self.fp8_stored
-        if version != self.weight._version or q.device != self.weight.device:
+        if torch.is_grad_enabled():
+            if self.weight.requires_grad:
+                s.operands = None
+            return None
+        if not s.current(self.weight):
             raise RuntimeError("the weight of a frozen 8-bit layer has changed: call freeze_fp8_block(model) again")
-        return q, scale
+        return s.operands
 
     plain_forward = forward     # what ``ops.gemm.plain_linear`` compares with: a replaced ``forward`` is never passed by
 
@@ -98,17 +102,50 @@ def apply_fp8_block(model: nn.Module, skip=("lm_head", "lc_proj")) -> int:
     return n
 
 
+class StoredFP8:
+    """8-bit form of the weight of a frozen layer, and what shows that the weight is still the one it was made from: the parameter itself, its
+    version counter and the memory it lies in, or, where an engine owns that memory (it gathers and frees it, and its optimizers write the
+    shards), the engine's count of changes.  The memory is kept alive, so that no later weight can lie at the same address."""
+
+    def __init__(self, weight: torch.Tensor, operands) -> None:
+        from archscale_b200.parallel.fsdp import engine_of
+        self.weight, self.operands, self.engine = weight, operands, engine_of(weight)
+        self.memory = None if self.engine is not None else weight.detach()
+        self.stamp = self._stamp()
+
+    def _stamp(self):
+        w = self.weight
+        return (w._version, self.engine.params_version) if self.engine is not None else (w._version, w.data_ptr(), w.shape, w.stride(), w.dtype, w.device)
+
+    def current(self, weight: torch.Tensor) -> bool:
+        return weight is self.weight and self.stamp == self._stamp()
+
+    def __reduce__(self):                               # copies and pickles of a frozen layer are frozen, unless its weight has changed
+        return StoredFP8, (self.weight, self.operands if self.current(self.weight) else None)
+
+
 @torch.no_grad()
 def freeze_fp8_block(model: nn.Module, frozen: bool = True) -> int:
     """Store the 8-bit form of the weights of all ``fp8_block`` layers for calls without gradients (evaluation, generation), which otherwise
-    quantise them every time; ``frozen=False`` drops it.  Weights that change afterwards make such a call raise.  Returns the number of
-    layers."""
+    quantise them every time; ``frozen=False`` drops it.  Returns the number of layers.
+
+    Weights that change afterwards make such a call raise: by an operation on the parameter, a state dict, a move, new memory, or a step
+    or load of the engine that shards the model.  What goes past PyTorch's version counters (in-place operations on ``weight.data``, NumPy views,
+    kernels that are given the address) cannot be seen; freeze again after it.  A layer that is called with gradients, as it is in training,
+    drops its stored form, so that the calls after it take the weights as they are then.
+
+    Of a sharded model every rank has to make this call, since the weights are gathered."""
+    from archscale_b200.parallel.fsdp import gathered
     n = 0
     for mod in model.modules():
         if isinstance(mod, Linear) and mod.fp8_block:
             mod.fp8_stored = None
             if frozen:
-                q, _, scale = ops.quantize_fp8_weight(mod.weight)
-                mod.fp8_stored = (q, scale, mod.weight._version)
+                if mod.weight.is_inference():
+                    raise RuntimeError("freeze_fp8_block: weights made under torch.inference_mode() keep no version that shows whether they "
+                                       "change; make them outside of it")
+                with gathered(mod.weight):
+                    q, _, scale = ops.quantize_fp8_weight(mod.weight)
+                    mod.fp8_stored = StoredFP8(mod.weight, (q, scale))
             n += 1
     return n

@@ -23,6 +23,7 @@ Optimizers consume the flat shards through :meth:`FSDPEngine.groups` and :meth:`
 from __future__ import annotations
 
 import contextlib
+import weakref
 from dataclasses import dataclass, field
 from typing import Callable, Dict, Iterable, List, Optional, Sequence, Tuple
 
@@ -178,6 +179,45 @@ class _PostBackward(torch.autograd.Function):
         return (None, None) + grads
 
 
+_ENGINES: List[weakref.ref] = []        # in the order of their construction
+
+
+def _home_of(param: torch.Tensor):
+    """(engine, unit) that ``param`` belongs to now."""
+    for ref in reversed(_ENGINES):
+        e = ref()
+        for u in e.units if e is not None else ():
+            for g in u.groups:
+                for s in g.specs:
+                    if s.param is param:
+                        return e, u
+    return None, None
+
+
+def engine_of(param: torch.Tensor) -> Optional["FSDPEngine"]:
+    """The engine whose shards ``param`` is gathered from, or None."""
+    return _home_of(param)[0]
+
+
+@contextlib.contextmanager
+def gathered(param: torch.Tensor):
+    """Within it a parameter of an engine has its values; the unit is sharded again afterwards if it was before.  A collective call for such a
+    parameter; nothing for any other."""
+    engine, unit = _home_of(param)
+    if engine is None:
+        yield
+        return
+    was = unit.unsharded
+    engine._unshard(unit)
+    for g in unit.groups:
+        engine.finish_pending_gather(g)
+    try:
+        yield
+    finally:
+        if not was and engine.world > 1:
+            engine._reshard(unit)
+
+
 class FSDPEngine:
     def __init__(self, model: nn.Module, mesh: Optional[Mesh] = None, unit_classes: Sequence[type] = (),
                  param_dtype: torch.dtype = torch.bfloat16, reshard_after_forward: bool = True,
@@ -203,8 +243,10 @@ class FSDPEngine:
         self._rs_events: List[object] = []
         self._fwd_order: List[Unit] = []
         self._order_frozen = False
+        self.params_version = 0          # optimizer steps and checkpoint loads so far
         self.units: List[Unit] = []
         self._build_units(unit_classes)
+        _ENGINES[:] = [r for r in _ENGINES if r() is not None] + [weakref.ref(self)]
         self._register_hooks()
         if self.fused_comm:
             from . import symm
@@ -634,6 +676,7 @@ class FSDPEngine:
         from archscale_b200.ops import mxfp8, nvfp4
         mxfp8.invalidate_weight_cache()          # quantised copies of the old weights are void
         nvfp4.invalidate_weight_cache()
+        self.params_version += 1
         for g in self.groups():
             g.lp_stale = True
         for u in self.units:
@@ -780,6 +823,7 @@ class FSDPEngine:
         from archscale_b200.ops import mxfp8, nvfp4
         mxfp8.invalidate_weight_cache()
         nvfp4.invalidate_weight_cache()
+        self.params_version += 1
         for g in self.groups():
             for s, lo, hi, slo in g.local_slices():
                 if s.name not in sd:
