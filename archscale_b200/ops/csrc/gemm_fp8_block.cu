@@ -140,6 +140,8 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     float sum[W], scale[8];
 #pragma unroll
     for (int i = 0; i < W; ++i) sum[i] = 0.f;
+    // A warp whose wait has run out goes on to the barriers of the table, which the others may still reach: every warp arrives at every one
+    // of them, and the others' waits end within their limit too.
     bool ok = true;
     for (int i = 0; i < nkb; ++i) {
       const int acc = i % T::ACC; const uint32_t aph = (i / T::ACC) & 1;
@@ -160,8 +162,8 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
       const float s45 = (i & 1) ? scale[5] : scale[4], s67 = (i & 1) ? scale[7] : scale[6];
       const float f = (i & 4) ? ((i & 2) ? s67 : s45) : ((i & 2) ? s23 : s01);
       const float4* sa = reinterpret_cast<const float4*>(table + i % FS_CHUNK * BT + c0);
-      ok = mbar_wait_warp(&tmem_full[acc], aph, abort_flag, p.status, STATUS_TIMEOUT_TMEM_FULL);
-      if (!ok) break;
+      ok = ok && mbar_wait_warp(&tmem_full[acc], aph, abort_flag, p.status, STATUS_TIMEOUT_TMEM_FULL);
+      if (!ok) continue;
       tc_fence_after();
       uint32_t r[W];
       const uint32_t taddr = tmem_base + acc * BT + c0 + (static_cast<uint32_t>(q * 32) << 16);
