@@ -217,6 +217,7 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     n0 = (r / gsz) * NT;
   };
 
+  uint32_t issued = 0;                                 // blocks that this warp has loaded (warp 0) or multiplied (warp 1)
   if (warp == 0) {                                     // converged: a load from inside a branch of one lane takes longer to issue
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     int stage = 0; uint32_t phase = 0;
@@ -231,6 +232,7 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
           tma_load_2d_2sm(sa, &tmap_a, &full_bar[stage], kb * F2_BK, ma);
           tma_load_2d_2sm(sa + T::A_BYTES, &tmap_b, &full_bar[stage], kb * F2_BK, nb);
         }
+        ++issued;
         if (++stage == T::STAGES) { stage = 0; phase ^= 1; }
       }
     }
@@ -256,6 +258,7 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             umma_commit_2sm(&tmem_full[acc], 3);
             umma_commit_2sm(&empty_bar[stage], 3);
           }
+          ++issued;
           if (++stage == T::STAGES) { stage = 0; phase ^= 1; }
         }
       }
@@ -476,10 +479,14 @@ gemm2_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
 done:
   if (warp >= 4) {
     tmem_ld_wait();                    // a wait that gave up can leave a load on its way
+    if (!BTILE) asm volatile("cp.async.wait_all;" ::: "memory");
     tma_store_wait<0>();
   }
   tc_fence_before();
   __syncthreads();
+  // full_bar is the leader's; the other CTA knows that its loads have ended by the products that read them
+  if (warp < 2 && *abort_flag) drain_ring(warp == 0 && rank == 0 ? full_bar : empty_bar, T::STAGES, issued);
+  __syncwarp();
   cluster_sync_all();
   if (warp == 1) {
     __syncwarp();

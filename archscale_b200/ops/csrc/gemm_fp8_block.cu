@@ -107,12 +107,15 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
+  uint32_t issued = 0;                                 // blocks that this warp has loaded (warp 0) or multiplied (warp 1)
 
   if (warp == 0) {
+    issued = min(T::STAGES, nkb);
     for (int i = T::STAGES; i < nkb; ++i) {
       const int st = i % T::STAGES; const uint32_t ph = (i / T::STAGES) & 1;
       if (!mbar_wait_warp(&empty_bar[st], ph ^ 1, abort_flag, p.status, STATUS_TIMEOUT_EMPTY)) break;
       if (elect_one_sync()) load(i, st);
+      ++issued;
     }
   } else if (warp == 1) {
     // e4m3 × e4m3, fp32 accumulate, both operands K-major
@@ -132,6 +135,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         umma_commit(&tmem_full[acc]);
         umma_commit(&empty_bar[st]);
       }
+      ++issued;
     }
   } else {
     const int q = warp & 3, t = threadIdx.x - 64, c0 = (warp - 2) / 4 * W;      // lane quarter, first row of A
@@ -190,6 +194,8 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   }
   tc_fence_before();
   __syncthreads();
+  if (warp < 2 && *abort_flag) drain_ring(warp == 0 ? full_bar : empty_bar, T::STAGES, issued);
+  __syncwarp();
   if (S > 1) cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();

@@ -87,6 +87,15 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code));
 }
 
+// For a kernel that gives up: waits, within the limit once more, until the last `issued` turns of a ring have ended, so that no copy still writes to
+// shared memory and no product to tensor memory when the CTA leaves.  Turn i completes phase i / stages of barrier i % stages.
+__device__ __forceinline__ void drain_ring(uint64_t* bars, int stages, uint32_t issued) {
+  const long long t0 = clock64();
+  for (uint32_t i = issued > static_cast<uint32_t>(stages) ? issued - stages : 0; i < issued; ++i)
+    while (!mbar_try_wait(&bars[i % stages], (i / stages) & 1))
+      if (clock64() - t0 > kWaitLimitCycles) return;
+}
+
 // The same bounded wait for roles that are not on the critical path (loaders, read-out warps): it sleeps between polls,
 // so the polling warp leaves the issue slots of its scheduler to the warps that compute.
 __device__ __forceinline__ bool mbar_wait_relaxed(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status,

@@ -41,3 +41,17 @@ def test_every_warp_reaches_every_named_barrier(name):
         assert not re.search(r"\b(break|goto|return)\b", loop), loop
         last = max(x.start() for x in re.finditer(r"bar\.sync [1-9]", loop))
         assert "continue" not in loop[:last]
+
+
+@pytest.mark.parametrize("name", ["gemm_fp8_block.cu", "gemm2_fp8_block.cu"])
+def test_a_kernel_that_gives_up_waits_for_what_it_has_issued(name):
+    """After the block's last barrier the warps of the loads and of the products look at the flag of a wait that ran out, and drain their rings before the
+    cluster parts and tensor memory is freed; copies of single threads are waited for by the threads themselves."""
+    text = _source(name)
+    kernel = _block(text, text.index("gemm2_fp8_block_kernel(" if "2" in name else "gemm_fp8_block_kernel("))
+    barrier, drain, free = (kernel.rindex(w) for w in ("__syncthreads()", "drain_ring(", "tmem_dealloc"))
+    assert barrier < drain < kernel.rindex("cluster_sync_all()") and drain < free
+    assert re.search(r"warp < 2 && \*abort_flag\) drain_ring\(", kernel)
+    assert kernel.count("++issued;") == 2
+    if "f2_cp_async" in kernel:
+        assert barrier > kernel.rindex("cp.async.wait_all") > kernel.index("done:")
