@@ -20,6 +20,9 @@ is below 2⁻¹²⁶ the block counts as zero.  Any size is taken: no dimension 
   rounded to 16 bits); :func:`add_rms_norm_linear_fp8` trains it with the layer behind it.  Its backward makes the transposed operand of
   the weight gradient from the residual stream, which is kept anyway, so that ``n`` itself is kept in no form.
 
+Quantisers, product, stored layer and :func:`add_rms_norm_fp8` have no gradients, on any device: with gradients enabled they refuse operands that ask
+for one (store weights under ``torch.no_grad()``).
+
 Scales are returned as ``(rows, blocks)``; in memory the rows are the fast dimension, which is what the GEMM reads.  Elements
 have rows of a multiple of 16 bytes (TMA); others are copied into such rows within the call.
 
@@ -128,8 +131,10 @@ def _kernel(x: torch.Tensor) -> bool:
 
 def _no_grad(name: str, *tensors) -> None:
     """A call that has no gradients must not cut a graph silently."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no gradients: call it under torch.no_grad(), or use the training form")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} has no gradients: call it under torch.no_grad(), or use the training form")
 
 
 def _ext():
@@ -140,6 +145,7 @@ def _ext():
 # ------------------------------------------------------------------------------------------------ quantisers
 def quantize_fp8_block(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x:(R,C) → (elements (R,C), scales (R, ⌈C/128⌉)), blocks along the rows."""
+    _no_grad("quantize_fp8_block", x)
     if _kernel(x):
         return tuple(_ext().fp8_quantize(x, 1))
     _need_matrix("quantize_fp8_block", x)
@@ -148,6 +154,7 @@ def quantize_fp8_block(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 def quantize_fp8_block_t(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x:(R,C) → (elements (C,R), scales (C, ⌈R/128⌉)) of the transposed matrix, blocks along the original columns."""
+    _no_grad("quantize_fp8_block_t", x)
     if _kernel(x):
         return tuple(_ext().fp8_quantize(x, 2))
     _need_matrix("quantize_fp8_block_t", x)
@@ -156,6 +163,7 @@ def quantize_fp8_block_t(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 def quantize_fp8_block_both(x: torch.Tensor):
     """:func:`quantize_fp8_block` and :func:`quantize_fp8_block_t` from one read of x: (q, scale, q_t, scale_t)."""
+    _no_grad("quantize_fp8_block_both", x)
     if _kernel(x):
         return tuple(_ext().fp8_quantize(x, 3))
     _need_matrix("quantize_fp8_block_both", x)
@@ -164,6 +172,7 @@ def quantize_fp8_block_both(x: torch.Tensor):
 
 def quantize_fp8_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """w:(N,K) → (elements (N,K), the same transposed (K,N), scales (⌈N/128⌉, ⌈K/128⌉) of 128 × 128 tiles)."""
+    _no_grad("quantize_fp8_weight", w)
     if _kernel(w):
         return tuple(_ext().fp8_quantize(w, 4))
     _need_matrix("quantize_fp8_weight", w)
@@ -177,6 +186,7 @@ def matmul_fp8_block(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_
     """``a:(M,K) · b:(N,K)ᵀ (+ bias)``, each operand with scales per row and block of 128, ``(rows, ⌈K/128⌉)``, or per 128 × 128 tile,
     ``(⌈rows/128⌉, ⌈K/128⌉)`` → (M,N) in ``out_dtype``; with ``acc`` (fp32) the product is added to it in place.  ``a`` may have more leading
     dimensions than one (M: their product), which the result then has too."""
+    _no_grad("matmul_fp8_block", a, a_scale, b, b_scale, bias, acc)
     if out_dtype not in _FLOATS:
         raise TypeError(f"matmul_fp8_block: out_dtype must be bfloat16 or float32, got {out_dtype}")
     if _kernel(a):
@@ -208,8 +218,9 @@ def linear_fp8_weight(x: Union[torch.Tensor, Quantised], weight: torch.Tensor, s
     pair (elements, scales) of :func:`add_rms_norm_fp8` / :func:`quantize_fp8_block` with any leading dimensions of the elements.  It has
     no gradients and refuses operands that ask for one."""
     if not isinstance(x, torch.Tensor):
+        _no_grad("linear_fp8_weight", x[1], scale, bias)
         return matmul_fp8_block(x[0], x[1], weight, scale, bias, out_dtype or torch.bfloat16)
-    _no_grad("linear_fp8_weight", x, bias)
+    _no_grad("linear_fp8_weight", x, scale, bias)
     dtype = out_dtype or x.dtype
     if dtype not in _FLOATS:
         raise TypeError(f"linear_fp8_weight: results are bfloat16 or float32, not {dtype}")
