@@ -21,7 +21,8 @@ is below 2⁻¹²⁶ the block counts as zero.  Any size is taken: no dimension 
   the weight gradient from the residual stream, which is kept anyway, so that ``n`` itself is kept in no form.
 
 Quantisers, product, stored layer and :func:`add_rms_norm_fp8` have no gradients, on any device: with gradients enabled they refuse operands that ask
-for one (store weights under ``torch.no_grad()``).
+for one (store weights under ``torch.no_grad()``), and operands with a forward-mode tangent.  Under ``vmap`` and ``torch.jit.trace`` they run as
+PyTorch operators.  The layers that train are traced in the same way; forward-mode and functorch transforms raise.
 
 Scales are returned as ``(rows, blocks)``; in memory the rows are the fast dimension, which is what the GEMM reads.  Elements
 have rows of a multiple of 16 bytes (TMA); others are copied into such rows within the call.
@@ -33,6 +34,7 @@ from __future__ import annotations
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import backend
@@ -126,7 +128,8 @@ def _need_matrix(name: str, x: torch.Tensor) -> None:
 
 
 def _kernel(x: torch.Tensor) -> bool:
-    return x.is_cuda and backend.use_cuda_kernel("fp8_block", x)
+    """Transforms and traces see the restatements, whose operators they know."""
+    return x.is_cuda and not backend.transformed() and backend.use_cuda_kernel("fp8_block", x)
 
 
 def _no_grad(name: str, *tensors) -> None:
@@ -135,6 +138,10 @@ def _no_grad(name: str, *tensors) -> None:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{name} has no gradients: call it under torch.no_grad(), or use the training form")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no gradients, nor forward-mode tangents")
 
 
 def _ext():

@@ -38,3 +38,48 @@ def test_calls_without_gradients_refuse_operands_that_ask_for_one(device):
                 call(*some)
             with torch.no_grad():
                 call(*some)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_mode_tangents_are_refused(device):
+    from torch.autograd import forward_ad
+    x, w, bias, nw, _, (wq, _, ws) = _operands(device)
+    calls = [ops.quantize_fp8_block, ops.quantize_fp8_weight, lambda t: ops.linear_fp8_weight(t, wq, ws),
+             lambda t: ops.add_rms_norm_fp8(t, None, nw), lambda t: ops.linear_fp8_block(t, w),
+             lambda t: ops.add_rms_norm_linear_fp8(t, None, nw, w)]
+    for call in calls:
+        for ctx in (torch.no_grad, torch.enable_grad):
+            with ctx(), forward_ad.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+                call(forward_ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            torch.func.jvp(call, (x,), (x,))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: call(t)[0].float().sum())(x)
+    with forward_ad.dual_level():                                  # operands without one
+        assert torch.equal(ops.linear_fp8_weight(x, wq, ws), ops.linear_fp8_weight(x, wq, ws))
+
+
+def _near(got, want, top):
+    """The same elements and scales through another order of sums: 160 products of fp32 and two blocks, every step rounded or cut; ``top`` bounds a product
+    of two values.  Results in bf16 may round to neighbours."""
+    tol = 160 * top * 170 * 2.0 ** -23 + (2.0 ** -7 * want.float().abs() if want.dtype == torch.bfloat16 else 0)
+    return bool(((got.float() - want.float()).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_vmap_and_traces(device):
+    x, w, bias, nw, _, (wq, _, ws) = _operands(device)
+    batch = torch.randn(3, 5, 160, generator=torch.Generator().manual_seed(1)).to(device)
+    top = float(batch.abs().max() * w.abs().max())
+    top_n = 160 ** 0.5 * float(nw.abs().max() * w.abs().max())          # a normalised value is at most the root of the width
+    stored = lambda t: ops.linear_fp8_weight(t, wq, ws, bias)  # noqa: E731
+    assert _near(torch.vmap(stored)(batch), stored(batch), top)
+    assert torch.equal(torch.vmap(lambda t: ops.quantize_fp8_block(t)[1])(batch)[1], ops.quantize_fp8_block(batch[1])[1])
+    _, q, s = torch.vmap(lambda t: ops.add_rms_norm_fp8(t, None, nw))(batch)
+    assert q.shape == (3, 5, 160) and s.shape == (3, 5, 2)
+    layers = ((stored, top), (lambda t: ops.linear_fp8_block(t, w), top), (lambda t: ops.add_rms_norm_linear_fp8(t, None, nw, w)[1], top_n))
+    for call, bound in layers:
+        for ctx in (torch.no_grad, torch.enable_grad):
+            with ctx():
+                traced = torch.jit.trace(call, (x,), check_trace=False)
+                assert _near(traced(batch[2]), call(batch[2]), bound) and not torch.allclose(traced(batch[2]), traced(x))
