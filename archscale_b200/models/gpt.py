@@ -262,7 +262,7 @@ class Block(nn.Module):
     def _fp8_mlp(self, x, compute_dtype) -> bool:
         """Whether the second norm may deliver 8-bit operands to the MLP: nothing but its first layer reads the normalised values."""
         mlp = self.mlp
-        return (type(mlp) is LLaMAMLP and mlp.w1.fp8_block and not (mlp.w1.mxfp8 or mlp.w1.nvfp4) and ops.gemm.bare_linear(mlp.w1)
+        return (type(mlp) is LLaMAMLP and getattr(mlp.w1, "fp8_block", False) and not (mlp.w1.mxfp8 or mlp.w1.nvfp4) and ops.gemm.bare_linear(mlp.w1)
                 and "forward" not in mlp.__dict__ and not (mlp._forward_hooks or mlp._forward_pre_hooks or mlp._backward_hooks
                                                            or mlp._backward_pre_hooks or self.norm_2._forward_hooks or self.norm_2._forward_pre_hooks)
                 and compute_dtype == torch.bfloat16 and x.dtype in (torch.bfloat16, torch.float32))

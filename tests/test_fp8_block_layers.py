@@ -1,0 +1,51 @@
+"""8-bit layers next to other modules: layers that were replaced, families of models, the evaluation loader."""
+import pytest
+import torch
+import torch.nn as nn
+
+from archscale_b200.config import Config
+from archscale_b200.models.gpt import GPT
+from archscale_b200.models.layers import apply_fp8_block
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+class _Wrapped(nn.Module):
+    """A layer around another one, as adapters are."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, x):
+        return self.inner(x)
+
+
+def _dense(device):
+    torch.manual_seed(3)
+    m = GPT(Config.from_name("transformer_gqa4_d8", n_layer=2, n_embd=128, ar=None, n_head=2, n_query_groups=1, head_dim=64, intermediate_size=256,
+                             block_size=64, padded_vocab_size=128, vocab_size=128)).to(device)
+    m.reset_parameters()
+    return m.to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fp8", [False, True])
+def test_models_with_replaced_layers(device, fp8):
+    m = _dense(device)
+    if fp8:
+        apply_fp8_block(m)
+    idx = torch.randint(0, 128, (1, 16), device=device)
+    with torch.no_grad():
+        want = m(idx).logits
+        mlp = m.transformer.h[0].mlp
+        mlp.w1 = _Wrapped(mlp.w1)
+        plain = nn.Linear(128, 512, bias=False, device=device, dtype=mlp.w3.weight.dtype)
+        plain.weight.copy_(m.transformer.h[1].mlp.w1.weight)
+        assert not m.transformer.h[0]._fp8_mlp(torch.zeros(1, dtype=torch.bfloat16), torch.bfloat16)
+        got = m(idx).logits
+        # the norm's own 8-bit output is not rounded to 16 bits first, which moves elements to their neighbours
+        assert (got - want).abs().max() <= (0.1 if device == "cuda" else 0) * want.abs().max()
+        m.transformer.h[1].mlp.w1 = plain
+        assert torch.isfinite(m(idx).logits).all()
+        assert not m.transformer.h[1]._fp8_mlp(torch.zeros(1, dtype=torch.bfloat16), torch.bfloat16)
