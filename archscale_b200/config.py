@@ -137,7 +137,7 @@ class Config:
     tp_size: int = 1   # tensor-parallel degree
     mxfp8: bool = False  # E4M3 values + E8M0 scale per 32 elements on every Linear except lm_head
     nvfp4: bool = False  # e2m1 values + E4M3 scale per 16 elements + one fp32 scale per tensor, same layers
-    fp8_block: bool = False  # E4M3 values + fp32 scale per 128 elements (weights: per 128 x 128 tile), same layers, any size
+    fp8_block: bool = False  # E4M3 values + fp32 scale per 128 elements (weights: per 128 x 128 tile), any size, but for routers, decays and gates per head
 
     def __post_init__(self) -> None:
         if self.padded_vocab_size is None:

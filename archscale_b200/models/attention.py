@@ -88,6 +88,7 @@ class CausalSelfAttention(nn.Module):
                 self.v_proj = Linear(n_embd, hs * G, bias=config.attn_bias)
             if config.gated_attn:
                 self.g_proj = Linear(n_embd, H, bias=config.attn_bias)
+                self.g_proj.steering = True
         else:
             shape = hs * H if yoco_cross else (H + 2 * G) * hs
             if config.gated_attn:

@@ -56,6 +56,7 @@ class GatedDeltaNet(nn.Module):
         self.v_proj = Linear(hidden_size, self.value_dim, bias=False)
         self.a_proj = Linear(hidden_size, self.num_v_heads, bias=False)
         self.b_proj = Linear(hidden_size, self.num_v_heads, bias=False)
+        self.a_proj.steering = self.b_proj.steering = True
         self.A_log = nn.Parameter(torch.empty(self.num_v_heads, dtype=torch.float32))
         self.dt_min, self.dt_max, self.dt_init_floor = 0.001, 0.1, 1e-4
         self.dt_bias = nn.Parameter(torch.empty(self.num_v_heads))

@@ -25,6 +25,7 @@ class Linear(nn.Linear):
     mxfp8: bool = False
     nvfp4: bool = False
     fp8_block: bool = False
+    steering: bool = False      # the outputs are routing scores, decays, step sizes or a gate per head: never in 8-bit blocks
     fp8_stored = None           # StoredFP8 of a frozen layer
     widen: bool = False         # odd feature counts on operands widened to a multiple of 8 (``ops.gemm.linear_widened``)
 
@@ -93,10 +94,12 @@ def apply_nvfp4(model: nn.Module, skip=("lm_head", "lc_proj")) -> int:
 
 def apply_fp8_block(model: nn.Module, skip=("lm_head", "lc_proj")) -> int:
     """Switch every :class:`Linear` of ``model`` to 8-bit operands with an fp32 scale per 128 elements, except modules whose name
-    contains one of ``skip``.  Returns the number of layers switched."""
+    contains one of ``skip`` and those that are ``steering``: few outputs that go into a softmax over experts, an exponential or a sigmoid
+    per head, where an operand's error of 2⁻⁴ is one of the whole token (sizes alone keep them out of the MXFP8 path).  Returns the number
+    of layers switched."""
     n = 0
     for name, mod in model.named_modules():
-        if isinstance(mod, Linear) and not any(s in name for s in skip):
+        if isinstance(mod, Linear) and not mod.steering and not any(s in name for s in skip):
             mod.fp8_block = True
             n += 1
     return n

@@ -48,6 +48,7 @@ class Mamba(nn.Module):
         self.x_proj = Linear(self.d_inner, self.dt_rank + 2 * d_state, bias=False, **fk)
         self.x_proj.widen = True
         self.dt_proj = Linear(self.dt_rank, self.d_inner, bias=True, **fk)
+        self.x_proj.steering = self.dt_proj.steering = True
         self.A_log = nn.Parameter(torch.ones(self.d_inner, d_state, dtype=torch.float32, device=device))
         self.D = nn.Parameter(torch.ones(self.d_inner, dtype=torch.float32, device=device))
         self.out_proj = Linear(self.d_inner, d_model, bias=bias, **fk)

@@ -54,6 +54,7 @@ class SonicMoE(nn.Module):
         self.ep_group = None  # set by parallel.ep.attach()
         C, I = config.n_embd, self.intermediate_size
         self.router = Linear(C, self.n_mods, bias=False)
+        self.router.steering = True
         self.mods_in = Experts(self.n_local, C, 2 * I, bias=config.bias)
         self.mods_out = Experts(self.n_local, I, C, bias=config.bias)
         if self.share_expert:
@@ -161,6 +162,7 @@ class _Router(nn.Module):
     def __init__(self, config: Config, route_size: int) -> None:
         super().__init__()
         self.lc_proj = Linear(config.n_embd, route_size, bias=config.bias)
+        self.lc_proj.steering = True
 
 
 class MoE(SonicMoE):

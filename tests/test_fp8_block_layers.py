@@ -5,7 +5,7 @@ import torch.nn as nn
 
 from archscale_b200.config import Config
 from archscale_b200.models.gpt import GPT
-from archscale_b200.models.layers import apply_fp8_block
+from archscale_b200.models.layers import Linear, apply_fp8_block, freeze_fp8_block
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 
@@ -49,3 +49,40 @@ def test_models_with_replaced_layers(device, fp8):
         m.transformer.h[1].mlp.w1 = plain
         assert torch.isfinite(m(idx).logits).all()
         assert not m.transformer.h[1]._fp8_mlp(torch.zeros(1, dtype=torch.bfloat16), torch.bfloat16)
+
+
+SMALL = dict(n_layer=2, ar=None, n_embd=256, n_head=2, n_query_groups=1, intermediate_size=256, block_size=64, padded_vocab_size=128, vocab_size=128)
+FAMILIES = {
+    "experts": ("transformer_gqa4_h2_moe_s2_k2_d8", dict(head_dim=128), ("router",)),
+    "experts, one by one": ("transformer_gqa4_h2_moe_s2_k2_d8", dict(head_dim=128, use_sonicmoe=False), ("router.lc_proj",)),
+    "gates per head": ("transformer_gqa4_d8", dict(head_dim=128, gated_attn=True), ("attn.g_proj",)),
+    "selective scan": ("samba_d8", {}, ("x_proj", "dt_proj")),
+    "state space duality": ("mambay2_d16", dict(n_layer=4), ()),
+    "delta rule": ("gdny_d16", dict(n_layer=4), ("a_proj", "b_proj")),
+}
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("family", FAMILIES)
+def test_families(device, family):
+    """One step of every family: which layers are switched, that gradients arrive everywhere, and that stored weights give what live ones give."""
+    name, more, kept = FAMILIES[family]
+    torch.manual_seed(3)
+    m = GPT(Config.from_name(name, **{**SMALL, **more})).to(device)
+    m.reset_parameters()
+    m = m.to(torch.bfloat16)
+    n = apply_fp8_block(m)
+    layers = {n: l for n, l in m.named_modules() if isinstance(l, Linear)}
+    steering = [n for n in layers if n.endswith(kept)] if kept else []
+    assert bool(steering) == bool(kept)
+    assert {n for n, l in layers.items() if not l.fp8_block} == {"lm_head", *steering} and n == len(layers) - 1 - len(steering)
+    idx = torch.randint(0, 128, (2, 32), device=device)
+    out = m(idx).logits
+    out.float().square().mean().backward()
+    assert torch.isfinite(out).all()
+    for n, l in layers.items():
+        assert l.weight.grad is not None and torch.isfinite(l.weight.grad).all(), n
+    with torch.no_grad():
+        live = m(idx).logits
+        assert freeze_fp8_block(m) == len(layers) - 1 - len(steering)
+        assert torch.equal(m(idx).logits, live)
