@@ -16,6 +16,7 @@ import torch.nn.functional as F
 
 from archscale_b200.config import Config
 from archscale_b200.models.gpt import GPT
+from archscale_b200.models.layers import apply_fp8_block, freeze_fp8_block
 
 
 def config_from_checkpoint_path(checkpoint_path: str, config_name: str) -> Config:
@@ -84,12 +85,18 @@ class ModelWrapper(torch.nn.Module):
         return sequences
 
 
-def load_model(checkpoint_path: str, config_name: str, device="cuda", dtype=torch.bfloat16) -> ModelWrapper:
+def load_model(checkpoint_path: str, config_name: str, device="cuda", dtype=torch.bfloat16, fp8_block: Optional[bool] = None) -> ModelWrapper:
+    """``fp8_block``: whether the linear layers run on stored 8-bit weights (``Config.fp8_block``); by default as the checkpoint says that the
+    model was trained."""
     config = config_from_checkpoint_path(checkpoint_path, config_name)
-    model = GPT(config)
     state = torch.load(checkpoint_path, map_location="cpu", weights_only=False)
+    config.fp8_block = bool((state.get("config") or {}).get("fp8_block", False)) if fp8_block is None else fp8_block
+    model = GPT(config)
     model.load_state_dict(state.get("model", state))
     model.to(device=device, dtype=dtype)
     model.compute_dtype = dtype
     model.eval()
+    if config.fp8_block:
+        apply_fp8_block(model)
+        freeze_fp8_block(model)
     return ModelWrapper(model)

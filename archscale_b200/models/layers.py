@@ -130,7 +130,8 @@ class StoredFP8:
 @torch.no_grad()
 def freeze_fp8_block(model: nn.Module, frozen: bool = True) -> int:
     """Store the 8-bit form of the weights of all ``fp8_block`` layers for calls without gradients (evaluation, generation), which otherwise
-    quantise them every time; ``frozen=False`` drops it.  Returns the number of layers.
+    quantise them every time; ``frozen=False`` drops it.  Returns the number of layers; a model without any (see :func:`apply_fp8_block`) is
+    refused.
 
     Weights that change afterwards make such a call raise: by an operation on the parameter, a state dict, a move, new memory, or a step
     or load of the engine that shards the model.  What goes past PyTorch's version counters (in-place operations on ``weight.data``, NumPy views,
@@ -151,4 +152,6 @@ def freeze_fp8_block(model: nn.Module, frozen: bool = True) -> int:
                     q, _, scale = ops.quantize_fp8_weight(mod.weight)
                     mod.fp8_stored = StoredFP8(mod.weight, (q, scale))
             n += 1
+    if frozen and not n:
+        raise ValueError("freeze_fp8_block: no layer of the model is in 8-bit blocks; call apply_fp8_block(model) first")
     return n

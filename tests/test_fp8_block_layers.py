@@ -4,6 +4,7 @@ import torch
 import torch.nn as nn
 
 from archscale_b200.config import Config
+from archscale_b200.eval import load_model
 from archscale_b200.models.gpt import GPT
 from archscale_b200.models.layers import Linear, apply_fp8_block, freeze_fp8_block
 
@@ -86,3 +87,46 @@ def test_families(device, family):
         live = m(idx).logits
         assert freeze_fp8_block(m) == len(layers) - 1 - len(steering)
         assert torch.equal(m(idx).logits, live)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_evaluation_loads_what_was_trained(device, tmp_path):
+    """A checkpoint of a model that was trained in this format is evaluated in it, on stored weights; the caller may say otherwise."""
+    name = "transformer_gqa4_d8"
+    torch.manual_seed(0)
+    cfg = Config.from_name(name)
+    cfg.rope_base = 10000
+    small = dict(n_layer=1, n_embd=128, n_head=1, n_query_groups=1, head_dim=128, intermediate_size=256, vocab_size=128, padded_vocab_size=128)
+    real = Config.from_name.__func__
+    with pytest.MonkeyPatch.context() as mp:
+        mp.setattr(Config, "from_name", classmethod(lambda cls, n, **kw: real(cls, n, **{**small, "ar": None, **kw})))
+        trained = GPT(Config.from_name(name))
+        trained.reset_parameters()
+        paths = {}
+        for fp8 in (False, True):
+            config = {**trained.config.to_dict(), "fp8_block": fp8}
+            paths[fp8] = str(tmp_path / f"{fp8}.pth")
+            torch.save({"model": trained.state_dict(), "config": config}, paths[fp8])
+        paths["bare"] = str(tmp_path / "bare.pth")
+        torch.save(trained.state_dict(), paths["bare"])
+        idx = torch.randint(0, 128, (1, 8), device=device)
+
+        def logits(path, **kw):
+            m = load_model(path, name, device=device, **kw).model
+            on = {l.fp8_block for n, l in m.named_modules() if isinstance(l, Linear) and n != "lm_head"}
+            with torch.no_grad():
+                stored = {l.stored_fp8() is not None for n, l in m.named_modules() if isinstance(l, Linear) and n != "lm_head"}
+                assert len(on) == 1 and on == stored == {m.config.fp8_block}
+                return m.config.fp8_block, m(idx).logits
+
+        assert [logits(paths[p])[0] for p in (False, True, "bare")] == [False, True, False]
+        assert logits(paths[True], fp8_block=False)[0] is False and logits(paths["bare"], fp8_block=True)[0] is True
+        plain, eight = logits(paths[False])[1], logits(paths[True])[1]
+        assert not torch.equal(plain, eight) and (plain - eight).norm() <= 0.25 * plain.norm()
+
+
+def test_freezing_needs_layers():
+    m = _dense("cpu")
+    with pytest.raises(ValueError, match="apply_fp8_block"):
+        freeze_fp8_block(m)
+    assert freeze_fp8_block(m, False) == 0
