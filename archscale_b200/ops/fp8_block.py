@@ -31,6 +31,7 @@ The functions ending in ``_ref`` are plain PyTorch restatements used as the CPU 
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple, Union
 
 import torch
@@ -45,6 +46,11 @@ _FLOATS = (torch.bfloat16, torch.float32)
 
 
 # ------------------------------------------------------------------------------------------------ references
+def _flat(x: torch.Tensor) -> torch.Tensor:
+    """x:(..., C) → (rows, C), of no rows or no columns too."""
+    return x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
+
+
 def _padded(x: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
     return torch.nn.functional.pad(x, (0, -x.shape[1] % cols, 0, -x.shape[0] % rows))
 
@@ -58,9 +64,10 @@ def _factors(amax: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 def quantize_ref(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     R, C = x.shape
-    xb = _padded(x.float(), 1, BLOCK).reshape(R, -1, BLOCK)
+    blocks = (C + BLOCK - 1) // BLOCK
+    xb = _padded(x.float(), 1, BLOCK).reshape(R, blocks, BLOCK)
     scale, u = _factors(xb.abs().amax(-1))
-    return (xb * u.unsqueeze(-1)).to(FP8).reshape(R, -1)[:, :C].contiguous(), scale
+    return (xb * u.unsqueeze(-1)).to(FP8).reshape(R, blocks * BLOCK)[:, :C].contiguous(), scale
 
 
 def quantize_weight_ref(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -99,7 +106,7 @@ def _norm_ref(res, h, weight, eps, h_scale, stream_dtype):
 
 def add_rms_norm_fp8_ref(res, h, weight, eps: float = 1e-5, h_scale: float = 1.0, stream_dtype: Optional[torch.dtype] = None):
     x, _, n = _norm_ref(res, h, weight, eps, h_scale, _stream(res, stream_dtype))
-    q, scale = quantize_ref(n.reshape(-1, n.shape[-1]))
+    q, scale = quantize_ref(_flat(n))
     return x, q, scale
 
 
@@ -202,7 +209,7 @@ def matmul_fp8_block(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_
         raise TypeError(f"matmul_fp8_block: operands must be float8_e4m3fn, got {a.dtype} and {b.dtype}")
     if a.dim() < 2 or b.dim() != 2 or a.shape[-1] != b.shape[1]:
         raise ValueError(f"matmul_fp8_block: contraction lengths differ: {tuple(a.shape)} and {tuple(b.shape)}")
-    lead, a = a.shape[:-1], a.reshape(-1, a.shape[-1])
+    lead, a = a.shape[:-1], _flat(a)
     blocks = (a.shape[1] + BLOCK - 1) // BLOCK
     for what, q, s in (("a_scale", a, a_scale), ("b_scale", b, b_scale)):
         if s.dtype != torch.float32 or s.dim() != 2 or s.shape[1] != blocks or s.shape[0] not in (q.shape[0], (q.shape[0] + BLOCK - 1) // BLOCK):
@@ -234,8 +241,7 @@ def linear_fp8_weight(x: Union[torch.Tensor, Quantised], weight: torch.Tensor, s
     if _kernel(x):
         backend.count_launch(2)
         return backend.require_extension().linear_fp8_stored(x, weight, scale, bias, dtype is torch.float32)
-    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    q, s = quantize_fp8_block(flat)
+    q, s = quantize_fp8_block(_flat(x))
     y = matmul_fp8_block(q, s, weight, scale, bias, dtype)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
 
@@ -253,7 +259,7 @@ def _layer_backward(gy2, w_t, w_scale, x_t, weight, want_x, x_dtype, want_w):
 class _LinearFP8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        x2 = x.reshape(-1, x.shape[-1])
+        x2 = _flat(x)
         wq, w_t, w_scale = quantize_fp8_weight(weight)
         q, scale = quantize_fp8_block(x2)
         need_w = bool(ctx.needs_input_grad) and ctx.needs_input_grad[1]
@@ -266,7 +272,7 @@ class _LinearFP8Fn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gy):
         w_t, w_scale, *x_t = ctx.saved_tensors
-        gy2 = gy.reshape(-1, gy.shape[-1])
+        gy2 = _flat(gy)
         need_x, need_w, need_b = ctx.needs_input_grad
         dx, dw = _layer_backward(gy2, w_t, w_scale, x_t, ctx.weight, need_x, ctx.x_dtype, need_w)
         return (None if dx is None else dx.view(ctx.x_shape)), dw, (gy2.sum(0, dtype=torch.float32).to(ctx.bias_dtype) if need_b else None)
@@ -307,7 +313,7 @@ def _norm_kernel(res, h, weight, eps, h_scale, stream_dtype, want_rstd):
     if not _kernel(res) or not 1 <= C <= 32768:
         _check_norm("add_rms_norm_fp8", res, h, weight, _stream(res, stream_dtype))
         x, rstd, n = _norm_ref(res, h, weight, eps, h_scale, _stream(res, stream_dtype))
-        return (x, *quantize_ref(n.reshape(-1, C)), rstd.reshape(-1))
+        return (x, *quantize_ref(_flat(n)), rstd.reshape(-1))
     return _ext().add_rmsnorm_fp8(res, h, weight, eps, h_scale, _stream_code(stream_dtype), want_rstd)
 
 
@@ -348,13 +354,13 @@ class _AddNormLinearFP8Fn(torch.autograd.Function):
     def backward(ctx, gx, gy):
         x, rstd, norm_weight, w_t, w_scale = ctx.saved_tensors
         C = ctx.shape[-1]
-        x = x.reshape(-1, C)
+        x = _flat(x)
         need_res, need_h, need_nw, need_w, need_b = ctx.needs_input_grad[:5]
         need_n = need_res or need_h or need_nw
-        gx2 = None if gx is None else gx.reshape(-1, C)
+        gx2 = None if gx is None else _flat(gx)
         dn = dw = db = dres = dh = dnw = None
         if gy is not None:
-            gy2 = gy.reshape(-1, gy.shape[-1])
+            gy2 = _flat(gy)
             if need_n or need_w:
                 x_t = quantize_ref((x.float() * rstd.view(-1, 1) * norm_weight.float()).t()) if need_w else None
                 dn, dw = _layer_backward(gy2, w_t, w_scale, x_t, ctx.weight, need_n, torch.float32, need_w)

@@ -83,3 +83,33 @@ def test_vmap_and_traces(device):
             with ctx():
                 traced = torch.jit.trace(call, (x,), check_trace=False)
                 assert _near(traced(batch[2]), call(batch[2]), bound) and not torch.allclose(traced(batch[2]), traced(x))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lead", [(0,), (4,), (2, 3), (0, 3), (2, 0)])
+@pytest.mark.parametrize("K,N", [(160, 40), (0, 40), (160, 0), (0, 0)])
+def test_sizes_of_zero(device, lead, K, N):
+    """No tokens, an empty sum, no outputs: the shapes and zeros that F.linear gives, gradients too."""
+    g = torch.Generator().manual_seed(0)
+    x, w, gy = (torch.randn(*s, generator=g).to(device) for s in ((*lead, K), (N, K), (*lead, N)))
+    x.requires_grad_(), w.requires_grad_()
+    bias = torch.ones(N, device=device)
+    y, z = ops.linear_fp8_block(x, w, bias), torch.nn.functional.linear(x, w, bias)
+    assert y.shape == z.shape and (K > 0 or (y == 1).all())
+    for got, want in zip(torch.autograd.grad(y, (x, w), gy), torch.autograd.grad(z, (x, w), gy)):
+        assert got.shape == want.shape and (want.numel() == 0 or want.abs().max() > 0 or (got == 0).all())
+    with torch.no_grad():
+        wq, wt, ws = ops.quantize_fp8_weight(w)
+        assert wq.shape == (N, K) and wt.shape == (K, N) and ws.shape == (-(-N // 128), -(-K // 128))
+        y = ops.linear_fp8_weight(x, wq, ws, bias)
+        assert y.shape == z.shape and (K > 0 or (y == 1).all())
+        if K:
+            n = torch.ones(K, device=device)
+            s, q, scale = ops.add_rms_norm_fp8(x, x.bfloat16(), n)
+            rows = z.numel() // N if N else x.numel() // K
+            assert s.shape == x.shape and q.shape == (rows, K) and scale.shape == (rows, -(-K // 128))
+            assert ops.linear_fp8_weight((q.view(x.shape), scale), wq, ws).shape == z.shape
+    if K:
+        s, y = ops.add_rms_norm_linear_fp8(x, None, n.requires_grad_(), w)
+        dx, dn, dw = torch.autograd.grad(y, (x, n, w), gy.bfloat16())
+        assert y.shape == z.shape and dx.shape == x.shape and dn.shape == n.shape and dw.shape == w.shape
