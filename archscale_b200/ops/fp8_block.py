@@ -51,6 +51,11 @@ def _flat(x: torch.Tensor) -> torch.Tensor:
     return x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
 
 
+def _to(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """``x.to(dtype)``; in a trace as a copy, since the fuser of ``torch.jit`` writes code for it that names an e4m3 type CUDA does not have."""
+    return x.to(dtype) if torch._C._get_tracing_state() is None else torch.empty_like(x, dtype=dtype).copy_(x)
+
+
 def _padded(x: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
     return torch.nn.functional.pad(x, (0, -x.shape[1] % cols, 0, -x.shape[0] % rows))
 
@@ -67,7 +72,7 @@ def quantize_ref(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     blocks = (C + BLOCK - 1) // BLOCK
     xb = _padded(x.float(), 1, BLOCK).reshape(R, blocks, BLOCK)
     scale, u = _factors(xb.abs().amax(-1))
-    return (xb * u.unsqueeze(-1)).to(FP8).reshape(R, blocks * BLOCK)[:, :C].contiguous(), scale
+    return _to(xb * u.unsqueeze(-1), FP8).reshape(R, blocks * BLOCK)[:, :C].contiguous(), scale
 
 
 def quantize_weight_ref(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -76,7 +81,7 @@ def quantize_weight_ref(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     nb, kb = wb.shape[0] // BLOCK, wb.shape[1] // BLOCK
     wb = wb.view(nb, BLOCK, kb, BLOCK)
     scale, u = _factors(wb.abs().amax((1, 3)))
-    return (wb * u.view(nb, 1, kb, 1)).to(FP8).view(nb * BLOCK, kb * BLOCK)[:N, :K].contiguous(), scale
+    return _to(wb * u.view(nb, 1, kb, 1), FP8).view(nb * BLOCK, kb * BLOCK)[:N, :K].contiguous(), scale
 
 
 def dequantize_ref(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -85,7 +90,7 @@ def dequantize_ref(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = to
     s = scale.to(dtype)
     if s.shape[0] != R:
         s = s.repeat_interleave(BLOCK, 0)[:R]
-    return q.to(dtype) * s.repeat_interleave(BLOCK, 1)[:, :C]
+    return _to(q, dtype) * s.repeat_interleave(BLOCK, 1)[:, :C]
 
 
 def matmul_fp8_block_ref(a, a_scale, b, b_scale, bias=None, out_dtype=torch.bfloat16, acc=None):
