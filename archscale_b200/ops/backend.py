@@ -92,7 +92,7 @@ def use_cuda_kernel(op: str, *tensors: torch.Tensor) -> bool:
 def transformed() -> bool:
     """True while a functorch transform, a forward-mode level or a ``torch.jit`` trace is active."""
     return (torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0
-            or torch._C._get_tracing_state() is not None)
+            or torch._C._is_tracing())
 
 
 def plain_call() -> bool:

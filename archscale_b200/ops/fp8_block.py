@@ -145,7 +145,7 @@ def _kernel(x: torch.Tensor) -> bool:
 
 
 def _no_grad(name: str, *tensors) -> None:
-    """A call that has no gradients must not cut a graph silently."""
+    """A call that has no gradients must not cut a graph silently (the bindings check the operands of the kernels)."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -164,36 +164,36 @@ def _ext():
 # ------------------------------------------------------------------------------------------------ quantisers
 def quantize_fp8_block(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x:(R,C) → (elements (R,C), scales (R, ⌈C/128⌉)), blocks along the rows."""
-    _no_grad("quantize_fp8_block", x)
     if _kernel(x):
         return tuple(_ext().fp8_quantize(x, 1))
+    _no_grad("quantize_fp8_block", x)
     _need_matrix("quantize_fp8_block", x)
     return quantize_ref(x)
 
 
 def quantize_fp8_block_t(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x:(R,C) → (elements (C,R), scales (C, ⌈R/128⌉)) of the transposed matrix, blocks along the original columns."""
-    _no_grad("quantize_fp8_block_t", x)
     if _kernel(x):
         return tuple(_ext().fp8_quantize(x, 2))
+    _no_grad("quantize_fp8_block_t", x)
     _need_matrix("quantize_fp8_block_t", x)
     return quantize_ref(x.t())
 
 
 def quantize_fp8_block_both(x: torch.Tensor):
     """:func:`quantize_fp8_block` and :func:`quantize_fp8_block_t` from one read of x: (q, scale, q_t, scale_t)."""
-    _no_grad("quantize_fp8_block_both", x)
     if _kernel(x):
         return tuple(_ext().fp8_quantize(x, 3))
+    _no_grad("quantize_fp8_block_both", x)
     _need_matrix("quantize_fp8_block_both", x)
     return (*quantize_ref(x), *quantize_ref(x.t()))
 
 
 def quantize_fp8_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """w:(N,K) → (elements (N,K), the same transposed (K,N), scales (⌈N/128⌉, ⌈K/128⌉) of 128 × 128 tiles)."""
-    _no_grad("quantize_fp8_weight", w)
     if _kernel(w):
         return tuple(_ext().fp8_quantize(w, 4))
+    _no_grad("quantize_fp8_weight", w)
     _need_matrix("quantize_fp8_weight", w)
     q, scale = quantize_weight_ref(w)
     return q, q.t().contiguous(), scale
@@ -205,11 +205,11 @@ def matmul_fp8_block(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_
     """``a:(M,K) · b:(N,K)ᵀ (+ bias)``, each operand with scales per row and block of 128, ``(rows, ⌈K/128⌉)``, or per 128 × 128 tile,
     ``(⌈rows/128⌉, ⌈K/128⌉)`` → (M,N) in ``out_dtype``; with ``acc`` (fp32) the product is added to it in place.  ``a`` may have more leading
     dimensions than one (M: their product), which the result then has too."""
-    _no_grad("matmul_fp8_block", a, a_scale, b, b_scale, bias, acc)
     if out_dtype not in _FLOATS:
         raise TypeError(f"matmul_fp8_block: out_dtype must be bfloat16 or float32, got {out_dtype}")
     if _kernel(a):
         return _ext().gemm_fp8_block(a, a_scale, b, b_scale, bias, out_dtype is torch.float32, acc)
+    _no_grad("matmul_fp8_block", a, a_scale, b, b_scale, bias, acc)
     if a.dtype != FP8 or b.dtype != FP8:
         raise TypeError(f"matmul_fp8_block: operands must be float8_e4m3fn, got {a.dtype} and {b.dtype}")
     if a.dim() < 2 or b.dim() != 2 or a.shape[-1] != b.shape[1]:
@@ -237,15 +237,14 @@ def linear_fp8_weight(x: Union[torch.Tensor, Quantised], weight: torch.Tensor, s
     pair (elements, scales) of :func:`add_rms_norm_fp8` / :func:`quantize_fp8_block` with any leading dimensions of the elements.  It has
     no gradients and refuses operands that ask for one."""
     if not isinstance(x, torch.Tensor):
-        _no_grad("linear_fp8_weight", x[1], scale, bias)
         return matmul_fp8_block(x[0], x[1], weight, scale, bias, out_dtype or torch.bfloat16)
-    _no_grad("linear_fp8_weight", x, scale, bias)
     dtype = out_dtype or x.dtype
     if dtype not in _FLOATS:
         raise TypeError(f"linear_fp8_weight: results are bfloat16 or float32, not {dtype}")
     if _kernel(x):
         backend.count_launch(2)
         return backend.require_extension().linear_fp8_stored(x, weight, scale, bias, dtype is torch.float32)
+    _no_grad("linear_fp8_weight", x, scale, bias)
     q, s = quantize_fp8_block(_flat(x))
     y = matmul_fp8_block(q, s, weight, scale, bias, dtype)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
