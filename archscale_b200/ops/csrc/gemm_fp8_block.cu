@@ -158,7 +158,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         const int blocks = min(FS_CHUNK, nkb - i);
         for (int j = t; j < blocks * BT; j += T::SUMMERS) {
           const int m = m0 + j % BT;
-          table[j] = m < p.M ? p.sa.p[static_cast<int64_t>(m >> p.sa.shift) * p.sa.row + (kb0 + i + j / BT) * p.sa.blk] : 0.f;
+          table[j] = m < p.M ? p.sa.p[static_cast<int64_t>(m >> p.sa.shift) * p.sa.row + (kb0 + i + j / BT) * p.sa.blk] * kFp8Down : 0.f;
         }
         asm volatile("bar.sync 1, %0;" ::"n"(T::SUMMERS) : "memory");
       }
@@ -189,7 +189,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     // the last products were waited for, so the loads before them have landed and the stages may be written
     if (ok) {
 #pragma unroll
-      for (int i = 0; i < W; ++i) part[(c0 + i) * FS_BN + q * 32 + lane] = sum[i];
+      for (int i = 0; i < W; ++i) part[(c0 + i) * FS_BN + q * 32 + lane] = sum[i] * kFp8Up;
     }
   }
   tc_fence_before();

@@ -382,6 +382,11 @@ __device__ __forceinline__ float2 unpack_f32x2(unsigned long long v) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
   return f;
 }
+// A block's sum of 128 products of e4m3 values, up to 2^24.6, times a scale of up to 2^119.2 = FLT_MAX / 448 does not fit fp32, though the other
+// operand's scale may bring it back.  So the scale that is multiplied first is held 2^-17 times as large, and sums are made good at the end; the
+// smallest scale of the quantisers, 2^-108.5 = 1e-30 / 448, stays a normal number by it.
+constexpr float kFp8Down = 1.f / 131072.f, kFp8Up = 131072.f;
+
 __device__ __forceinline__ float2 fma_f32x2(float2 a, float2 b, float2 c) {
   unsigned long long r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pack_f32x2(a)), "l"(pack_f32x2(b)), "l"(pack_f32x2(c)));

@@ -9,8 +9,8 @@ With ``a = max(max|block|, 1e-30)``, every operation in fp32 and rounded once,
 
     ``out[m, n] = Σ_b sa[m, b] · sb[n, b] · Σ_{k in b} a[m, k] · b[n, k]``                        (:func:`matmul_fp8_block`)
 
-with the inner sums on the tensor cores and the outer ones in fp32.  Where both scales of a block are so small that their product
-is below 2⁻¹²⁶ the block counts as zero.  Any size is taken: no dimension has to be a multiple of 128.
+with the inner sums on the tensor cores and the outer ones in fp32.  One scale of a block may be as large as the other is small.  Where their
+product is below 2⁻¹²⁶, or one of them below 2⁻¹⁰⁹ (the quantisers make none), the block may count as zero, and where the product is past the range of fp32 as infinite.  Any size is taken: no dimension has to be a multiple of 128.
 
 * :func:`linear_fp8_block` trains: ``y = Q(x) Q(W)ᵀ``, ``dx = Q(dy) Q(W)``, ``dW = Qᵗ(dy)ᵀ Qᵗ(x)``, where ``Qᵗ`` takes its blocks along the
   tokens; the rounding itself has gradient one.  Weights stay bf16 / fp32 and are quantised in every call.
