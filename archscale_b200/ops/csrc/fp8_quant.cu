@@ -718,7 +718,7 @@ static int launch_norm_bwd(const Fp8NormBwdParams& p, int grid, cudaStream_t st)
 }  // namespace b200
 
 // x [rows, cols] (dtype 0 fp32, 1 bf16, rows ldx elements apart).  mode: 1 rows (q, s), 2 columns (qt, st), 3 both, 4 tiles of
-// 128 × 128 (q, s and, unless null, qt).  With rstd, w: the values are (x · rstd[row]) · w[col] (modes 1 to 3).  ldq, ldqt: multiples of 16.
+// 128 × 128 (q, s and, unless null, qt).  With rstd, w: the values are (x · rstd[row]) · w[col] (mode 2).  ldq, ldqt: multiples of 16.
 extern "C" int b200_fp8_quantize(const void* x, int dtype, int64_t ldx, int rows, int cols, int mode, void* q, int64_t ldq, float* s,
                                  int64_t lds, void* qt, int64_t ldqt, float* st, int64_t ldst, const float* rstd, const void* w,
                                  int w_dtype, cudaStream_t stream) {
