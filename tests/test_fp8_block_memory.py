@@ -49,3 +49,25 @@ def test_any_set_of_gradients(want):
     some = [t.clone().requires_grad_(i in want) for i, t in enumerate(given)]
     got = torch.autograd.grad(ops.linear_fp8_block(*some), [some[i] for i in want], gy)
     assert all(torch.equal(a, all_[i]) for a, i in zip(got, want))
+
+
+@pytest.mark.parametrize("branch", [False, True])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_any_set_of_gradients_behind_a_norm(branch, with_bias):
+    g = torch.Generator(device="cuda").manual_seed(0)
+    shapes = {"res": (30, 160), "h": (30, 160), "norm": (160,), "weight": (200, 160), "bias": (200,)}
+    names = [n for n in shapes if (n != "h" or branch) and (n != "bias" or with_bias)]
+    given = {n: torch.randn(*shapes[n], generator=g, device="cuda").bfloat16() for n in names}
+    gx, gy = (torch.randn(30, k, generator=g, device="cuda").bfloat16() for k in (160, 200))
+
+    def grads(want):
+        t = {n: v.clone().requires_grad_(n in want) for n, v in given.items()}
+        x, y = ops.add_rms_norm_linear_fp8(t["res"], t.get("h"), t["norm"], t["weight"], bias=t.get("bias"))
+        outs, ins = [(o, d) for o, d in ((x, gx), (y, gy)) if o.requires_grad], [t[n] for n in names if n in want]
+        return dict(zip([n for n in names if n in want], torch.autograd.grad([o for o, _ in outs], ins, [d for _, d in outs])))
+
+    full = grads(names)
+    for bits in range(1, 2 ** len(names)):
+        want = [n for i, n in enumerate(names) if bits >> i & 1]
+        for n, got in grads(want).items():
+            assert torch.equal(got, full[n]), (want, n)

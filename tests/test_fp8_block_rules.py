@@ -113,3 +113,19 @@ def test_sizes_of_zero(device, lead, K, N):
         s, y = ops.add_rms_norm_linear_fp8(x, None, n.requires_grad_(), w)
         dx, dn, dw = torch.autograd.grad(y, (x, n, w), gy.bfloat16())
         assert y.shape == z.shape and dx.shape == x.shape and dn.shape == n.shape and dw.shape == w.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [160, 200])
+def test_operands_on_two_devices(K):
+    """Refused as such, whether or not the rows of the elements would have to be copied first."""
+    x, w = torch.randn(5, K, device="cuda"), torch.randn(40, K, device="cuda")
+    (q, s), (wq, _, ws) = ops.quantize_fp8_block(x), ops.quantize_fp8_weight(w)
+    host = lambda t: t.cpu().contiguous()  # noqa: E731
+    for args in ((q, s, host(wq), ws), (q, s, wq, host(ws)), (q, host(s), wq, ws), (q, s, wq, ws, torch.zeros(40))):
+        with pytest.raises(ValueError):
+            ops.matmul_fp8_block(*args)
+    for call in (lambda: ops.linear_fp8_block(x, host(w)), lambda: ops.linear_fp8_weight(x, host(wq), ws),
+                 lambda: ops.add_rms_norm_fp8(x, None, torch.ones(K)), lambda: ops.add_rms_norm_linear_fp8(x, None, torch.ones(K, device="cuda"), host(w))):
+        with pytest.raises(ValueError):
+            call()
