@@ -50,3 +50,19 @@ def test_empty_blocks_against_large_ones(M, kinds):
     out = ops.matmul_fp8_block(a, sa, b, sb, out_dtype=torch.float32)
     want = 128 * 1e-30 * 3e38
     assert ((out - want).abs() <= want * 200 * 2.0 ** -23).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(1, 128, 40000), (5, 300, 70000), (30, 2000, 20000), (64, 1000, 36100), (64, 20000, 9000)])
+@pytest.mark.parametrize("kinds", ["row,tile", "row,row", "tile,row"])
+def test_few_rows_of_long_contractions(M, N, K, kinds):
+    """More than 32 blocks of K per CTA, so that the table of scales is filled more than once.  The bound is that of any product; a few hundred blocks are
+    added in an order that is the same from call to call."""
+    g = torch.Generator(device="cuda").manual_seed(K)
+    quant = {"row": ops.quantize_fp8_block, "tile": lambda t: ops.quantize_fp8_weight(t)[::2]}
+    (a, sa), (b, sb) = (quant[k](torch.randn(r, K, generator=g, device="cuda").bfloat16()) for k, r in zip(kinds.split(","), (M, N)))
+    A, B = (fb.dequantize_ref(*t, torch.float64) for t in ((a, sa), (b, sb)))
+    want, mag = A @ B.t(), A.abs() @ B.abs().t()
+    out = ops.matmul_fp8_block(a, sa, b, sb, out_dtype=torch.float32)
+    assert ((out.double() - want).abs() <= mag * (128 * 2.0 ** -23 + (-(-K // 128) + 3) * 2.0 ** -24)).all()
+    assert torch.equal(out, ops.matmul_fp8_block(a, sa, b, sb, out_dtype=torch.float32))
