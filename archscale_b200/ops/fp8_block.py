@@ -17,7 +17,8 @@ product is below 2⁻¹²⁶, or one of them below 2⁻¹⁰⁹ (the quantisers 
 * :func:`linear_fp8_weight` serves weights that were quantised beforehand (``quantize_fp8_weight``, or a checkpoint's elements and
   scales), from one token on.
 * :func:`add_rms_norm_fp8` is the block entry ``x = res + h_scale · h``, ``n = rmsnorm(x) · w`` with ``n`` delivered in this format (it is never
-  rounded to 16 bits); :func:`add_rms_norm_linear_fp8` trains it with the layer behind it.  Its backward makes the transposed operand of
+  rounded to 16 bits; an element is what ``n · 448 / a`` rounds to as a real number, which the formula in fp32 misses for about one value in ten
+  thousand, those half way between two elements); :func:`add_rms_norm_linear_fp8` trains it with the layer behind it.  Its backward makes the transposed operand of
   the weight gradient from the residual stream, which is kept anyway, so that ``n`` itself is kept in no form.
 
 Quantisers, product, stored layer and :func:`add_rms_norm_fp8` have no gradients, on any device: with gradients enabled they refuse operands that ask
