@@ -207,3 +207,25 @@ def test_two_ranks():
     for _ in range(2):
         rank, got, again, raised, same = q.get()
         assert got and again and raised and not same, rank
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_inference_mode(device):
+    """Frozen and live layers in it, a store that was made in it, and a change that is made in it."""
+    lin, x = _layer()
+    lin, x = lin.to(device), x.to(device)
+    with torch.no_grad():
+        want = lin(x)
+    with torch.inference_mode():
+        assert torch.equal(lin(x), want)
+        freeze_fp8_block(lin)
+        assert lin.stored_fp8() is not None and torch.equal(lin(x), want)
+    with torch.no_grad():
+        assert torch.equal(lin(x), want)
+    with torch.inference_mode():
+        lin.weight.mul_(2.0)
+        with pytest.raises(RuntimeError, match="frozen"):
+            lin(x)
+    freeze_fp8_block(lin)
+    lin(x).sum().backward()
+    assert lin.weight.grad is not None
