@@ -14,6 +14,8 @@ from .moe import (load_balance_loss, moe_ffn, moe_ffn_ref, router_topk_softmax, 
                   stable_topk)
 from .newton_schulz import newton_schulz, newton_schulz_ref  # noqa: F401
 from .norm import add_rms_norm, add_rms_norm_ref, gated_rms_norm, layer_norm, rms_norm, rms_norm_ref, layer_norm_ref, gated_rms_norm_ref  # noqa: F401
+from .paged import (PagedCache, new_paged_cache, paged_attention, paged_attention_ref, paged_cache_read, paged_cache_read_ref,  # noqa: F401
+                    paged_cache_write, paged_cache_write_ref, paged_diff_attention, paged_diff_attention_ref)
 from .rope import apply_rotary_emb, build_rope_cache, qk_norm_rope, qkv_norm_rope, qkv_norm_rope_supported  # noqa: F401
 from .selective_scan import selective_scan, selective_scan_ref  # noqa: F401
 from .ssd import ssd_scan, ssd_scan_ref  # noqa: F401

@@ -311,6 +311,34 @@ int b200_gemm2_fp8_block(const void* A, int64_t lda, const float* sa, int64_t sa
                          int accumulate, void* ws, int num_sms, int* status, cudaStream_t stream);
 int64_t b200_gemm2_fp8_block_workspace(int M, int N, int K, int num_sms);      // bytes
 
+// Paged key-value cache (paged_cache.cu, paged_attention.cu, paged_attention_rows.cu; layout in paged.cuh).  Types: 0 fp32, 1 bf16, 2 e4m3.  Strides
+// in elements.
+struct b200_paged_view {
+  void *k, *v;
+  uint8_t *ks, *vs;                        // scale bytes, with e4m3
+  int64_t k_page, k_group, k_slot, v_page, v_group, v_slot;
+  int64_t ks_page, ks_group, ks_slot, vs_page, vs_group, vs_slot;
+  const int *table, *lengths, *new_lengths;   // new_lengths: null where all rows are real
+  int64_t table_row;
+  int pages, groups, page_size, dim, type, table_cols;
+  int* status;
+};
+// New rows k, v [B, T, G, D] of type `type` into the cache; strides of batch, token, head (D dense).
+int b200_paged_write(const struct b200_paged_view* c, const void* k, const void* v, int type, int64_t kb, int64_t kt, int64_t kh, int64_t vb, int64_t vt,
+                     int64_t vh, int B, int T, cudaStream_t st);
+// The first `tokens` tokens of each sequence into dense k, v [B, tokens, G, D] of type `type`, zeros where a sequence has none.
+int b200_paged_read(const struct b200_paged_view* c, void* k, void* v, int type, int B, int tokens, cudaStream_t st);
+// Attention of T new tokens: q [B, T, H, D] of type `type` with strides of batch, token, head; out dense of that type; lse fp32 [B, H, T] or null.
+// window < 0: none.  sink [H] or null.  diff: pairs of heads, a1 − λ·a2 normalised over 2 D, times w [2 D] and gain.  sink, λ and w: fp32 or bf16.
+struct b200_paged_query {
+  const void* q; void* out; float* lse;
+  const void *sink, *lam, *w;
+  int64_t q_batch, q_token, q_head;
+  float scale, gain, eps;
+  int B, T, H, type, window, diff, sink_type, lam_type, w_type;
+};
+int b200_paged_attention_rows(const struct b200_paged_view* c, const struct b200_paged_query* a, cudaStream_t st);
+
 #ifdef __cplusplus
 }
 #endif

@@ -240,6 +240,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qknorm_rope_bwd(
 
 #include "bindings_extra.inc"
 #include "bindings_fp8.inc"
+#include "bindings_paged.inc"
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_bf16", &gemm_bf16, "bf16 tcgen05 GEMM", py::arg("a"), py::arg("b"), py::arg("mode"), py::arg("out_dtype"),
@@ -261,4 +262,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qknorm_rope_bwd", &qknorm_rope_bwd);
   register_extra(m);
   register_fp8(m);
+  register_paged(m);
 }
