@@ -23,7 +23,8 @@ BUILD = os.path.join(PKG, "_build")
 OUT = os.path.join(PKG, "_C.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-PRECISE = {"gdn_pieces.cu", "fp8_quant.cu", "paged_cache.cu", "paged_attention_rows.cu"}     # built without --use_fast_math: expf and divisions at their documented accuracy, subnormal numbers kept
+PRECISE = {"gdn_pieces.cu", "fp8_quant.cu", "paged_cache.cu", "paged_attention.cu", "paged_attention_bf16.cu",
+           "paged_attention_e4m3.cu", "paged_attention_rows.cu"}     # built without --use_fast_math: expf and divisions at their documented accuracy, subnormal numbers kept
 
 
 def _newer(src: str, dst: str, headers) -> bool:

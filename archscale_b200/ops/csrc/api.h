@@ -337,6 +337,10 @@ struct b200_paged_query {
   float scale, gain, eps;
   int B, T, H, type, window, diff, sink_type, lam_type, w_type;
 };
+// ws: b200_paged_attention_workspace bytes, 16-byte aligned.
+int64_t b200_paged_attention_workspace(const struct b200_paged_view* c, const struct b200_paged_query* a, int num_sms);
+int b200_paged_attention(const struct b200_paged_view* c, const struct b200_paged_query* a, void* ws, int num_sms, cudaStream_t st);
+// What that one does not take (fp32, other strides), called by it: a CTA per query row.
 int b200_paged_attention_rows(const struct b200_paged_view* c, const struct b200_paged_query* a, cudaStream_t st);
 
 #ifdef __cplusplus
