@@ -3,7 +3,7 @@
 
 namespace b200 {
 
-struct PaPlan { PaArgs p; int dt, mode, span, tiles, nrt, nb; bool gen, ok; };
+struct PaPlan { PaArgs p; int dt, nc, span, tiles, nrt, nb; bool gen, ok; };
 
 static PaPlan pa_plan(const PagedView& c, const b200_paged_query& a) {
   PaPlan s = {};
@@ -19,11 +19,15 @@ static PaPlan pa_plan(const PagedView& c, const b200_paged_query& a) {
   p.per = a.H / c.groups;                                                       // query heads, or pairs of them, of a key head or pair
   p.rows = p.per * a.T;
   p.heads = a.diff ? c.groups / 2 : c.groups;
-  s.mode = a.diff ? PA_PAIRS : p.rows <= 8 ? PA_ROWS8 : PA_ROWS16;
+  s.nc = p.rows <= (a.diff ? 4 : 8) ? 1 : 2;
   s.dt = a.diff ? (D <= 64 ? 128 : 256) : D <= 64 ? 64 : D <= 128 ? 128 : 256;
-  s.gen = p.piece != 16 || D != (a.diff ? s.dt / 2 : s.dt);
+  const int64_t far = (static_cast<int64_t>(c.pages) * p.page_b + static_cast<int64_t>(c.page_size) * p.slot_b) / 16;
+  p.page_16 = static_cast<uint32_t>(p.page_b / 16); p.slot_16 = static_cast<uint32_t>(p.slot_b / 16);
+  p.page_shift = -1;
+  for (int i = 0; i < 31; ++i) if (c.page_size == 1 << i) p.page_shift = i;
+  s.gen = far > 0xffffffffLL || p.piece != 16 || D != (a.diff ? s.dt / 2 : s.dt);
   p.q_words = reinterpret_cast<uintptr_t>(a.q) % 4 == 0 && (a.q_batch | a.q_token | a.q_head) % 2 == 0;
-  const int qrows = s.mode == PA_ROWS16 ? 16 : 8;
+  const int qrows = (a.diff ? 4 : 8) * s.nc;
   const int64_t room = static_cast<int64_t>(c.table_cols) * c.page_size, seen = a.window >= 0 ? static_cast<int64_t>(a.window) + qrows + 1 : room;
   const int64_t span = room < seen ? room : seen;
   s.span = static_cast<int>(span < 0x7fffff00 ? span : 0x7fffff00);
@@ -36,7 +40,7 @@ static PaPlan pa_plan(const PagedView& c, const b200_paged_query& a) {
   return s;
 }
 static int pa_go(const PaPlan& s, PaArgs& p, int num_sms, void* ws, int64_t* need, cudaStream_t st) {
-  return (p.c.type == 2 ? pa_run_e4m3 : pa_run_bf16)(p, s.dt, s.mode, s.gen, s.span, num_sms, ws, need, st);
+  return (p.c.type == 2 ? pa_run_e4m3 : pa_run_bf16)(p, s.dt, p.a.diff != 0, s.nc, s.gen, s.span, num_sms, ws, need, st);
 }
 
 }  // namespace b200

@@ -5,18 +5,20 @@
 // In e4m3 a key's power of two multiplies its score; a value's, 2^e_j, goes into the weight, p'_j = 2^(x_j + e_j − m' + 14), whose maximum m' is kept
 // beside m: no value is too small or large beside another, whatever their scales.
 //
-// Rows.  The query rows of a key head (its H/G heads times T tokens) are the 16 rows of an MMA m16n8k16, its columns keys (scores) or values (outputs):
-//   ROWS8    up to 8 rows: the weights p enter the second product as two 16-bit halves, hi in rows 0-7 and lo = p − hi in rows 8-15 of one MMA
-//   ROWS16   up to 16: two MMAs, for hi and lo
-//   PAIRS    differential attention: 8 rows of branch 1 as [q1 | 0], the same 8 of branch 2 as [0 | q2], keys [k1 | k2], values [v1 | v2]: one product
-//            each for both branches, and a1 − λ a2 is in one thread
-// The halves make p as good as 2⁻¹⁷ (bf16; e4m3 runs in fp16: 2⁻²²), which costs nothing where the tensor cores wait for memory.  q is exact:
-// bf16 as it is, for fp16 times a power of two of its row.
+// Tokens are the rows of the MMAs (m16n8k16), query rows their 8 columns: scores are K · Qᵀ, outputs Vᵀ · Pᵀ.  So a call of a few query rows wastes nothing,
+// a warp's sums take D · 8 floats, and keys and values are left operands straight from memory order.  P turns from a result (tokens down) into a right
+// operand (tokens along k) by transposing 8 × 8 blocks between registers.  Columns:
+//   plain    the H/G heads of the key head times T tokens, 8 · NC to a tile
+//   PAIRS    differential attention: 4 rows of branch 1 as [q1 | 0], then the same 4 of branch 2 as [0 | q2], against keys [k1 | k2] and
+//            values [v1 | v2]: one read and one product for both branches
+// Rounding: q is exact (bf16; for fp16 times a power of two of its row).  In bf16 P enters as two halves, hi and p − hi, so that it is good to 2⁻¹⁷: its plain
+// rounding, 2⁻⁹ of each weight, would be as large as that of the result, and the second product costs nothing where the tensor cores wait for memory.
+// In e4m3 the products run in fp16, whose 2⁻¹² is an eighth of the result's rounding: one half is enough (weights from 2¹⁴ down to 2⁻²⁴).
 //
-// What bounds it: memory.  16 rows are 32 operations a byte at most, and tcgen05 would want 128 rows, keys and P written back through shared memory; so the
-// keys feed mma.sync from shared memory (4 warps per scheduler would keep up with 1.5 times the bandwidth).  Each warp is on its own: it
-// loads its tokens with cp.async into its own ring of three stages (16 to 32 tokens, 8 KB), and no barrier joins warps before the
-// end of a work item.  Pages are looked up one step ahead, so that their latency is not in the chain.
+// What bounds it: memory.  At most 16 columns are 32 operations a byte; tcgen05 would take 128 rows of keys too, but wants P through shared memory and its sums
+// through tensor memory for every tile, which is the longer chain where a CTA has a handful of tiles.  Each warp is on its own: it loads its
+// tokens with cp.async into its own ring (steps of 16 or 32 tokens, 8 KB), and no barrier joins warps before the end of a work item.  Pages are looked
+// up one step ahead, so that their latency is not in the chain.
 //
 // Work.  Lengths are known on the device only.  An item is (sequence, tile of rows, key head); its keys are chunks of 4 warps' steps.  Every CTA adds
 // up the chunks of all items from the lengths and takes an equal, contiguous share of them, so that one long sequence or many short ones fill the
@@ -24,14 +26,13 @@
 // do not depend on scheduling), which the first one starts early and which needs no counters, so that nothing has to be zero beforehand.
 #pragma once
 #include <cuda_fp16.h>
+#include <type_traits>
 
 #include "paged.cuh"
 
 namespace b200 {
 
-enum { PA_ROWS8 = 0, PA_ROWS16 = 1, PA_PAIRS = 2 };
 constexpr int PA_WARPS = 4;
-constexpr int PA_STAGES = 3;
 constexpr int PA_ENTRIES = 1024;           // (sequence, tile of rows) of one launch
 
 struct PaArgs {
@@ -42,30 +43,50 @@ struct PaArgs {
   int heads;                               // key heads, or pairs of them
   int ncta, piece, q_words;                // bytes of a copy where rows are not whole 16-byte pieces; queries start on 4-byte boundaries
   int64_t page_b, group_b, slot_b;         // strides in bytes, of keys as of values
+  uint32_t page_16, slot_16;               // the same in units of 16 bytes (not GEN)
+  int page_shift;                          // log2 of the page size, or -1
   float* parts;                            // [ncta][2] parts of items
   int* prefix;                             // chunks before each entry, from CTA 0
 };
 
-// What a shape needs.
-template <int ES, int DT, int MODE>
+// What a shape needs.  ES: bytes of an element; DT: values of a row of keys, of both heads of a pair; NC: groups of 8 columns.
+#ifndef PA_ST
+#define PA_ST 2
+#endif
+#ifndef PA_TS8
+#define PA_TS8 32
+#endif
+template <int ES, int DT, bool PAIRS, int NC>
 struct PaShape {
   static constexpr int ROW = DT * ES;                                          // bytes of a token in a stage
-  static constexpr int TS = ES == 2 ? (DT == 64 ? 32 : 16) : (DT == 256 ? 16 : 32);   // tokens of a warp's step
-  static constexpr int HEADS = MODE == PA_PAIRS ? 2 : 1;
+  static constexpr int TS = ES == 2 ? (DT == 64 ? 32 : 16) : (DT == 256 ? 16 : DT == 128 ? PA_TS8 : 32);   // tokens of a warp's step
+  static constexpr int HEADS = PAIRS ? 2 : 1;
   static constexpr int TILE = TS * ROW;
   static constexpr int SCALES = ES == 1 ? HEADS * TS * 8 : 0;                  // factors of keys, exponents of values
   static constexpr int STAGE = 2 * TILE + SCALES + 16;                         // and the mask of tokens
-  static constexpr int RING = PA_WARPS * PA_STAGES * STAGE;
-  static constexpr int QROWS = MODE == PA_ROWS16 ? 16 : 8;                     // query rows of a tile
-  static constexpr int OROWS = MODE == PA_ROWS8 ? 8 : 16;                      // rows of the output product
-  static constexpr int LD = DT + 8;                                            // floats between rows in shared memory: no bank twice
-  static constexpr int SLABS = PA_WARPS * OROWS * LD * 4;
+  static constexpr int STAGES = PA_ST;
+  static constexpr int RING = PA_WARPS * STAGES * STAGE;
+  static constexpr int COLS = 8 * NC;
+  static constexpr int QROWS = PAIRS ? 4 * NC : 8 * NC;                        // query rows of a tile
+  static constexpr int LD = DT + 4;                                            // floats between rows in shared memory: no bank twice
+  static constexpr int SLABS = PA_WARPS * COLS * LD * 4;
   static constexpr int SMEM = RING > SLABS ? RING : SLABS;
   static constexpr int CHUNK = PA_WARPS * TS;
-  static constexpr int NG = ES == 1 ? HEADS : 0;                               // groups of columns with maxima of their own
-  static constexpr int PART = OROWS * (DT + 4);                                // floats of a part: sums, then m, l, m' of each row
+  static constexpr int NG = ES == 1 ? HEADS : 0;                               // groups of values with maxima of their own
+  static constexpr int PART = COLS * (DT + 4);                                 // floats of a part: sums, then m, l, m' of each column
   static_assert(SMEM <= 227 * 1024 - 6144, "shared memory");
 };
+// column of a tile's query row r, in branch 0 or 1
+template <bool PAIRS>
+__host__ __device__ constexpr int pa_column(int r, int branch) { return PAIRS ? (r >> 2) * 8 + (r & 3) + 4 * branch : r; }
+
+// CTAs of an SM: as many as its shared memory and the registers of the sums allow
+template <int ES, int DT, bool PAIRS, int NC>
+constexpr int pa_resident() {
+  constexpr int one = PaShape<ES, DT, PAIRS, NC>::SMEM + (PA_ENTRIES + 1) * 4 + 2304;      // its static part and what the system keeps
+  constexpr int fit = 228 * 1024 / one, regs = DT * NC >= 512 ? 2 : DT * NC >= 256 ? 3 : 4;
+  return fit < regs ? fit : regs;
+}
 
 __device__ __forceinline__ float pa_ex2(float x) {
   float y;
@@ -94,12 +115,12 @@ __device__ __forceinline__ PaSpan pa_span(const PaArgs& p, int entry) {
 }
 
 // Epilogue of a row, by a warp: v[i] is the sum of column lane + 32 i (and v2 of branch 2), scaled to maxima m, m' and with l the sum of weights.
-template <int ES, int DT, int MODE>
+template <int ES, int DT, bool PAIRS>
 __device__ __forceinline__ void pa_finish(const PaArgs& p, int b, int head, int row, bool there, float (&v)[DT / 32], float (&v2)[DT / 32], const float (&m)[2],
                                           const float (&l)[2], const float (&mv)[2][2], int lane) {
   constexpr int N = DT / 32;
   const int D = p.c.dim, t = row / p.per, hh = row % p.per;
-  if constexpr (MODE != PA_PAIRS) {
+  if constexpr (!PAIRS) {
     const int h = head * p.per + hh;
     float top = m[0], sum = l[0];
     if (p.a.sink != nullptr && there) {
@@ -148,6 +169,12 @@ __device__ __forceinline__ void pa_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the transpose of an 8 × 8 block of 16-bit values
+__device__ __forceinline__ uint32_t pa_turn(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 template <bool TRANS>
 __device__ __forceinline__ void pa_ldsm(uint32_t (&r)[4], uint32_t addr) {
   if constexpr (TRANS)
@@ -161,21 +188,16 @@ __device__ __forceinline__ uint32_t pa_half2(uint32_t two) {
   asm("{ .reg .b16 lo; cvt.u16.u32 lo, %1; cvt.rn.f16x2.e4m3x2 %0, lo; }" : "=r"(h) : "r"(two));
   return h;
 }
-// x, y as 16-bit hi halves, and what these leave
+// x, y in 16 bits, and what that leaves
 template <int ES>
-__device__ __forceinline__ void pa_split(float x, float y, uint32_t& hi, uint32_t& lo) {
-  if constexpr (ES == 2) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    const __nv_bfloat162 r = __floats2bfloat162_rn(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
-    lo = *reinterpret_cast<const uint32_t*>(&r);
-  } else {
-    const __half2 h = __floats2half2_rn(x, y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    const float2 f = __half22float2(h);
-    const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
-    lo = *reinterpret_cast<const uint32_t*>(&r);
-  }
+__device__ __forceinline__ uint32_t pa_pack(float x, float y) {
+  if constexpr (ES == 2) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
+  else { const __half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
+}
+__device__ __forceinline__ uint32_t pa_rest(float x, float y, uint32_t hi) { return pa_pack<2>(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u)); }
+template <int BYTES>
+__device__ __forceinline__ void pa_copy(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 template <int BYTES>
 __device__ __forceinline__ void pa_copy(uint32_t dst, const void* src, bool live) {
@@ -190,11 +212,11 @@ __device__ __forceinline__ uint32_t pa_at(int t, int chunk) {
 }
 
 // GEN: rows that are not whole 16-byte pieces, or shorter than DT
-template <int ES, int DT, int MODE, bool GEN>
-__global__ void __launch_bounds__(PA_WARPS * 32) paged_attention_kernel(const PaArgs p) {
-  using S = PaShape<ES, DT, MODE>;
+template <int ES, int DT, bool PAIRS, int NC, bool GEN>
+__global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>()) paged_attention_kernel(const PaArgs p) {
+  using S = PaShape<ES, DT, PAIRS, NC>;
   constexpr bool E8 = ES == 1;
-  constexpr int TS = S::TS, NT = TS / 8, KS = DT / 16, NV = DT / 8, NR = MODE == PA_ROWS8 ? 1 : 2, HEADS = S::HEADS, NG = S::NG;
+  constexpr int TS = S::TS, MT = TS / 16, KS = DT / 16, HEADS = S::HEADS, NG = S::NG, NGX = NG > 0 ? NG : 1;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int s_prefix[PA_ENTRIES + 1];
   __shared__ int s_scan[PA_WARPS];
@@ -231,9 +253,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attention_kernel(const Pa
 
   const int64_t all = static_cast<int64_t>(s_prefix[entries]) * p.heads, share = (all + p.ncta - 1) / p.ncta;
   const int64_t end = min(all, (blockIdx.x + 1) * share);
-  uint8_t* const ring = smem + warp * PA_STAGES * S::STAGE;
+  uint8_t* const ring = smem + warp * S::STAGES * S::STAGE;
   const uint32_t ring_u = smem_u32(ring);
   constexpr float LOG2E = 1.4426950408889634f;
+  constexpr uint32_t FULL = TS == 32 ? 0xffffffffu : (1u << (TS & 31)) - 1u;
 
   for (int64_t at = blockIdx.x * share; at < end;) {
     // ---- the item
@@ -250,15 +273,21 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attention_kernel(const Pa
     // ---- loads: lane i < TS knows token i of a step
     const uint8_t* const kb = static_cast<const uint8_t*>(p.c.k) + static_cast<int64_t>(head) * HEADS * p.group_b;
     const uint8_t* const vb = static_cast<const uint8_t*>(p.c.v) + static_cast<int64_t>(head) * HEADS * p.group_b;
+    const int piece0 = lane % (S::ROW / 16);
+    const int64_t lane_b = HEADS == 2 && piece0 >= S::ROW / 32 ? p.group_b + (piece0 - S::ROW / 32) * 16 : piece0 * 16;
+    const uint8_t* const k_lane = kb + lane_b;
+    const uint8_t* const v_lane = vb + lane_b;
     int next_page = -1;
+    auto page_of = [&](int j) { return p.page_shift >= 0 ? j >> p.page_shift : j / p.c.page_size; };
     uint32_t pend_k[HEADS] = {}, pend_v[HEADS] = {};
     auto look = [&](int step) {                                                 // page of this lane's token, or -1
       const int64_t j = static_cast<int64_t>(j_base) + static_cast<int64_t>(step) * S::CHUNK + lane;
-      next_page = step < steps && lane < TS && j < sp.hi ? paged_page(p.c, b, static_cast<int>(j) / p.c.page_size) : -1;
+      next_page = -1;
+      if (step < steps && lane < TS && j < sp.hi) next_page = paged_page(p.c, b, page_of(static_cast<int>(j)));
     };
     auto issue = [&](int step) {
       if (E8 && step > 0 && lane < TS) {                                        // scales asked for one step ago
-        uint8_t* st = ring + ((step - 1) % PA_STAGES) * S::STAGE + 2 * S::TILE;
+        uint8_t* st = ring + ((step - 1) % S::STAGES) * S::STAGE + 2 * S::TILE;
 #pragma unroll
         for (int h = 0; h < HEADS; ++h) {
           reinterpret_cast<float*>(st)[h * TS + lane] = paged_pow2(pend_k[h]);
@@ -267,11 +296,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attention_kernel(const Pa
       }
       if (step < steps) {
         const int j = j_base + step * S::CHUNK + lane, page = next_page;
-        const int slot = page >= 0 ? j % p.c.page_size : 0;
-        const int64_t mine = page >= 0 ? page * p.page_b + slot * p.slot_b : -1;
+        const int slot = page >= 0 ? j - page_of(j) * p.c.page_size : 0;
         const uint32_t live = __ballot_sync(0xffffffffu, page >= 0);
-        const uint32_t st = ring_u + (step % PA_STAGES) * S::STAGE;
-        if (lane == 0) *reinterpret_cast<uint32_t*>(ring + (step % PA_STAGES) * S::STAGE + 2 * S::TILE + S::SCALES) = live;
+        const uint32_t st = ring_u + (step % S::STAGES) * S::STAGE;
+        if (lane == 0) *reinterpret_cast<uint32_t*>(ring + (step % S::STAGES) * S::STAGE + 2 * S::TILE + S::SCALES) = live;
         look(step + 1);
         if (live != 0) {
           if (E8 && page >= 0) {
@@ -282,18 +310,29 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attention_kernel(const Pa
             }
           }
           if constexpr (!GEN) {
-            constexpr int PPR = S::ROW / 16;
+            constexpr int PPR = S::ROW / 16;                                    // a lane has one piece of every (32 / PPR)-th token
+            const uint32_t mine = page >= 0 ? page * p.page_16 + slot * p.slot_16 : 0u;
+            if (live == FULL) {
 #pragma unroll
-            for (int i = 0; i < TS * PPR / 32; ++i) {
-              const int idx = i * 32 + lane, t = idx / PPR, pc = idx % PPR;
-              const int64_t o = __shfl_sync(0xffffffffu, mine, t);
-              const int64_t from = o < 0 ? 0 : o + (HEADS == 2 && pc >= PPR / 2 ? p.group_b + (pc - PPR / 2) * 16 : pc * 16);
-              const uint32_t to = st + pa_at<S::ROW>(t, pc);
-              pa_copy<16>(to, kb + from, o >= 0);
-              pa_copy<16>(to + S::TILE, vb + from, o >= 0);
+              for (int i = 0; i < TS * PPR / 32; ++i) {
+                const int64_t o = static_cast<int64_t>(__shfl_sync(0xffffffffu, mine, i * (32 / PPR) + lane / PPR)) * 16;
+                const uint32_t to = st + pa_at<S::ROW>(i * (32 / PPR) + lane / PPR, lane % PPR);
+                pa_copy<16>(to, k_lane + o);
+                pa_copy<16>(to + S::TILE, v_lane + o);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < TS * PPR / 32; ++i) {
+                const int t = i * (32 / PPR) + lane / PPR;
+                const int64_t o = static_cast<int64_t>(__shfl_sync(0xffffffffu, mine, t)) * 16;
+                const uint32_t to = st + pa_at<S::ROW>(t, lane % PPR);
+                pa_copy<16>(to, k_lane + o, live >> t & 1u);
+                pa_copy<16>(to + S::TILE, v_lane + o, live >> t & 1u);
+              }
             }
           } else {
             const int ppr = p.c.dim * ES / p.piece;
+            const int64_t mine = page >= 0 ? page * p.page_b + slot * p.slot_b : -1;
             for (int t = 0; t < TS; ++t) {
               const int64_t o = __shfl_sync(0xffffffffu, mine, t);
 #pragma unroll
@@ -314,183 +353,231 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attention_kernel(const Pa
     };
     look(0);
 #pragma unroll
-    for (int i = 0; i < PA_STAGES - 1; ++i) issue(i);
+    for (int i = 0; i < S::STAGES; ++i) issue(i);
 
-    // ---- rows of this thread: gq and, except with 8 rows, gq + 8 of the product
-    int row[NR], kmin[NR], kmax[NR];
-    float factor[NR];
-    uint32_t qa[KS][MODE == PA_ROWS16 ? 4 : 2];
+    // ---- queries: column gq of each group is loaded by this thread
+    auto column = [&](int n, int& row, int& branch) {                           // column n of 8 · NC
+      row = row0 + (PAIRS ? (n >> 3) * 4 + (n & 3) : n);
+      branch = PAIRS ? n >> 2 & 1 : 0;
+    };
+    uint32_t qb[NC][KS][2];
+    float factor[NC][2];                                                        // of the columns 2 cq, 2 cq + 1 whose scores this thread gets
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      row[i] = row0 + gq + (MODE == PA_ROWS16 ? 8 * i : 0);
-      const int t = row[i] / p.per;
-      const bool there = row[i] < p.rows && t <= sp.t1;
-      const int64_t pos = sp.pos0 + t;
-      kmax[i] = there ? static_cast<int>(max(int64_t(-1), min(pos, int64_t(0x7fffffff)))) : -1;
-      kmin[i] = p.a.window >= 0 ? static_cast<int>(max(int64_t(0), pos - p.a.window)) : 0;
-      const int h = MODE == PA_PAIRS ? 2 * (head * p.per + row[i] % p.per) + i : head * p.per + row[i] % p.per;
+    for (int c = 0; c < NC; ++c) {
+      int row, branch;
+      column(c * 8 + gq, row, branch);
+      const int t = row / p.per, h = PAIRS ? 2 * (head * p.per + row % p.per) + branch : head * p.per + row % p.per;
+      const bool there = row < p.rows && t <= sp.t1;
       const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.a.q) + b * p.a.q_batch + t * p.a.q_token + h * p.a.q_head;
-      auto two = [&](int d) -> uint32_t {                                       // values d, d + 1 (d even; so is D)
-        if (!there || d >= p.c.dim) return 0u;
+      auto two = [&](int ks, int w) -> uint32_t {                               // values d, d + 1 (d even; so is D)
+        int d = E8 ? 16 * ks + 4 * cq + 2 * w : 16 * ks + 2 * cq + 8 * w;
+        if (PAIRS) d -= branch * (DT / 2);
+        if (!there || d < 0 || d >= p.c.dim || (PAIRS && d >= DT / 2)) return 0u;
         if (p.q_words) return *reinterpret_cast<const uint32_t*>(src + d);
         return static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(src + d)) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(src + d + 1)) << 16;
       };
-      constexpr int MINE = MODE == PA_PAIRS ? KS / 2 : KS;                      // steps of the product in which the row is not zero
-      factor[i] = p.a.scale * LOG2E;
-      float up = 1.f;
+      float up = 1.f, f = p.a.scale * LOG2E;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) qb[c][ks][w] = two(ks, w);
       if constexpr (E8) {
         uint32_t top = 0;
 #pragma unroll
-        for (int ks = 0; ks < MINE; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const uint32_t u = two(16 * ks + 4 * cq + 2 * w);
-            top = max(top, max(u << 16 & 0x7fffffffu, u & 0x7fff0000u));
-          }
+          for (int w = 0; w < 2; ++w) top = max(top, max(qb[c][ks][w] << 16 & 0x7fffffffu, qb[c][ks][w] & 0x7fff0000u));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         if (top != 0 && top < 0x7f800000u) {                                    // the largest becomes 2^13 … 2^14
           const int k = min(13 - (static_cast<int>(top >> 23) - 127), 126);
           up = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
-          factor[i] *= __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+          f *= __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
         }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t u = qb[c][ks][w];
+            qb[c][ks][w] = pa_pack<1>(__uint_as_float(u << 16) * up, __uint_as_float(u & 0xffff0000u) * up);
+          }
       }
 #pragma unroll
-      for (int ks = 0; ks < MINE; ++ks)
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          uint32_t u = two(E8 ? 16 * ks + 4 * cq + 2 * w : 16 * ks + 2 * cq + 8 * w);
-          if constexpr (E8) {
-            const __half2 hv = __floats2half2_rn(__uint_as_float(u << 16) * up, __uint_as_float(u & 0xffff0000u) * up);
-            u = *reinterpret_cast<const uint32_t*>(&hv);
-          }
-          if constexpr (MODE == PA_ROWS16) qa[ks][2 * w + i] = u;
-          else if constexpr (MODE == PA_PAIRS) qa[i * (KS / 2) + ks][w] = u;
-          else qa[ks][w] = u;
-        }
+      for (int k = 0; k < 2; ++k) factor[c][k] = __shfl_sync(0xffffffffu, f, 4 * (2 * cq + k));
     }
+    int kmin[NC][2], kmax[NC][2];
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        int row, branch;
+        column(c * 8 + 2 * cq + k, row, branch);
+        const int t = row / p.per;
+        const int64_t pos = sp.pos0 + t;
+        kmax[c][k] = row < p.rows && t <= sp.t1 ? static_cast<int>(max(int64_t(-1), min(pos, int64_t(0x7fffffff)))) : -1;
+        kmin[c][k] = p.a.window >= 0 ? static_cast<int>(max(int64_t(0), pos - p.a.window)) : 0;
+      }
     // a step from all_lo to all_hi is seen by every row that is there
     const int64_t all_hi = sp.pos0 + sp.t0, all_lo = p.a.window >= 0 ? sp.pos0 + sp.t1 - p.a.window : 0;
+    const int kh = PAIRS ? cq >> 1 : 0;                                         // key head of this thread's columns
 
-    float acc[NV][4], m[NR], l[NR], mv[NR][2];
+    float acc[NC][KS][4], m[NC][2], l[NC][2], mv[NC][2][2];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int c = 0; c < NC; ++c) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[i][k] = 0.f;
+      for (int i = 0; i < KS; ++i)
 #pragma unroll
-    for (int i = 0; i < NR; ++i) { m[i] = mv[i][0] = mv[i][1] = -INFINITY; l[i] = 0.f; }
+        for (int k = 0; k < 4; ++k) acc[c][i][k] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) { m[c][k] = mv[c][k][0] = mv[c][k][1] = -INFINITY; l[c][k] = 0.f; }
+    }
 
     for (int step = 0; step < steps; ++step) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(PA_STAGES - 2) : "memory");
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 1) : "memory");
       __syncwarp();
-      const int stage = step % PA_STAGES;
+      const int stage = step % S::STAGES;
       const uint8_t* const st = ring + stage * S::STAGE;
       const uint32_t kt_u = ring_u + stage * S::STAGE, vt_u = kt_u + S::TILE;
       const uint32_t live = *reinterpret_cast<const uint32_t*>(st + 2 * S::TILE + S::SCALES);
       const int j0 = j_base + step * S::CHUNK;
       if (live != 0) {
-        // ---- scores
-        float x[NT][4];
+        // ---- scores: x[c][mt][k] of token mt · 16 + gq (k < 2) or + 8, column 2 cq + (k & 1)
+        float x[NC][MT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) x[n][k] = 0.f;
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[c][mt][k] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < (E8 ? KS / 2 : KS); ++ks)
 #pragma unroll
-          for (int np = 0; np < NT / 2; ++np) {
+          for (int mt = 0; mt < MT; ++mt) {
             uint32_t r[4];
-            pa_ldsm<false>(r, kt_u + pa_at<S::ROW>(np * 16 + ((lane >> 4) & 1) * 8 + (lane & 7), ks * 2 + ((lane >> 3) & 1)));
-            auto mul = [&](int n, int k, uint32_t b0, uint32_t b1) {
-              if constexpr (MODE == PA_ROWS16) pa_mma<ES>(x[n], qa[k][0], qa[k][1], qa[k][2], qa[k][3], b0, b1);
-              else if constexpr (MODE == PA_PAIRS) {
-                if (k < KS / 2) pa_mma<ES>(x[n], qa[k][0], 0u, qa[k][1], 0u, b0, b1);
-                else pa_mma<ES>(x[n], 0u, qa[k][0], 0u, qa[k][1], b0, b1);
-              } else pa_mma<ES>(x[n], qa[k][0], 0u, qa[k][1], 0u, b0, b1);
-            };
+            pa_ldsm<false>(r, kt_u + pa_at<S::ROW>(mt * 16 + (lane & 15), ks * 2 + (lane >> 4)));
             if constexpr (E8) {                                                 // 16 bytes are a whole step of the product; q is laid out alike
-              mul(2 * np, 2 * ks, pa_half2(r[0]), pa_half2(r[0] >> 16));
-              mul(2 * np, 2 * ks + 1, pa_half2(r[1]), pa_half2(r[1] >> 16));
-              mul(2 * np + 1, 2 * ks, pa_half2(r[2]), pa_half2(r[2] >> 16));
-              mul(2 * np + 1, 2 * ks + 1, pa_half2(r[3]), pa_half2(r[3] >> 16));
-            } else {
-              mul(2 * np, ks, r[0], r[1]);
-              mul(2 * np + 1, ks, r[2], r[3]);
-            }
-          }
-        const bool masked = live != (TS == 32 ? 0xffffffffu : (1u << (TS & 31)) - 1u) || j0 + TS - 1 > all_hi || j0 < all_lo;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t a0 = pa_half2(r[2 * h]), a1 = pa_half2(r[2 * h + 1]), a2 = pa_half2(r[2 * h] >> 16), a3 = pa_half2(r[2 * h + 1] >> 16);
 #pragma unroll
-          for (int k = 0; k < 2 * NR; ++k) {
-            const int i = k >> 1, t = n * 8 + 2 * cq + (k & 1);
-            x[n][k] *= factor[i];
-            if (E8) x[n][k] *= reinterpret_cast<const float*>(st + 2 * S::TILE)[(HEADS == 2 ? i : 0) * TS + t];
-            if (masked && !((live >> t & 1u) && j0 + t <= kmax[i] && j0 + t >= kmin[i])) x[n][k] = -INFINITY;
-          }
-        // ---- running maxima; the sums follow where one grew
-        float top[NR], tv[NR][2];
-#pragma unroll
-        for (int i = 0; i < NR; ++i) {
-          top[i] = m[i]; tv[i][0] = mv[i][0]; tv[i][1] = mv[i][1];
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              top[i] = fmaxf(top[i], x[n][2 * i + k]);
-#pragma unroll
-              for (int g = 0; g < NG; ++g)
-                tv[i][g] = fmaxf(tv[i][g], x[n][2 * i + k] + reinterpret_cast<const float*>(st + 2 * S::TILE)[(HEADS + g) * TS + n * 8 + 2 * cq + k]);
-            }
-#pragma unroll
-          for (int o = 1; o < 4; o *= 2) {
-            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
-#pragma unroll
-            for (int g = 0; g < NG; ++g) tv[i][g] = fmaxf(tv[i][g], __shfl_xor_sync(0xffffffffu, tv[i][g], o));
-          }
-        }
-        bool grew = false;
-#pragma unroll
-        for (int i = 0; i < NR; ++i) grew = grew || top[i] > m[i] || (NG > 0 && tv[i][0] > mv[i][0]) || (NG > 1 && tv[i][1] > mv[i][1]);
-        if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-          for (int i = 0; i < NR; ++i) {
-            const float f = pa_step(m[i], top[i]);
-            l[i] *= f;
-            const float f0 = E8 ? pa_step(mv[i][0], tv[i][0]) : f, f1 = NG == 2 ? pa_step(mv[i][1], tv[i][1]) : f0;
-#pragma unroll
-            for (int n = 0; n < NV; ++n) {
-              const float fn = n < NV / 2 ? f0 : f1;
-              if constexpr (MODE == PA_ROWS8) { acc[n][0] *= fn; acc[n][1] *= fn; acc[n][2] *= fn; acc[n][3] *= fn; }
-              else { acc[n][2 * i] *= fn; acc[n][2 * i + 1] *= fn; }
-            }
-            m[i] = top[i]; mv[i][0] = tv[i][0]; mv[i][1] = tv[i][1];
-          }
-        }
-        // ---- weights: 16 tokens at a time are the left operand of the second product
-        uint32_t hi[HEADS][NT][NR], lo[HEADS][NT][NR];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < NR; ++i) {
-            float w[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) { const float y = x[n][2 * i + k]; w[k] = pa_step(y, m[i]); l[i] += w[k]; }
-            if constexpr (E8) {
-#pragma unroll
-              for (int g = 0; g < NG; ++g) {
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  const float y = x[n][2 * i + k];
-                  w[k] = y == -INFINITY ? 0.f : pa_ex2(y + reinterpret_cast<const float*>(st + 2 * S::TILE)[(HEADS + g) * TS + n * 8 + 2 * cq + k] - mv[i][g] + 14.f);
-                }
-                pa_split<ES>(w[0], w[1], hi[g][n][i], lo[g][n][i]);
+                for (int c = 0; c < NC; ++c) pa_mma<ES>(x[c][mt], a0, a1, a2, a3, qb[c][2 * ks + h][0], qb[c][2 * ks + h][1]);
               }
             } else {
-              pa_split<ES>(w[0], w[1], hi[0][n][i], lo[0][n][i]);
-              if (HEADS == 2) { hi[HEADS - 1][n][i] = hi[0][n][i]; lo[HEADS - 1][n][i] = lo[0][n][i]; }
+#pragma unroll
+              for (int c = 0; c < NC; ++c) pa_mma<ES>(x[c][mt], r[0], r[1], r[2], r[3], qb[c][ks][0], qb[c][ks][1]);
             }
           }
+        const bool masked = live != FULL || j0 + TS - 1 > all_hi || j0 < all_lo;
+        const float* const scales = reinterpret_cast<const float*>(st + 2 * S::TILE);
+        float ev[NGX][MT][2];                                                   // exponents of the values' scales
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int t = mt * 16 + 8 * h + gq;
+            float f = 1.f;
+            if constexpr (E8) {
+              f = scales[kh * TS + t];
+#pragma unroll
+              for (int g = 0; g < NG; ++g) ev[g][mt][h] = scales[(HEADS + g) * TS + t];
+            }
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) x[c][mt][2 * h + k] *= E8 ? factor[c][k] * f : factor[c][k];
+          }
+        if (masked) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int t = mt * 16 + 8 * h + gq;
+              const bool is = live >> t & 1u;
+#pragma unroll
+              for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                  if (!(is && j0 + t <= kmax[c][k] && j0 + t >= kmin[c][k])) x[c][mt][2 * h + k] = -INFINITY;
+            }
+        }
+        // ---- running maxima: lanes compare their own values, and only where one is larger do they meet and the sums follow
+        bool grew = false;
+        float top[NC][2], tv[NC][2][NGX];
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            top[c][k] = m[c][k];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) tv[c][k][g] = mv[c][k][g];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                top[c][k] = fmaxf(top[c][k], x[c][mt][2 * h + k]);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) tv[c][k][g] = fmaxf(tv[c][k][g], x[c][mt][2 * h + k] + ev[g][mt][h]);
+              }
+            grew = grew || top[c][k] > m[c][k];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) grew = grew || tv[c][k][g] > mv[c][k][g];
+          }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            float f[2][2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+#pragma unroll
+              for (int o = 4; o < 32; o *= 2) {
+                top[c][k] = fmaxf(top[c][k], __shfl_xor_sync(0xffffffffu, top[c][k], o));
+#pragma unroll
+                for (int g = 0; g < NG; ++g) tv[c][k][g] = fmaxf(tv[c][k][g], __shfl_xor_sync(0xffffffffu, tv[c][k][g], o));
+              }
+              f[k][0] = f[k][1] = pa_step(m[c][k], top[c][k]);
+              l[c][k] *= f[k][0];
+              m[c][k] = top[c][k];
+#pragma unroll
+              for (int g = 0; g < NG; ++g) { f[k][g] = pa_step(mv[c][k][g], tv[c][k][g]); mv[c][k][g] = tv[c][k][g]; }
+              if (NG == 1) f[k][1] = f[k][0];
+            }
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) acc[c][i][k] *= f[k & 1][i >= KS / 2];
+          }
+        }
+        // ---- weights, turned into right operands: 16 tokens at a time
+        uint32_t hi[NC][NGX][MT][2], lo[NC][MT][2];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          float base[2], bv[2][NGX];                                            // where nothing is seen yet every x is −∞: its weight is 0
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            base[k] = m[c][k] == -INFINITY ? 0.f : m[c][k];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) bv[k][g] = mv[c][k][g] == -INFINITY ? 14.f : 14.f - mv[c][k][g];
+          }
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float y0 = x[c][mt][2 * h], y1 = x[c][mt][2 * h + 1], w0 = pa_ex2(y0 - base[0]), w1 = pa_ex2(y1 - base[1]);
+              l[c][0] += w0; l[c][1] += w1;
+              if constexpr (E8) {
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                  const float e = ev[g][mt][h];
+                  hi[c][g][mt][h] = pa_turn(pa_pack<1>(masked && y0 == -INFINITY ? 0.f : pa_ex2(y0 + e + bv[0][g]),
+                                                       masked && y1 == -INFINITY ? 0.f : pa_ex2(y1 + e + bv[1][g])));
+                }
+              } else {
+                const uint32_t u = pa_pack<2>(w0, w1);
+                hi[c][0][mt][h] = pa_turn(u);
+                lo[c][mt][h] = pa_turn(pa_rest(w0, w1, u));
+              }
+            }
+        }
         // ---- outputs.  A weight of zero times an infinity or NaN is NaN: where rows see different tokens and one of these is not finite, the tokens of
         // each new token's rows go into a product of their own, of which those rows alone are taken.
         bool odd = false;
@@ -503,64 +590,68 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attention_kernel(const Pa
           }
           odd = __any_sync(0xffffffffu, odd);
         }
-        auto out_mul = [&](float (&d)[4], int n, int kt, uint32_t b0, uint32_t b1) {
-          const int g = HEADS == 2 && n >= NV / 2 ? 1 : 0;
-          if constexpr (MODE == PA_ROWS8) {
-            pa_mma<ES>(d, hi[g][2 * kt][0], lo[g][2 * kt][0], hi[g][2 * kt + 1][0], lo[g][2 * kt + 1][0], b0, b1);
-          } else {
-            pa_mma<ES>(d, hi[g][2 * kt][0], hi[g][2 * kt][1], hi[g][2 * kt + 1][0], hi[g][2 * kt + 1][1], b0, b1);
-            pa_mma<ES>(d, lo[g][2 * kt][0], lo[g][2 * kt][1], lo[g][2 * kt + 1][0], lo[g][2 * kt + 1][1], b0, b1);
-          }
+        auto out_mul = [&](float (&d)[4], int c, int i, int mt, const uint32_t (&a)[4]) {
+          const int g = NG == 2 && i >= KS / 2 ? 1 : 0;
+          pa_mma<ES>(d, a[0], a[1], a[2], a[3], hi[c][g][mt][0], hi[c][g][mt][1]);
+          if (!E8) pa_mma<ES>(d, a[0], a[1], a[2], a[3], lo[c][mt][0], lo[c][mt][1]);
         };
-        auto values = [&](int kt, int dp, uint32_t (&r)[4]) {
-          pa_ldsm<true>(r, vt_u + pa_at<S::ROW>(kt * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), dp * 2 + (lane >> 4)));
-        };
-        // operands of the columns of `values`: NB tiles of 8 columns
-        constexpr int NB = E8 ? 4 : 2;
-        auto tiles = [&](const uint32_t (&r)[4], uint32_t (&b0)[NB], uint32_t (&b1)[NB]) {
-          if constexpr (E8) {                                                   // even columns, odd columns of 16
+        // left operands of the 16 or 32 columns of a matrix load: rows gq, gq + 8 are columns gq, gq + 8 (bf16) or 2 gq, 2 gq + 1 of 16 (e4m3)
+        constexpr int NB = E8 ? 2 : 1;
+        auto values = [&](int mt, int i, uint32_t (&a)[NB][4]) {
+          uint32_t r[4];
+          if constexpr (E8) {
+            pa_ldsm<true>(r, vt_u + pa_at<S::ROW>(mt * 16 + (lane & 15), i * 2 + (lane >> 4)));
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const uint32_t u = __byte_perm(r[2 * h], 0, 0x3120), w = __byte_perm(r[2 * h + 1], 0, 0x3120);
-              b0[2 * h] = pa_half2(u); b0[2 * h + 1] = pa_half2(u >> 16);
-              b1[2 * h] = pa_half2(w); b1[2 * h + 1] = pa_half2(w >> 16);
+              a[h][0] = pa_half2(u); a[h][1] = pa_half2(u >> 16); a[h][2] = pa_half2(w); a[h][3] = pa_half2(w >> 16);
             }
-          } else { b0[0] = r[0]; b1[0] = r[1]; b0[1] = r[2]; b1[1] = r[3]; }
+          } else {
+            pa_ldsm<true>(r, vt_u + pa_at<S::ROW>(mt * 16 + (lane & 7) + (lane >> 4) * 8, i * 2 + (lane >> 3 & 1)));
+            a[0][0] = r[0]; a[0][1] = r[1]; a[0][2] = r[2]; a[0][3] = r[3];
+          }
         };
         if (!odd) {
 #pragma unroll
-          for (int kt = 0; kt < TS / 16; ++kt)
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int dp = 0; dp < NV / NB; ++dp) {
-              uint32_t r[4], b0[NB], b1[NB];
-              values(kt, dp, r);
-              tiles(r, b0, b1);
+            for (int i = 0; i < KS / NB; ++i) {
+              uint32_t a[NB][4];
+              values(mt, i, a);
 #pragma unroll
-              for (int i = 0; i < NB; ++i) out_mul(acc[dp * NB + i], dp * NB + i, kt, b0[i], b1[i]);
+              for (int h = 0; h < NB; ++h)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) out_mul(acc[c][i * NB + h], c, i * NB + h, mt, a[h]);
             }
         } else {
           for (int t = sp.t0; t <= sp.t1; ++t) {
             const int64_t pos = sp.pos0 + t, back = p.a.window >= 0 ? pos - p.a.window : 0;
-            const bool take0 = row[0] / p.per == t, take1 = row[NR - 1] / p.per == t;
 #pragma unroll
-            for (int kt = 0; kt < TS / 16; ++kt) {
+            for (int mt = 0; mt < MT; ++mt) {
               uint32_t keep[2];
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                const int64_t j = j0 + kt * 16 + 8 * h + 2 * cq;
+                const int64_t j = j0 + mt * 16 + 8 * h + 2 * cq;
                 keep[h] = (j >= back && j <= pos ? 0xffffu : 0u) | (j + 1 >= back && j + 1 <= pos ? 0xffff0000u : 0u);
               }
 #pragma unroll
-              for (int dp = 0; dp < NV / NB; ++dp) {
-                uint32_t r[4], b0[NB], b1[NB];
-                values(kt, dp, r);
-                tiles(r, b0, b1);
+              for (int i = 0; i < KS / NB; ++i) {
+                uint32_t a[NB][4];
+                values(mt, i, a);
 #pragma unroll
-                for (int i = 0; i < NB; ++i) {
-                  float d[4] = {0.f, 0.f, 0.f, 0.f};
-                  out_mul(d, dp * NB + i, kt, b0[i] & keep[0], b1[i] & keep[1]);
-                  if (take0) { acc[dp * NB + i][0] += d[0]; acc[dp * NB + i][1] += d[1]; }
-                  if (take1) { acc[dp * NB + i][2] += d[2]; acc[dp * NB + i][3] += d[3]; }
+                for (int h = 0; h < NB; ++h) {
+                  a[h][0] &= keep[0]; a[h][1] &= keep[0]; a[h][2] &= keep[1]; a[h][3] &= keep[1];
+#pragma unroll
+                  for (int c = 0; c < NC; ++c) {
+                    float d[4] = {0.f, 0.f, 0.f, 0.f};
+                    out_mul(d, c, i * NB + h, mt, a[h]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                      int row, branch;
+                      column(c * 8 + 2 * cq + (k & 1), row, branch);
+                      if (row / p.per == t) acc[c][i * NB + h][k] += d[k];
+                    }
+                  }
                 }
               }
             }
@@ -568,47 +659,40 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attention_kernel(const Pa
         }
       }
       __syncwarp();
-      issue(step + PA_STAGES - 1);
+      issue(step + S::STAGES);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 
     // ---- the warps' parts, through the memory of the ring
 #pragma unroll
-    for (int i = 0; i < NR; ++i)
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int o = 1; o < 4; o *= 2) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int o = 4; o < 32; o *= 2) l[c][k] += __shfl_xor_sync(0xffffffffu, l[c][k], o);
     __syncthreads();
-    float* const slab = reinterpret_cast<float*>(smem) + warp * S::OROWS * S::LD;
-    if (cq == 0)
+    float* const slab = reinterpret_cast<float*>(smem) + warp * S::COLS * S::LD;
 #pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        s_stat[warp][0][gq + 8 * i] = m[i]; s_stat[warp][1][gq + 8 * i] = l[i];
-        s_stat[warp][2][gq + 8 * i] = mv[i][0]; s_stat[warp][3][gq + 8 * i] = mv[i][1];
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int n = c * 8 + 2 * cq + k;
+        if (gq == 0) { s_stat[warp][0][n] = m[c][k]; s_stat[warp][1][n] = l[c][k]; s_stat[warp][2][n] = mv[c][k][0]; s_stat[warp][3][n] = mv[c][k][1]; }
+        float* const to = slab + n * S::LD;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          if constexpr (E8) *reinterpret_cast<float2*>(to + i * 16 + 2 * gq) = make_float2(acc[c][i][k], acc[c][i][k + 2]);
+          else { to[i * 16 + gq] = acc[c][i][k]; to[i * 16 + gq + 8] = acc[c][i][k + 2]; }
+        }
       }
-    if constexpr (MODE == PA_ROWS8) {
-#pragma unroll
-      for (int n = 0; n < NV; ++n) { acc[n][0] += acc[n][2]; acc[n][1] += acc[n][3]; }
-    }
-#pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      float* const to = slab + (gq + 8 * i) * S::LD;
-      if constexpr (E8) {
-#pragma unroll
-        for (int n = 0; n < NV; n += 2)
-          *reinterpret_cast<float4*>(to + n * 8 + 4 * cq) = make_float4(acc[n][2 * i], acc[n + 1][2 * i], acc[n][2 * i + 1], acc[n + 1][2 * i + 1]);
-      } else {
-#pragma unroll
-        for (int n = 0; n < NV; ++n) *reinterpret_cast<float2*>(to + n * 8 + 2 * cq) = make_float2(acc[n][2 * i], acc[n][2 * i + 1]);
-      }
-    }
     __syncthreads();
     const bool whole = c0 == 0 && c1 == chunks;
     float* const part = whole ? nullptr : p.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (c0 == 0)) * S::PART;
     for (int r = warp; r < S::QROWS; r += PA_WARPS) {
       float v[2][DT / 32], mm[2], ll[2], mmv[2][2];
 #pragma unroll
-      for (int br = 0; br < (MODE == PA_PAIRS ? 2 : 1); ++br) {
-        const int k = r + 8 * br;
+      for (int br = 0; br < HEADS; ++br) {
+        const int k = pa_column<PAIRS>(r, br);
         mm[br] = mmv[br][0] = mmv[br][1] = -INFINITY; ll[br] = 0.f;
 #pragma unroll
         for (int w = 0; w < PA_WARPS; ++w) {
@@ -625,16 +709,16 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attention_kernel(const Pa
           const float f0 = E8 ? pa_step(s_stat[w][2][k], mmv[br][0]) : f, f1 = NG == 2 ? pa_step(s_stat[w][3][k], mmv[br][1]) : f0;
 #pragma unroll
           for (int i = 0; i < DT / 32; ++i)
-            v[br][i] += reinterpret_cast<const float*>(smem)[(w * S::OROWS + k) * S::LD + lane + 32 * i] * (i < DT / 64 ? f0 : f1);
+            v[br][i] += reinterpret_cast<const float*>(smem)[(w * S::COLS + k) * S::LD + lane + 32 * i] * (i < DT / 64 ? f0 : f1);
         }
         if (!whole) {
 #pragma unroll
           for (int i = 0; i < DT / 32; ++i) part[k * DT + lane + 32 * i] = v[br][i];
-          if (lane < 4) part[S::OROWS * DT + k * 4 + lane] = lane == 0 ? mm[br] : lane == 1 ? ll[br] : lane == 2 ? mmv[br][0] : mmv[br][1];
+          if (lane < 4) part[S::COLS * DT + k * 4 + lane] = lane == 0 ? mm[br] : lane == 1 ? ll[br] : lane == 2 ? mmv[br][0] : mmv[br][1];
         }
       }
       if (whole && row0 + r < p.rows)
-        pa_finish<ES, DT, MODE>(p, b, head, row0 + r, (row0 + r) / p.per <= sp.t1, v[0], v[1], mm, ll, mmv, lane);
+        pa_finish<ES, DT, PAIRS>(p, b, head, row0 + r, (row0 + r) / p.per <= sp.t1, v[0], v[1], mm, ll, mmv, lane);
     }
     __syncthreads();                                                            // the ring is used again
     if (GEN)                                                                    // and its unused columns are zero again
@@ -645,10 +729,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_attention_kernel(const Pa
 }
 
 // The parts of items that lie in several CTAs: one CTA per item and row.
-template <int ES, int DT, int MODE>
+template <int ES, int DT, bool PAIRS, int NC>
 __global__ void __launch_bounds__(PA_WARPS * 32) paged_join_kernel(const PaArgs p) {
-  using S = PaShape<ES, DT, MODE>;
-  constexpr int N = DT / 32, BR = MODE == PA_PAIRS ? 2 : 1;
+  using S = PaShape<ES, DT, PAIRS, NC>;
+  constexpr int N = DT / 32, BR = PAIRS ? 2 : 1;
   constexpr bool E8 = ES == 1;
   __shared__ float s_sum[PA_WARPS][BR][DT];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -667,10 +751,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_join_kernel(const PaArgs 
   float m[2], l[2], mv[2][2], v[2][N];
 #pragma unroll
   for (int br = 0; br < BR; ++br) {
-    const int k = r + 8 * br;
+    const int k = pa_column<PAIRS>(r, br);
     m[br] = mv[br][0] = mv[br][1] = -INFINITY; l[br] = 0.f;
     for (int i = lane; i < n; i += 32) {
-      const float4 s = *reinterpret_cast<const float4*>(part(i) + S::OROWS * DT + k * 4);
+      const float4 s = *reinterpret_cast<const float4*>(part(i) + S::COLS * DT + k * 4);
       m[br] = fmaxf(m[br], s.x); mv[br][0] = fmaxf(mv[br][0], s.z); mv[br][1] = fmaxf(mv[br][1], s.w);
     }
 #pragma unroll
@@ -680,7 +764,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_join_kernel(const PaArgs 
       mv[br][1] = fmaxf(mv[br][1], __shfl_xor_sync(0xffffffffu, mv[br][1], o));
     }
     for (int i = lane; i < n; i += 32) {
-      const float4 s = *reinterpret_cast<const float4*>(part(i) + S::OROWS * DT + k * 4);
+      const float4 s = *reinterpret_cast<const float4*>(part(i) + S::COLS * DT + k * 4);
       l[br] += s.y * pa_step(s.x, m[br]);
     }
 #pragma unroll
@@ -691,7 +775,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_join_kernel(const PaArgs 
 #pragma unroll 4
     for (int i = warp; i < n; i += PA_WARPS) {
       const float* src = part(i);
-      const float4 s = *reinterpret_cast<const float4*>(src + S::OROWS * DT + k * 4);
+      const float4 s = *reinterpret_cast<const float4*>(src + S::COLS * DT + k * 4);
       const float f = pa_step(s.x, m[br]), f0 = E8 ? pa_step(s.z, mv[br][0]) : f, f1 = S::NG == 2 ? pa_step(s.w, mv[br][1]) : f0;
 #pragma unroll
       for (int j = 0; j < N; ++j) sum[j] += src[k * DT + lane + 32 * j] * (j < N / 2 ? f0 : f1);
@@ -710,20 +794,13 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_join_kernel(const PaArgs 
       for (int w = 0; w < PA_WARPS; ++w) v[br][j] += s_sum[w][br][lane + 32 * j];
     }
   const PaSpan sp = pa_span<S::QROWS>(p, e);
-  pa_finish<ES, DT, MODE>(p, b, head, row0 + r, (row0 + r) / p.per <= sp.t1, v[0], v[1], m, l, mv, lane);
+  pa_finish<ES, DT, PAIRS>(p, b, head, row0 + r, (row0 + r) / p.per <= sp.t1, v[0], v[1], m, l, mv, lane);
 }
 
-// CTAs that fit an SM beside one another, by shared memory
-template <int ES, int DT, int MODE>
-constexpr int pa_resident() {
-  constexpr int one = PaShape<ES, DT, MODE>::SMEM + (PA_ENTRIES + 1) * 4 + 2048;      // its static part and what the system keeps
-  return 228 * 1024 / one < 4 ? 228 * 1024 / one : 4;
-}
-
-template <int ES, int DT, int MODE, bool GEN>
+template <int ES, int DT, bool PAIRS, int NC, bool GEN>
 static int pa_launch(PaArgs& p, int max_chunks, int num_sms, cudaStream_t st) {
-  using S = PaShape<ES, DT, MODE>;
-  auto kernel = paged_attention_kernel<ES, DT, MODE, GEN>;
+  using S = PaShape<ES, DT, PAIRS, NC>;
+  auto kernel = paged_attention_kernel<ES, DT, PAIRS, NC, GEN>;
   if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); e != cudaSuccess) return static_cast<int>(e);
   kernel<<<p.ncta, PA_WARPS * 32, S::SMEM, st>>>(p);
   if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return static_cast<int>(e);
@@ -737,39 +814,37 @@ static int pa_launch(PaArgs& p, int max_chunks, int num_sms, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, paged_join_kernel<ES, DT, MODE>, p));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, paged_join_kernel<ES, DT, PAIRS, NC>, p));
 }
 
 // A launch of the sequences and tiles that p names; with `need` only the bytes of its workspace and its CTAs are worked out.
-int pa_run_bf16(PaArgs& p, int dt, int mode, bool gen, int span, int num_sms, void* ws, int64_t* need, cudaStream_t st);
-int pa_run_e4m3(PaArgs& p, int dt, int mode, bool gen, int span, int num_sms, void* ws, int64_t* need, cudaStream_t st);
+int pa_run_bf16(PaArgs& p, int dt, bool pairs, int nc, bool gen, int span, int num_sms, void* ws, int64_t* need, cudaStream_t st);
+int pa_run_e4m3(PaArgs& p, int dt, bool pairs, int nc, bool gen, int span, int num_sms, void* ws, int64_t* need, cudaStream_t st);
 
-template <int ES, int DT, int MODE>
+template <int ES, int DT, bool PAIRS, int NC>
 static int pa_prepare(PaArgs& p, bool gen, int span, int num_sms, void* ws, int64_t* need, cudaStream_t st) {
-  using S = PaShape<ES, DT, MODE>;
+  using S = PaShape<ES, DT, PAIRS, NC>;
   const int max_chunks = span <= S::CHUNK ? 1 : (span + S::CHUNK - 1) / S::CHUNK;
-  const int64_t work = static_cast<int64_t>(p.nb) * p.nrt * p.heads * max_chunks, full = static_cast<int64_t>(num_sms) * pa_resident<ES, DT, MODE>();
+  const int64_t work = static_cast<int64_t>(p.nb) * p.nrt * p.heads * max_chunks, full = static_cast<int64_t>(num_sms) * pa_resident<ES, DT, PAIRS, NC>();
   p.ncta = static_cast<int>(work < full ? work : full);
   const int64_t bytes = max_chunks > 1 ? static_cast<int64_t>(p.ncta) * 2 * S::PART * 4 + (PA_ENTRIES + 4) * 4 : 0;
   if (need != nullptr) { *need = bytes; return 0; }
   p.parts = static_cast<float*>(ws);
   p.prefix = max_chunks > 1 ? reinterpret_cast<int*>(p.parts + static_cast<int64_t>(p.ncta) * 2 * S::PART) : nullptr;
-  return gen ? pa_launch<ES, DT, MODE, true>(p, max_chunks, num_sms, st) : pa_launch<ES, DT, MODE, false>(p, max_chunks, num_sms, st);
+  return gen ? pa_launch<ES, DT, PAIRS, NC, true>(p, max_chunks, num_sms, st) : pa_launch<ES, DT, PAIRS, NC, false>(p, max_chunks, num_sms, st);
 }
 template <int ES>
-static int pa_run(PaArgs& p, int dt, int mode, bool gen, int span, int num_sms, void* ws, int64_t* need, cudaStream_t st) {
-  if (mode == PA_PAIRS) {
-    if (dt == 128) return pa_prepare<ES, 128, PA_PAIRS>(p, gen, span, num_sms, ws, need, st);
-    return pa_prepare<ES, 256, PA_PAIRS>(p, gen, span, num_sms, ws, need, st);
-  }
-  if (mode == PA_ROWS8) {
-    if (dt == 64) return pa_prepare<ES, 64, PA_ROWS8>(p, gen, span, num_sms, ws, need, st);
-    if (dt == 128) return pa_prepare<ES, 128, PA_ROWS8>(p, gen, span, num_sms, ws, need, st);
-    return pa_prepare<ES, 256, PA_ROWS8>(p, gen, span, num_sms, ws, need, st);
-  }
-  if (dt == 64) return pa_prepare<ES, 64, PA_ROWS16>(p, gen, span, num_sms, ws, need, st);
-  if (dt == 128) return pa_prepare<ES, 128, PA_ROWS16>(p, gen, span, num_sms, ws, need, st);
-  return pa_prepare<ES, 256, PA_ROWS16>(p, gen, span, num_sms, ws, need, st);
+static int pa_run(PaArgs& p, int dt, bool pairs, int nc, bool gen, int span, int num_sms, void* ws, int64_t* need, cudaStream_t st) {
+  auto go = [&](auto dtc, auto pairsc) {
+    constexpr int DT = decltype(dtc)::value;
+    constexpr bool PAIRS = decltype(pairsc)::value;
+    return nc == 1 ? pa_prepare<ES, DT, PAIRS, 1>(p, gen, span, num_sms, ws, need, st) : pa_prepare<ES, DT, PAIRS, 2>(p, gen, span, num_sms, ws, need, st);
+  };
+  using D64 = std::integral_constant<int, 64>;
+  using D128 = std::integral_constant<int, 128>;
+  using D256 = std::integral_constant<int, 256>;
+  if (pairs) return dt == 128 ? go(D128{}, std::true_type{}) : go(D256{}, std::true_type{});
+  return dt == 64 ? go(D64{}, std::false_type{}) : dt == 128 ? go(D128{}, std::false_type{}) : go(D256{}, std::false_type{});
 }
 
 }  // namespace b200

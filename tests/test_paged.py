@@ -213,14 +213,15 @@ def attn_inputs(case, cache_type, q_type, device, order="groups", seed=0):
     return q, cache, table.to(device), ints(lengths), ints(new), window, s
 
 
-def attn_bound(q, cache, spread, L, split):
+def attn_bound(q, cache, spread, L):
     """What an output may be off before its rounding, relative to the largest value.  A score of D products and a scale is rounded D + 2 times
     (2⁻²⁴ each, of at most Σ|q k|), and once more where log₂ e is folded in (of |s| ≤ Σ|q k|); its exponential is off by that and by 2⁻²¹ (exp2 in
     hardware: 2⁻²²; the rescaling by the maximum once more).  Numerator and denominator both count.  Sums of L terms are rounded L times.
-    Weights enter the product in two 16-bit halves: 2⁻¹⁶ (bf16) at most, ``split``."""
+    Weights enter the product rounded: over e4m3 to fp16, by half a step of 2⁻¹¹ at most; else as two halves in bf16, where the second, at most 2⁻⁸ of a
+    weight, is off by 2⁻⁸ of itself.  Σ p |v| / Σ p is at most the largest value."""
     D = q.shape[-1]
     score = (D + 4) * 2.0 ** -24 * spread
-    return 2 * (score + 2.0 ** -20) + 2 * L * 2.0 ** -24 + (2.0 ** -16 if split else 0)
+    return 2 * (score + 2.0 ** -20) + 2 * L * 2.0 ** -24 + (2.0 ** -11 if cache.k.dtype == FP8 else 2.0 ** -16)
 
 
 def visible_top(cache, table, lengths):
@@ -239,7 +240,7 @@ def check_attn(q, cache, table, lengths, new, window, sink, scale=None):
     assert torch.equal(out, alone)
     want, want_lse, spread = oracle.attention(q, cache, table.cpu(), lengths, new, scale, window, sink)
     L = max([0, *lengths.tolist()])
-    rel = attn_bound(q, cache, spread, L, True)
+    rel = attn_bound(q, cache, spread, L)
     tol = half_step(q.dtype) * want.abs() + rel * visible_top(cache, table, lengths) * (1 + half_step(q.dtype))
     err = (out.double().cpu() - want).abs()
     assert bool((err <= tol).all()), float((err - tol).max())
@@ -382,7 +383,7 @@ def check_diff(q, cache, table, lengths, new, window, lam, w, scale=None, c=0.4,
     want, spread, low = oracle.diff_attention(q, cache, table.cpu(), lengths, lam, w, c, eps, new, scale, window)
     L = max([0, *lengths.tolist()])
     # a1 − λ a2 is off by a; its root mean square by no more, so that y is off by (a / rms) (1 + |y| / (w c)), and |y| ≤ w c √(2 D)
-    a = attn_bound(q, cache, spread, L, True) * (1 + abs(float(lam))) * visible_top(cache, table, lengths)
+    a = attn_bound(q, cache, spread, L) * (1 + abs(float(lam))) * visible_top(cache, table, lengths)
     gain = float(w.float().abs().max()) * c
     size = want.abs()
     tol = half_step(q.dtype) * size + (a / low if math.isfinite(low) else 0) * (gain + size) * 1.1 + 2.0 ** -20 * size
