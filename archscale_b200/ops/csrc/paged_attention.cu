@@ -34,8 +34,9 @@ static PaPlan pa_plan(const PagedView& c, const b200_paged_query& a) {
   s.tiles = (p.rows + qrows - 1) / qrows;
   s.nrt = s.tiles < PA_ENTRIES ? s.tiles : PA_ENTRIES;
   s.nb = PA_ENTRIES / s.nrt;
-  const int64_t fit = 0x40000000LL / (static_cast<int64_t>(s.nrt) * (s.span / 64 + 1));       // chunks are counted in 32 bits
-  if (s.nb > fit) s.nb = fit < 1 ? 1 : static_cast<int>(fit);
+  const int64_t fit = 0x40000000LL / (static_cast<int64_t>(s.nrt) * p.heads * (s.span / 64 + 1));       // chunks are counted in 32 bits
+  if (fit < 1) { s.ok = false; return s; }
+  if (s.nb > fit) s.nb = static_cast<int>(fit);
   if (s.nb > a.B) s.nb = a.B;
   return s;
 }

@@ -53,6 +53,9 @@ struct PaArgs {
 #ifndef PA_ST
 #define PA_ST 2
 #endif
+#ifndef PA_F
+#define PA_F 1
+#endif
 #ifndef PA_TS8
 #define PA_TS8 32
 #endif
@@ -251,24 +254,51 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
   if (blockIdx.x == 0 && p.prefix != nullptr)
     for (int i = threadIdx.x; i <= entries; i += PA_WARPS * 32) p.prefix[i] = s_prefix[i];
 
-  const int64_t all = static_cast<int64_t>(s_prefix[entries]) * p.heads, share = (all + p.ncta - 1) / p.ncta;
-  const int64_t end = min(all, (blockIdx.x + 1) * share);
+  const uint32_t all = static_cast<uint32_t>(s_prefix[entries]) * p.heads, share = (all + p.ncta - 1) / p.ncta;
+  const uint32_t end = min(all, (blockIdx.x + 1) * share);
   uint8_t* const ring = smem + warp * S::STAGES * S::STAGE;
   const uint32_t ring_u = smem_u32(ring);
   constexpr float LOG2E = 1.4426950408889634f;
   constexpr uint32_t FULL = TS == 32 ? 0xffffffffu : (1u << (TS & 31)) - 1u;
 
-  for (int64_t at = blockIdx.x * share; at < end;) {
+#pragma unroll 1
+  for (uint32_t at = blockIdx.x * share; at < end;) {
     // ---- the item
     int e = 0;
-    for (int hi = entries; hi - e > 1;) { const int mid = (e + hi) >> 1; if (static_cast<int64_t>(s_prefix[mid]) * p.heads <= at) e = mid; else hi = mid; }
-    const int chunks = s_prefix[e + 1] - s_prefix[e];
-    const int64_t off = at - static_cast<int64_t>(s_prefix[e]) * p.heads;
-    const int head = static_cast<int>(off / chunks), c0 = static_cast<int>(off % chunks), c1 = static_cast<int>(min(static_cast<int64_t>(chunks), c0 + end - at));
+    for (int hi = entries; hi - e > 1;) { const int mid = (e + hi) >> 1; if (static_cast<uint32_t>(s_prefix[mid]) * p.heads <= at) e = mid; else hi = mid; }
+    const uint32_t chunks = s_prefix[e + 1] - s_prefix[e], off = at - static_cast<uint32_t>(s_prefix[e]) * p.heads;
+    const uint32_t head = off / chunks, c0 = off - head * chunks, c1 = min(chunks, c0 + end - at);
     const int b = p.b0 + e / p.nrt, row0 = (p.rt0 + e % p.nrt) * S::QROWS;
     const PaSpan sp = pa_span<S::QROWS>(p, e);
     const int j_base = sp.lo + c0 * S::CHUNK + warp * TS;                       // first token of this warp's step 0
-    const int steps = c1 - c0;
+    const int steps = static_cast<int>(c1 - c0);
+
+    // ---- queries: column gq of each group is loaded by this thread
+    auto column = [&](int n, int& row, int& branch) {                           // column n of 8 · NC
+      row = row0 + (PAIRS ? (n >> 3) * 4 + (n & 3) : n);
+      branch = PAIRS ? n >> 2 & 1 : 0;
+    };
+    uint32_t qb[NC][KS][2];
+    float factor[NC][2];                                                        // of the columns 2 cq, 2 cq + 1 whose scores this thread gets
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      int row, branch;
+      column(c * 8 + gq, row, branch);
+      const int t = row / p.per, h = PAIRS ? 2 * (head * p.per + row % p.per) + branch : head * p.per + row % p.per;
+      const bool there = row < p.rows && t <= sp.t1;
+      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.a.q) + b * p.a.q_batch + t * p.a.q_token + h * p.a.q_head;
+      auto two = [&](int ks, int w) -> uint32_t {                               // values d, d + 1 (d even; so is D)
+        int d = E8 ? 16 * ks + 4 * cq + 2 * w : 16 * ks + 2 * cq + 8 * w;
+        if (PAIRS) d -= branch * (DT / 2);
+        if (!there || d < 0 || d >= p.c.dim || (PAIRS && d >= DT / 2)) return 0u;
+        if (p.q_words) return *reinterpret_cast<const uint32_t*>(src + d);
+        return static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(src + d)) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(src + d + 1)) << 16;
+      };
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) qb[c][ks][w] = two(ks, w);
+    }
 
     // ---- loads: lane i < TS knows token i of a step
     const uint8_t* const kb = static_cast<const uint8_t*>(p.c.k) + static_cast<int64_t>(head) * HEADS * p.group_b;
@@ -277,38 +307,34 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
     const int64_t lane_b = HEADS == 2 && piece0 >= S::ROW / 32 ? p.group_b + (piece0 - S::ROW / 32) * 16 : piece0 * 16;
     const uint8_t* const k_lane = kb + lane_b;
     const uint8_t* const v_lane = vb + lane_b;
-    int next_page = -1;
+    const int* const table = p.c.table + b * p.c.table_row;
+    const uint8_t* const ks = E8 ? p.c.ks + static_cast<int>(head) * HEADS * p.c.ks_group : nullptr;
+    const uint8_t* const vs = E8 ? p.c.vs + static_cast<int>(head) * HEADS * p.c.vs_group : nullptr;
     auto page_of = [&](int j) { return p.page_shift >= 0 ? j >> p.page_shift : j / p.c.page_size; };
-    uint32_t pend_k[HEADS] = {}, pend_v[HEADS] = {};
     auto look = [&](int step) {                                                 // page of this lane's token, or -1
       const int64_t j = static_cast<int64_t>(j_base) + static_cast<int64_t>(step) * S::CHUNK + lane;
-      next_page = -1;
-      if (step < steps && lane < TS && j < sp.hi) next_page = paged_page(p.c, b, page_of(static_cast<int>(j)));
+      if (step >= steps || lane >= TS || j >= sp.hi) return -1;
+      return table[page_of(static_cast<int>(j))];                               // hi is within the table
     };
+    int page_a = look(0), page_b = look(1);
+    uint32_t pend_k[HEADS] = {}, pend_v[HEADS] = {};
     auto issue = [&](int step) {
-      if (E8 && step > 0 && lane < TS) {                                        // scales asked for one step ago
-        uint8_t* st = ring + ((step - 1) % S::STAGES) * S::STAGE + 2 * S::TILE;
-#pragma unroll
-        for (int h = 0; h < HEADS; ++h) {
-          reinterpret_cast<float*>(st)[h * TS + lane] = paged_pow2(pend_k[h]);
-          reinterpret_cast<float*>(st)[(HEADS + h) * TS + lane] = pend_v[h] == 255u ? __int_as_float(0x7fffffff) : static_cast<float>(static_cast<int>(pend_v[h]) - 127);
-        }
-      }
+      int64_t scale_at = -1, scale_at_v = 0;
       if (step < steps) {
-        const int j = j_base + step * S::CHUNK + lane, page = next_page;
+        const int j = j_base + step * S::CHUNK + lane;
+        int page = page_a;
+        if (lane < TS && j < sp.hi && (page < 0 || page >= p.c.pages)) {        // not of this cache
+          if (p.c.status) atomicCAS(p.c.status, 0, STATUS_INDEX_RANGE);
+          page = -1;
+        }
+        page_a = page_b;
+        page_b = look(step + 2);
         const int slot = page >= 0 ? j - page_of(j) * p.c.page_size : 0;
+        if (E8 && page >= 0) { scale_at = page * p.c.ks_page + slot * p.c.ks_slot; scale_at_v = page * p.c.vs_page + slot * p.c.vs_slot; }
         const uint32_t live = __ballot_sync(0xffffffffu, page >= 0);
         const uint32_t st = ring_u + (step % S::STAGES) * S::STAGE;
         if (lane == 0) *reinterpret_cast<uint32_t*>(ring + (step % S::STAGES) * S::STAGE + 2 * S::TILE + S::SCALES) = live;
-        look(step + 1);
         if (live != 0) {
-          if (E8 && page >= 0) {
-#pragma unroll
-            for (int h = 0; h < HEADS; ++h) {
-              pend_k[h] = p.c.ks[page * p.c.ks_page + (head * HEADS + h) * p.c.ks_group + slot * p.c.ks_slot];
-              pend_v[h] = p.c.vs[page * p.c.vs_page + (head * HEADS + h) * p.c.vs_group + slot * p.c.vs_slot];
-            }
-          }
           if constexpr (!GEN) {
             constexpr int PPR = S::ROW / 16;                                    // a lane has one piece of every (32 / PPR)-th token
             const uint32_t mine = page >= 0 ? page * p.page_16 + slot * p.slot_16 : 0u;
@@ -350,56 +376,47 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    look(0);
+      if constexpr (E8) {
+        if (step > 0 && lane < TS) {                                            // scales asked for one step ago
+          float* const to = reinterpret_cast<float*>(ring + ((step - 1) % S::STAGES) * S::STAGE + 2 * S::TILE);
 #pragma unroll
-    for (int i = 0; i < S::STAGES; ++i) issue(i);
-
-    // ---- queries: column gq of each group is loaded by this thread
-    auto column = [&](int n, int& row, int& branch) {                           // column n of 8 · NC
-      row = row0 + (PAIRS ? (n >> 3) * 4 + (n & 3) : n);
-      branch = PAIRS ? n >> 2 & 1 : 0;
+          for (int h = 0; h < HEADS; ++h) {
+            to[h * TS + lane] = paged_pow2(pend_k[h]);
+            to[(HEADS + h) * TS + lane] = pend_v[h] == 255u ? __int_as_float(0x7fffffff) : static_cast<float>(static_cast<int>(pend_v[h]) - 127);
+          }
+        }
+        if (scale_at >= 0) {
+#pragma unroll
+          for (int h = 0; h < HEADS; ++h) {
+            pend_k[h] = ks[scale_at + h * p.c.ks_group];
+            pend_v[h] = vs[scale_at_v + h * p.c.vs_group];
+          }
+        }
+      }
     };
-    uint32_t qb[NC][KS][2];
-    float factor[NC][2];                                                        // of the columns 2 cq, 2 cq + 1 whose scores this thread gets
+
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      int row, branch;
-      column(c * 8 + gq, row, branch);
-      const int t = row / p.per, h = PAIRS ? 2 * (head * p.per + row % p.per) + branch : head * p.per + row % p.per;
-      const bool there = row < p.rows && t <= sp.t1;
-      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.a.q) + b * p.a.q_batch + t * p.a.q_token + h * p.a.q_head;
-      auto two = [&](int ks, int w) -> uint32_t {                               // values d, d + 1 (d even; so is D)
-        int d = E8 ? 16 * ks + 4 * cq + 2 * w : 16 * ks + 2 * cq + 8 * w;
-        if (PAIRS) d -= branch * (DT / 2);
-        if (!there || d < 0 || d >= p.c.dim || (PAIRS && d >= DT / 2)) return 0u;
-        if (p.q_words) return *reinterpret_cast<const uint32_t*>(src + d);
-        return static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(src + d)) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(src + d + 1)) << 16;
-      };
       float up = 1.f, f = p.a.scale * LOG2E;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int w = 0; w < 2; ++w) qb[c][ks][w] = two(ks, w);
       if constexpr (E8) {
         uint32_t top = 0;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
-          for (int w = 0; w < 2; ++w) top = max(top, max(qb[c][ks][w] << 16 & 0x7fffffffu, qb[c][ks][w] & 0x7fff0000u));
+          for (int w = 0; w < 2; ++w) top = max(top, max(qb[c][k][w] << 16 & 0x7fffffffu, qb[c][k][w] & 0x7fff0000u));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         if (top != 0 && top < 0x7f800000u) {                                    // the largest becomes 2^13 … 2^14
-          const int k = min(13 - (static_cast<int>(top >> 23) - 127), 126);
-          up = __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
-          f *= __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+          const int by = min(13 - (static_cast<int>(top >> 23) - 127), 126);
+          up = __uint_as_float(static_cast<uint32_t>(127 + by) << 23);
+          f *= __uint_as_float(static_cast<uint32_t>(127 - by) << 23);
         }
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            const uint32_t u = qb[c][ks][w];
-            qb[c][ks][w] = pa_pack<1>(__uint_as_float(u << 16) * up, __uint_as_float(u & 0xffff0000u) * up);
+            const uint32_t u = qb[c][k][w];
+            qb[c][k][w] = pa_pack<1>(__uint_as_float(u << 16) * up, __uint_as_float(u & 0xffff0000u) * up);
           }
       }
 #pragma unroll
@@ -432,7 +449,9 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
       for (int k = 0; k < 2; ++k) { m[c][k] = mv[c][k][0] = mv[c][k][1] = -INFINITY; l[c][k] = 0.f; }
     }
 
-    for (int step = 0; step < steps; ++step) {
+#pragma unroll 1
+    for (int step = -S::STAGES; step < steps; ++step) {                         // loads run STAGES steps ahead; one loop, so that they are in the code once
+      if (step >= 0) {
       asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 1) : "memory");
       __syncwarp();
       const int stage = step % S::STAGES;
@@ -548,7 +567,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
           }
         }
         // ---- weights, turned into right operands: 16 tokens at a time
-        uint32_t hi[NC][NGX][MT][2], lo[NC][MT][2];
+        uint32_t hi[NC][NGX][MT][2], lo[E8 ? 1 : NC][E8 ? 1 : MT][2];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           float base[2], bv[2][NGX];                                            // where nothing is seen yet every x is −∞: its weight is 0
@@ -593,7 +612,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
         auto out_mul = [&](float (&d)[4], int c, int i, int mt, const uint32_t (&a)[4]) {
           const int g = NG == 2 && i >= KS / 2 ? 1 : 0;
           pa_mma<ES>(d, a[0], a[1], a[2], a[3], hi[c][g][mt][0], hi[c][g][mt][1]);
-          if (!E8) pa_mma<ES>(d, a[0], a[1], a[2], a[3], lo[c][mt][0], lo[c][mt][1]);
+          if constexpr (!E8) pa_mma<ES>(d, a[0], a[1], a[2], a[3], lo[c][mt][0], lo[c][mt][1]);
         };
         // left operands of the 16 or 32 columns of a matrix load: rows gq, gq + 8 are columns gq, gq + 8 (bf16) or 2 gq, 2 gq + 1 of 16 (e4m3)
         constexpr int NB = E8 ? 2 : 1;
@@ -659,6 +678,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
         }
       }
       __syncwarp();
+      }
       issue(step + S::STAGES);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -728,72 +748,96 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
   }
 }
 
-// The parts of items that lie in several CTAs: one CTA per item and row.
-template <int ES, int DT, bool PAIRS, int NC>
-__global__ void __launch_bounds__(PA_WARPS * 32) paged_join_kernel(const PaArgs p) {
+// The parts of items that lie in several CTAs.  WPR warps share a row, each takes every WPR-th part with all of its loads in flight; a CTA has the rows of
+// 16 / WPR (at most 8) neighbours of (item, row).  Few items have many parts each and want warps, many items have few parts and want to be over in
+// one wave: 16, 4 or 1, whichever fits the device at once (256 items of 2 to 3 parts: 6 us with 1, 20 with 16; 4 items of 103 parts: 15 with 4, 8 with 16).
+template <int ES, int DT, bool PAIRS, int NC, int WPR>
+__global__ void __launch_bounds__(512 / (WPR == 1 ? 2 : 1)) paged_join_kernel(const PaArgs p) {
   using S = PaShape<ES, DT, PAIRS, NC>;
-  constexpr int N = DT / 32, BR = PAIRS ? 2 : 1;
+  constexpr int RPB = WPR == 1 ? 8 : 16 / WPR;
+  constexpr int N = DT / 32, BR = PAIRS ? 2 : 1, AHEAD = DT == 256 ? 4 : 8;
   constexpr bool E8 = ES == 1;
-  __shared__ float s_sum[PA_WARPS][BR][DT];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int e = blockIdx.x / p.heads, head = blockIdx.x % p.heads, r = blockIdx.y;
+  __shared__ float s_sum[RPB][WPR][BR][WPR == 1 ? 1 : DT];
+  __shared__ float4 s_stat[RPB][WPR][BR];
+  const int warp = threadIdx.x / 32 % WPR, slot = threadIdx.x / 32 / WPR, lane = threadIdx.x & 31;
+  const int64_t which = static_cast<int64_t>(blockIdx.x) * RPB + slot;
+  const int item = static_cast<int>(which / S::QROWS), r = static_cast<int>(which % S::QROWS);
+  const int e = item / p.heads, head = item % p.heads;
+  if (e >= p.nb * p.nrt) return;
   const int row0 = (p.rt0 + e % p.nrt) * S::QROWS, b = p.b0 + e / p.nrt;
+  const PaSpan sp = pa_span<S::QROWS>(p, e);                                    // nothing of the first kernel is needed for it
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (row0 + r >= p.rows) return;
   const int entries = p.nb * p.nrt;
-  const int64_t all = static_cast<int64_t>(p.prefix[entries]) * p.heads, share = (all + p.ncta - 1) / p.ncta;
-  const int before = p.prefix[e], chunks = p.prefix[e + 1] - before;
-  const int64_t from = static_cast<int64_t>(before) * p.heads + static_cast<int64_t>(head) * chunks;
-  const int first = static_cast<int>(from / share), last = static_cast<int>((from + chunks - 1) / share);
+  const uint32_t before = p.prefix[e], chunks = p.prefix[e + 1] - before;
+  const uint32_t all = static_cast<uint32_t>(p.prefix[entries]) * p.heads, share = (all + p.ncta - 1) / p.ncta;
+  const uint32_t from = before * p.heads + head * chunks;
+  const int first = from / share, last = (from + chunks - 1) / share;
   if (first == last) return;                                                    // one CTA had it all
   const int n = last - first + 1;
-  auto part = [&](int i) { return p.parts + ((static_cast<int64_t>(first) + i) * 2 + (i == 0)) * S::PART; };
   float m[2], l[2], mv[2][2], v[2][N];
 #pragma unroll
   for (int br = 0; br < BR; ++br) {
     const int k = pa_column<PAIRS>(r, br);
     m[br] = mv[br][0] = mv[br][1] = -INFINITY; l[br] = 0.f;
-    for (int i = lane; i < n; i += 32) {
-      const float4 s = *reinterpret_cast<const float4*>(part(i) + S::COLS * DT + k * 4);
-      m[br] = fmaxf(m[br], s.x); mv[br][0] = fmaxf(mv[br][0], s.z); mv[br][1] = fmaxf(mv[br][1], s.w);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[br][j] = 0.f;
+    for (int i0 = warp; i0 < n; i0 += WPR * AHEAD) {
+      float4 st[AHEAD];
+      float x[AHEAD][N];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const int i = i0 + a * WPR;
+        const float* src = p.parts + ((static_cast<int64_t>(first) + i) * 2 + (i == 0)) * S::PART;
+        st[a] = i < n ? *reinterpret_cast<const float4*>(src + S::COLS * DT + k * 4) : make_float4(-INFINITY, 0.f, -INFINITY, -INFINITY);
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[a][j] = i < n ? src[k * DT + lane + 32 * j] : 0.f;
+      }
+      float top = m[br], t0 = mv[br][0], t1 = mv[br][1];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) { top = fmaxf(top, st[a].x); t0 = fmaxf(t0, st[a].z); t1 = fmaxf(t1, st[a].w); }
+      const float f = pa_step(m[br], top), f0 = E8 ? pa_step(mv[br][0], t0) : f, f1 = S::NG == 2 ? pa_step(mv[br][1], t1) : f0;
+      l[br] *= f;
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[br][j] *= j < N / 2 ? f0 : f1;
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const float g = pa_step(st[a].x, top), g0 = E8 ? pa_step(st[a].z, t0) : g, g1 = S::NG == 2 ? pa_step(st[a].w, t1) : g0;
+        l[br] += st[a].y * g;
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[br][j] += x[a][j] * (j < N / 2 ? g0 : g1);
+      }
+      m[br] = top; mv[br][0] = t0; mv[br][1] = t1;
     }
+    if constexpr (WPR > 1) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      m[br] = fmaxf(m[br], __shfl_xor_sync(0xffffffffu, m[br], o));
-      mv[br][0] = fmaxf(mv[br][0], __shfl_xor_sync(0xffffffffu, mv[br][0], o));
-      mv[br][1] = fmaxf(mv[br][1], __shfl_xor_sync(0xffffffffu, mv[br][1], o));
+      for (int j = 0; j < N; ++j) s_sum[slot][warp][br][lane + 32 * j] = v[br][j];
+      if (lane == 0) s_stat[slot][warp][br] = make_float4(m[br], l[br], mv[br][0], mv[br][1]);
     }
-    for (int i = lane; i < n; i += 32) {
-      const float4 s = *reinterpret_cast<const float4*>(part(i) + S::COLS * DT + k * 4);
-      l[br] += s.y * pa_step(s.x, m[br]);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) l[br] += __shfl_xor_sync(0xffffffffu, l[br], o);
-    float sum[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) sum[j] = 0.f;
-#pragma unroll 4
-    for (int i = warp; i < n; i += PA_WARPS) {
-      const float* src = part(i);
-      const float4 s = *reinterpret_cast<const float4*>(src + S::COLS * DT + k * 4);
-      const float f = pa_step(s.x, m[br]), f0 = E8 ? pa_step(s.z, mv[br][0]) : f, f1 = S::NG == 2 ? pa_step(s.w, mv[br][1]) : f0;
-#pragma unroll
-      for (int j = 0; j < N; ++j) sum[j] += src[k * DT + lane + 32 * j] * (j < N / 2 ? f0 : f1);
-    }
-#pragma unroll
-    for (int j = 0; j < N; ++j) s_sum[warp][br][lane + 32 * j] = sum[j];
   }
-  __syncthreads();
-  if (warp != 0) return;
+  if constexpr (WPR > 1) {
+    asm volatile("bar.sync %0, %1;" ::"r"(slot + 1), "n"(WPR * 32) : "memory");  // the warps of a row: others may have left
+    if (warp != 0) return;
 #pragma unroll
-  for (int br = 0; br < BR; ++br)
+    for (int br = 0; br < BR; ++br) {
+      m[br] = mv[br][0] = mv[br][1] = -INFINITY; l[br] = 0.f;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      v[br][j] = 0.f;
+      for (int w = 0; w < WPR; ++w) {
+        const float4 st = s_stat[slot][w][br];
+        m[br] = fmaxf(m[br], st.x); mv[br][0] = fmaxf(mv[br][0], st.z); mv[br][1] = fmaxf(mv[br][1], st.w);
+      }
 #pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) v[br][j] += s_sum[w][br][lane + 32 * j];
+      for (int j = 0; j < N; ++j) v[br][j] = 0.f;
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) {
+        const float4 st = s_stat[slot][w][br];
+        const float f = pa_step(st.x, m[br]), f0 = E8 ? pa_step(st.z, mv[br][0]) : f, f1 = S::NG == 2 ? pa_step(st.w, mv[br][1]) : f0;
+        l[br] += st.y * f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[br][j] += s_sum[slot][w][br][lane + 32 * j] * (j < N / 2 ? f0 : f1);
+      }
     }
-  const PaSpan sp = pa_span<S::QROWS>(p, e);
+  }
   pa_finish<ES, DT, PAIRS>(p, b, head, row0 + r, (row0 + r) / p.per <= sp.t1, v[0], v[1], m, l, mv, lane);
 }
 
@@ -806,15 +850,18 @@ static int pa_launch(PaArgs& p, int max_chunks, int num_sms, cudaStream_t st) {
   if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return static_cast<int>(e);
   if (p.prefix == nullptr) return 0;                                            // items of one chunk each: nothing to join
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.nb * p.nrt * p.heads), S::QROWS);
-  cfg.blockDim = dim3(PA_WARPS * 32);
+  const int64_t rows = static_cast<int64_t>(p.nb) * p.nrt * p.heads * S::QROWS, room = static_cast<int64_t>(num_sms) * 32;      // warps of the device, with 64 registers
+  const int wpr = rows * 16 <= room ? 16 : rows * 4 <= room ? 4 : 1, rpb = wpr == 1 ? 8 : 16 / wpr;
+  cfg.gridDim = dim3(static_cast<unsigned>((rows + rpb - 1) / rpb));
+  cfg.blockDim = dim3(wpr * rpb * 32);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, paged_join_kernel<ES, DT, PAIRS, NC>, p));
+  auto join = wpr == 16 ? paged_join_kernel<ES, DT, PAIRS, NC, 16> : wpr == 4 ? paged_join_kernel<ES, DT, PAIRS, NC, 4> : paged_join_kernel<ES, DT, PAIRS, NC, 1>;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, join, p));
 }
 
 // A launch of the sequences and tiles that p names; with `need` only the bytes of its workspace and its CTAs are worked out.
@@ -825,7 +872,7 @@ template <int ES, int DT, bool PAIRS, int NC>
 static int pa_prepare(PaArgs& p, bool gen, int span, int num_sms, void* ws, int64_t* need, cudaStream_t st) {
   using S = PaShape<ES, DT, PAIRS, NC>;
   const int max_chunks = span <= S::CHUNK ? 1 : (span + S::CHUNK - 1) / S::CHUNK;
-  const int64_t work = static_cast<int64_t>(p.nb) * p.nrt * p.heads * max_chunks, full = static_cast<int64_t>(num_sms) * pa_resident<ES, DT, PAIRS, NC>();
+  const int64_t work = static_cast<int64_t>(p.nb) * p.nrt * p.heads * max_chunks, full = static_cast<int64_t>(num_sms) * pa_resident<ES, DT, PAIRS, NC>() * PA_F;
   p.ncta = static_cast<int>(work < full ? work : full);
   const int64_t bytes = max_chunks > 1 ? static_cast<int64_t>(p.ncta) * 2 * S::PART * 4 + (PA_ENTRIES + 4) * 4 : 0;
   if (need != nullptr) { *need = bytes; return 0; }
