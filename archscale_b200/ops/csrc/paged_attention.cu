@@ -25,7 +25,10 @@ static PaPlan pa_plan(const PagedView& c, const b200_paged_query& a) {
   p.page_16 = static_cast<uint32_t>(p.page_b / 16); p.slot_16 = static_cast<uint32_t>(p.slot_b / 16);
   p.page_shift = -1;
   for (int i = 0; i < 31; ++i) if (c.page_size == 1 << i) p.page_shift = i;
-  s.gen = far > 0xffffffffLL || p.piece != 16 || D != (a.diff ? s.dt / 2 : s.dt);
+  const int64_t far_s = static_cast<int64_t>(c.pages) * (c.ks_page > c.vs_page ? c.ks_page : c.vs_page) + static_cast<int64_t>(c.page_size) * (c.ks_slot > c.vs_slot ? c.ks_slot : c.vs_slot);
+  p.ks_page = static_cast<uint32_t>(c.ks_page); p.ks_slot = static_cast<uint32_t>(c.ks_slot);
+  p.vs_page = static_cast<uint32_t>(c.vs_page); p.vs_slot = static_cast<uint32_t>(c.vs_slot);
+  s.gen = far > 0xffffffffLL || far_s > 0xffffffffLL || p.piece != 16 || D != (a.diff ? s.dt / 2 : s.dt);
   p.q_words = reinterpret_cast<uintptr_t>(a.q) % 4 == 0 && (a.q_batch | a.q_token | a.q_head) % 2 == 0;
   const int qrows = (a.diff ? 4 : 8) * s.nc;
   const int64_t room = static_cast<int64_t>(c.table_cols) * c.page_size, seen = a.window >= 0 ? static_cast<int64_t>(a.window) + qrows + 1 : room;

@@ -44,6 +44,7 @@ struct PaArgs {
   int ncta, piece, q_words;                // bytes of a copy where rows are not whole 16-byte pieces; queries start on 4-byte boundaries
   int64_t page_b, group_b, slot_b;         // strides in bytes, of keys as of values
   uint32_t page_16, slot_16;               // the same in units of 16 bytes (not GEN)
+  uint32_t ks_page, ks_slot, vs_page, vs_slot;      // strides of the scales (not GEN)
   int page_shift;                          // log2 of the page size, or -1
   float* parts;                            // [ncta][2] parts of items
   int* prefix;                             // chunks before each entry, from CTA 0
@@ -66,9 +67,9 @@ struct PaShape {
   static constexpr int HEADS = PAIRS ? 2 : 1;
   static constexpr int TILE = TS * ROW;
   static constexpr int SCALES = ES == 1 ? HEADS * TS * 8 : 0;                  // factors of keys, exponents of values
-  static constexpr int STAGE = 2 * TILE + SCALES + 16;                         // and the mask of tokens
+  static constexpr int STAGE = 2 * TILE, EXTRA = SCALES + 16;                  // keys and values; beside them the scales and the mask of tokens
   static constexpr int STAGES = PA_ST;
-  static constexpr int RING = PA_WARPS * STAGES * STAGE;
+  static constexpr int RING = PA_WARPS * STAGES * (STAGE + EXTRA);
   static constexpr int COLS = 8 * NC;
   static constexpr int QROWS = PAIRS ? 4 * NC : 8 * NC;                        // query rows of a tile
   static constexpr int LD = DT + 4;                                            // floats between rows in shared memory: no bank twice
@@ -210,9 +211,9 @@ __device__ __forceinline__ void pa_copy(uint32_t dst, const void* src, bool live
 }
 // byte of 16-byte piece `chunk` of token t in a tile: pieces of 8 tokens that a matrix load takes together lie in 8 different bank groups
 template <int ROW>
-__device__ __forceinline__ uint32_t pa_at(int t, int chunk) {
-  return t * ROW + ((ROW >= 128 ? chunk ^ (t & 7) : chunk ^ ((t >> 1) & 3)) << 4);
-}
+__device__ __forceinline__ constexpr uint32_t pa_swizzle(int t) { return (ROW >= 128 ? t & 7 : t >> 1 & 3) << 4; }
+template <int ROW>
+__device__ __forceinline__ uint32_t pa_at(int t, int chunk) { return t * ROW + ((chunk << 4) ^ pa_swizzle<ROW>(t)); }
 
 // GEN: rows that are not whole 16-byte pieces, or shorter than DT
 template <int ES, int DT, bool PAIRS, int NC, bool GEN>
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
   using S = PaShape<ES, DT, PAIRS, NC>;
   constexpr bool E8 = ES == 1;
   constexpr int TS = S::TS, MT = TS / 16, KS = DT / 16, HEADS = S::HEADS, NG = S::NG, NGX = NG > 0 ? NG : 1;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(512) uint8_t smem[];
   __shared__ int s_prefix[PA_ENTRIES + 1];
   __shared__ int s_scan[PA_WARPS];
   __shared__ float s_stat[PA_WARPS][4][16];                                     // m, l, m' of both groups
@@ -256,8 +257,11 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
 
   const uint32_t all = static_cast<uint32_t>(s_prefix[entries]) * p.heads, share = (all + p.ncta - 1) / p.ncta;
   const uint32_t end = min(all, (blockIdx.x + 1) * share);
-  uint8_t* const ring = smem + warp * S::STAGES * S::STAGE;
+  uint8_t* const ring = smem + warp * S::STAGES * S::STAGE;                     // stages start at multiples of 512 bytes, so that addresses in a row are XORs
+  uint8_t* const extra = smem + PA_WARPS * S::STAGES * S::STAGE + warp * S::STAGES * S::EXTRA;
   const uint32_t ring_u = smem_u32(ring);
+  // this lane's row and piece in the matrix loads: keys by rows of tokens, values transposed
+  const uint32_t own_k = pa_at<S::ROW>(lane & 15, lane >> 4), own_v = E8 ? own_k : pa_at<S::ROW>((lane & 7) + (lane >> 4) * 8, lane >> 3 & 1);
   constexpr float LOG2E = 1.4426950408889634f;
   constexpr uint32_t FULL = TS == 32 ? 0xffffffffu : (1u << (TS & 31)) - 1u;
 
@@ -319,7 +323,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
     int page_a = look(0), page_b = look(1);
     uint32_t pend_k[HEADS] = {}, pend_v[HEADS] = {};
     auto issue = [&](int step) {
-      int64_t scale_at = -1, scale_at_v = 0;
+      bool scaled = false;
+      int64_t scale_at = 0, scale_at_v = 0;
       if (step < steps) {
         const int j = j_base + step * S::CHUNK + lane;
         int page = page_a;
@@ -330,28 +335,34 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
         page_a = page_b;
         page_b = look(step + 2);
         const int slot = page >= 0 ? j - page_of(j) * p.c.page_size : 0;
-        if (E8 && page >= 0) { scale_at = page * p.c.ks_page + slot * p.c.ks_slot; scale_at_v = page * p.c.vs_page + slot * p.c.vs_slot; }
+        if (E8 && page >= 0) {
+          scaled = true;
+          if constexpr (GEN) { scale_at = page * p.c.ks_page + slot * p.c.ks_slot; scale_at_v = page * p.c.vs_page + slot * p.c.vs_slot; }
+          else { scale_at = page * p.ks_page + slot * p.ks_slot; scale_at_v = page * p.vs_page + slot * p.vs_slot; }
+        }
         const uint32_t live = __ballot_sync(0xffffffffu, page >= 0);
         const uint32_t st = ring_u + (step % S::STAGES) * S::STAGE;
-        if (lane == 0) *reinterpret_cast<uint32_t*>(ring + (step % S::STAGES) * S::STAGE + 2 * S::TILE + S::SCALES) = live;
+        if (lane == 0) *reinterpret_cast<uint32_t*>(extra + (step % S::STAGES) * S::EXTRA + S::SCALES) = live;
         if (live != 0) {
           if constexpr (!GEN) {
             constexpr int PPR = S::ROW / 16;                                    // a lane has one piece of every (32 / PPR)-th token
             const uint32_t mine = page >= 0 ? page * p.page_16 + slot * p.slot_16 : 0u;
+            constexpr int TPI = 32 / PPR;
+            const uint32_t own = pa_at<S::ROW>(lane / PPR, lane % PPR);
             if (live == FULL) {
 #pragma unroll
-              for (int i = 0; i < TS * PPR / 32; ++i) {
-                const int64_t o = static_cast<int64_t>(__shfl_sync(0xffffffffu, mine, i * (32 / PPR) + lane / PPR)) * 16;
-                const uint32_t to = st + pa_at<S::ROW>(i * (32 / PPR) + lane / PPR, lane % PPR);
+              for (int i = 0; i < TS / TPI; ++i) {
+                const int64_t o = static_cast<int64_t>(__shfl_sync(0xffffffffu, mine, i * TPI + lane / PPR)) * 16;
+                const uint32_t to = st + (own ^ pa_swizzle<S::ROW>(i * TPI)) + i * TPI * S::ROW;
                 pa_copy<16>(to, k_lane + o);
                 pa_copy<16>(to + S::TILE, v_lane + o);
               }
             } else {
 #pragma unroll
-              for (int i = 0; i < TS * PPR / 32; ++i) {
-                const int t = i * (32 / PPR) + lane / PPR;
+              for (int i = 0; i < TS / TPI; ++i) {
+                const int t = i * TPI + lane / PPR;
                 const int64_t o = static_cast<int64_t>(__shfl_sync(0xffffffffu, mine, t)) * 16;
-                const uint32_t to = st + pa_at<S::ROW>(t, lane % PPR);
+                const uint32_t to = st + (own ^ pa_swizzle<S::ROW>(i * TPI)) + i * TPI * S::ROW;
                 pa_copy<16>(to, k_lane + o, live >> t & 1u);
                 pa_copy<16>(to + S::TILE, v_lane + o, live >> t & 1u);
               }
@@ -378,14 +389,14 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
       asm volatile("cp.async.commit_group;" ::: "memory");
       if constexpr (E8) {
         if (step > 0 && lane < TS) {                                            // scales asked for one step ago
-          float* const to = reinterpret_cast<float*>(ring + ((step - 1) % S::STAGES) * S::STAGE + 2 * S::TILE);
+          float* const to = reinterpret_cast<float*>(extra + ((step - 1) % S::STAGES) * S::EXTRA);
 #pragma unroll
           for (int h = 0; h < HEADS; ++h) {
             to[h * TS + lane] = paged_pow2(pend_k[h]);
             to[(HEADS + h) * TS + lane] = pend_v[h] == 255u ? __int_as_float(0x7fffffff) : static_cast<float>(static_cast<int>(pend_v[h]) - 127);
           }
         }
-        if (scale_at >= 0) {
+        if (scaled) {
 #pragma unroll
           for (int h = 0; h < HEADS; ++h) {
             pend_k[h] = ks[scale_at + h * p.c.ks_group];
@@ -456,8 +467,9 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
       __syncwarp();
       const int stage = step % S::STAGES;
       const uint8_t* const st = ring + stage * S::STAGE;
-      const uint32_t kt_u = ring_u + stage * S::STAGE, vt_u = kt_u + S::TILE;
-      const uint32_t live = *reinterpret_cast<const uint32_t*>(st + 2 * S::TILE + S::SCALES);
+      const uint32_t kt_u = ring_u + stage * S::STAGE + own_k, vt_u = ring_u + stage * S::STAGE + S::TILE + own_v;
+      const uint8_t* const ex = extra + stage * S::EXTRA;
+      const uint32_t live = *reinterpret_cast<const uint32_t*>(ex + S::SCALES);
       const int j0 = j_base + step * S::CHUNK;
       if (live != 0) {
         // ---- scores: x[c][mt][k] of token mt · 16 + gq (k < 2) or + 8, column 2 cq + (k & 1)
@@ -473,7 +485,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
             uint32_t r[4];
-            pa_ldsm<false>(r, kt_u + pa_at<S::ROW>(mt * 16 + (lane & 15), ks * 2 + (lane >> 4)));
+            pa_ldsm<false>(r, (kt_u ^ (ks << 5)) + mt * 16 * S::ROW);
             if constexpr (E8) {                                                 // 16 bytes are a whole step of the product; q is laid out alike
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
@@ -487,7 +499,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
             }
           }
         const bool masked = live != FULL || j0 + TS - 1 > all_hi || j0 < all_lo;
-        const float* const scales = reinterpret_cast<const float*>(st + 2 * S::TILE);
+        const float* const scales = reinterpret_cast<const float*>(ex);
         float ev[NGX][MT][2];                                                   // exponents of the values' scales
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -619,14 +631,14 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
         auto values = [&](int mt, int i, uint32_t (&a)[NB][4]) {
           uint32_t r[4];
           if constexpr (E8) {
-            pa_ldsm<true>(r, vt_u + pa_at<S::ROW>(mt * 16 + (lane & 15), i * 2 + (lane >> 4)));
+            pa_ldsm<true>(r, (vt_u ^ (i << 5)) + mt * 16 * S::ROW);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const uint32_t u = __byte_perm(r[2 * h], 0, 0x3120), w = __byte_perm(r[2 * h + 1], 0, 0x3120);
               a[h][0] = pa_half2(u); a[h][1] = pa_half2(u >> 16); a[h][2] = pa_half2(w); a[h][3] = pa_half2(w >> 16);
             }
           } else {
-            pa_ldsm<true>(r, vt_u + pa_at<S::ROW>(mt * 16 + (lane & 7) + (lane >> 4) * 8, i * 2 + (lane >> 3 & 1)));
+            pa_ldsm<true>(r, (vt_u ^ (i << 5)) + mt * 16 * S::ROW);
             a[0][0] = r[0]; a[0][1] = r[1]; a[0][2] = r[2]; a[0][3] = r[3];
           }
         };
