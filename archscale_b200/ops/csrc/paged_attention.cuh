@@ -32,7 +32,6 @@
 
 namespace b200 {
 
-constexpr int PA_WARPS = 4;
 constexpr int PA_ENTRIES = 1024;           // (sequence, tile of rows) of one launch
 
 struct PaArgs {
@@ -51,31 +50,23 @@ struct PaArgs {
 };
 
 // What a shape needs.  ES: bytes of an element; DT: values of a row of keys, of both heads of a pair; NC: groups of 8 columns.
-#ifndef PA_ST
-#define PA_ST 2
-#endif
-#ifndef PA_F
-#define PA_F 1
-#endif
-#ifndef PA_TS8
-#define PA_TS8 32
-#endif
 template <int ES, int DT, bool PAIRS, int NC>
 struct PaShape {
   static constexpr int ROW = DT * ES;                                          // bytes of a token in a stage
-  static constexpr int TS = ES == 2 ? (DT == 64 ? 32 : 16) : (DT == 256 ? 16 : DT == 128 ? PA_TS8 : 32);   // tokens of a warp's step
+  static constexpr int TS = ES == 2 ? (DT == 64 ? 32 : 16) : (DT == 256 ? 16 : 32);   // tokens of a warp's step
   static constexpr int HEADS = PAIRS ? 2 : 1;
   static constexpr int TILE = TS * ROW;
   static constexpr int SCALES = ES == 1 ? HEADS * TS * 8 : 0;                  // factors of keys, exponents of values
   static constexpr int STAGE = 2 * TILE, EXTRA = SCALES + 16;                  // keys and values; beside them the scales and the mask of tokens
-  static constexpr int STAGES = PA_ST;
-  static constexpr int RING = PA_WARPS * STAGES * (STAGE + EXTRA);
+  static constexpr int STAGES = 2;
+  static constexpr int WARPS = STAGE > 12288 ? 6 : 4;                          // six where one CTA has the SM to itself
+  static constexpr int RING = WARPS * STAGES * (STAGE + EXTRA);
   static constexpr int COLS = 8 * NC;
   static constexpr int QROWS = PAIRS ? 4 * NC : 8 * NC;                        // query rows of a tile
   static constexpr int LD = DT + 4;                                            // floats between rows in shared memory: no bank twice
-  static constexpr int SLABS = PA_WARPS * COLS * LD * 4;
+  static constexpr int SLABS = WARPS * COLS * LD * 4;
   static constexpr int SMEM = RING > SLABS ? RING : SLABS;
-  static constexpr int CHUNK = PA_WARPS * TS;
+  static constexpr int CHUNK = WARPS * TS;
   static constexpr int NG = ES == 1 ? HEADS : 0;                               // groups of values with maxima of their own
   static constexpr int PART = COLS * (DT + 4);                                 // floats of a part: sums, then m, l, m' of each column
   static_assert(SMEM <= 227 * 1024 - 6144, "shared memory");
@@ -217,21 +208,21 @@ __device__ __forceinline__ uint32_t pa_at(int t, int chunk) { return t * ROW + (
 
 // GEN: rows that are not whole 16-byte pieces, or shorter than DT
 template <int ES, int DT, bool PAIRS, int NC, bool GEN>
-__global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>()) paged_attention_kernel(const PaArgs p) {
+__global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_resident<ES, DT, PAIRS, NC>()) paged_attention_kernel(const PaArgs p) {
   using S = PaShape<ES, DT, PAIRS, NC>;
   constexpr bool E8 = ES == 1;
   constexpr int TS = S::TS, MT = TS / 16, KS = DT / 16, HEADS = S::HEADS, NG = S::NG, NGX = NG > 0 ? NG : 1;
   extern __shared__ __align__(512) uint8_t smem[];
   __shared__ int s_prefix[PA_ENTRIES + 1];
-  __shared__ int s_scan[PA_WARPS];
-  __shared__ float s_stat[PA_WARPS][4][16];                                     // m, l, m' of both groups
+  __shared__ int s_scan[S::WARPS];
+  __shared__ float s_stat[S::WARPS][4][16];                                     // m, l, m' of both groups
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, cq = lane & 3;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- chunks before every entry
   const int entries = p.nb * p.nrt;
   {
-    const int each = (entries + PA_WARPS * 32 - 1) / (PA_WARPS * 32), from = threadIdx.x * each;
+    const int each = (entries + S::WARPS * 32 - 1) / (S::WARPS * 32), from = threadIdx.x * each;
     int sum = 0;
     for (int i = from; i < min(from + each, entries); ++i) {
       const PaSpan s = pa_span<S::QROWS>(p, i);
@@ -247,18 +238,18 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
     int base = scan - sum;
     for (int w = 0; w < warp; ++w) base += s_scan[w];
     for (int i = from; i < min(from + each, entries); ++i) { const int n = s_prefix[i]; s_prefix[i] = base; base += n; }
-    if (threadIdx.x == 0) { int all = 0; for (int w = 0; w < PA_WARPS; ++w) all += s_scan[w]; s_prefix[entries] = all; }
+    if (threadIdx.x == 0) { int all = 0; for (int w = 0; w < S::WARPS; ++w) all += s_scan[w]; s_prefix[entries] = all; }
   }
   if (GEN)                                                                      // columns past D stay zero
-    for (int i = threadIdx.x; i < S::RING / 16; i += PA_WARPS * 32) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < S::RING / 16; i += S::WARPS * 32) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   if (blockIdx.x == 0 && p.prefix != nullptr)
-    for (int i = threadIdx.x; i <= entries; i += PA_WARPS * 32) p.prefix[i] = s_prefix[i];
+    for (int i = threadIdx.x; i <= entries; i += S::WARPS * 32) p.prefix[i] = s_prefix[i];
 
   const uint32_t all = static_cast<uint32_t>(s_prefix[entries]) * p.heads, share = (all + p.ncta - 1) / p.ncta;
   const uint32_t end = min(all, (blockIdx.x + 1) * share);
   uint8_t* const ring = smem + warp * S::STAGES * S::STAGE;                     // stages start at multiples of 512 bytes, so that addresses in a row are XORs
-  uint8_t* const extra = smem + PA_WARPS * S::STAGES * S::STAGE + warp * S::STAGES * S::EXTRA;
+  uint8_t* const extra = smem + S::WARPS * S::STAGES * S::STAGE + warp * S::STAGES * S::EXTRA;
   const uint32_t ring_u = smem_u32(ring);
   // this lane's row and piece in the matrix loads: keys by rows of tokens, values transposed
   const uint32_t own_k = pa_at<S::ROW>(lane & 15, lane >> 4), own_v = E8 ? own_k : pa_at<S::ROW>((lane & 7) + (lane >> 4) * 8, lane >> 3 & 1);
@@ -720,14 +711,14 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
     __syncthreads();
     const bool whole = c0 == 0 && c1 == chunks;
     float* const part = whole ? nullptr : p.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (c0 == 0)) * S::PART;
-    for (int r = warp; r < S::QROWS; r += PA_WARPS) {
+    for (int r = warp; r < S::QROWS; r += S::WARPS) {
       float v[2][DT / 32], mm[2], ll[2], mmv[2][2];
 #pragma unroll
       for (int br = 0; br < HEADS; ++br) {
         const int k = pa_column<PAIRS>(r, br);
         mm[br] = mmv[br][0] = mmv[br][1] = -INFINITY; ll[br] = 0.f;
 #pragma unroll
-        for (int w = 0; w < PA_WARPS; ++w) {
+        for (int w = 0; w < S::WARPS; ++w) {
           mm[br] = fmaxf(mm[br], s_stat[w][0][k]);
           mmv[br][0] = fmaxf(mmv[br][0], s_stat[w][2][k]);
           mmv[br][1] = fmaxf(mmv[br][1], s_stat[w][3][k]);
@@ -735,7 +726,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
 #pragma unroll
         for (int i = 0; i < DT / 32; ++i) v[br][i] = 0.f;
 #pragma unroll
-        for (int w = 0; w < PA_WARPS; ++w) {
+        for (int w = 0; w < S::WARPS; ++w) {
           const float f = pa_step(s_stat[w][0][k], mm[br]);
           ll[br] += s_stat[w][1][k] * f;
           const float f0 = E8 ? pa_step(s_stat[w][2][k], mmv[br][0]) : f, f1 = NG == 2 ? pa_step(s_stat[w][3][k], mmv[br][1]) : f0;
@@ -754,7 +745,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, pa_resident<ES, DT, PAIRS, NC>(
     }
     __syncthreads();                                                            // the ring is used again
     if (GEN)                                                                    // and its unused columns are zero again
-      for (int i = threadIdx.x; i < S::SLABS / 16; i += PA_WARPS * 32) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+      for (int i = threadIdx.x; i < S::SLABS / 16; i += S::WARPS * 32) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
     if (GEN) __syncthreads();
     at += c1 - c0;
   }
@@ -858,7 +849,7 @@ static int pa_launch(PaArgs& p, int max_chunks, int num_sms, cudaStream_t st) {
   using S = PaShape<ES, DT, PAIRS, NC>;
   auto kernel = paged_attention_kernel<ES, DT, PAIRS, NC, GEN>;
   if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); e != cudaSuccess) return static_cast<int>(e);
-  kernel<<<p.ncta, PA_WARPS * 32, S::SMEM, st>>>(p);
+  kernel<<<p.ncta, S::WARPS * 32, S::SMEM, st>>>(p);
   if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return static_cast<int>(e);
   if (p.prefix == nullptr) return 0;                                            // items of one chunk each: nothing to join
   cudaLaunchConfig_t cfg = {};
@@ -884,8 +875,12 @@ template <int ES, int DT, bool PAIRS, int NC>
 static int pa_prepare(PaArgs& p, bool gen, int span, int num_sms, void* ws, int64_t* need, cudaStream_t st) {
   using S = PaShape<ES, DT, PAIRS, NC>;
   const int max_chunks = span <= S::CHUNK ? 1 : (span + S::CHUNK - 1) / S::CHUNK;
-  const int64_t work = static_cast<int64_t>(p.nb) * p.nrt * p.heads * max_chunks, full = static_cast<int64_t>(num_sms) * pa_resident<ES, DT, PAIRS, NC>() * PA_F;
-  p.ncta = static_cast<int>(work < full ? work : full);
+  // As many CTAs as run at once, each with an equal share; twice as many where a share is long beside the fixed costs of a CTA, so that SMs that are
+  // nearer to memory take more of them: bf16, 64 sequences up to 8192, 97 -> 98 us with the cache in the L2, 119 -> 113 without; 32 in pairs 139 -> 135;
+  // e4m3, whose warps compute half of the time, 47 -> 51.
+  const int64_t work = static_cast<int64_t>(p.nb) * p.nrt * p.heads * max_chunks, full = static_cast<int64_t>(num_sms) * pa_resident<ES, DT, PAIRS, NC>();
+  const int64_t most = ES == 2 && work >= 48 * full ? 2 * full : full;
+  p.ncta = static_cast<int>(work < most ? work : most);
   const int64_t bytes = max_chunks > 1 ? static_cast<int64_t>(p.ncta) * 2 * S::PART * 4 + (PA_ENTRIES + 4) * 4 : 0;
   if (need != nullptr) { *need = bytes; return 0; }
   p.parts = static_cast<float*>(ws);

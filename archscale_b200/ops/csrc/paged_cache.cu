@@ -7,42 +7,45 @@
 //   read    x = q · 2^e into dense rows, zeros past the end of a sequence.
 //
 // Memory-bound.  A head's row is held by D / 8 lanes, 8 values each (one 16-byte load of bf16), keys and values by the same lanes; rows that no 16 bytes
-// divide go value by value on a whole warp.
+// divide go value by value on a whole warp.  A row waits for its length, its page and then its data, so a thread has four rows under way where there are
+// enough of them to fill the device all the same (8 x 8192 tokens from e4m3: @READ@; 4 x 4096 tokens into e4m3: @WRITE@), and one
+// where latency counts.
 #include <cuda_fp8.h>
+#include <type_traits>
 
 #include "paged.cuh"
 
 namespace b200 {
 
-template <class T> struct Vals;          // 8 values as they are loaded and stored
-template <> struct Vals<__nv_bfloat16> {
-  static __device__ void load(const __nv_bfloat16* p, float (&x)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+template <class T> struct Eight;         // 8 values as they are loaded, and as they are stored
+template <> struct Eight<__nv_bfloat16> {
+  uint4 u;
+  __device__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ void get(float (&x)[8]) const {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
   }
   static __device__ void store(__nv_bfloat16* p, const float (&x)[8]) {
-    uint4 u;
-    uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+    uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) { const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t*>(&h); }
-    *reinterpret_cast<uint4*>(p) = u;
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
-template <> struct Vals<float> {
-  static __device__ void load(const float* p, float (&x)[8]) {
-    *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
-    *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(p + 4);
-  }
+template <> struct Eight<float> {
+  float4 u, v;
+  __device__ void load(const float* p) { u = *reinterpret_cast<const float4*>(p); v = *reinterpret_cast<const float4*>(p + 4); }
+  __device__ void get(float (&x)[8]) const { x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w; }
   static __device__ void store(float* p, const float (&x)[8]) {
-    *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(x);
-    *reinterpret_cast<float4*>(p + 4) = *reinterpret_cast<const float4*>(x + 4);
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
   }
 };
-template <> struct Vals<__nv_fp8_e4m3> {
-  static __device__ void load(const __nv_fp8_e4m3* p, float (&x)[8]) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
+template <> struct Eight<__nv_fp8_e4m3> {
+  uint2 u;
+  __device__ void load(const __nv_fp8_e4m3* p) { u = *reinterpret_cast<const uint2*>(p); }
+  __device__ void get(float (&x)[8]) const {
     const uint32_t w[2] = {u.x, u.y};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -66,26 +69,28 @@ __device__ __forceinline__ void put_value(__nv_bfloat16* p, float x) { *p = __fl
 __device__ __forceinline__ void put_value(__nv_fp8_e4m3* p, float x) { p->__x = __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
 
 // A lane's share of a row: 8 neighbouring values (VEC), or every 32nd value, up to 8 of them.
-template <bool VEC, class T>
-__device__ __forceinline__ void load_share(const T* row, int lane, int D, float (&x)[8]) {
-  if constexpr (VEC) {
-    if (8 * lane < D) { Vals<T>::load(row + 8 * lane, x); return; }
+template <bool VEC, class T> struct Share;
+template <class T> struct Share<true, T> {
+  Eight<T> e;
+  __device__ void load(const T* row, int lane, int D) { if (8 * lane < D) e.load(row + 8 * lane); else e = {}; }
+  __device__ void get(float (&x)[8]) const { e.get(x); }
+  static __device__ void store(T* row, int lane, int D, const float (&x)[8]) { if (8 * lane < D) Eight<T>::store(row + 8 * lane, x); }
+};
+template <class T> struct Share<false, T> {
+  float v[8];
+  __device__ void load(const T* row, int lane, int D) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = lane + 32 * i < D ? one_value(row + lane + 32 * i) : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = lane + 32 * i < D ? one_value(row + lane + 32 * i) : 0.f;
   }
-}
-template <bool VEC, class T>
-__device__ __forceinline__ void store_share(T* row, int lane, int D, const float (&x)[8]) {
-  if constexpr (VEC) {
-    if (8 * lane < D) Vals<T>::store(row + 8 * lane, x);
-  } else {
+  __device__ void get(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = v[i];
+  }
+  static __device__ void store(T* row, int lane, int D, const float (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) if (lane + 32 * i < D) put_value(row + lane + 32 * i, x[i]);
   }
-}
+};
 
 // Scale byte of a row from its values, which become x · 2^−e.  LANES neighbouring lanes hold the row.
 template <int LANES>
@@ -109,62 +114,94 @@ __device__ __forceinline__ uint32_t to_scale(float (&x)[8]) {
 
 constexpr int PC_THREADS = 256;
 
-template <class In, class Cache, int LANES, bool VEC>
+// ROWS: rows (token, head) of a thread, a grid's step apart from each other
+template <class In, class Cache, int LANES, bool VEC, int ROWS>
 __global__ void __launch_bounds__(PC_THREADS) paged_write_kernel(const PagedView c, const In* k, const In* v, int64_t kb, int64_t kt, int64_t kh, int64_t vb,
                                                                  int64_t vt, int64_t vh, int B, int T) {
   constexpr bool E8 = sizeof(Cache) == 1;
+  constexpr int STEP = PC_THREADS / LANES;
   const int lane = threadIdx.x % LANES;
-  const uint32_t row = blockIdx.x * (PC_THREADS / LANES) + threadIdx.x / LANES;                            // (token, head)
-  const int t = static_cast<int>(row / static_cast<uint32_t>(c.groups)), g = static_cast<int>(row % static_cast<uint32_t>(c.groups));
+  const uint32_t row0 = blockIdx.x * (STEP * ROWS) + threadIdx.x / LANES;
   for (int b = blockIdx.y; b < B; b += gridDim.y) {
     const int n = paged_new(c, b, T);
-    int page = -1, slot = 0;
-    if (t < n) {
-      const int64_t pos = static_cast<int64_t>(c.lengths[b]) - n + t;
-      if (pos >= 0) { page = paged_page(c, b, static_cast<int>(pos) / c.page_size); slot = static_cast<int>(pos) % c.page_size; }
+    const int64_t first = static_cast<int64_t>(c.lengths[b]) - n;
+    Share<VEC, In> x[ROWS], y[ROWS];
+    int page[ROWS], slot[ROWS], g[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const uint32_t row = row0 + i * STEP;
+      const int t = static_cast<int>(row / static_cast<uint32_t>(c.groups));
+      g[i] = static_cast<int>(row % static_cast<uint32_t>(c.groups));
+      page[i] = -1; slot[i] = 0;
+      if (t < n && first + t >= 0) {
+        const int pos = static_cast<int>(first + t);
+        page[i] = paged_page(c, b, pos / c.page_size);
+        slot[i] = pos % c.page_size;
+        x[i].load(k + b * kb + t * kt + g[i] * kh, lane, c.dim);
+        y[i].load(v + b * vb + t * vt + g[i] * vh, lane, c.dim);
+      } else x[i] = y[i] = {};
     }
-    const bool live = page >= 0;           // the same for the lanes of a row; all lanes take part in the exchange of maxima
-    float x[8] = {}, y[8] = {};
-    if (live) {
-      load_share<VEC>(k + b * kb + t * kt + g * kh, lane, c.dim, x);
-      load_share<VEC>(v + b * vb + t * vt + g * vh, lane, c.dim, y);
-    }
-    uint32_t ex = 0, ey = 0;
-    if constexpr (E8) { ex = to_scale<LANES>(x); ey = to_scale<LANES>(y); }
-    if (live) {
-      store_share<VEC>(static_cast<Cache*>(c.k) + page * c.k_page + g * c.k_group + slot * c.k_slot, lane, c.dim, x);
-      store_share<VEC>(static_cast<Cache*>(c.v) + page * c.v_page + g * c.v_group + slot * c.v_slot, lane, c.dim, y);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      float p[8], q[8];
+      x[i].get(p); y[i].get(q);
+      uint32_t ex = 0, ey = 0;
+      if constexpr (E8) { ex = to_scale<LANES>(p); ey = to_scale<LANES>(q); }   // all lanes take part in the exchange of maxima
+      if (page[i] < 0) continue;                                                // the same for the lanes of a row
+      Share<VEC, Cache>::store(static_cast<Cache*>(c.k) + page[i] * c.k_page + g[i] * c.k_group + slot[i] * c.k_slot, lane, c.dim, p);
+      Share<VEC, Cache>::store(static_cast<Cache*>(c.v) + page[i] * c.v_page + g[i] * c.v_group + slot[i] * c.v_slot, lane, c.dim, q);
       if (E8 && lane == 0) {
-        c.ks[page * c.ks_page + g * c.ks_group + slot * c.ks_slot] = ex;
-        c.vs[page * c.vs_page + g * c.vs_group + slot * c.vs_slot] = ey;
+        c.ks[page[i] * c.ks_page + g[i] * c.ks_group + slot[i] * c.ks_slot] = ex;
+        c.vs[page[i] * c.vs_page + g[i] * c.vs_group + slot[i] * c.vs_slot] = ey;
       }
     }
   }
 }
 
-template <class Cache, class Out, int LANES, bool VEC>
+template <class Cache, class Out, int LANES, bool VEC, int ROWS>
 __global__ void __launch_bounds__(PC_THREADS) paged_read_kernel(const PagedView c, Out* k, Out* v, int B, int tokens) {
   constexpr bool E8 = sizeof(Cache) == 1;
+  constexpr int STEP = PC_THREADS / LANES;
   const int lane = threadIdx.x % LANES;
-  const uint32_t row = blockIdx.x * (PC_THREADS / LANES) + threadIdx.x / LANES;
-  const int t = static_cast<int>(row / static_cast<uint32_t>(c.groups)), g = static_cast<int>(row % static_cast<uint32_t>(c.groups));
-  if (t >= tokens) return;
+  const uint32_t row0 = blockIdx.x * (STEP * ROWS) + threadIdx.x / LANES;
   for (int b = blockIdx.y; b < B; b += gridDim.y) {
-    const int page = t < c.lengths[b] ? paged_page(c, b, t / c.page_size) : -1, slot = t % c.page_size;
-    float x[8] = {}, y[8] = {};
-    if (page >= 0) {
-      load_share<VEC>(static_cast<const Cache*>(c.k) + page * c.k_page + g * c.k_group + slot * c.k_slot, lane, c.dim, x);
-      load_share<VEC>(static_cast<const Cache*>(c.v) + page * c.v_page + g * c.v_group + slot * c.v_slot, lane, c.dim, y);
-      if constexpr (E8) {
-        const float sx = paged_pow2(c.ks[page * c.ks_page + g * c.ks_group + slot * c.ks_slot]);
-        const float sy = paged_pow2(c.vs[page * c.vs_page + g * c.vs_group + slot * c.vs_slot]);
+    const int length = c.lengths[b];
+    Share<VEC, Cache> x[ROWS], y[ROWS];
+    int page[ROWS], slot[ROWS], g[ROWS];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { x[i] *= sx; y[i] *= sy; }
+    for (int i = 0; i < ROWS; ++i) {                                            // all pages, then all rows
+      const uint32_t row = row0 + i * STEP;
+      const int t = static_cast<int>(row / static_cast<uint32_t>(c.groups));
+      g[i] = static_cast<int>(row % static_cast<uint32_t>(c.groups));
+      page[i] = t < tokens && t < length ? paged_page(c, b, t / c.page_size) : -1;
+      slot[i] = t % c.page_size;
+    }
+    float sx[ROWS], sy[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      sx[i] = sy[i] = 0.f;
+      if (page[i] < 0) { x[i] = y[i] = {}; continue; }
+      x[i].load(static_cast<const Cache*>(c.k) + page[i] * c.k_page + g[i] * c.k_group + slot[i] * c.k_slot, lane, c.dim);
+      y[i].load(static_cast<const Cache*>(c.v) + page[i] * c.v_page + g[i] * c.v_group + slot[i] * c.v_slot, lane, c.dim);
+      if constexpr (E8) {
+        sx[i] = paged_pow2(c.ks[page[i] * c.ks_page + g[i] * c.ks_group + slot[i] * c.ks_slot]);
+        sy[i] = paged_pow2(c.vs[page[i] * c.vs_page + g[i] * c.vs_group + slot[i] * c.vs_slot]);
       }
     }
-    const int64_t at = (static_cast<int64_t>(b) * tokens * c.groups + row) * c.dim;
-    store_share<VEC>(k + at, lane, c.dim, x);
-    store_share<VEC>(v + at, lane, c.dim, y);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const uint32_t row = row0 + i * STEP;
+      if (row / static_cast<uint32_t>(c.groups) >= static_cast<uint32_t>(tokens)) continue;
+      float p[8], q[8];
+      x[i].get(p); y[i].get(q);
+      if constexpr (E8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { p[j] *= sx[i]; q[j] *= sy[i]; }
+      }
+      const int64_t at = (static_cast<int64_t>(b) * tokens * c.groups + row) * c.dim;
+      Share<VEC, Out>::store(k + at, lane, c.dim, p);
+      Share<VEC, Out>::store(v + at, lane, c.dim, q);
+    }
   }
 }
 
@@ -177,34 +214,47 @@ static bool cache_vec(const PagedView& c) {
   return c.dim % 8 == 0 && strides % (align8(c.type) / element(c.type)) == 0 && whole(c.k, align8(c.type)) && whole(c.v, align8(c.type));
 }
 
+// Lanes of a row.
+template <class F>
+static void pc_lanes(int dim, bool vec, F&& go) {
+  if (!vec) go(std::integral_constant<int, 32>{}, std::false_type{});
+  else if (dim <= 64) go(std::integral_constant<int, 8>{}, std::true_type{});
+  else if (dim <= 128) go(std::integral_constant<int, 16>{}, std::true_type{});
+  else go(std::integral_constant<int, 32>{}, std::true_type{});
+}
+// Rows of a thread: four where that still gives every SM its 2048 threads.
+template <class F>
+static void pc_grid(int64_t rows, int B, int lanes, F&& go) {
+  const int step = PC_THREADS / lanes, per = rows * lanes * B >= 8LL * 148 * 2048 ? 4 : rows * lanes * B >= 2LL * 148 * 2048 ? 2 : 1;
+  go(per, dim3(static_cast<unsigned>((rows + step * per - 1) / (step * per)), static_cast<unsigned>(B < 65535 ? B : 65535)));
+}
+
 template <class In, class Cache>
 static int write_as(const PagedView& c, const void* k, const void* v, int64_t kb, int64_t kt, int64_t kh, int64_t vb, int64_t vt, int64_t vh, int B, int T,
                     bool vec, cudaStream_t st) {
-  const int64_t rows = static_cast<int64_t>(T) * c.groups;
-  auto go = [&](auto kernel, int lanes) {
-    const int64_t per = PC_THREADS / lanes;
-    kernel<<<dim3(static_cast<unsigned>((rows + per - 1) / per), static_cast<unsigned>(B < 65535 ? B : 65535)), PC_THREADS, 0, st>>>(
-        c, static_cast<const In*>(k), static_cast<const In*>(v), kb, kt, kh, vb, vt, vh, B, T);
+  auto go = [&](auto lanes_c, auto vec_c) {
+    constexpr int LANES = decltype(lanes_c)::value;
+    constexpr bool VEC = decltype(vec_c)::value;
+    pc_grid(static_cast<int64_t>(T) * c.groups, B, LANES, [&](int per, dim3 grid) {
+      auto kernel = per == 1 ? paged_write_kernel<In, Cache, LANES, VEC, 1> : per == 2 ? paged_write_kernel<In, Cache, LANES, VEC, 2> : paged_write_kernel<In, Cache, LANES, VEC, 4>;
+      kernel<<<grid, PC_THREADS, 0, st>>>(c, static_cast<const In*>(k), static_cast<const In*>(v), kb, kt, kh, vb, vt, vh, B, T);
+    });
   };
-  if (!vec) go(paged_write_kernel<In, Cache, 32, false>, 32);
-  else if (c.dim <= 64) go(paged_write_kernel<In, Cache, 8, true>, 8);
-  else if (c.dim <= 128) go(paged_write_kernel<In, Cache, 16, true>, 16);
-  else go(paged_write_kernel<In, Cache, 32, true>, 32);
+  pc_lanes(c.dim, vec, go);
   return static_cast<int>(cudaGetLastError());
 }
 
 template <class Cache, class Out>
 static int read_as(const PagedView& c, void* k, void* v, int B, int tokens, bool vec, cudaStream_t st) {
-  const int64_t rows = static_cast<int64_t>(tokens) * c.groups;
-  auto go = [&](auto kernel, int lanes) {
-    const int64_t per = PC_THREADS / lanes;
-    kernel<<<dim3(static_cast<unsigned>((rows + per - 1) / per), static_cast<unsigned>(B < 65535 ? B : 65535)), PC_THREADS, 0, st>>>(
-        c, static_cast<Out*>(k), static_cast<Out*>(v), B, tokens);
+  auto go = [&](auto lanes_c, auto vec_c) {
+    constexpr int LANES = decltype(lanes_c)::value;
+    constexpr bool VEC = decltype(vec_c)::value;
+    pc_grid(static_cast<int64_t>(tokens) * c.groups, B, LANES, [&](int per, dim3 grid) {
+      auto kernel = per == 1 ? paged_read_kernel<Cache, Out, LANES, VEC, 1> : per == 2 ? paged_read_kernel<Cache, Out, LANES, VEC, 2> : paged_read_kernel<Cache, Out, LANES, VEC, 4>;
+      kernel<<<grid, PC_THREADS, 0, st>>>(c, static_cast<Out*>(k), static_cast<Out*>(v), B, tokens);
+    });
   };
-  if (!vec) go(paged_read_kernel<Cache, Out, 32, false>, 32);
-  else if (c.dim <= 64) go(paged_read_kernel<Cache, Out, 8, true>, 8);
-  else if (c.dim <= 128) go(paged_read_kernel<Cache, Out, 16, true>, 16);
-  else go(paged_read_kernel<Cache, Out, 32, true>, 32);
+  pc_lanes(c.dim, vec, go);
   return static_cast<int>(cudaGetLastError());
 }
 
