@@ -46,6 +46,11 @@ class DiffAttention(nn.Module):
             nn.init.normal_(getattr(self, n), mean=0.0, std=0.1)
         self.subln.reset_parameters()
 
+    def lam(self, dtype: torch.dtype) -> torch.Tensor:
+        lam1 = torch.exp(torch.sum(self.lambda_q1 * self.lambda_k1, dim=-1).float()).to(dtype)
+        lam2 = torch.exp(torch.sum(self.lambda_q2 * self.lambda_k2, dim=-1).float()).to(dtype)
+        return lam1 - lam2 + self.lambda_init
+
     def forward(self, q, k, v, cu_seqlens=None):
         # heads are interleaved pairs: (H two) → two groups of H/2 heads
         B, T, H, D = q.shape
@@ -64,10 +69,7 @@ class DiffAttention(nn.Module):
         o = ops.attention(qs, ks, vs, **kw).view(B, T, 4, H // 2, D)
         a1 = torch.cat((o[:, :, 0], o[:, :, 1]), dim=-1)
         a2 = torch.cat((o[:, :, 2], o[:, :, 3]), dim=-1)
-        lam1 = torch.exp(torch.sum(self.lambda_q1 * self.lambda_k1, dim=-1).float()).type_as(q)
-        lam2 = torch.exp(torch.sum(self.lambda_q2 * self.lambda_k2, dim=-1).float()).type_as(q)
-        lam = lam1 - lam2 + self.lambda_init
-        a = ops.diff_combine(a1, a2, lam, self.subln.weight, 1 - self.lambda_init, 1e-5)
+        a = ops.diff_combine(a1, a2, self.lam(q.dtype), self.subln.weight, 1 - self.lambda_init, 1e-5)
         # (B,T,H/2,2D) → (B,T,H,D)
         return a.reshape(B, T, H // 2, 2, D).reshape(B, T, H, D)
 
@@ -150,7 +152,7 @@ class CausalSelfAttention(nn.Module):
             nn.init.zeros_(self.softmax_offset)
 
     # -- rope for ada_rope layers --------------------------------------------------
-    def _ada_rope(self, x: torch.Tensor, T: int):
+    def _ada_rope(self, x: torch.Tensor, start: int, T: int):
         cfg = self.config
         if cfg.yoco_window and cfg.local_window == cfg.block_size // 2:
             initial_window, sf = 4096, cfg.scaling_factor
@@ -162,9 +164,25 @@ class CausalSelfAttention(nn.Module):
                                                    torch.bfloat16, x.device, base=0.09 * initial_window ** 1.628,
                                                    scaling_factor=sf)
         cos, sin = self.rope_cache
-        return cos[:T], sin[:T]
+        return cos[start:T], sin[start:T]
 
-    def _attend(self, q, k, v, cu_seqlens):
+    def _window(self):
+        win = self.win_tuple
+        if self.config.full_swa_extend and win == (-1, -1) and not self.training:
+            win = (self.config.block_size - 1, 0)
+        return win
+
+    def _attend_cached(self, q, cache):
+        """The new tokens over everything the cache holds (:mod:`archscale_b200.models.decode`)."""
+        self.z_mean = None
+        if self.use_da:
+            da = self.da
+            return cache.attend_diff(q, da.softmax_scale, da.window_size, da.lam(q.dtype), da.subln.weight, 1 - da.lambda_init, 1e-5)
+        return cache.attend(q, self.scale, self._window(), self.softmax_offset if self.config.sink_attn else None)
+
+    def _attend(self, q, k, v, cu_seqlens, cache=None):
+        if cache is not None and not cache.filling:
+            return self._attend_cached(q, cache)
         if not self.config.fa2:
             # the reference's non-flash path: sqrt of the softmax weights over silu(v), no window / packing (`:426-441`)
             self.z_mean = None
@@ -176,9 +194,7 @@ class CausalSelfAttention(nn.Module):
         if self.use_da:
             self.z_mean = None
             return self.da(q, k, v, cu_seqlens=cu_seqlens)
-        win = self.win_tuple
-        if self.config.full_swa_extend and win == (-1, -1) and not self.training:
-            win = (self.config.block_size - 1, 0)
+        win = self._window()
         sink = self.softmax_offset if self.config.sink_attn else None
         want_lse = self.collect_stats
         out = ops.attention(q, k, v, scale=self.scale, window=win, cu_seqlens=cu_seqlens, sink=sink,
@@ -193,12 +209,13 @@ class CausalSelfAttention(nn.Module):
     collect_stats: bool = False
 
     def forward(self, x: torch.Tensor, rope, max_seq_length: int, cu_seqlens: Optional[torch.Tensor] = None,
-                input_pos=None, kv_cache=None, gmu_mems=None):
+                input_pos=None, kv_cache=None, gmu_mems=None, cache=None):
         B, T, C = x.shape
         cfg = self.config
         if cfg.ada_rope:
             assert cfg.local_window > 0
-            rope = self._ada_rope(x, T)
+            start = cache.tokens if cache is not None else 0
+            rope = self._ada_rope(x, start, start + T)
         H, G, hs = self.n_head, self.n_query_groups, self.head_size
         g = None
         if self.yoco_cross:
@@ -216,7 +233,7 @@ class CausalSelfAttention(nn.Module):
                 cos, sin = rope
                 q = ops.apply_rotary_emb(q, cos, sin)
             k, v = kv_cache
-            y = self._attend(q, k, v, cu_seqlens)
+            y = self._attend(q, k, v, cu_seqlens, cache)
             if cfg.gated_attn:
                 y = ops.glu(g, y)
             return self.proj(y.reshape(B, T, -1)), kv_cache, gmu_mems
@@ -266,7 +283,9 @@ class CausalSelfAttention(nn.Module):
             q, k = ops.qk_norm_rope(q, k, self.q_norm.weight if self.qk_norm else None,
                                     self.k_norm.weight if self.qk_norm else None, cos, sin, cfg.norm_eps)
         kv_cache = (k, v)
-        y = self._attend(q, k, v, cu_seqlens)
+        if cache is not None:
+            cache.write(k, v)
+        y = self._attend(q, k, v, cu_seqlens, cache)
         if cfg.gated_attn:
             y = ops.glu(g, y)
         y = y.reshape(B, T, -1)

@@ -287,6 +287,7 @@ class Block(nn.Module):
         cu_seqlens = seq_meta.get("cu_seqlens") if seq_meta else None
         seq_idx = seq_meta.get("seq_idx") if seq_meta else None
         pad_mask = seq_meta.get("pad_mask") if seq_meta else None
+        cache = seq_meta.get("cache") if seq_meta else None
         stream = self._stream_dtype(compute_dtype)
         x, n_1 = ops.add_rms_norm(x, h_pending, self.norm_1.weight, self.norm_1.eps, scale, compute_dtype, stream)
         new_kv_cache = kv_cache
@@ -300,7 +301,7 @@ class Block(nn.Module):
         elif self.use_gmu:
             h, gmu_mems = self.attn(n_1, gmu_mems)
         else:
-            h, new_kv_cache, gmu_mems = self.attn(n_1, rope, max_seq_length, cu_seqlens, None, kv_cache, gmu_mems)
+            h, new_kv_cache, gmu_mems = self.attn(n_1, rope, max_seq_length, cu_seqlens, None, kv_cache, gmu_mems, cache)
         if self.collect_stats:
             with torch.no_grad():
                 self.attn_output_rmsnorm = compute_rmsnorm(h) * scale
@@ -332,6 +333,7 @@ class Block(nn.Module):
         cu_seqlens = seq_meta.get("cu_seqlens") if seq_meta else None
         seq_idx = seq_meta.get("seq_idx") if seq_meta else None
         pad_mask = seq_meta.get("pad_mask") if seq_meta else None
+        cache = seq_meta.get("cache") if seq_meta else None
         if hasattr(self, "layer_configurator"):
             lc = self.layer_configurator
         ox_src = x
@@ -356,7 +358,7 @@ class Block(nn.Module):
         elif self.use_gmu:
             h, gmu_mems = self.attn(n_1, gmu_mems)
         else:
-            h, new_kv_cache, gmu_mems = self.attn(n_1, rope, max_seq_length, cu_seqlens, input_pos, kv_cache, gmu_mems)
+            h, new_kv_cache, gmu_mems = self.attn(n_1, rope, max_seq_length, cu_seqlens, input_pos, kv_cache, gmu_mems, cache)
         x, h, input_embed = self.post_process_residual(h, ox, lc, input_embed, residual_dropout)
         if self.collect_stats:
             with torch.no_grad():
@@ -518,18 +520,23 @@ class GPT(nn.Module):
     # -- forward -------------------------------------------------------------------------
     def forward(self, idx: torch.Tensor, max_seq_length: Optional[int] = None,
                 attn_mask: Optional[torch.Tensor] = None, residual_dropout: float = 0.0,
-                use_flce_loss: bool = False) -> CausalLMOutput:
+                use_flce_loss: bool = False, cache=None) -> CausalLMOutput:
+        """``cache``: a :class:`archscale_b200.models.decode.DecodeCache`, to which the tokens are appended and over which they are computed."""
         cfg = self.config
         B, T = idx.shape
         seq_meta = self._seq_meta(idx, attn_mask)
+        start = 0
+        if cache is not None:
+            start = cache.begin(idx)
+            seq_meta = dict(seq_meta or {}, cache=cache)
         if max_seq_length is None:
             max_seq_length = cfg.block_size
         rope = None
         if not (cfg.nope or cfg.ada_rope):
-            if self.rope_cache is None or T > self.max_len or self.rope_cache[0].device != idx.device:
-                self.max_len = max(T, self.max_len)
+            if self.rope_cache is None or start + T > self.max_len or self.rope_cache[0].device != idx.device:
+                self.max_len = max(start + T, self.max_len)
                 self.rope_cache = self.build_rope_cache(idx, self.max_len)
-            rope = (self.rope_cache[0][:T], self.rope_cache[1][:T])
+            rope = (self.rope_cache[0][start:start + T], self.rope_cache[1][start:start + T])
         x = self.transformer.wte(idx)
         if self.scale_embed:
             x = x * math.sqrt(cfg.n_embd)
@@ -586,6 +593,8 @@ class GPT(nn.Module):
         else:
             for block in self.transformer.h:
                 run(block)
+        if cache is not None:
+            cache.end(T)
         if cfg.sum_skip:
             x = input_embed
         if use_deferred:

@@ -384,7 +384,7 @@ def check_diff(q, cache, table, lengths, new, window, lam, w, scale=None, c=0.4,
     L = max([0, *lengths.tolist()])
     # a1 − λ a2 is off by a; its root mean square by no more, so that y is off by (a / rms) (1 + |y| / (w c)), and |y| ≤ w c √(2 D)
     a = attn_bound(q, cache, spread, L) * (1 + abs(float(lam))) * visible_top(cache, table, lengths)
-    gain = float(w.float().abs().max()) * c
+    gain = float(w.float().abs().max()) * abs(c)
     size = want.abs()
     tol = half_step(q.dtype) * size + (a / low if math.isfinite(low) else 0) * (gain + size) * 1.1 + 2.0 ** -20 * size
     err = (out.double().cpu() - want).abs()
