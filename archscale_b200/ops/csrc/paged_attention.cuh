@@ -83,6 +83,12 @@ constexpr int pa_resident() {
   return fit < regs ? fit : regs;
 }
 
+// Shares of `all` chunks: CTA c has those from pa_first(c) to pa_first(c + 1), one more or less than any other; pa_owner is the CTA of a chunk.
+__device__ __forceinline__ uint32_t pa_first(uint32_t c, uint32_t all, uint32_t ctas) { return static_cast<uint32_t>(static_cast<uint64_t>(c) * all / ctas); }
+__device__ __forceinline__ uint32_t pa_owner(uint32_t chunk, uint32_t all, uint32_t ctas) {
+  return static_cast<uint32_t>((static_cast<uint64_t>(chunk + 1) * ctas - 1) / all);
+}
+
 __device__ __forceinline__ float pa_ex2(float x) {
   float y;
   asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -246,8 +252,9 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
   if (blockIdx.x == 0 && p.prefix != nullptr)
     for (int i = threadIdx.x; i <= entries; i += S::WARPS * 32) p.prefix[i] = s_prefix[i];
 
-  const uint32_t all = static_cast<uint32_t>(s_prefix[entries]) * p.heads, share = (all + p.ncta - 1) / p.ncta;
-  const uint32_t end = min(all, (blockIdx.x + 1) * share);
+  const uint32_t all = static_cast<uint32_t>(s_prefix[entries]) * p.heads, ctas = min(all, static_cast<uint32_t>(p.ncta));
+  if (blockIdx.x >= ctas) return;
+  const uint32_t begin = pa_first(blockIdx.x, all, ctas), end = pa_first(blockIdx.x + 1, all, ctas);
   uint8_t* const ring = smem + warp * S::STAGES * S::STAGE;                     // stages start at multiples of 512 bytes, so that addresses in a row are XORs
   uint8_t* const extra = smem + S::WARPS * S::STAGES * S::STAGE + warp * S::STAGES * S::EXTRA;
   const uint32_t ring_u = smem_u32(ring);
@@ -257,7 +264,7 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
   constexpr uint32_t FULL = TS == 32 ? 0xffffffffu : (1u << (TS & 31)) - 1u;
 
 #pragma unroll 1
-  for (uint32_t at = blockIdx.x * share; at < end;) {
+  for (uint32_t at = begin; at < end;) {
     // ---- the item
     int e = 0;
     for (int hi = entries; hi - e > 1;) { const int mid = (e + hi) >> 1; if (static_cast<uint32_t>(s_prefix[mid]) * p.heads <= at) e = mid; else hi = mid; }
@@ -773,9 +780,9 @@ __global__ void __launch_bounds__(512 / (WPR == 1 ? 2 : 1)) paged_join_kernel(co
   if (row0 + r >= p.rows) return;
   const int entries = p.nb * p.nrt;
   const uint32_t before = p.prefix[e], chunks = p.prefix[e + 1] - before;
-  const uint32_t all = static_cast<uint32_t>(p.prefix[entries]) * p.heads, share = (all + p.ncta - 1) / p.ncta;
+  const uint32_t all = static_cast<uint32_t>(p.prefix[entries]) * p.heads, ctas = min(all, static_cast<uint32_t>(p.ncta));
   const uint32_t from = before * p.heads + head * chunks;
-  const int first = from / share, last = (from + chunks - 1) / share;
+  const int first = pa_owner(from, all, ctas), last = pa_owner(from + chunks - 1, all, ctas);
   if (first == last) return;                                                    // one CTA had it all
   const int n = last - first + 1;
   float m[2], l[2], mv[2][2], v[2][N];
