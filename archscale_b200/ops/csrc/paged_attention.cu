@@ -29,6 +29,8 @@ static PaPlan pa_plan(const PagedView& c, const b200_paged_query& a) {
   p.ks_page = static_cast<uint32_t>(c.ks_page); p.ks_slot = static_cast<uint32_t>(c.ks_slot);
   p.vs_page = static_cast<uint32_t>(c.vs_page); p.vs_slot = static_cast<uint32_t>(c.vs_slot);
   s.gen = far > 0xffffffffLL || far_s > 0xffffffffLL || p.piece != 16 || D != (a.diff ? s.dt / 2 : s.dt);
+  p.same_scales = p.ks_page == p.vs_page && p.ks_slot == p.vs_slot;
+  p.q_wide = reinterpret_cast<uintptr_t>(a.q) % 8 == 0 && (a.q_batch | a.q_token | a.q_head) % 4 == 0;
   p.q_words = reinterpret_cast<uintptr_t>(a.q) % 4 == 0 && (a.q_batch | a.q_token | a.q_head) % 2 == 0;
   const int qrows = (a.diff ? 4 : 8) * s.nc;
   const int64_t room = static_cast<int64_t>(c.table_cols) * c.page_size, seen = a.window >= 0 ? static_cast<int64_t>(a.window) + qrows + 1 : room;

@@ -44,6 +44,7 @@ struct PaArgs {
   int64_t page_b, group_b, slot_b;         // strides in bytes, of keys as of values
   uint32_t page_16, slot_16;               // the same in units of 16 bytes (not GEN)
   uint32_t ks_page, ks_slot, vs_page, vs_slot;      // strides of the scales (not GEN)
+  int same_scales, q_wide;                 // those of keys as of values; queries start on 8-byte boundaries
   int page_shift;                          // log2 of the page size, or -1
   float* parts;                            // [ncta][2] parts of items
   int* prefix;                             // chunks before each entry, from CTA 0
@@ -183,11 +184,9 @@ __device__ __forceinline__ void pa_ldsm(uint32_t (&r)[4], uint32_t addr) {
   else
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-// two e4m3 values as fp16
-__device__ __forceinline__ uint32_t pa_half2(uint32_t two) {
-  uint32_t h;
-  asm("{ .reg .b16 lo; cvt.u16.u32 lo, %1; cvt.rn.f16x2.e4m3x2 %0, lo; }" : "=r"(h) : "r"(two));
-  return h;
+// four e4m3 values as fp16: the lower two, the upper two
+__device__ __forceinline__ void pa_halves(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{ .reg .b16 x, y; mov.b32 {x, y}, %2; cvt.rn.f16x2.e4m3x2 %0, x; cvt.rn.f16x2.e4m3x2 %1, y; }" : "=r"(lo), "=r"(hi) : "r"(four));
 }
 // x, y in 16 bits, and what that leaves
 template <int ES>
@@ -286,7 +285,7 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
     for (int c = 0; c < NC; ++c) {
       int row, branch;
       column(c * 8 + gq, row, branch);
-      const int t = row / p.per, h = PAIRS ? 2 * (head * p.per + row % p.per) + branch : head * p.per + row % p.per;
+      const int t = p.a.T == 1 ? 0 : row / p.per, in_group = head * p.per + row - t * p.per, h = PAIRS ? 2 * in_group + branch : in_group;
       const bool there = row < p.rows && t <= sp.t1;
       const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.a.q) + b * p.a.q_batch + t * p.a.q_token + h * p.a.q_head;
       auto two = [&](int ks, int w) -> uint32_t {                               // values d, d + 1 (d even; so is D)
@@ -296,10 +295,23 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
         if (p.q_words) return *reinterpret_cast<const uint32_t*>(src + d);
         return static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(src + d)) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(src + d + 1)) << 16;
       };
+      if (!GEN && p.q_wide) {                                                   // whole rows: no checks, and 8 bytes at a time where values are neighbours
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+        for (int ks = 0; ks < KS; ++ks) {
+          uint2 u = make_uint2(0u, 0u);
+          if (there && (!PAIRS || (ks >= KS / 2) == (branch == 1))) {
+            const __nv_bfloat16* const at_ks = src + 16 * ks - (PAIRS ? branch * (DT / 2) : 0);
+            if constexpr (E8) u = *reinterpret_cast<const uint2*>(at_ks + 4 * cq);
+            else u = make_uint2(*reinterpret_cast<const uint32_t*>(at_ks + 2 * cq), *reinterpret_cast<const uint32_t*>(at_ks + 2 * cq + 8));
+          }
+          qb[c][ks][0] = u.x; qb[c][ks][1] = u.y;
+        }
+      } else {
 #pragma unroll
-        for (int w = 0; w < 2; ++w) qb[c][ks][w] = two(ks, w);
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) qb[c][ks][w] = two(ks, w);
+      }
     }
 
     // ---- loads: lane i < TS knows token i of a step
@@ -313,21 +325,19 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
     const uint8_t* const ks = E8 ? p.c.ks + static_cast<int>(head) * HEADS * p.c.ks_group : nullptr;
     const uint8_t* const vs = E8 ? p.c.vs + static_cast<int>(head) * HEADS * p.c.vs_group : nullptr;
     auto page_of = [&](int j) { return p.page_shift >= 0 ? j >> p.page_shift : j / p.c.page_size; };
-    auto look = [&](int step) {                                                 // page of this lane's token, or -1
-      const int64_t j = static_cast<int64_t>(j_base) + static_cast<int64_t>(step) * S::CHUNK + lane;
-      if (step >= steps || lane >= TS || j >= sp.hi) return -1;
-      return table[page_of(static_cast<int>(j))];                               // hi is within the table
-    };
+    // this lane's token of a step, and how many steps have one: hi is within the table, and a step of the item begins before hi
+    const int j_lane = j_base + lane, mine_of = lane < TS && j_lane < sp.hi ? min(steps, (sp.hi - j_lane + S::CHUNK - 1) / S::CHUNK) : 0;
+    auto look = [&](int step) { return step < mine_of ? table[page_of(j_lane + step * S::CHUNK)] : -1; };      // its page, or -1
     int page_a = look(0), page_b = look(1);
     uint32_t pend_k[HEADS] = {}, pend_v[HEADS] = {};
     auto issue = [&](int step) {
       bool scaled = false;
       int64_t scale_at = 0, scale_at_v = 0;
       if (step < steps) {
-        const int j = j_base + step * S::CHUNK + lane;
+        const int j = j_lane + step * S::CHUNK;
         int page = page_a;
-        if (lane < TS && j < sp.hi && (page < 0 || page >= p.c.pages)) {        // not of this cache
-          if (p.c.status) atomicCAS(p.c.status, 0, STATUS_INDEX_RANGE);
+        if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(p.c.pages)) {  // no token, or not a page of this cache
+          if (step < mine_of && p.c.status) atomicCAS(p.c.status, 0, STATUS_INDEX_RANGE);
           page = -1;
         }
         page_a = page_b;
@@ -336,7 +346,7 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
         if (E8 && page >= 0) {
           scaled = true;
           if constexpr (GEN) { scale_at = page * p.c.ks_page + slot * p.c.ks_slot; scale_at_v = page * p.c.vs_page + slot * p.c.vs_slot; }
-          else { scale_at = page * p.ks_page + slot * p.ks_slot; scale_at_v = page * p.vs_page + slot * p.vs_slot; }
+          else { scale_at = page * p.ks_page + slot * p.ks_slot; scale_at_v = p.same_scales ? scale_at : page * p.vs_page + slot * p.vs_slot; }
         }
         const uint32_t live = __ballot_sync(0xffffffffu, page >= 0);
         const uint32_t st = ring_u + (step % S::STAGES) * S::STAGE;
@@ -390,16 +400,15 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
           float* const to = reinterpret_cast<float*>(extra + ((step - 1) % S::STAGES) * S::EXTRA);
 #pragma unroll
           for (int h = 0; h < HEADS; ++h) {
-            to[h * TS + lane] = paged_pow2(pend_k[h]);
-            to[(HEADS + h) * TS + lane] = pend_v[h] == 255u ? __int_as_float(0x7fffffff) : static_cast<float>(static_cast<int>(pend_v[h]) - 127);
+            // 2^(byte − 127), and byte − 127 by the fraction of 2^23 + byte; 255 is NaN in both
+            to[h * TS + lane] = __uint_as_float(max(pend_k[h] << 23 | (pend_k[h] + 1) >> 8, 0x400000u));
+            to[(HEADS + h) * TS + lane] = pend_v[h] == 255u ? __int_as_float(0x7fffffff) : __uint_as_float(0x4b000000u | pend_v[h]) - 8388735.f;
           }
         }
-        if (scaled) {
 #pragma unroll
-          for (int h = 0; h < HEADS; ++h) {
-            pend_k[h] = ks[scale_at + h * p.c.ks_group];
-            pend_v[h] = vs[scale_at_v + h * p.c.vs_group];
-          }
+        for (int h = 0; h < HEADS; ++h) {
+          pend_k[h] = pend_v[h] = 127u;                                         // tokens that are not there: finite, whatever lies there
+          if (scaled) { pend_k[h] = ks[scale_at + h * p.c.ks_group]; pend_v[h] = vs[scale_at_v + h * p.c.vs_group]; }
         }
       }
     };
@@ -438,7 +447,7 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
       for (int k = 0; k < 2; ++k) {
         int row, branch;
         column(c * 8 + 2 * cq + k, row, branch);
-        const int t = row / p.per;
+        const int t = p.a.T == 1 ? 0 : row / p.per;
         const int64_t pos = sp.pos0 + t;
         kmax[c][k] = row < p.rows && t <= sp.t1 ? static_cast<int>(max(int64_t(-1), min(pos, int64_t(0x7fffffff)))) : -1;
         kmin[c][k] = p.a.window >= 0 ? static_cast<int>(max(int64_t(0), pos - p.a.window)) : 0;
@@ -487,7 +496,9 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
             if constexpr (E8) {                                                 // 16 bytes are a whole step of the product; q is laid out alike
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                const uint32_t a0 = pa_half2(r[2 * h]), a1 = pa_half2(r[2 * h + 1]), a2 = pa_half2(r[2 * h] >> 16), a3 = pa_half2(r[2 * h + 1] >> 16);
+                uint32_t a0, a1, a2, a3;
+                pa_halves(r[2 * h], a0, a2);
+                pa_halves(r[2 * h + 1], a1, a3);
 #pragma unroll
                 for (int c = 0; c < NC; ++c) pa_mma<ES>(x[c][mt], a0, a1, a2, a3, qb[c][2 * ks + h][0], qb[c][2 * ks + h][1]);
               }
@@ -576,6 +587,16 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
               for (int k = 0; k < 4; ++k) acc[c][i][k] *= f[k & 1][i >= KS / 2];
           }
         }
+        bool unscaled = false;                                                  // a token that some rows may not see has no scale: −∞ + NaN is not −∞
+        if (E8 && masked) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int g = 0; g < NG; ++g) unscaled = unscaled || ev[g][mt][h] != ev[g][mt][h];
+          unscaled = __any_sync(0xffffffffu, unscaled);
+        }
         // ---- weights, turned into right operands: 16 tokens at a time
         uint32_t hi[NC][NGX][MT][2], lo[E8 ? 1 : NC][E8 ? 1 : MT][2];
 #pragma unroll
@@ -597,8 +618,9 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                   const float e = ev[g][mt][h];
-                  hi[c][g][mt][h] = pa_turn(pa_pack<1>(masked && y0 == -INFINITY ? 0.f : pa_ex2(y0 + e + bv[0][g]),
-                                                       masked && y1 == -INFINITY ? 0.f : pa_ex2(y1 + e + bv[1][g])));
+                  float w2 = pa_ex2(y0 + e + bv[0][g]), w3 = pa_ex2(y1 + e + bv[1][g]);
+                  if (unscaled) { w2 = y0 == -INFINITY ? 0.f : w2; w3 = y1 == -INFINITY ? 0.f : w3; }
+                  hi[c][g][mt][h] = pa_turn(pa_pack<1>(w2, w3));
                 }
               } else {
                 const uint32_t u = pa_pack<2>(w0, w1);
@@ -632,8 +654,8 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
             pa_ldsm<true>(r, (vt_u ^ (i << 5)) + mt * 16 * S::ROW);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t u = __byte_perm(r[2 * h], 0, 0x3120), w = __byte_perm(r[2 * h + 1], 0, 0x3120);
-              a[h][0] = pa_half2(u); a[h][1] = pa_half2(u >> 16); a[h][2] = pa_half2(w); a[h][3] = pa_half2(w >> 16);
+              pa_halves(__byte_perm(r[2 * h], 0, 0x3120), a[h][0], a[h][1]);
+              pa_halves(__byte_perm(r[2 * h + 1], 0, 0x3120), a[h][2], a[h][3]);
             }
           } else {
             pa_ldsm<true>(r, (vt_u ^ (i << 5)) + mt * 16 * S::ROW);
