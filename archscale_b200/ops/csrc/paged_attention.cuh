@@ -26,6 +26,7 @@
 // do not depend on scheduling), which the first one starts early and which needs no counters, so that nothing has to be zero beforehand.
 #pragma once
 #include <cuda_fp16.h>
+#include <atomic>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -66,10 +67,10 @@ struct PaShape {
   static constexpr int QROWS = PAIRS ? 4 * NC : 8 * NC;                        // query rows of a tile
   static constexpr int LD = DT + 4;                                            // floats between rows in shared memory: no bank twice
   static constexpr int SLABS = WARPS * COLS * LD * 4;
-  static constexpr int SMEM = RING > SLABS ? RING : SLABS;
   static constexpr int CHUNK = WARPS * TS;
   static constexpr int NG = ES == 1 ? HEADS : 0;                               // groups of values with maxima of their own
   static constexpr int PART = COLS * (DT + 4);                                 // floats of a part: sums, then m, l, m' of each column
+  static constexpr int SMEM = RING > SLABS + PART * 4 ? RING : SLABS + PART * 4;
   static_assert(SMEM <= 227 * 1024 - 6144, "shared memory");
 };
 // column of a tile's query row r, in branch 0 or 1
@@ -211,8 +212,20 @@ __device__ __forceinline__ constexpr uint32_t pa_swizzle(int t) { return (ROW >=
 template <int ROW>
 __device__ __forceinline__ uint32_t pa_at(int t, int chunk) { return t * ROW + ((chunk << 4) ^ pa_swizzle<ROW>(t)); }
 
-// GEN: rows that are not whole 16-byte pieces, or shorter than DT
-template <int ES, int DT, bool PAIRS, int NC, bool GEN>
+// the CTAs of a cluster, all threads
+__device__ __forceinline__ void pa_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// a float at the place of `p` in the shared memory of the cluster's CTA `rank`
+__device__ __forceinline__ float pa_remote(const float* p, int rank) {
+  float x;
+  asm volatile("{ .reg .b32 a; mapa.shared::cluster.u32 a, %1, %2; ld.shared::cluster.f32 %0, [a]; }" : "=f"(x) : "r"(smem_u32(p)), "r"(rank) : "memory");
+  return x;
+}
+
+// GEN: rows that are not whole 16-byte pieces, or shorter than DT.  CLUSTER: an item is eight CTAs, which share its keys evenly and join their parts
+// through each other's shared memory, each the rows of its rank
+template <int ES, int DT, bool PAIRS, int NC, bool GEN, bool CLUSTER>
 __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_resident<ES, DT, PAIRS, NC>()) paged_attention_kernel(const PaArgs p) {
   using S = PaShape<ES, DT, PAIRS, NC>;
   constexpr bool E8 = ES == 1;
@@ -222,11 +235,11 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
   __shared__ int s_scan[S::WARPS];
   __shared__ float s_stat[S::WARPS][4][16];                                     // m, l, m' of both groups
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, cq = lane & 3;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if constexpr (!CLUSTER) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- chunks before every entry
   const int entries = p.nb * p.nrt;
-  {
+  if constexpr (!CLUSTER) {
     const int each = (entries + S::WARPS * 32 - 1) / (S::WARPS * 32), from = threadIdx.x * each;
     int sum = 0;
     for (int i = from; i < min(from + each, entries); ++i) {
@@ -248,12 +261,15 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
   if (GEN)                                                                      // columns past D stay zero
     for (int i = threadIdx.x; i < S::RING / 16; i += S::WARPS * 32) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
-  if (blockIdx.x == 0 && p.prefix != nullptr)
+  if (!CLUSTER && blockIdx.x == 0 && p.prefix != nullptr)
     for (int i = threadIdx.x; i <= entries; i += S::WARPS * 32) p.prefix[i] = s_prefix[i];
 
-  const uint32_t all = static_cast<uint32_t>(s_prefix[entries]) * p.heads, ctas = min(all, static_cast<uint32_t>(p.ncta));
-  if (blockIdx.x >= ctas) return;
-  const uint32_t begin = pa_first(blockIdx.x, all, ctas), end = pa_first(blockIdx.x + 1, all, ctas);
+  uint32_t begin = 0, end = 1;
+  if constexpr (!CLUSTER) {
+    const uint32_t all = static_cast<uint32_t>(s_prefix[entries]) * p.heads, ctas = min(all, static_cast<uint32_t>(p.ncta));
+    if (blockIdx.x >= ctas) return;
+    begin = pa_first(blockIdx.x, all, ctas); end = pa_first(blockIdx.x + 1, all, ctas);
+  }
   uint8_t* const ring = smem + warp * S::STAGES * S::STAGE;                     // stages start at multiples of 512 bytes, so that addresses in a row are XORs
   uint8_t* const extra = smem + S::WARPS * S::STAGES * S::STAGE + warp * S::STAGES * S::EXTRA;
   const uint32_t ring_u = smem_u32(ring);
@@ -266,11 +282,21 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
   for (uint32_t at = begin; at < end;) {
     // ---- the item
     int e = 0;
-    for (int hi = entries; hi - e > 1;) { const int mid = (e + hi) >> 1; if (static_cast<uint32_t>(s_prefix[mid]) * p.heads <= at) e = mid; else hi = mid; }
-    const uint32_t chunks = s_prefix[e + 1] - s_prefix[e], off = at - static_cast<uint32_t>(s_prefix[e]) * p.heads;
-    const uint32_t head = off / chunks, c0 = off - head * chunks, c1 = min(chunks, c0 + end - at);
+    uint32_t chunks = 0, head = 0, c0 = 0, c1 = 0;
+    if constexpr (CLUSTER) {
+      e = blockIdx.x / 8 / p.heads; head = blockIdx.x / 8 % p.heads;
+    } else {
+      for (int hi = entries; hi - e > 1;) { const int mid = (e + hi) >> 1; if (static_cast<uint32_t>(s_prefix[mid]) * p.heads <= at) e = mid; else hi = mid; }
+      chunks = s_prefix[e + 1] - s_prefix[e];
+      const uint32_t off = at - static_cast<uint32_t>(s_prefix[e]) * p.heads;
+      head = off / chunks; c0 = off - head * chunks; c1 = min(chunks, c0 + end - at);
+    }
     const int b = p.b0 + e / p.nrt, row0 = (p.rt0 + e % p.nrt) * S::QROWS;
     const PaSpan sp = pa_span<S::QROWS>(p, e);
+    if constexpr (CLUSTER) {
+      chunks = (sp.hi - sp.lo + S::CHUNK - 1) / S::CHUNK;
+      c0 = blockIdx.x % 8 * chunks / 8; c1 = (blockIdx.x % 8 + 1) * chunks / 8;
+    }
     const int j_base = sp.lo + c0 * S::CHUNK + warp * TS;                       // first token of this warp's step 0
     const int steps = static_cast<int>(c1 - c0);
 
@@ -738,8 +764,8 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
         }
       }
     __syncthreads();
-    const bool whole = c0 == 0 && c1 == chunks;
-    float* const part = whole ? nullptr : p.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (c0 == 0)) * S::PART;
+    const bool whole = !CLUSTER && c0 == 0 && c1 == chunks;
+    float* const part = CLUSTER ? reinterpret_cast<float*>(smem + S::SLABS) : whole ? nullptr : p.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (c0 == 0)) * S::PART;
     for (int r = warp; r < S::QROWS; r += S::WARPS) {
       float v[2][DT / 32], mm[2], ll[2], mmv[2][2];
 #pragma unroll
@@ -771,6 +797,39 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
       }
       if (whole && row0 + r < p.rows)
         pa_finish<ES, DT, PAIRS>(p, b, head, row0 + r, (row0 + r) / p.per <= sp.t1, v[0], v[1], mm, ll, mmv, lane);
+    }
+    if constexpr (CLUSTER) {
+      pa_cluster_sync();                                                        // every CTA's part is in its shared memory
+      for (int r = blockIdx.x % 8 + 8 * warp; r < S::QROWS && row0 + r < p.rows; r += 8 * S::WARPS) {
+        float v[2][DT / 32], mm[2], ll[2], mmv[2][2];
+#pragma unroll
+        for (int br = 0; br < HEADS; ++br) {
+          const int k = pa_column<PAIRS>(r, br);
+          float st[8][4], x[8][DT / 32];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st[c][i] = i < 2 || E8 ? pa_remote(part + S::COLS * DT + k * 4 + i, c) : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < DT / 32; ++i) x[c][i] = pa_remote(part + k * DT + lane + 32 * i, c);
+          }
+          mm[br] = mmv[br][0] = mmv[br][1] = -INFINITY; ll[br] = 0.f;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) { mm[br] = fmaxf(mm[br], st[c][0]); mmv[br][0] = fmaxf(mmv[br][0], st[c][2]); mmv[br][1] = fmaxf(mmv[br][1], st[c][3]); }
+#pragma unroll
+          for (int i = 0; i < DT / 32; ++i) v[br][i] = 0.f;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const float f = pa_step(st[c][0], mm[br]), f0 = E8 ? pa_step(st[c][2], mmv[br][0]) : f, f1 = NG == 2 ? pa_step(st[c][3], mmv[br][1]) : f0;
+            ll[br] += st[c][1] * f;
+#pragma unroll
+            for (int i = 0; i < DT / 32; ++i) v[br][i] += x[c][i] * (i < DT / 64 ? f0 : f1);
+          }
+        }
+        pa_finish<ES, DT, PAIRS>(p, b, head, row0 + r, (row0 + r) / p.per <= sp.t1, v[0], v[1], mm, ll, mmv, lane);
+      }
+      pa_cluster_sync();                                                        // nobody leaves while another reads
+      return;
     }
     __syncthreads();                                                            // the ring is used again
     if (GEN)                                                                    // and its unused columns are zero again
@@ -873,13 +932,35 @@ __global__ void __launch_bounds__(512 / (WPR == 1 ? 2 : 1)) paged_join_kernel(co
   pa_finish<ES, DT, PAIRS>(p, b, head, row0 + r, (row0 + r) / p.per <= sp.t1, v[0], v[1], m, l, mv, lane);
 }
 
-template <int ES, int DT, bool PAIRS, int NC, bool GEN>
-static int pa_launch(PaArgs& p, int max_chunks, int num_sms, cudaStream_t st) {
+template <int ES, int DT, bool PAIRS, int NC, bool GEN, bool CLUSTER>
+static int pa_main(const PaArgs& p, int ctas, cudaStream_t st) {
   using S = PaShape<ES, DT, PAIRS, NC>;
-  auto kernel = paged_attention_kernel<ES, DT, PAIRS, NC, GEN>;
-  if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); e != cudaSuccess) return static_cast<int>(e);
-  kernel<<<p.ncta, S::WARPS * 32, S::SMEM, st>>>(p);
-  if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return static_cast<int>(e);
+  auto kernel = paged_attention_kernel<ES, DT, PAIRS, NC, GEN, CLUSTER>;
+  static std::atomic<uint64_t> ready{0};                                        // devices (of the first 64) on which the kernel has its shared memory
+  int device = 0;
+  if (const cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return static_cast<int>(e);
+  const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+  if (!(ready.load(std::memory_order_acquire) & bit)) {
+    if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); e != cudaSuccess) return static_cast<int>(e);
+    ready.fetch_or(bit, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(S::WARPS * 32);
+  cfg.dynamicSmemBytes = S::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 8; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CLUSTER ? 1 : 0;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, p));
+}
+template <int ES, int DT, bool PAIRS, int NC, bool GEN>
+static int pa_launch(const PaArgs& p, bool cluster, int num_sms, cudaStream_t st) {
+  using S = PaShape<ES, DT, PAIRS, NC>;
+  if (cluster) return pa_main<ES, DT, PAIRS, NC, GEN, true>(p, p.nb * p.nrt * p.heads * 8, st);
+  if (const int rc = pa_main<ES, DT, PAIRS, NC, GEN, false>(p, p.ncta, st)) return rc;
   if (p.prefix == nullptr) return 0;                                            // items of one chunk each: nothing to join
   cudaLaunchConfig_t cfg = {};
   const int64_t rows = static_cast<int64_t>(p.nb) * p.nrt * p.heads * S::QROWS, room = static_cast<int64_t>(num_sms) * 32;      // warps of the device, with 64 registers
@@ -910,11 +991,17 @@ static int pa_prepare(PaArgs& p, bool gen, int span, int num_sms, void* ws, int6
   const int64_t work = static_cast<int64_t>(p.nb) * p.nrt * p.heads * max_chunks, full = static_cast<int64_t>(num_sms) * pa_resident<ES, DT, PAIRS, NC>();
   const int64_t most = ES == 2 && work >= 48 * full ? 2 * full : full;
   p.ncta = static_cast<int>(work < most ? work : most);
-  const int64_t bytes = max_chunks > 1 ? static_cast<int64_t>(p.ncta) * 2 * S::PART * 4 + (PA_ENTRIES + 4) * 4 : 0;
+  // Few items of a few chunks: clusters of eight CTAs, one launch and no second kernel.  A CTA then has an eighth of an item instead of its share of all
+  // chunks, which may be three (bf16, up to 128 values a row: four and a half) chunks more before it costs what the second kernel does; clusters leave places of an SM unused, hence four fifths.
+  // One sequence of 1000 tokens, 4 key heads of 128: 10.3 -> 8.3 us, 8 of 2500: 17.2 -> 12.3, 8 of 5000 in e4m3: 22.6 -> 16.4; on the other side of the
+  // rule 13 of 2500: 18.4 -> 22.5, one of 5000 in e4m3: 12.3 -> 14.4.
+  const int64_t items = static_cast<int64_t>(p.nb) * p.nrt * p.heads;
+  const bool cluster = max_chunks > 1 && max_chunks <= 64 && 10 * items <= full && max_chunks * (full - 8 * items) <= (ES == 2 && DT <= 128 ? 36 : 24) * full;
+  const int64_t bytes = max_chunks > 1 && !cluster ? static_cast<int64_t>(p.ncta) * 2 * S::PART * 4 + (PA_ENTRIES + 4) * 4 : 0;
   if (need != nullptr) { *need = bytes; return 0; }
   p.parts = static_cast<float*>(ws);
-  p.prefix = max_chunks > 1 ? reinterpret_cast<int*>(p.parts + static_cast<int64_t>(p.ncta) * 2 * S::PART) : nullptr;
-  return gen ? pa_launch<ES, DT, PAIRS, NC, true>(p, max_chunks, num_sms, st) : pa_launch<ES, DT, PAIRS, NC, false>(p, max_chunks, num_sms, st);
+  p.prefix = bytes > 0 ? reinterpret_cast<int*>(p.parts + static_cast<int64_t>(p.ncta) * 2 * S::PART) : nullptr;
+  return gen ? pa_launch<ES, DT, PAIRS, NC, true>(p, cluster, num_sms, st) : pa_launch<ES, DT, PAIRS, NC, false>(p, cluster, num_sms, st);
 }
 template <int ES>
 static int pa_run(PaArgs& p, int dt, bool pairs, int nc, bool gen, int span, int num_sms, void* ws, int64_t* need, cudaStream_t st) {
