@@ -21,6 +21,10 @@ template <class T> struct Eight;         // 8 values as they are loaded, and as 
 template <> struct Eight<__nv_bfloat16> {
   uint4 u;
   __device__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ uint32_t top() const {                                             // of two at a time: magnitudes order as their bits do
+    const uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu), __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
+    return max(m << 16, m & 0xffff0000u);
+  }
   __device__ void get(float (&x)[8]) const {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -36,6 +40,14 @@ template <> struct Eight<__nv_bfloat16> {
 template <> struct Eight<float> {
   float4 u, v;
   __device__ void load(const float* p) { u = *reinterpret_cast<const float4*>(p); v = *reinterpret_cast<const float4*>(p + 4); }
+  __device__ uint32_t top() const {
+    float x[8];
+    get(x);
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    return m;
+  }
   __device__ void get(float (&x)[8]) const { x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w; }
   static __device__ void store(float* p, const float (&x)[8]) {
     *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
@@ -74,6 +86,7 @@ template <class T> struct Share<true, T> {
   Eight<T> e;
   __device__ void load(const T* row, int lane, int D) { if (8 * lane < D) e.load(row + 8 * lane); else e = {}; }
   __device__ void get(float (&x)[8]) const { e.get(x); }
+  __device__ uint32_t top() const { return e.top(); }
   static __device__ void store(T* row, int lane, int D, const float (&x)[8]) { if (8 * lane < D) Eight<T>::store(row + 8 * lane, x); }
 };
 template <class T> struct Share<false, T> {
@@ -86,38 +99,49 @@ template <class T> struct Share<false, T> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = v[i];
   }
+  __device__ uint32_t top() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    return m;
+  }
   static __device__ void store(T* row, int lane, int D, const float (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) if (lane + 32 * i < D) put_value(row + lane + 32 * i, x[i]);
   }
 };
 
-// Scale byte of a row from its values, which become x · 2^−e.  LANES neighbouring lanes hold the row.
+// Scale byte of a row from the bits of a lane's largest magnitude (NaN above all), and the power of two that its values are multiplied with (0: they are
+// zeros).  LANES neighbouring lanes hold the row.
 template <int LANES>
-__device__ __forceinline__ uint32_t to_scale(float (&x)[8]) {
-  uint32_t top = 0;                        // magnitudes order as their bits do, NaN above all
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+__device__ __forceinline__ uint32_t to_scale(uint32_t top, float& up) {
 #pragma unroll
   for (int o = 1; o < LANES; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (top >= 0x7f800000u) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    return 255u;
-  }
-  const int code = max(0, static_cast<int>((top + 0x1fffffu) >> 23) - 8);
-  const float up = __uint_as_float(static_cast<uint32_t>(254 - code) << 23);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] *= up;
-  return code;
+  const uint32_t code = max(0, static_cast<int>((top + 0x1fffffu) >> 23) - 8);
+  up = __uint_as_float((254u - code) << 23);
+  return top >= 0x7f800000u ? 255u : code;
 }
+// token and head of a row, and the steps to this thread's next one
+struct Place {
+  int t, g, dt, dg, groups;
+  __device__ Place(uint32_t row, uint32_t step, int groups_) : groups(groups_) {
+    const uint32_t n = groups_;
+    t = row / n; g = row % n; dt = step / n; dg = step % n;
+  }
+  __device__ void next() {
+    t += dt; g += dg;
+    if (g >= groups) { g -= groups; ++t; }
+  }
+};
+// page of a token's position in its sequence, and slot in the page
+__device__ __forceinline__ int page_index(int pos, int size, int shift) { return shift >= 0 ? pos >> shift : pos / size; }
 
 constexpr int PC_THREADS = 256;
 
 // ROWS: rows (token, head) of a thread, a grid's step apart from each other
 template <class In, class Cache, int LANES, bool VEC, int ROWS>
 __global__ void __launch_bounds__(PC_THREADS) paged_write_kernel(const PagedView c, const In* k, const In* v, int64_t kb, int64_t kt, int64_t kh, int64_t vb,
-                                                                 int64_t vt, int64_t vh, int B, int T) {
+                                                                 int64_t vt, int64_t vh, int B, int T, int shift, bool alike) {
   constexpr bool E8 = sizeof(Cache) == 1;
   constexpr int STEP = PC_THREADS / LANES;
   const int lane = threadIdx.x % LANES;
@@ -127,18 +151,16 @@ __global__ void __launch_bounds__(PC_THREADS) paged_write_kernel(const PagedView
     const int64_t first = static_cast<int64_t>(c.lengths[b]) - n;
     Share<VEC, In> x[ROWS], y[ROWS];
     int page[ROWS], slot[ROWS], g[ROWS];
+    Place at(row0, STEP, c.groups);
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const uint32_t row = row0 + i * STEP;
-      const int t = static_cast<int>(row / static_cast<uint32_t>(c.groups));
-      g[i] = static_cast<int>(row % static_cast<uint32_t>(c.groups));
-      page[i] = -1; slot[i] = 0;
-      if (t < n && first + t >= 0) {
-        const int pos = static_cast<int>(first + t);
-        page[i] = paged_page(c, b, pos / c.page_size);
-        slot[i] = pos % c.page_size;
-        x[i].load(k + b * kb + t * kt + g[i] * kh, lane, c.dim);
-        y[i].load(v + b * vb + t * vt + g[i] * vh, lane, c.dim);
+    for (int i = 0; i < ROWS; ++i, at.next()) {
+      page[i] = -1; slot[i] = 0; g[i] = at.g;
+      if (at.t < n && first + at.t >= 0) {
+        const int pos = static_cast<int>(first + at.t), index = page_index(pos, c.page_size, shift);
+        page[i] = paged_page(c, b, index);
+        slot[i] = pos - index * c.page_size;
+        x[i].load(k + b * kb + at.t * kt + at.g * kh, lane, c.dim);
+        y[i].load(v + b * vb + at.t * vt + at.g * vh, lane, c.dim);
       } else x[i] = y[i] = {};
     }
 #pragma unroll
@@ -146,10 +168,16 @@ __global__ void __launch_bounds__(PC_THREADS) paged_write_kernel(const PagedView
       float p[8], q[8];
       x[i].get(p); y[i].get(q);
       uint32_t ex = 0, ey = 0;
-      if constexpr (E8) { ex = to_scale<LANES>(p); ey = to_scale<LANES>(q); }   // all lanes take part in the exchange of maxima
+      if constexpr (E8) {                                                       // all lanes take part in the exchange of maxima
+        float px, py;
+        ex = to_scale<LANES>(x[i].top(), px); ey = to_scale<LANES>(y[i].top(), py);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { p[j] = ex == 255u ? 0.f : p[j] * px; q[j] = ey == 255u ? 0.f : q[j] * py; }
+      }
       if (page[i] < 0) continue;                                                // the same for the lanes of a row
-      Share<VEC, Cache>::store(static_cast<Cache*>(c.k) + page[i] * c.k_page + g[i] * c.k_group + slot[i] * c.k_slot, lane, c.dim, p);
-      Share<VEC, Cache>::store(static_cast<Cache*>(c.v) + page[i] * c.v_page + g[i] * c.v_group + slot[i] * c.v_slot, lane, c.dim, q);
+      const int64_t to = page[i] * c.k_page + g[i] * c.k_group + slot[i] * c.k_slot;
+      Share<VEC, Cache>::store(static_cast<Cache*>(c.k) + to, lane, c.dim, p);
+      Share<VEC, Cache>::store(static_cast<Cache*>(c.v) + (alike ? to : page[i] * c.v_page + g[i] * c.v_group + slot[i] * c.v_slot), lane, c.dim, q);
       if (E8 && lane == 0) {
         c.ks[page[i] * c.ks_page + g[i] * c.ks_group + slot[i] * c.ks_slot] = ex;
         c.vs[page[i] * c.vs_page + g[i] * c.vs_group + slot[i] * c.vs_slot] = ey;
@@ -159,7 +187,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_write_kernel(const PagedView
 }
 
 template <class Cache, class Out, int LANES, bool VEC, int ROWS>
-__global__ void __launch_bounds__(PC_THREADS) paged_read_kernel(const PagedView c, Out* k, Out* v, int B, int tokens) {
+__global__ void __launch_bounds__(PC_THREADS) paged_read_kernel(const PagedView c, Out* k, Out* v, int B, int tokens, int shift, bool alike) {
   constexpr bool E8 = sizeof(Cache) == 1;
   constexpr int STEP = PC_THREADS / LANES;
   const int lane = threadIdx.x % LANES;
@@ -168,43 +196,51 @@ __global__ void __launch_bounds__(PC_THREADS) paged_read_kernel(const PagedView 
     const int length = c.lengths[b];
     Share<VEC, Cache> x[ROWS], y[ROWS];
     int page[ROWS], slot[ROWS], g[ROWS];
+    Place at(row0, STEP, c.groups);
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {                                            // all pages, then all rows
-      const uint32_t row = row0 + i * STEP;
-      const int t = static_cast<int>(row / static_cast<uint32_t>(c.groups));
-      g[i] = static_cast<int>(row % static_cast<uint32_t>(c.groups));
-      page[i] = t < tokens && t < length ? paged_page(c, b, t / c.page_size) : -1;
-      slot[i] = t % c.page_size;
+    for (int i = 0; i < ROWS; ++i, at.next()) {                                 // all pages, then all rows
+      const int index = page_index(at.t, c.page_size, shift);
+      g[i] = at.g;
+      page[i] = at.t < tokens && at.t < length ? paged_page(c, b, index) : -1;
+      slot[i] = at.t - index * c.page_size;
     }
     float sx[ROWS], sy[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       sx[i] = sy[i] = 0.f;
       if (page[i] < 0) { x[i] = y[i] = {}; continue; }
-      x[i].load(static_cast<const Cache*>(c.k) + page[i] * c.k_page + g[i] * c.k_group + slot[i] * c.k_slot, lane, c.dim);
-      y[i].load(static_cast<const Cache*>(c.v) + page[i] * c.v_page + g[i] * c.v_group + slot[i] * c.v_slot, lane, c.dim);
+      const int64_t from = page[i] * c.k_page + g[i] * c.k_group + slot[i] * c.k_slot;
+      x[i].load(static_cast<const Cache*>(c.k) + from, lane, c.dim);
+      y[i].load(static_cast<const Cache*>(c.v) + (alike ? from : page[i] * c.v_page + g[i] * c.v_group + slot[i] * c.v_slot), lane, c.dim);
       if constexpr (E8) {
         sx[i] = paged_pow2(c.ks[page[i] * c.ks_page + g[i] * c.ks_group + slot[i] * c.ks_slot]);
         sy[i] = paged_pow2(c.vs[page[i] * c.vs_page + g[i] * c.vs_group + slot[i] * c.vs_slot]);
       }
     }
+    const uint32_t rows = static_cast<uint32_t>(tokens) * c.groups;
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const uint32_t row = row0 + i * STEP;
-      if (row / static_cast<uint32_t>(c.groups) >= static_cast<uint32_t>(tokens)) continue;
+      if (row >= rows) continue;
       float p[8], q[8];
       x[i].get(p); y[i].get(q);
       if constexpr (E8) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) { p[j] *= sx[i]; q[j] *= sy[i]; }
       }
-      const int64_t at = (static_cast<int64_t>(b) * tokens * c.groups + row) * c.dim;
-      Share<VEC, Out>::store(k + at, lane, c.dim, p);
-      Share<VEC, Out>::store(v + at, lane, c.dim, q);
+      const int64_t to = (static_cast<int64_t>(b) * rows + row) * c.dim;
+      Share<VEC, Out>::store(k + to, lane, c.dim, p);
+      Share<VEC, Out>::store(v + to, lane, c.dim, q);
     }
   }
 }
 
+// log2 of the page size, or -1
+static int pc_shift(const PagedView& c) {
+  for (int i = 0; i < 31; ++i) if (c.page_size == 1 << i) return i;
+  return -1;
+}
+static bool pc_alike(const PagedView& c) { return c.k_page == c.v_page && c.k_group == c.v_group && c.k_slot == c.v_slot; }
 static bool whole(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 static int element(int type) { return type == 0 ? 4 : type == 1 ? 2 : 1; }
 static int align8(int type) { return type == 2 ? 8 : 16; }             // bytes of the widest access to 8 values
@@ -237,7 +273,7 @@ static int write_as(const PagedView& c, const void* k, const void* v, int64_t kb
     constexpr bool VEC = decltype(vec_c)::value;
     pc_grid(static_cast<int64_t>(T) * c.groups, B, LANES, [&](int per, dim3 grid) {
       auto kernel = per == 1 ? paged_write_kernel<In, Cache, LANES, VEC, 1> : per == 2 ? paged_write_kernel<In, Cache, LANES, VEC, 2> : paged_write_kernel<In, Cache, LANES, VEC, 4>;
-      kernel<<<grid, PC_THREADS, 0, st>>>(c, static_cast<const In*>(k), static_cast<const In*>(v), kb, kt, kh, vb, vt, vh, B, T);
+      kernel<<<grid, PC_THREADS, 0, st>>>(c, static_cast<const In*>(k), static_cast<const In*>(v), kb, kt, kh, vb, vt, vh, B, T, pc_shift(c), pc_alike(c));
     });
   };
   pc_lanes(c.dim, vec, go);
@@ -251,7 +287,7 @@ static int read_as(const PagedView& c, void* k, void* v, int B, int tokens, bool
     constexpr bool VEC = decltype(vec_c)::value;
     pc_grid(static_cast<int64_t>(tokens) * c.groups, B, LANES, [&](int per, dim3 grid) {
       auto kernel = per == 1 ? paged_read_kernel<Cache, Out, LANES, VEC, 1> : per == 2 ? paged_read_kernel<Cache, Out, LANES, VEC, 2> : paged_read_kernel<Cache, Out, LANES, VEC, 4>;
-      kernel<<<grid, PC_THREADS, 0, st>>>(c, static_cast<Out*>(k), static_cast<Out*>(v), B, tokens);
+      kernel<<<grid, PC_THREADS, 0, st>>>(c, static_cast<Out*>(k), static_cast<Out*>(v), B, tokens, pc_shift(c), pc_alike(c));
     });
   };
   pc_lanes(c.dim, vec, go);
