@@ -15,15 +15,20 @@
 // rounding, 2⁻⁹ of each weight, would be as large as that of the result, and the second product costs nothing where the tensor cores wait for memory.
 // In e4m3 the products run in fp16, whose 2⁻¹² is an eighth of the result's rounding: one half is enough (weights from 2¹⁴ down to 2⁻²⁴).
 //
-// What bounds it: memory.  At most 16 columns are 32 operations a byte; tcgen05 would take 128 rows of keys too, but wants P through shared memory and its sums
-// through tensor memory for every tile, which is the longer chain where a CTA has a handful of tiles.  Each warp is on its own: it loads its
-// tokens with cp.async into its own ring (steps of 16 or 32 tokens, 8 KB), and no barrier joins warps before the end of a work item.  Pages are looked
-// up one step ahead, so that their latency is not in the chain.
+// What bounds it: memory in bf16 (64 ragged sequences up to 8192, H 16, G 4, D 128: 550 MB in 96 us, 0.87 of the copy rate; 32 in pairs of heads of 64, G 20:
+// 702 MB in 116 us, 0.92).  At most 16 columns are 32 operations a byte; tcgen05 would take 128 rows of keys too, but wants P through shared memory
+// and its sums through tensor memory for every tile, which is the longer chain where a CTA has a handful of tiles.  In e4m3 instructions and their
+// latency: 730 for a step of 32 tokens, 220 of them conversions (one sequence of 131072 tokens: 135 MB in 35 us, 0.59), after some 12 us of first loads, last
+// steps and the second kernel.  Few and short sequences: latency (1000 tokens 4 us behind the launch).
 //
-// Work.  Lengths are known on the device only.  An item is (sequence, tile of rows, key head); its keys are chunks of 4 warps' steps.  Every CTA adds
-// up the chunks of all items from the lengths and takes an equal, contiguous share of them, so that one long sequence or many short ones fill the
-// device alike.  Items that lie in one CTA are finished there; the parts of the others meet in a second kernel (joined in the order of the keys: results
-// do not depend on scheduling), which the first one starts early and which needs no counters, so that nothing has to be zero beforehand.
+// Each warp is on its own: it loads its tokens with cp.async into its own ring (two stages of 16 or 32 tokens, 8 KB; three CTAs an SM; three stages on two
+// CTAs were no faster), and no barrier joins warps before the end of a work item.  Pages are looked up two steps ahead, so that their latency is not in the chain.
+//
+// Work.  Lengths are known on the device only.  An item is (sequence, tile of rows, key head); its keys are chunks, one step of each warp.  Every CTA adds
+// up the chunks of all items from the lengths and takes a contiguous share of them, equal to one chunk, so that one long sequence or many short ones fill
+// the device alike.  Items that lie in one CTA are finished there; the parts of the others meet in a second kernel (joined in the order of the keys: results
+// do not depend on scheduling), which the first one starts early and which needs no counters, so that nothing has to be zero beforehand.  Few items of
+// a few chunks run on clusters of eight CTAs instead, which join their parts in shared memory (pa_prepare).
 #pragma once
 #include <cuda_fp16.h>
 #include <atomic>
@@ -841,7 +846,8 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
 
 // The parts of items that lie in several CTAs.  WPR warps share a row, each takes every WPR-th part with all of its loads in flight; a CTA has the rows of
 // 16 / WPR (at most 8) neighbours of (item, row).  Few items have many parts each and want warps, many items have few parts and want to be over in
-// one wave: 16, 4 or 1, whichever fits the device at once (256 items of 2 to 3 parts: 6 us with 1, 20 with 16; 4 items of 103 parts: 15 with 4, 8 with 16).
+// one wave: 16, 4 or 1, whichever fits the device at once (256 items of 2 to 3 parts: 6 us with 1, 20 with 16; 4 items of 103 parts: 15 with 4, 6 with 16).
+// Loads in turn are what such a kernel waits for: factors of all parts first and then a thread per column took 12 us instead of 6.
 template <int ES, int DT, bool PAIRS, int NC, int WPR>
 __global__ void __launch_bounds__(512 / (WPR == 1 ? 2 : 1)) paged_join_kernel(const PaArgs p) {
   using S = PaShape<ES, DT, PAIRS, NC>;
@@ -900,34 +906,44 @@ __global__ void __launch_bounds__(512 / (WPR == 1 ? 2 : 1)) paged_join_kernel(co
       }
       m[br] = top; mv[br][0] = t0; mv[br][1] = t1;
     }
-    if constexpr (WPR > 1) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) s_sum[slot][warp][br][lane + 32 * j] = v[br][j];
-      if (lane == 0) s_stat[slot][warp][br] = make_float4(m[br], l[br], mv[br][0], mv[br][1]);
-    }
   }
   if constexpr (WPR > 1) {
-    asm volatile("bar.sync %0, %1;" ::"r"(slot + 1), "n"(WPR * 32) : "memory");  // the warps of a row: others may have left
-    if (warp != 0) return;
+    // the warps of a row (others may have left): common maxima, sums scaled to them, then columns added up by as many threads as there are
+    auto together = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(slot + 1), "n"(WPR * 32) : "memory"); };
+#pragma unroll
+    for (int br = 0; br < BR; ++br) if (lane == 0) s_stat[slot][warp][br] = make_float4(m[br], l[br], mv[br][0], mv[br][1]);
+    together();
 #pragma unroll
     for (int br = 0; br < BR; ++br) {
-      m[br] = mv[br][0] = mv[br][1] = -INFINITY; l[br] = 0.f;
+      const float4 st = lane < WPR ? s_stat[slot][lane][br] : make_float4(-INFINITY, 0.f, -INFINITY, -INFINITY);
+      float top = st.x, t0 = st.z, t1 = st.w;
 #pragma unroll
-      for (int w = 0; w < WPR; ++w) {
-        const float4 st = s_stat[slot][w][br];
-        m[br] = fmaxf(m[br], st.x); mv[br][0] = fmaxf(mv[br][0], st.z); mv[br][1] = fmaxf(mv[br][1], st.w);
+      for (int o = 16; o; o >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (E8) { t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o)); t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o)); }
       }
+      float sum = st.y * pa_step(st.x, top);
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[br][j] = 0.f;
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const float f = pa_step(m[br], top), f0 = E8 ? pa_step(mv[br][0], t0) : f, f1 = S::NG == 2 ? pa_step(mv[br][1], t1) : f0;
 #pragma unroll
-      for (int w = 0; w < WPR; ++w) {
-        const float4 st = s_stat[slot][w][br];
-        const float f = pa_step(st.x, m[br]), f0 = E8 ? pa_step(st.z, mv[br][0]) : f, f1 = S::NG == 2 ? pa_step(st.w, mv[br][1]) : f0;
-        l[br] += st.y * f;
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[br][j] += s_sum[slot][w][br][lane + 32 * j] * (j < N / 2 ? f0 : f1);
-      }
+      for (int j = 0; j < N; ++j) s_sum[slot][warp][br][lane + 32 * j] = v[br][j] * (j < N / 2 ? f0 : f1);
+      m[br] = top; l[br] = sum; mv[br][0] = t0; mv[br][1] = t1;
     }
+    together();
+#pragma unroll
+    for (int i = warp * 32 + lane; i < BR * DT; i += WPR * 32) {
+      float x = 0.f;
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) x += s_sum[slot][w][i / DT][i % DT];
+      s_sum[slot][0][i / DT][i % DT] = x;
+    }
+    together();
+    if (warp != 0) return;
+#pragma unroll
+    for (int br = 0; br < BR; ++br)
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[br][j] = s_sum[slot][0][br][lane + 32 * j];
   }
   pa_finish<ES, DT, PAIRS>(p, b, head, row0 + r, (row0 + r) / p.per <= sp.t1, v[0], v[1], m, l, mv, lane);
 }

@@ -7,9 +7,10 @@
 //   read    x = q · 2^e into dense rows, zeros past the end of a sequence.
 //
 // Memory-bound.  A head's row is held by D / 8 lanes, 8 values each (one 16-byte load of bf16), keys and values by the same lanes; rows that no 16 bytes
-// divide go value by value on a whole warp.  A row waits for its length, its page and then its data, so a thread has four rows under way where there are
-// enough of them to fill the device all the same (8 x 8192 tokens from e4m3: @READ@; 4 x 4096 tokens into e4m3: @WRITE@), and one
-// where latency counts.
+// divide go value by value on a whole warp.  A row waits for its length, its page and then its data, so a thread has two or four rows under way where
+// there are enough of them to fill the device all the same, and one where latency counts.  Instructions were the next bound: no division per row,
+// maxima of two bf16 values at a time.  G 4, D 128: 8 x 8192 tokens read from e4m3 41 us (4.9 TB/s; 65 with one row a thread), 4 x 4096 tokens written
+// into e4m3 10.3 us (4.9 TB/s), both without the launch; one token 8.5 us, all of it the host's.
 #include <cuda_fp8.h>
 #include <type_traits>
 
