@@ -4,8 +4,8 @@
   (``_mup_``, ``_tie``, ``_rbase_``, ``_swa<N>``, ``_ctx<N>`` with the matching RoPE scaling factor) — the
   convention of `eval.py:113-141`.
 * ``ModelWrapper.generate`` is token-by-token decoding that re-runs the whole prefix each step,
-  greedy or sampled, with EOS and external stopping criteria (`eval.py:36-111`); with ``use_cache`` a step computes its own
-  token over a paged key-value cache (attention models; ``cache_dtype``: bfloat16, float32 or float8_e4m3fn).
+  greedy or sampled, with EOS and external stopping criteria (`eval.py:36-111`); with ``kv_cache`` a step computes its own
+  token over a paged key-value cache (attention models; ``kv_cache_dtype``: bfloat16, float32 or float8_e4m3fn).
 """
 from __future__ import annotations
 
@@ -59,8 +59,8 @@ class ModelWrapper(torch.nn.Module):
     def generate(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None, max_length: Optional[int] = None,
                  return_dict_in_generate: bool = True, pad_token_id: Optional[int] = None, eos_token_id: Optional[int] = None,
                  do_sample: bool = False, temperature: Optional[float] = None,
-                 stopping_criteria: Optional[Sequence[Callable]] = None, max_gen_toks: int = 128, use_cache: bool = False,
-                 cache_dtype: Optional[torch.dtype] = None, **_unused):
+                 stopping_criteria: Optional[Sequence[Callable]] = None, max_gen_toks: int = 128, kv_cache: bool = False,
+                 kv_cache_dtype: Optional[torch.dtype] = None, **_unused):
         sequences = input_ids.clone()
         max_new = max_length - input_ids.shape[1] if max_length else max_gen_toks
         if attention_mask is None:
@@ -68,8 +68,8 @@ class ModelWrapper(torch.nn.Module):
         use_mask = bool((attention_mask == 0).any())
         active = torch.ones(input_ids.shape[0], dtype=torch.bool, device=input_ids.device)
         cache = None
-        if use_cache and max_new > 0:
-            cache = DecodeCache(self.model, input_ids.shape[0], input_ids.shape[1] + max_new, dtype=cache_dtype)
+        if kv_cache and max_new > 0:
+            cache = DecodeCache(self.model, input_ids.shape[0], input_ids.shape[1] + max_new, dtype=kv_cache_dtype)
         for _ in range(max(max_new, 0)):
             if cache is not None:
                 logits = self.model(sequences[:, cache.tokens:], cache=cache).logits[:, -1, :].float()

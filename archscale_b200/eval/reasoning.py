@@ -178,8 +178,8 @@ def evaluate(task_name: str, lines: Iterable[Dict], generate: Callable[[str, int
             f"pass@1:{n}_samples": sum(scores) / max(len(scores), 1)}
 
 
-def model_generator(wrapper, tokenizer, max_new_tokens: int = 32768, temperature: float = 0.6, use_cache: bool = False,
-                    cache_dtype=None) -> Callable[[str, int], List[str]]:
+def model_generator(wrapper, tokenizer, max_new_tokens: int = 32768, temperature: float = 0.6, kv_cache: bool = False,
+                    kv_cache_dtype=None) -> Callable[[str, int], List[str]]:
     """Sampling generator on :class:`archscale_b200.eval.common.ModelWrapper` (n completions as one batch)."""
     import torch
 
@@ -189,7 +189,7 @@ def model_generator(wrapper, tokenizer, max_new_tokens: int = 32768, temperature
         x = ids.to(wrapper.device).long().unsqueeze(0).repeat(n, 1)
         room = max(1, min(max_new_tokens, wrapper.config.block_size - x.shape[1]))
         out = wrapper.generate(x, max_gen_toks=room, do_sample=True, temperature=temperature,
-                               eos_token_id=getattr(tokenizer, "eos_id", None), use_cache=use_cache, cache_dtype=cache_dtype)
+                               eos_token_id=getattr(tokenizer, "eos_id", None), kv_cache=kv_cache, kv_cache_dtype=kv_cache_dtype)
         return [tokenizer.decode(s[x.shape[1]:].cpu()) for s in out.sequences]
     return gen
 
@@ -223,16 +223,16 @@ def main(argv: Optional[List[str]] = None) -> None:
     ap.add_argument("--n_samples", type=int, default=None)
     ap.add_argument("--max_new_tokens", type=int, default=32768)
     ap.add_argument("--temperature", type=float, default=0.6)
-    ap.add_argument("--use_cache", action="store_true", help="generate over a paged key-value cache (attention models)")
-    ap.add_argument("--cache_fp8", action="store_true", help="keep that cache in e4m3 with a power of two per token and head")
+    ap.add_argument("--kv_cache", action="store_true", help="generate over a paged key-value cache (attention models)")
+    ap.add_argument("--kv_cache_fp8", action="store_true", help="keep that cache in e4m3 with a power of two per token and head")
     a = ap.parse_args(argv)
     import torch
     from archscale_b200.data.tokenizer import Tokenizer
     from archscale_b200.eval.common import load_model
     wrapper = load_model(a.checkpoint, a.config)
     tok = Tokenizer(a.tokenizer)
-    res = evaluate(a.task, load_jsonl(a.data), model_generator(wrapper, tok, a.max_new_tokens, a.temperature, a.use_cache or a.cache_fp8,
-                                                                       torch.float8_e4m3fn if a.cache_fp8 else None), a.n_samples)
+    res = evaluate(a.task, load_jsonl(a.data), model_generator(wrapper, tok, a.max_new_tokens, a.temperature, a.kv_cache or a.kv_cache_fp8,
+                                                                       torch.float8_e4m3fn if a.kv_cache_fp8 else None), a.n_samples)
     print(json.dumps(res))
 
 

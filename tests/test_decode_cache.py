@@ -74,7 +74,7 @@ def test_generation(name, device):
     w = ModelWrapper(m)
     ids = torch.randint(0, 96, (2, 6), generator=torch.Generator().manual_seed(2)).to(device)
     plain = w.generate(ids, max_gen_toks=12, return_dict_in_generate=False)
-    cached = w.generate(ids, max_gen_toks=12, return_dict_in_generate=False, use_cache=True)
+    cached = w.generate(ids, max_gen_toks=12, return_dict_in_generate=False, kv_cache=True)
     assert cached.shape == plain.shape == (2, 18) and torch.equal(cached[:, :6], ids)
     # greedy choices agree up to ties of what the orders of sums leave
     with torch.no_grad():
@@ -82,11 +82,11 @@ def test_generation(name, device):
     chosen = logits.gather(-1, cached[:, 6:, None]).squeeze(-1)
     assert bool((chosen >= logits.amax(-1) - 4e-4 * max(1.0, float(logits.abs().max()))).all())
     stop = int(cached[0, 8])
-    short = w.generate(ids, max_gen_toks=12, eos_token_id=stop, use_cache=True)
+    short = w.generate(ids, max_gen_toks=12, eos_token_id=stop, kv_cache=True)
     assert short.sequences.shape[1] <= 18
-    eight = w.generate(ids, max_gen_toks=12, return_dict_in_generate=False, use_cache=True, cache_dtype=torch.float8_e4m3fn)
+    eight = w.generate(ids, max_gen_toks=12, return_dict_in_generate=False, kv_cache=True, kv_cache_dtype=torch.float8_e4m3fn)
     assert eight.shape == (2, 18)
-    assert w.generate(ids, max_gen_toks=0, return_dict_in_generate=False, use_cache=True).shape == ids.shape
+    assert w.generate(ids, max_gen_toks=0, return_dict_in_generate=False, kv_cache=True).shape == ids.shape
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -176,7 +176,7 @@ def test_what_a_cache_refuses():
         with pytest.raises(ValueError, match="does not cover"):
             DecodeCache(other, 1, 8)
         with pytest.raises(ValueError, match="does not cover"):
-            ModelWrapper(other.eval()).generate(ids, max_gen_toks=2, use_cache=True)
+            ModelWrapper(other.eval()).generate(ids, max_gen_toks=2, kv_cache=True)
 
 
 def test_a_call_that_failed_leaves_the_cache_as_it_was():
