@@ -340,8 +340,49 @@ def bench_fp8_block(res: list) -> None:
         print(r, flush=True)
 
 
+def paged_inputs(B, L, H, G, D, dtype, page=64, ragged=False):
+    """(q, cache, table, lengths) of one new token each over sequences of L tokens (ragged: L / 8 … L)."""
+    n = -(-L // page)
+    cache = ops.new_paged_cache(B * n, G, page, D, dtype, "cuda")
+    table = torch.randperm(B * n, device="cuda").to(torch.int32).view(B, n)
+    lengths = torch.randint(L // 8, L + 1, (B,), device="cuda", dtype=torch.int32) if ragged else torch.full((B,), L, device="cuda", dtype=torch.int32)
+    for t in range(0, L, 4096):
+        k, v = (torch.randn(B, min(4096, L - t), G, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+        ops.paged_cache_write(cache, k, v, table, torch.full((B,), t + k.shape[1], device="cuda", dtype=torch.int32))
+    return torch.randn(B, 1, H, D, device="cuda", dtype=torch.bfloat16), cache, table, lengths
+
+
+def bench_paged(res: list) -> None:
+    """Paged key-value cache: attention of one new token each, plain and differential, writing a chunk and reading a prefix."""
+    pk = peaks()
+    e4m3 = torch.float8_e4m3fn
+    for B, L, H, G, D, dtype, ragged, diff in ((1, 1000, 16, 4, 128, torch.bfloat16, False, False), (64, 8192, 16, 4, 128, torch.bfloat16, True, False),
+                                               (1, 131072, 32, 4, 128, e4m3, False, False), (1, 2000, 40, 20, 64, torch.bfloat16, False, True),
+                                               (32, 8192, 40, 20, 64, torch.bfloat16, True, True), (4, 32768, 16, 4, 128, e4m3, False, True)):
+        q, cache, table, lengths = paged_inputs(B, L, H, G, D, dtype, ragged=ragged)
+        lam, w = torch.full((1,), 0.3, device="cuda"), torch.ones(2 * D, device="cuda")
+        t = time_ms((lambda: ops.paged_diff_attention(q, cache, table, lengths, lam, w, 0.4)) if diff else (lambda: ops.paged_attention(q, cache, table, lengths)))
+        nbytes = 2 * int(lengths.sum()) * G * (D + 1 if dtype is e4m3 else 2 * D) + 4 * q.numel()
+        r = {"kernel": "paged_diff_attention" if diff else "paged_attention", "B": B, "L": L, "ragged": ragged, "H": H, "G": G, "D": D, "cache": str(dtype)[6:],
+             "ms": t, "frac_of_" + pk["kind"] + "_hbm": nbytes / t / 1e6 / pk["hbm_gbs"]}
+        res.append(r)
+        print(r, flush=True)
+    for dtype in (torch.bfloat16, e4m3):
+        B, L, G, D = 8, 8192, 4, 128
+        _, cache, table, lengths = paged_inputs(B, L, 4, G, D, dtype)
+        k, v = (torch.randn(B, 2048, G, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+        size = D + 1 if dtype is e4m3 else 2 * D
+        for name, tokens, fn in (("paged_cache_write", B * 2048, lambda: ops.paged_cache_write(cache, k, v, table, lengths)),
+                                 ("paged_cache_read", B * L, lambda: ops.paged_cache_read(cache, table, lengths, L))):
+            t = time_ms(fn)
+            r = {"kernel": name, "tokens": tokens, "G": G, "D": D, "cache": str(dtype)[6:], "ms": t, "frac_of_" + pk["kind"] + "_hbm": 2 * tokens * G * (size + 2 * D) / t / 1e6 / pk["hbm_gbs"]}
+            res.append(r)
+            print(r, flush=True)
+
+
 ALL = {"gemm": bench_gemm, "rmsnorm": bench_rmsnorm, "swiglu": bench_swiglu, "ce": bench_ce, "rope": bench_rope,
-       "attn": bench_attn, "mamba": bench_mamba, "mxfp8": bench_mxfp8, "nvfp4": bench_nvfp4, "fp8_block": bench_fp8_block, "gdn": bench_gdn}
+       "attn": bench_attn, "mamba": bench_mamba, "mxfp8": bench_mxfp8, "nvfp4": bench_nvfp4, "fp8_block": bench_fp8_block, "gdn": bench_gdn,
+       "paged": bench_paged}
 
 
 def main() -> None:

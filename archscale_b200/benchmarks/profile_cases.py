@@ -181,6 +181,19 @@ def case_gdn():
     torch.cuda.synchronize()
 
 
+def case_paged():
+    """Attention of one new token each over a paged cache, in bf16 and in e4m3, plain and in pairs, with the write and the read of such a cache."""
+    from archscale_b200 import ops
+    from archscale_b200.benchmarks.kernels import paged_inputs
+    lam, w = torch.full((1,), 0.3, device="cuda"), torch.ones(256, device="cuda")
+    for dtype in (torch.bfloat16, torch.float8_e4m3fn):
+        q, cache, table, lengths = paged_inputs(16, 16384, 16, 4, 128, dtype)
+        ops.paged_attention(q, cache, table, lengths)
+        ops.paged_diff_attention(q, cache, table, lengths, lam, w, 0.4)
+        ops.paged_cache_read(cache, table, lengths, 8192)
+    torch.cuda.synchronize()
+
+
 CASES = {k[5:]: v for k, v in list(globals().items()) if k.startswith("case_")}
 
 
