@@ -306,7 +306,7 @@ def paged_cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table
         raise ValueError(f"{name}: new keys and values must be (batch, new tokens, {cache.k.shape[1]}, {cache.k.shape[3]}), got {tuple(k.shape)} and {tuple(v.shape)}")
     if k.dtype != v.dtype:
         raise TypeError(f"{name}: new keys and values must be of one type, got {k.dtype} and {v.dtype}")
-    if any(t.shape[d] > 1 and t.stride(d) == 0 for t in (cache.k, cache.v) for d in range(3)):
+    if any(t is not None and t.shape[d] > 1 and t.stride(d) == 0 for t in cache for d in range(3)):
         raise ValueError(f"{name}: an expanded cache cannot be written")
     paged_cache_write_ref(cache, k, v, table, lengths, new_lengths)
     return cache

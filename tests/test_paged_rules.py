@@ -99,6 +99,18 @@ def test_wrong_operands(device):
     assert torch.equal(attn(c=expanded), attn(c=dense))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("field", ["k", "v", "k_scale", "v_scale"])
+def test_expanded_parts_are_not_written(device, field):
+    _, table, lengths, k, v, *_ = operands(device)
+    cache = ops.new_paged_cache(6, 4, 8, 64, torch.float8_e4m3fn, device)
+    whole = getattr(cache, field)
+    wrong = cache._replace(**{field: whole[:, :, :1].expand(whole.shape)})
+    with pytest.raises(ValueError, match="an expanded cache"):
+        ops.paged_cache_write(wrong, k, v, table, lengths)
+    ops.paged_cache_read(wrong, table, lengths, 4)
+
+
 @pytest.mark.gpu
 def test_operands_on_two_devices():
     cache, table, lengths, k, v, q, lam, w = operands("cuda")
