@@ -13,12 +13,12 @@
 //            values [v1 | v2]: one read and one product for both branches
 // Rounding: q is exact (bf16; for fp16 times a power of two of its row).  In bf16 P enters as two halves, hi and p − hi, so that it is good to 2⁻¹⁷: its plain
 // rounding, 2⁻⁹ of each weight, would be as large as that of the result, and the second product costs nothing where the tensor cores wait for memory.
-// In e4m3 the products run in fp16, whose 2⁻¹² is an eighth of the result's rounding: one half is enough (weights from 2¹⁴ down to 2⁻²⁴).
+// In e4m3 the products run in fp16, weights (from 2¹⁴ down to 2⁻²⁴) as two halves too: good to 2⁻²² where one half left 2⁻¹¹.
 //
 // What bounds it: memory in bf16 (64 ragged sequences up to 8192, H 16, G 4, D 128: 550 MB in 96 us, 0.87 of the copy rate; 32 in pairs of heads of 64, G 20:
 // 702 MB in 116 us, 0.92).  At most 16 columns are 32 operations a byte; tcgen05 would take 128 rows of keys too, but wants P through shared memory
 // and its sums through tensor memory for every tile, which is the longer chain where a CTA has a handful of tiles.  In e4m3 instructions and their
-// latency: 730 for a step of 32 tokens, 220 of them conversions (one sequence of 131072 tokens: 135 MB in 35 us, 0.59), after some 12 us of first loads, last
+// latency: 730 for a step of 32 tokens, 220 of them conversions (one sequence of 131072 tokens: 135 MB in 37 us, 0.55), after some 12 us of first loads, last
 // steps and the second kernel.  Few and short sequences: latency (1000 tokens 4 us behind the launch).
 //
 // Each warp is on its own: it loads its tokens with cp.async into its own ring (two stages of 16 or 32 tokens, 8 KB; three CTAs an SM; three stages on two
@@ -200,7 +200,11 @@ __device__ __forceinline__ uint32_t pa_pack(float x, float y) {
   if constexpr (ES == 2) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
   else { const __half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
 }
-__device__ __forceinline__ uint32_t pa_rest(float x, float y, uint32_t hi) { return pa_pack<2>(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u)); }
+template <int ES>
+__device__ __forceinline__ uint32_t pa_rest(float x, float y, uint32_t hi) {
+  if constexpr (ES == 2) return pa_pack<2>(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+  else { const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi)); return pa_pack<1>(x - h.x, y - h.y); }
+}
 template <int BYTES>
 __device__ __forceinline__ void pa_copy(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -629,7 +633,7 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
           unscaled = __any_sync(0xffffffffu, unscaled);
         }
         // ---- weights, turned into right operands: 16 tokens at a time
-        uint32_t hi[NC][NGX][MT][2], lo[E8 ? 1 : NC][E8 ? 1 : MT][2];
+        uint32_t hi[NC][NGX][MT][2], lo[NC][NGX][MT][2];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           float base[2], bv[2][NGX];                                            // where nothing is seen yet every x is −∞: its weight is 0
@@ -651,12 +655,14 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
                   const float e = ev[g][mt][h];
                   float w2 = pa_ex2(y0 + e + bv[0][g]), w3 = pa_ex2(y1 + e + bv[1][g]);
                   if (unscaled) { w2 = y0 == -INFINITY ? 0.f : w2; w3 = y1 == -INFINITY ? 0.f : w3; }
-                  hi[c][g][mt][h] = pa_turn(pa_pack<1>(w2, w3));
+                  const uint32_t u = pa_pack<1>(w2, w3);
+                  hi[c][g][mt][h] = pa_turn(u);
+                  lo[c][g][mt][h] = pa_turn(pa_rest<1>(w2, w3, u));
                 }
               } else {
                 const uint32_t u = pa_pack<2>(w0, w1);
                 hi[c][0][mt][h] = pa_turn(u);
-                lo[c][mt][h] = pa_turn(pa_rest(w0, w1, u));
+                lo[c][0][mt][h] = pa_turn(pa_rest<2>(w0, w1, u));
               }
             }
         }
@@ -675,7 +681,7 @@ __global__ void __launch_bounds__(PaShape<ES, DT, PAIRS, NC>::WARPS * 32, pa_res
         auto out_mul = [&](float (&d)[4], int c, int i, int mt, const uint32_t (&a)[4]) {
           const int g = NG == 2 && i >= KS / 2 ? 1 : 0;
           pa_mma<ES>(d, a[0], a[1], a[2], a[3], hi[c][g][mt][0], hi[c][g][mt][1]);
-          if constexpr (!E8) pa_mma<ES>(d, a[0], a[1], a[2], a[3], lo[c][mt][0], lo[c][mt][1]);
+          pa_mma<ES>(d, a[0], a[1], a[2], a[3], lo[c][g][mt][0], lo[c][g][mt][1]);
         };
         // left operands of the 16 or 32 columns of a matrix load: rows gq, gq + 8 are columns gq, gq + 8 (bf16) or 2 gq, 2 gq + 1 of 16 (e4m3)
         constexpr int NB = E8 ? 2 : 1;
