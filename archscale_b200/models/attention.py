@@ -152,7 +152,7 @@ class CausalSelfAttention(nn.Module):
             nn.init.zeros_(self.softmax_offset)
 
     # -- rope for ada_rope layers --------------------------------------------------
-    def _ada_rope(self, x: torch.Tensor, start: int, T: int):
+    def _ada_rope(self, x: torch.Tensor, T: int):
         cfg = self.config
         if cfg.yoco_window and cfg.local_window == cfg.block_size // 2:
             initial_window, sf = 4096, cfg.scaling_factor
@@ -163,8 +163,7 @@ class CausalSelfAttention(nn.Module):
             self.rope_cache = ops.build_rope_cache(self.max_len, int(cfg.rotary_percentage * cfg.head_size),
                                                    torch.bfloat16, x.device, base=0.09 * initial_window ** 1.628,
                                                    scaling_factor=sf)
-        cos, sin = self.rope_cache
-        return cos[start:T], sin[start:T]
+        return self.rope_cache
 
     def _window(self):
         win = self.win_tuple
@@ -214,8 +213,7 @@ class CausalSelfAttention(nn.Module):
         cfg = self.config
         if cfg.ada_rope:
             assert cfg.local_window > 0
-            start = cache.tokens if cache is not None else 0
-            rope = self._ada_rope(x, start, start + T)
+            rope = tuple(t[:T] for t in self._ada_rope(x, T)) if cache is None else cache.positions(self, lambda: self._ada_rope(x, cache.capacity), T)
         H, G, hs = self.n_head, self.n_query_groups, self.head_size
         g = None
         if self.yoco_cross:

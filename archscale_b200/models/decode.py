@@ -7,7 +7,7 @@ cache of the layer that made their keys.
 """
 from __future__ import annotations
 
-from typing import List, Optional
+from typing import Callable, Dict, List, Optional, Tuple
 
 import torch
 
@@ -34,8 +34,11 @@ class DecodeCache:
     """``model(idx, cache=cache)`` appends the tokens ``idx`` (B, T) to it and computes them over everything it holds.
 
     ``dtype``: bfloat16 or float32 (default: the model's compute type), or float8_e4m3fn with a power of two per token and head.  All sequences
-    have the same number of tokens.  A call under ``torch.cuda.graph`` must not be the one that fills an empty cache, and its replays
-    add to ``lengths`` on the device, not to ``tokens``."""
+    have the same number of tokens.
+
+    Once a cache holds tokens, calls can be captured by ``torch.cuda.graph``.  A capture appends nothing; each replay takes its positions from
+    ``lengths`` on the device and advances them.  A replay that the capacity has no room for gives NaN.  Replays and other calls may follow one another
+    in any order: after a capture ``tokens`` (and so the next call that is not captured) reads ``lengths``, which waits for the device."""
 
     def __init__(self, model, batch: int, capacity: int, page_size: int = 64, dtype: Optional[torch.dtype] = None, device=None) -> None:
         why = unsupported(model)
@@ -48,36 +51,78 @@ class DecodeCache:
         reps = bc.n_layer // bc.share_group // bc.share_per_layer if bc.share_per_layer > 0 else 1
         layers = reps * sum(not block.yoco_cross for block in model.transformer.h)
         pages = -(-capacity // page_size)
-        self.batch, self.capacity, self.tokens = batch, capacity, 0
+        self.batch, self.capacity = batch, capacity
         self.table = torch.arange(batch * pages, dtype=torch.int32, device=device).view(batch, pages)
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.layers: List[ops.PagedCache] = [ops.new_paged_cache(batch * pages, cfg.n_query_groups, page_size, cfg.head_size, dtype or model.compute_dtype, device)
                                              for _ in range(layers)]
-        self._at, self._open = -1, 0
+        self._at, self._open, self._tokens = -1, 0, 0
+        self._capturing, self._captured = False, False
+        self._rows: Optional[torch.Tensor] = None                 # positions of a captured call's tokens
+        self._tables: Dict[torch.nn.Module, Tuple[torch.Tensor, torch.Tensor]] = {}      # captured calls read them: they live as long as the cache
 
-    def begin(self, idx: torch.Tensor) -> int:
-        """Before the first layer: room for the tokens; returns the position of the first one."""
+    def _in_capture(self) -> bool:
+        if not self.lengths.is_cuda:
+            return False
+        with torch.cuda.device(self.lengths.device):
+            return torch.cuda.is_current_stream_capturing()
+
+    @property
+    def tokens(self) -> int:
+        """Tokens of each sequence."""
+        if self._captured and not self._in_capture():             # replays have moved lengths
+            self._tokens = int(self.lengths[0]) - self._open
+        return self._tokens
+
+    def begin(self, idx: torch.Tensor) -> None:
+        """Before the first layer: room for the tokens."""
         B, T = idx.shape
+        self._capturing = self._in_capture()
         if B != self.batch:
             raise ValueError(f"the cache holds {self.batch} sequences, got {B}")
         if self.tokens + T > self.capacity:
-            raise ValueError(f"the cache holds {self.capacity} tokens: {self.tokens} are there, {T} more were given")
+            raise ValueError(f"the cache holds {self.capacity} tokens: {self._tokens} are there, {T} more were given")
         if torch.is_grad_enabled():
             raise RuntimeError("a key-value cache has no gradients: call the model under torch.no_grad()")
+        self._at = -1
+        if self._capturing:
+            if self._tokens == 0:
+                raise RuntimeError("the first tokens of a cache cannot be captured: its replays would be further ones")
+            if self._open:
+                raise RuntimeError("the last call with this cache failed: call the model once before a capture")
+            self._captured = True
+            self.lengths += T
+            self._rows = (self.lengths[:1] - T + torch.arange(T, dtype=torch.int32, device=self.lengths.device)).clamp(0, self.capacity - 1)
+            return
         if self._open:                                             # the call before did not come to its end
             self.lengths -= self._open
         self.lengths += T
-        self._at, self._open = -1, T
-        return self.tokens
+        self._open = T
 
     def end(self, T: int) -> None:
-        self.tokens += T
-        self._open = 0
+        """After the last operation of a call."""
+        self._rows = None
+        if not self._capturing:
+            self._tokens += T
+            self._open = 0
 
     @property
     def filling(self) -> bool:
         """Whether the tokens of this call are the first ones: attention over them alone."""
-        return self.tokens == 0
+        return self._tokens == 0
+
+    def positions(self, owner: torch.nn.Module, table: Callable[[], Tuple[torch.Tensor, torch.Tensor]], T: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Rows of the rotary table of a model or layer, which covers the capacity, at the positions of the T new tokens.  It is kept as the first call
+        had it, since graphs read it; a captured call gathers the rows on the device."""
+        if owner not in self._tables and not self._capturing:
+            self._tables[owner] = table()
+        if self._capturing:
+            return tuple(t.index_select(0, self._rows) for t in self._tables[owner])
+        return tuple(t[self._tokens:self._tokens + T] for t in self._tables[owner])
+
+    def bounded(self, x: torch.Tensor) -> torch.Tensor:
+        """The model's output, NaN in replays past the capacity."""
+        return x.masked_fill(self.lengths[0] > self.capacity, float("nan")) if self._capturing else x
 
     def write(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """Keys and values (B, T, G, D) of the next attention layer; layers that only read use the last ones written."""

@@ -525,18 +525,19 @@ class GPT(nn.Module):
         cfg = self.config
         B, T = idx.shape
         seq_meta = self._seq_meta(idx, attn_mask)
-        start = 0
         if cache is not None:
-            start = cache.begin(idx)
+            cache.begin(idx)
             seq_meta = dict(seq_meta or {}, cache=cache)
         if max_seq_length is None:
             max_seq_length = cfg.block_size
         rope = None
         if not (cfg.nope or cfg.ada_rope):
-            if self.rope_cache is None or start + T > self.max_len or self.rope_cache[0].device != idx.device:
-                self.max_len = max(start + T, self.max_len)
-                self.rope_cache = self.build_rope_cache(idx, self.max_len)
-            rope = (self.rope_cache[0][start:start + T], self.rope_cache[1][start:start + T])
+            def table(n):
+                if self.rope_cache is None or n > self.max_len or self.rope_cache[0].device != idx.device:
+                    self.max_len = max(n, self.max_len)
+                    self.rope_cache = self.build_rope_cache(idx, self.max_len)
+                return self.rope_cache
+            rope = tuple(t[:T] for t in table(T)) if cache is None else cache.positions(self, lambda: table(cache.capacity), T)
         x = self.transformer.wte(idx)
         if self.scale_embed:
             x = x * math.sqrt(cfg.n_embd)
@@ -606,6 +607,8 @@ class GPT(nn.Module):
             x = _norm_to(self.transformer.ln_f, x, self.compute_dtype)
         if self.logit_scale != 1.0:
             x = x * self.logit_scale
+        if cache is not None:
+            x = cache.bounded(x)
         if use_flce_loss:
             return CausalLMOutput(logits=x, weight=self.lm_head.weight)
         return CausalLMOutput(logits=self.lm_head(x).float())
