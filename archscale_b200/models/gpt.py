@@ -594,8 +594,6 @@ class GPT(nn.Module):
         else:
             for block in self.transformer.h:
                 run(block)
-        if cache is not None:
-            cache.end(T)
         if cfg.sum_skip:
             x = input_embed
         if use_deferred:
@@ -609,6 +607,7 @@ class GPT(nn.Module):
             x = x * self.logit_scale
         if cache is not None:
             x = cache.bounded(x)
-        if use_flce_loss:
-            return CausalLMOutput(logits=x, weight=self.lm_head.weight)
-        return CausalLMOutput(logits=self.lm_head(x).float())
+        out = CausalLMOutput(logits=x, weight=self.lm_head.weight) if use_flce_loss else CausalLMOutput(logits=self.lm_head(x).float())
+        if cache is not None:
+            cache.end(T)
+        return out

@@ -60,6 +60,23 @@ def test_captures_that_are_refused(monkeypatch):
         assert near(m(IDS[:, 4:6], cache=cache).logits, m(IDS[:, :6]).logits[:, 4:]) and cache.lengths.tolist() == [6] * 3
 
 
+@pytest.mark.parametrize("part", ["ln_f", "lm_head"])
+def test_a_call_that_fails_behind_the_last_layer(part):
+    m = make("grouped")
+    cache = DecodeCache(m, 3, 9)
+    with torch.no_grad():
+        want = m(IDS[:, :9]).logits
+        for a, b in ((0, 6), (6, 9)):
+            module = m.lm_head if part == "lm_head" else m.transformer.ln_f
+            hook = module.register_forward_pre_hook(lambda *a: (_ for _ in ()).throw(MemoryError("stop")))
+            with pytest.raises(MemoryError):
+                m(IDS[:, a:b], cache=cache)
+            hook.remove()
+            assert cache.tokens == a
+            assert near(m(IDS[:, a:b], cache=cache).logits, want[:, a:b])
+    assert cache.tokens == 9 and cache.lengths.tolist() == [9] * 3
+
+
 def captured(m, cache, token):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
