@@ -17,7 +17,10 @@ static PaPlan pa_plan(const PagedView& c, const b200_paged_query& a) {
   s.ok = a.type == 1 && c.type != 0 && alike && p.piece != 0 && D <= (a.diff ? 128 : 256);
   if (!s.ok) return s;
   p.per = a.H / c.groups;                                                       // query heads, or pairs of them, of a key head or pair
-  p.rows = p.per * a.T;
+  const int64_t rows = static_cast<int64_t>(p.per) * a.T;
+  s.ok = rows <= 0x7fff0000LL;                                                  // counted in 32 bits, tiles of them rounded up
+  if (!s.ok) return s;
+  p.rows = static_cast<int>(rows);
   p.heads = a.diff ? c.groups / 2 : c.groups;
   s.nc = p.rows <= (a.diff ? 4 : 8) ? 1 : 2;
   s.dt = a.diff ? (D <= 64 ? 128 : 256) : D <= 64 ? 64 : D <= 128 ? 128 : 256;
