@@ -6,6 +6,7 @@ from archscale_b200.eval import ModelWrapper
 from archscale_b200.models.decode import DecodeCache
 from test_decode_cache import MODELS, make, run
 
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 IDS = torch.randint(0, 96, (3, 40), generator=torch.Generator().manual_seed(1))
 
 
@@ -75,6 +76,30 @@ def test_a_call_that_fails_behind_the_last_layer(part):
             assert cache.tokens == a
             assert near(m(IDS[:, a:b], cache=cache).logits, want[:, a:b])
     assert cache.tokens == 9 and cache.lengths.tolist() == [9] * 3
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [None, torch.float8_e4m3fn])
+@pytest.mark.parametrize("name", ["grouped", "differential"])
+def test_generation_ends_with_its_token(name, dtype, device):
+    """The choices are those of the steps' logits; with one of them as the end of a text, that is where it ends."""
+    m = make(name, device)
+    w = ModelWrapper(m)
+    ids = IDS[:1, :6].repeat(2, 1).to(device)
+    kw = dict(max_gen_toks=12, return_dict_in_generate=False, kv_cache=True, kv_cache_dtype=dtype)
+    out = w.generate(ids, **kw)
+    logits = run(m, out, list(range(6, 18)), dtype=dtype)[:, 5:-1]
+    chosen = logits.gather(-1, out[:, 6:, None]).squeeze(-1)
+    assert bool((chosen >= logits.amax(-1) - 4e-4 * max(1.0, float(logits.abs().max()))).all())
+    with torch.no_grad():
+        exact = m(out).logits[:, 5:-1]
+    # fp32: other orders of sums; e4m3: elements off by half a step of 2⁻³ at most, 0.036 of their size if even, in every layer
+    assert near(logits, exact) if dtype is None else float((logits - exact).norm() / exact.norm()) < 0.1
+    for step in (0, 7, 11):
+        eos = int(out[0, 6 + step])
+        first = out[0, 6:].tolist().index(eos)
+        short = w.generate(ids, **kw, eos_token_id=eos)
+        assert torch.equal(short, out[:, :6 + first + 1])
 
 
 def captured(m, cache, token):
