@@ -380,9 +380,58 @@ def bench_paged(res: list) -> None:
             print(r, flush=True)
 
 
+def bench_generate(res: list) -> None:
+    """Greedy generation, batch 8, prompt 1024, 128 new tokens: wall time per token of ``ModelWrapper.generate`` re-running the prefix and over a cache, and
+    of a step of the model over a cache, as called and captured."""
+    import time
+
+    from archscale_b200.config import Config
+    from archscale_b200.eval import ModelWrapper
+    from archscale_b200.models.decode import DecodeCache
+    from archscale_b200.models.gpt import GPT
+
+    def wall_ms(fn, n):
+        torch.cuda.synchronize()
+        t = time.perf_counter()
+        fn()
+        torch.cuda.synchronize()
+        return (time.perf_counter() - t) * 1e3 / n
+
+    for name in ("transformer_gqa4_d8", "transformer_gqa4_d16"):
+        torch.manual_seed(0)
+        with torch.device("cuda"):
+            model = GPT(Config.from_name(name))
+        model.reset_parameters()
+        model.compute_dtype = torch.bfloat16
+        model = model.to(torch.bfloat16).eval()
+        w, ids, new = ModelWrapper(model), torch.randint(0, model.config.vocab_size, (8, 1024), device="cuda"), 128
+        r = {"kernel": "generate", "model": name, "batch": 8, "prompt": 1024, "new_tokens": new}
+        for what, kw in (("prefix", {}), ("cache", dict(kv_cache=True)), ("cache_e4m3", dict(kv_cache=True, kv_cache_dtype=torch.float8_e4m3fn))):
+            w.generate(ids, max_gen_toks=4, **kw)
+            r[what + "_ms_per_token"] = wall_ms(lambda: w.generate(ids, max_gen_toks=new, **kw), new)
+        with torch.no_grad():
+            cache, token = DecodeCache(model, 8, 1024 + 2 * new + 8), ids[:, :1].clone()
+            model(ids, cache=cache)
+
+            def steps():
+                for _ in range(new):
+                    model(token, cache=cache)
+
+            model(token, cache=cache)
+            r["step_ms"] = wall_ms(steps, new)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                model(token, cache=cache)
+            graph.replay()
+            r["step_captured_ms"] = wall_ms(lambda: [graph.replay() for _ in range(new)], new)
+        res.append(r)
+        print(r, flush=True)
+        del graph, cache, w, model
+
+
 ALL = {"gemm": bench_gemm, "rmsnorm": bench_rmsnorm, "swiglu": bench_swiglu, "ce": bench_ce, "rope": bench_rope,
        "attn": bench_attn, "mamba": bench_mamba, "mxfp8": bench_mxfp8, "nvfp4": bench_nvfp4, "fp8_block": bench_fp8_block, "gdn": bench_gdn,
-       "paged": bench_paged}
+       "paged": bench_paged, "generate": bench_generate}
 
 
 def main() -> None:
