@@ -1,4 +1,6 @@
-// Attention of a few new tokens over a paged key-value cache (layout in paged.cuh), keys and values read once for all query rows of a key head.
+// Attention of a few new tokens over a paged key-value cache (layout in paged.cuh), keys and values read once for every tile of at most 16 query rows of a
+// key head, or 8 of a pair of them: once for a token or a few drafts.  Whole prompt parts are right, but every tile reads the prefix again (2048 new tokens over
+// 8192, H 16, G 4, D 128: 1084 us, where the products alone need 94).
 //
 // Mathematics.  One pass over the keys with a running maximum and sum (base 2, 32 bits):  x_j = log₂e · scale · q·k_j,  p_j = 2^(x_j − m),
 // o = Σ p_j v_j / Σ p_j.  Parts of a sequence are joined by  m = max m_i,  l = Σ l_i 2^(m_i − m),  o = Σ o_i 2^(m_i − m).
@@ -15,10 +17,10 @@
 // rounding, 2⁻⁹ of each weight, would be as large as that of the result, and the second product costs nothing where the tensor cores wait for memory.
 // In e4m3 the products run in fp16, weights (from 2¹⁴ down to 2⁻²⁴) as two halves too: good to 2⁻²² where one half left 2⁻¹¹.
 //
-// What bounds it: memory in bf16 (64 ragged sequences up to 8192, H 16, G 4, D 128: 550 MB in 96 us, 0.87 of the copy rate; 32 in pairs of heads of 64, G 20:
-// 702 MB in 116 us, 0.92).  At most 16 columns are 32 operations a byte; tcgen05 would take 128 rows of keys too, but wants P through shared memory
+// What bounds it: memory in bf16 (16 sequences of 16384, H 16, G 4, D 128: 537 MB in 91 us by the kernel alone with cold caches, 0.90 of the copy rate, in pairs
+// 93; as called, with launch and join, 64 ragged sequences up to 8192, 605 MB: 111 us, 0.83; 32 in pairs of heads of 64, G 20, 755 MB: 135 us, 0.85).  At most 16 columns are 32 operations a byte; tcgen05 would take 128 rows of keys too, but wants P through shared memory
 // and its sums through tensor memory for every tile, which is the longer chain where a CTA has a handful of tiles.  In e4m3 instructions and their
-// latency: 730 for a step of 32 tokens, 220 of them conversions (one sequence of 131072 tokens: 135 MB in 37 us, 0.55), after some 12 us of first loads, last
+// latency: 770 for a step of 32 tokens, 220 of them conversions (one sequence of 131072 tokens: 135 MB in 37 us, 0.55), with some 12 us of first loads, last
 // steps and the second kernel.  Few and short sequences: latency (1000 tokens 4 us behind the launch).
 //
 // Each warp is on its own: it loads its tokens with cp.async into its own ring (two stages of 16 or 32 tokens, 8 KB; three CTAs an SM; three stages on two
@@ -1016,7 +1018,8 @@ static int pa_prepare(PaArgs& p, bool gen, int span, int num_sms, void* ws, int6
   // Few items of a few chunks: clusters of eight CTAs, one launch and no second kernel.  A CTA then has an eighth of an item instead of its share of all
   // chunks, which may be three (bf16, up to 128 values a row: four and a half) chunks more before it costs what the second kernel does; clusters leave places of an SM unused, hence four fifths.
   // One sequence of 1000 tokens, 4 key heads of 128: 10.3 -> 8.3 us, 8 of 2500: 17.2 -> 12.3, 8 of 5000 in e4m3: 22.6 -> 16.4; on the other side of the
-  // rule 13 of 2500: 18.4 -> 22.5, one of 5000 in e4m3: 12.3 -> 14.4.
+  // rule 13 of 2500: 18.4 -> 22.5, one of 5000 in e4m3: 12.3 -> 14.4.  The chunks are those of the table, since lengths lie on the device: in a table with room for
+  // 8192 tokens the sequence of 1000 takes 10.3 us, 8 of 1000 16.4 instead of 8.4, 8 of 2500 16.5 instead of 12.4.
   const int64_t items = static_cast<int64_t>(p.nb) * p.nrt * p.heads;
   const bool cluster = max_chunks > 1 && max_chunks <= 64 && 10 * items <= full && max_chunks * (full - 8 * items) <= (ES == 2 && DT <= 128 ? 36 : 24) * full;
   const int64_t bytes = max_chunks > 1 && !cluster ? static_cast<int64_t>(p.ncta) * 2 * S::PART * 4 + (PA_ENTRIES + 4) * 4 : 0;

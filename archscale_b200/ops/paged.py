@@ -14,7 +14,8 @@ position ``lengths[b] − new_lengths[b] + i``.  Tables and lengths stay on the 
   tensors, which :func:`~archscale_b200.ops.attention` takes.
 * :func:`paged_attention` is ``o_i = Σ_j softmax_j(scale · q_i·k_j) v_j`` over the positions ``j`` up to the row's own, at most ``window[0]`` back,
   with the options of :func:`~archscale_b200.ops.attention` (grouped heads, window, sink, log-sum-exp).  Any number of new tokens is right; it is made
-  for a few, and reads keys and values once for all of them and all heads of a group.
+  for a few: keys and values are read once for every 16 rows (tokens times heads) of a group, or 8 of a pair of heads.  Queries in float32, and caches in
+  float32 or of odd layouts, take a kernel that reads them once for each row.  Weights are good to 2⁻¹⁷, sums are in 32 bits.
 * :func:`paged_diff_attention` is the same for pairs of heads ``(1, 2)``: ``a_i = softmax(q_i k_iᵀ) [v_1 | v_2]`` and
   ``y = RMSNorm(a_1 − λ a_2) · weight · c`` over the 2 D values of a pair, in fp32 up to the one rounding of y (the training layer rounds ``a_1`` and ``a_2``).
 
