@@ -152,12 +152,14 @@ class CausalSelfAttention(nn.Module):
             nn.init.zeros_(self.softmax_offset)
 
     # -- rope for ada_rope layers --------------------------------------------------
+    def _ada_window(self):
+        """(window that sets the base, scaling factor), which is all that the tables of layers differ in."""
+        cfg = self.config
+        return (4096, cfg.scaling_factor) if cfg.yoco_window and cfg.local_window == cfg.block_size // 2 else (cfg.local_window, 1.0)
+
     def _ada_rope(self, x: torch.Tensor, T: int):
         cfg = self.config
-        if cfg.yoco_window and cfg.local_window == cfg.block_size // 2:
-            initial_window, sf = 4096, cfg.scaling_factor
-        else:
-            initial_window, sf = cfg.local_window, 1.0
+        initial_window, sf = self._ada_window()
         if self.rope_cache is None or T > self.max_len:
             self.max_len = max(T, self.max_len)
             self.rope_cache = ops.build_rope_cache(self.max_len, int(cfg.rotary_percentage * cfg.head_size),
@@ -213,7 +215,7 @@ class CausalSelfAttention(nn.Module):
         cfg = self.config
         if cfg.ada_rope:
             assert cfg.local_window > 0
-            rope = tuple(t[:T] for t in self._ada_rope(x, T)) if cache is None else cache.positions(self, lambda: self._ada_rope(x, cache.capacity), T)
+            rope = tuple(t[:T] for t in self._ada_rope(x, T)) if cache is None else cache.positions(self._ada_window(), lambda: self._ada_rope(x, cache.capacity), T)
         H, G, hs = self.n_head, self.n_query_groups, self.head_size
         g = None
         if self.yoco_cross:

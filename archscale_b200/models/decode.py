@@ -7,7 +7,7 @@ cache of the layer that made their keys.
 """
 from __future__ import annotations
 
-from typing import Callable, Dict, List, Optional, Tuple
+from typing import Callable, Dict, Hashable, List, Optional, Tuple
 
 import torch
 
@@ -59,7 +59,7 @@ class DecodeCache:
         self._at, self._open, self._tokens = -1, 0, 0
         self._capturing, self._captured = False, False
         self._rows: Optional[torch.Tensor] = None                 # positions of a captured call's tokens
-        self._tables: Dict[torch.nn.Module, Tuple[torch.Tensor, torch.Tensor]] = {}      # captured calls read them: they live as long as the cache
+        self._tables: Dict[Hashable, Tuple[torch.Tensor, torch.Tensor]] = {}       # captured calls read them: they live as long as the cache
 
     def _in_capture(self) -> bool:
         if not self.lengths.is_cuda:
@@ -111,14 +111,14 @@ class DecodeCache:
         """Whether the tokens of this call are the first ones: attention over them alone."""
         return self._tokens == 0
 
-    def positions(self, owner: torch.nn.Module, table: Callable[[], Tuple[torch.Tensor, torch.Tensor]], T: int) -> Tuple[torch.Tensor, torch.Tensor]:
-        """Rows of the rotary table of a model or layer, which covers the capacity, at the positions of the T new tokens.  It is kept as the first call
-        had it, since graphs read it; a captured call gathers the rows on the device."""
-        if owner not in self._tables and not self._capturing:
-            self._tables[owner] = table()
+    def positions(self, name: Hashable, table: Callable[[], Tuple[torch.Tensor, torch.Tensor]], T: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Rows of a rotary table, which covers the capacity, at the positions of the T new tokens.  ``name`` tells the tables of a model apart.  One is kept
+        as the first call had it, since graphs read it; a captured call gathers the rows on the device."""
+        if name not in self._tables and not self._capturing:
+            self._tables[name] = table()
         if self._capturing:
-            return tuple(t.index_select(0, self._rows) for t in self._tables[owner])
-        return tuple(t[self._tokens:self._tokens + T] for t in self._tables[owner])
+            return tuple(t.index_select(0, self._rows) for t in self._tables[name])
+        return tuple(t[self._tokens:self._tokens + T] for t in self._tables[name])
 
     def bounded(self, x: torch.Tensor) -> torch.Tensor:
         """The model's output, NaN in replays past the capacity."""

@@ -537,7 +537,7 @@ class GPT(nn.Module):
                     self.max_len = max(n, self.max_len)
                     self.rope_cache = self.build_rope_cache(idx, self.max_len)
                 return self.rope_cache
-            rope = tuple(t[:T] for t in table(T)) if cache is None else cache.positions(self, lambda: table(cache.capacity), T)
+            rope = tuple(t[:T] for t in table(T)) if cache is None else cache.positions("rope", lambda: table(cache.capacity), T)
         x = self.transformer.wte(idx)
         if self.scale_embed:
             x = x * math.sqrt(cfg.n_embd)

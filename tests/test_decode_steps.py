@@ -1,4 +1,6 @@
 """Steps over a key-value cache that are captured, replayed, mixed with others, or fail."""
+import copy
+
 import pytest
 import torch
 
@@ -143,3 +145,26 @@ def test_replays(name, dtype):
         assert bool(graphs[0][1].isnan().all())
         with pytest.raises(ValueError, match="41 are there"):
             m(token, cache=cache)
+
+
+@pytest.mark.parametrize("name", ["grouped", "windowed_rotary"])
+def test_copies_of_a_cache(name, monkeypatch):
+    """A copy goes on by itself, captured or not, and holds no copy of the model."""
+    m = make(name)
+
+    def refuse(self, memo):
+        raise AssertionError("a copy of a module")
+
+    cache = DecodeCache(m, 3, 12, page_size=5)
+    with torch.no_grad():
+        want = m(IDS[:, :12]).logits
+        m(IDS[:, :7], cache=cache)
+        with monkeypatch.context() as patch:
+            patch.setattr(torch.nn.Module, "__deepcopy__", refuse, raising=False)
+            other = copy.deepcopy(cache)
+        for c in (other, cache):
+            assert near(m(IDS[:, 7:9], cache=c).logits, want[:, 7:9])
+            with monkeypatch.context() as patch:
+                patch.setattr(DecodeCache, "_in_capture", lambda self: True)
+                for t in (9, 10, 11):
+                    assert near(m(IDS[:, t:t + 1], cache=c).logits, want[:, t:t + 1])
