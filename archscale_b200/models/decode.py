@@ -38,7 +38,7 @@ class DecodeCache:
 
     Once a cache holds tokens, calls can be captured by ``torch.cuda.graph``.  A capture appends nothing; each replay takes its positions from
     ``lengths`` on the device and advances them.  A replay that the capacity has no room for gives NaN.  Replays and other calls may follow one another
-    in any order: after a capture ``tokens`` (and so the next call that is not captured) reads ``lengths``, which waits for the device."""
+    on a stream in any order: after a capture ``tokens`` (and so the next call that is not captured) reads ``lengths``, which waits for the device."""
 
     def __init__(self, model, batch: int, capacity: int, page_size: int = 64, dtype: Optional[torch.dtype] = None, device=None) -> None:
         why = unsupported(model)
